@@ -559,6 +559,66 @@ int rt_search_epilogue(int64_t* ids, const int32_t* raw_dots, float* out_scores,
                        int64_t k, const int64_t* sort_perm, int64_t n_perm, const float* q_scales,
                        const float* global_scale, rt_stream_t stream);
 
+/* --- a paged key/value cache searched by block -------------------------------------------------
+ * No counterpart in the reference: the scoring-and-selection path applied to a language model's
+ * cache. Conventions of the three calls: T packed tokens, token t at positions[t] of sequence
+ * seq_ids[t] (a row of page_table int32 [B, max_pages]: the physical page of each block of `page`
+ * tokens; an entry outside [0, P) is absent). A token whose position is negative or past the page
+ * table, or whose sequence is outside [0, B), is padding. Hq query heads, Hq / Hkv of them to a
+ * key/value head. dtype 0 = bf16, 1 = fp16 (queries, keys, values, outputs). D in {64, 96, 128, 192,
+ * 256}; page in {16, 32, 64, 128}. k_cache, v_cache [P, Hkv, page, D]; bounds int8 [P, Hkv, 2 D];
+ * bound_scales float [P, Hkv]. q, k, v are [T, heads, D] with the strides given (in elements, D's
+ * is 1); every row starts on 16 bytes. */
+
+/* Queries, keys and values of new tokens: queries rotated into q_out [T, Hq, D], keys rotated and
+ * values as they are written to their slots. cos_sin float [table_len, rot]: a position's rot / 2
+ * cosines, then its sines; channels (i, i + rot / 2) make a pair, (2 i, 2 i + 1) where
+ * `interleaved`; channels from rot on stay; rot even, 0: no rotation. Products and sums are each
+ * rounded to float once. A token at the last slot of its block fills the block's bounds: over the
+ * page's stored keys mid = (max + min) / 2, half = (max - min) / 2 per channel, [mid | half] as
+ * codes rint(x / a * 127) with a = max(max |x|, 1e-8) and scale a / 127. The block's earlier keys are
+ * taken from this call where they are the tokens right before it (same sequence, consecutive
+ * positions), else from the cache: a sequence's tokens come in order, side by side. Padding
+ * tokens, and tokens past cos_sin or without a page, write nothing but a zero row of q_out. Two tokens at
+ * one slot are not allowed. */
+int rt_kv_append(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                 int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                 int64_t v_token_stride, int64_t v_head_stride, int64_t T, int64_t Hq, int64_t Hkv,
+                 int64_t D, int dtype, const float* cos_sin, int64_t table_len, int64_t rot,
+                 int interleaved, const int32_t* positions, const int32_t* seq_ids,
+                 const int32_t* page_table, int64_t B, int64_t max_pages, void* k_cache,
+                 void* v_cache, int64_t P, int64_t page, int8_t* bounds, float* bound_scales,
+                 void* q_out, rt_stream_t stream);
+
+/* The blocks each token and key/value head attends to -> out int32 [T, Hkv, count], ascending, -1 at
+ * the end. The token's own block is last = position / page. Blocks below `sink` and the `recent`
+ * ones up to last are always kept (recent >= 1: the own block may have no bounds yet; sink +
+ * recent <= count <= 1024); the other places go to the blocks between, by (score desc, block asc). A
+ * query head's row is quantised as bounds are (codes c, scale s); score(b) = max over the group's
+ * heads of float(c . mid_b + |c| . half_b) * s, times the block's scale (the sum exact in int32,
+ * two float products); not a number ranks last. Blocks without a page are not candidates. */
+size_t rt_kv_select_workspace(int64_t T, int64_t Hkv, int64_t max_pages);
+int rt_kv_select(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t T,
+                 int64_t Hq, int64_t Hkv, int64_t D, int dtype, const int8_t* bounds,
+                 const float* bound_scales, int64_t P, int64_t page, const int32_t* positions,
+                 const int32_t* seq_ids, const int32_t* page_table, int64_t B, int64_t max_pages,
+                 int64_t count, int64_t sink, int64_t recent, int32_t* out, void* workspace,
+                 size_t workspace_bytes, rt_stream_t stream);
+
+/* Softmax attention over listed blocks: blocks int32 [T, Hkv, count] (each block at most once a row,
+ * any order; entries below 0, past the token's block or without a page are skipped), the keys at
+ * positions up to the token's, scores scale * q . k -> out [T, Hq, D], lse float [T, Hq] (natural
+ * log of the weights' sum). A row without a key: zeros and -inf. Cache slots past a token's
+ * position are never used, whatever they hold. */
+size_t rt_kv_attention_workspace(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t page,
+                                 int64_t count);
+int rt_kv_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t T,
+                    int64_t Hq, int64_t Hkv, int64_t D, int dtype, const void* k_cache,
+                    const void* v_cache, int64_t P, int64_t page, const int32_t* blocks,
+                    int64_t count, const int32_t* positions, const int32_t* seq_ids,
+                    const int32_t* page_table, int64_t B, int64_t max_pages, float scale, void* out,
+                    float* lse, void* workspace, size_t workspace_bytes, rt_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

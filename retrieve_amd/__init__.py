@@ -4,14 +4,15 @@ path: hand-written HIP kernels behind a C ABI (``include/retrieve_amd.h``,
 ``torch.ops.st.*`` ops.
 
 ``import retrieve_amd`` registers nothing; ``retrieve_amd.hip`` registers the
-``torch.ops.retrieve.*`` ops when imported.
+``torch.ops.retrieve.*`` ops when imported, ``retrieve_amd.kv`` the paged-cache ops
+``torch.ops.retrieve_kv.*``.
 """
 
 from __future__ import annotations
 
 import importlib
 
-_SUBMODULES = ("hip",)
+_SUBMODULES = ("hip", "kv")
 
 
 def __getattr__(name: str):
