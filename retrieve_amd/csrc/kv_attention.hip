@@ -1,8 +1,25 @@
 // Softmax attention of each token over the blocks chosen for it and its key/value head.
 //
-// out = sum_j exp(x_j - m) v_j / l over the keys j of the listed blocks at positions up to the token's,
-// with x_j = scale q . k_j, m their maximum and l the sum of the weights, kept running over one
-// pass (a new maximum rescales what is summed); lse = m + log l. Rows without a key: 0 and -inf.
+// out = sum_j exp(x_j - m) v_j / l over the keys j of the listed blocks at positions up to the
+// token's, with x_j = scale q . k_j, m their maximum and l the sum of the weights, kept running
+// over one pass; lse = m + log l. Rows without a key: 0 and -inf.
+//
+// A wave holds up to 16 query heads of one key/value head (the heads that share it: its keys and
+// values are read once for all of them) and takes 32 keys a step:
+//   S^T [keys x heads] = K Q^T   K's rows straight from memory in the operand's layout (a lane has
+//                                16 bytes of one key), Q^T in registers throughout;
+//   O^T [channels x heads] += V^T P^T   the weights are where the first product left them (lane l:
+//                                head l % 16, keys 4 (l / 16) + r of each 16), so P^T needs no
+//                                exchange; V is staged through the wave's own LDS, swizzled, and
+//                                read transposed (ds_read_tr: 4 keys of one channel a lane).
+// A lane's column is one head in both products: maxima, sums and rescaling stay in the lane. The
+// maximum is raised only where a score passes it by 8 (in powers of two: weights reach 256 at
+// most, far inside both types), so most steps do not touch the accumulators or exchange lanes.
+// Weights are rounded to the values' 16 bits for the matrix cores (l sums them unrounded):
+// relative 2^-9 / 2^-12 a weight, the size of the output's own rounding.
+//
+// Memory: a wave keeps the next step's keys and values in flight (registers) while it works on
+// this one. Slots past the token's position are read but replaced: scores by -inf, values by 0.
 #include <type_traits>
 
 #include "../../include/retrieve_amd.h"
@@ -10,87 +27,398 @@
 
 namespace rt {
 
+constexpr int kAttendWaves = 4;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
 struct AttendArgs {
   const void* q;
   int64_t q_st, q_sh;
   int64_t T;
-  int32_t Hq, Hkv;
+  int32_t Hq, Hkv, G, tiles;  // G query heads a key/value head, in tiles of 16
   const void *k_cache, *v_cache;
   const int32_t* blocks;  // [T, Hkv, count]
   int32_t count;
   KvTokens tok;
-  float scale;
-  void* out;   // [T, Hq, D]
-  float* lse;  // [T, Hq]
+  float scale;      // times log2 e
+  int32_t parts;    // workgroups that share a row
+  void* out;        // [T, Hq, D]
+  float* lse;       // [T, Hq]
+  float* part_out;  // [rows, parts, 16, D], sums of weights times values
+  float* part_ml;   // [rows, parts, 16, 2], maxima (powers of two) and sums
 };
 
-// One wave a token and query head; a lane scores one key of 64, then sums its own channels.
-template <class E, int D>
-__global__ void __launch_bounds__(kWave) kv_attention_kernel(AttendArgs a) {
-  using V8 = typename Kv<E>::V8;
-  constexpr int R = (D + kWave - 1) / kWave;
-  __shared__ float qs[D];
-  const int64_t t = blockIdx.x / a.Hq;
-  const int hq = blockIdx.x % a.Hq, h = hq / (a.Hq / a.Hkv);
-  const int lane = lane_id();
-  const KvPlace p = kv_place(a.tok, t);
-  const E* q = static_cast<const E*>(a.q) + t * a.q_st + hq * a.q_sh;
-  for (int d = lane; d < D; d += kWave) qs[d] = static_cast<float>(q[d]) * a.scale;
-  __syncthreads();
-  const int size = 1 << a.tok.shift;
-  const int32_t* list = a.blocks + (t * a.Hkv + h) * a.count;
-  float m = -INFINITY, l = 0.0f, acc[R] = {};
-  for (int i = 0; i < a.count; ++i) {
-    const int32_t block = list[i];
-    if (block < 0 || block > p.last) continue;
-    const int32_t page = kv_page(a.tok, p, block);
-    if (page < 0) continue;
-    const int64_t base = ((static_cast<int64_t>(page) * a.Hkv + h) << a.tok.shift) * D;
-    const int64_t first = static_cast<int64_t>(block) << a.tok.shift;
-    const int keys = p.pos - first + 1 < size ? static_cast<int>(p.pos - first + 1) : size;
-    for (int j0 = 0; j0 < keys; j0 += kWave) {
-      const int j = j0 + lane;
-      float x = -INFINITY;
-      if (j < keys) {
-        const E* k = static_cast<const E*>(a.k_cache) + base + static_cast<int64_t>(j) * D;
-        x = 0.0f;
-        for (int d = 0; d < D; d += 8) {
-          const V8 kv = *reinterpret_cast<const V8*>(k + d);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x = fmaf(static_cast<float>(kv[e]), qs[d + e], x);
-        }
-      }
-      float top = x;
-      for (int s = 1; s < kWave; s <<= 1) top = fmaxf(top, __shfl_xor(top, s));
-      const float next = fmaxf(m, top);
-      const float safe = next == -INFINITY ? 0.0f : next;
-      const float w = __expf(x - safe), keep = __expf(m - safe);
-      float sum = w;
-      for (int s = 1; s < kWave; s <<= 1) sum += __shfl_xor(sum, s);
-      l = l * keep + sum;
-      m = next;
-#pragma unroll
-      for (int r = 0; r < R; ++r) acc[r] *= keep;
-      const int n = keys - j0 < kWave ? keys - j0 : kWave;
-      for (int jj = 0; jj < n; ++jj) {
-        const float wj = __shfl(w, jj);
-        const E* v = static_cast<const E*>(a.v_cache) + base + static_cast<int64_t>(j0 + jj) * D;
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-          const int d = r * kWave + lane;
-          if (d < D) acc[r] = fmaf(wj, static_cast<float>(v[d]), acc[r]);
+template <class E>
+struct AttendOp;
+template <>
+struct AttendOp<__bf16> {
+  using V8 = Kv<__bf16>::V8;
+  typedef __bf16 V4 __attribute__((ext_vector_type(4)));
+  __device__ static v4f mma(V8 a, V8 b, v4f c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+  __device__ static V4 read_tr(const char* lds) {
+    typedef __attribute__((address_space(3))) V4 LdsV4;
+    return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((LdsV4*)lds);
+  }
+};
+template <>
+struct AttendOp<_Float16> {
+  using V8 = Kv<_Float16>::V8;
+  typedef _Float16 V4 __attribute__((ext_vector_type(4)));
+  __device__ static v4f mma(V8 a, V8 b, v4f c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+  __device__ static V4 read_tr(const char* lds) {
+    typedef __fp16 Raw __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) Raw LdsRaw;
+    return __builtin_bit_cast(V4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((LdsRaw*)lds));
+  }
+};
+
+// The staged values: 32 rows of D channels; the 32-byte granules of a row are permuted by the row
+// so that the 16 rows a transposed read takes at one channel lie in different banks.
+template <int D>
+__device__ inline int granule_swizzle(int row) {
+  return D % 128 == 0 ? row & 7 : D % 64 == 0 ? (row >> 1) & 3 : (row >> 2) & 1;
+}
+
+// A step's two tiles of 16 keys: their first rows in the caches and how many keys count.
+struct Tiles {
+  int64_t row[2];
+  int n[2];
+};
+
+// The tiles of one wave: of a row's list in units of 64 keys, units part, part + parts, ... A chunk
+// of 16 units is looked up at a time, one tile a lane; steps (two neighbouring tiles) without keys
+// are left out.
+struct TileList {
+  const int32_t* list;
+  KvPlace place;
+  int32_t head, part, parts, chunk;
+  uint64_t left;  // tiles of this chunk with keys to come
+  int32_t page, at;  // this lane's: physical page, first slot * 32 + keys
+
+  __device__ void fetch(const AttendArgs& a) {
+    const int64_t unit = part + static_cast<int64_t>(parts) * (16 * chunk + (lane_id() >> 2));
+    const int64_t key = unit * 64 + 16 * (lane_id() & 3);
+    const int64_t entry = key >> a.tok.shift;
+    page = 0;
+    at = 0;
+    if (entry < a.count) {
+      const int32_t block = list[entry];
+      if (block >= 0 && block <= place.last) {
+        const int32_t p = kv_page(a.tok, place, block);
+        const int32_t slot = static_cast<int32_t>(key) & ((1 << a.tok.shift) - 1);
+        const int32_t n = place.pos - (block << a.tok.shift) - slot + 1;
+        if (p >= 0 && n > 0) {
+          page = p;
+          at = slot * 32 + (n < 16 ? n : 16);
         }
       }
     }
+    left = __ballot(at != 0);
   }
-  const float inv = l > 0.0f ? 1.0f / l : l == l ? 0.0f : l;
-  E* out = static_cast<E*>(a.out) + (t * a.Hq + hq) * D;
+  __device__ bool next(const AttendArgs& a, Tiles& s) {
+    while (left == 0) {
+      ++chunk;
+      const int64_t first = (part + static_cast<int64_t>(parts) * 16 * chunk) * 64;
+      if (first >= static_cast<int64_t>(a.count) << a.tok.shift) return false;
+      fetch(a);
+    }
+    const int i = __builtin_ctzll(left) & ~1;
+    left &= ~(uint64_t{3} << i);
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int d = r * kWave + lane;
-    if (d < D) out[d] = static_cast<E>(acc[r] * inv);
+    for (int j = 0; j < 2; ++j) {
+      const int32_t p = __builtin_amdgcn_readlane(page, i + j);
+      const int32_t x = __builtin_amdgcn_readlane(at, i + j);
+      s.row[j] = ((static_cast<int64_t>(p) * a.Hkv + head) << a.tok.shift) + (x >> 5);
+      s.n[j] = x & 31;
+    }
+    return true;
   }
-  if (lane == 0) a.lse[t * a.Hq + hq] = l > 0.0f || l != l ? m + logf(l) : -INFINITY;
+};
+
+// One wave's pass over its tiles: the accumulators (channel 16 i + 4 (lane / 16) + r of head
+// lane % 16), the maximum and this lane's share of the sum.
+template <class E, int D>
+struct AttendWave {
+  using Op = AttendOp<E>;
+  using V8 = typename Op::V8;
+  static constexpr int KS = D / 32, DT = D / 16, VL = D / 16;  // VL: 16-byte loads of V a lane
+  v4f acc[DT];
+  float m, l;
+
+  __device__ void run(const AttendArgs& a, int64_t t, int head, int tile, int part, int parts,
+                      char* lds) {
+    const int lane = lane_id(), col = lane & 15, grp = lane >> 4;
+#pragma unroll
+    for (int i = 0; i < DT; ++i) acc[i] = v4f{0.f, 0.f, 0.f, 0.f};
+    m = -3.402823466e38f;
+    l = 0.0f;
+    TileList tiles;
+    tiles.place = kv_place(a.tok, t);
+    if (tiles.place.last < 0) return;
+    tiles.list = a.blocks + (t * a.Hkv + head) * a.count;
+    tiles.head = head;
+    tiles.part = part;
+    tiles.parts = parts;
+    tiles.chunk = -1;
+    tiles.left = 0;
+
+    V8 qf[KS];
+    const bool real = tile * 16 + col < a.G;
+    const E* q = static_cast<const E*>(a.q) + t * a.q_st +
+                 static_cast<int64_t>(head * a.G + (real ? tile * 16 + col : 0)) * a.q_sh + grp * 8;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const V8 x = *reinterpret_cast<const V8*>(q + 32 * s);
+      qf[s] = real ? x : V8{};
+    }
+
+    V8 kf[2][KS], vf[VL];
+    auto load_k = [&](const Tiles& s) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const E* base = static_cast<const E*>(a.k_cache) + s.row[j] * D;
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+          kf[j][i] = *reinterpret_cast<const V8*>(base + (col * D + grp * 8 + 32 * i));
+        }
+      }
+    };
+    auto load_v = [&](const Tiles& s) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const E* base = static_cast<const E*>(a.v_cache) + s.row[j] * D;
+#pragma unroll
+        for (int i = 0; i < VL / 2; ++i) {
+          vf[j * (VL / 2) + i] = *reinterpret_cast<const V8*>(base + (i * 64 + lane) * 8);
+        }
+      }
+    };
+
+    Tiles now, then;
+    bool more = tiles.next(a, then);
+    if (more) {
+      load_k(then);
+      load_v(then);
+    }
+    while (more) {
+      now = then;
+      more = tiles.next(a, then);
+      v4f sc[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        sc[j] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < KS; ++i) sc[j] = Op::mma(kf[j][i], qf[i], sc[j]);
+      }
+      if (more) load_k(then);
+      const bool whole = now.n[0] == 16 && now.n[1] == 16;
+      if (!whole) {
+#pragma unroll
+        for (int i = 0; i < VL; ++i) {
+          const int row = ((i % (VL / 2)) * 64 + lane) / (D / 8);
+          if (row >= now.n[i / (VL / 2)]) vf[i] = V8{};
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < VL; ++i) {
+        const int at = i * 64 + lane, row = at / (D / 8), c = at % (D / 8);
+        *reinterpret_cast<V8*>(lds + row * (D * 2) + (((c >> 1) ^ granule_swizzle<D>(row)) << 5) +
+                               (c & 1) * 16) = vf[i];
+      }
+      if (more) load_v(then);
+      float w[8];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float y = sc[j][r] * a.scale;
+          w[4 * j + r] = whole || 4 * grp + r < now.n[j] ? y : -INFINITY;
+        }
+      }
+      float top = w[0];
+#pragma unroll
+      for (int r = 1; r < 8; ++r) top = fmaxf(top, w[r]);
+      if (__any(top > m + 8.0f)) {
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float next = fmaxf(m, top);
+        const float keep = __builtin_amdgcn_exp2f(m - next);
+        m = next;
+        l *= keep;
+#pragma unroll
+        for (int i = 0; i < DT; ++i) acc[i] *= keep;
+      }
+      V8 p;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        const float e = __builtin_amdgcn_exp2f(w[r] - m);
+        l += e;
+        p[r] = static_cast<E>(e);
+      }
+      asm volatile("" ::: "memory");  // (the staged rows are read by other lanes of this wave)
+#pragma unroll
+      for (int i = 0; i < DT; ++i) {
+        typename Op::V4 x[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int row = 16 * j + 4 * grp + (col >> 2);
+          x[j] = Op::read_tr(lds + row * (D * 2) + ((i ^ granule_swizzle<D>(row)) << 5) +
+                             (col & 3) * 8);
+        }
+        const V8 v = {x[0][0], x[0][1], x[0][2], x[0][3], x[1][0], x[1][1], x[1][2], x[1][3]};
+        acc[i] = Op::mma(v, p, acc[i]);
+      }
+      asm volatile("" ::: "memory");
+    }
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+  }
+};
+
+// 1 / l; 0 for a row without a key; NaN stays.
+__device__ inline float inverse_sum(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
+__device__ inline float log_sum(float m, float l) {
+  return l == 0.0f ? -INFINITY : (m + __log2f(l)) * kLn2;
+}
+
+// Many rows: a wave a row, four neighbouring tokens of one head a workgroup (they mostly choose the
+// same blocks).
+template <class E, int D>
+__global__ void __launch_bounds__(kAttendWaves* kWave, D <= 128 ? 2 : 1)
+    kv_attend_rows_kernel(AttendArgs a) {
+  typedef E V4 __attribute__((ext_vector_type(4)));
+  __shared__ __attribute__((aligned(16))) char lds[kAttendWaves][64 * D];
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int heads = a.Hkv * a.tiles;
+  const int64_t t = static_cast<int64_t>(blockIdx.x / heads) * kAttendWaves + wave;
+  if (t >= a.T) return;
+  const int head = blockIdx.x % heads / a.tiles, tile = blockIdx.x % heads % a.tiles;
+  AttendWave<E, D> w;
+  w.run(a, t, head, tile, 0, 1, lds[wave]);
+  const int col = lane_id() & 15, grp = lane_id() >> 4, g = tile * 16 + col;
+  if (g >= a.G) return;
+  const int64_t row = t * a.Hq + head * a.G + g;
+  const float inv = inverse_sum(w.l);
+  E* out = static_cast<E*>(a.out) + row * D + 4 * grp;
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) {
+    V4 x;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) x[r] = static_cast<E>(w.acc[i][r] * inv);
+    *reinterpret_cast<V4*>(out + 16 * i) = x;
+  }
+  if (grp == 0) a.lse[row] = log_sum(w.m, w.l);
+}
+
+// Few rows: the workgroup's waves (and `parts` workgroups) share a row's list; their sums are joined
+// at the largest maximum, here where one workgroup has the whole row, else by kv_join_kernel.
+template <class E, int D>
+__global__ void __launch_bounds__(kAttendWaves* kWave, D <= 128 ? 2 : 1)
+    kv_attend_split_kernel(AttendArgs a) {
+  __shared__ __attribute__((aligned(16))) char lds[kAttendWaves][64 * D];
+  __shared__ float ml[kAttendWaves][16][2];
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int part = blockIdx.x % a.parts;
+  const int64_t row = blockIdx.x / a.parts;  // (token, key/value head, tile)
+  const int tile = static_cast<int>(row % a.tiles);
+  const int head = static_cast<int>(row / a.tiles % a.Hkv);
+  const int64_t t = row / a.tiles / a.Hkv;
+  AttendWave<E, D> w;
+  w.run(a, t, head, tile, part * kAttendWaves + wave, a.parts * kAttendWaves, lds[wave]);
+  // the sums as fp32 rows of a head, 16-byte chunks permuted by the head (bank conflicts)
+  const int col = lane_id() & 15, grp = lane_id() >> 4;
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) {
+    *reinterpret_cast<v4f*>(lds[wave] + col * (D * 4) + (((4 * i + grp) ^ (col & 7)) << 4)) =
+        w.acc[i];
+  }
+  if (grp == 0) {
+    ml[wave][col][0] = w.m;
+    ml[wave][col][1] = w.l;
+  }
+  __syncthreads();
+  const int heads = a.G - tile * 16 < 16 ? a.G - tile * 16 : 16;
+  for (int i = threadIdx.x; i < heads * (D / 4); i += kAttendWaves * kWave) {
+    const int g = i / (D / 4), c = i % (D / 4);
+    float m = ml[0][g][0];
+#pragma unroll
+    for (int j = 1; j < kAttendWaves; ++j) m = fmaxf(m, ml[j][g][0]);
+    float l = 0.0f;
+    v4f sum{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < kAttendWaves; ++j) {
+      const float f = __builtin_amdgcn_exp2f(ml[j][g][0] - m);
+      l += f * ml[j][g][1];
+      sum += f * *reinterpret_cast<const v4f*>(lds[j] + g * (D * 4) + ((c ^ (g & 7)) << 4));
+    }
+    if (a.parts == 1) {
+      typedef E V4 __attribute__((ext_vector_type(4)));
+      const int64_t r = t * a.Hq + head * a.G + tile * 16 + g;
+      const float inv = inverse_sum(l);
+      V4 x;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = static_cast<E>(sum[e] * inv);
+      *reinterpret_cast<V4*>(static_cast<E*>(a.out) + r * D + 4 * c) = x;
+      if (c == 0) a.lse[r] = log_sum(m, l);
+    } else {
+      const int64_t r = (row * a.parts + part) * 16 + g;
+      *reinterpret_cast<v4f*>(a.part_out + r * D + 4 * c) = sum;
+      if (c == 0) {
+        a.part_ml[2 * r] = m;
+        a.part_ml[2 * r + 1] = l;
+      }
+    }
+  }
+}
+
+// The parts of a row joined at their largest maximum, in order: a thread has 4 channels of a head.
+template <class E, int D>
+__global__ void __launch_bounds__(D / 4) kv_join_kernel(AttendArgs a) {
+  typedef E V4 __attribute__((ext_vector_type(4)));
+  const int64_t r = blockIdx.x;  // (token, query head)
+  const int64_t t = r / a.Hq;
+  const int hq = static_cast<int>(r % a.Hq), head = hq / a.G, g = hq % a.G;
+  const int64_t row = (t * a.Hkv + head) * a.tiles + g / 16;
+  const int64_t first = row * a.parts * 16 + g % 16;
+  float m = a.part_ml[2 * first];
+  for (int p = 1; p < a.parts; ++p) m = fmaxf(m, a.part_ml[2 * (first + 16 * p)]);
+  float l = 0.0f;
+  v4f sum{0.f, 0.f, 0.f, 0.f};
+  for (int p = 0; p < a.parts; ++p) {
+    const int64_t at = first + 16 * p;
+    const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * at] - m);
+    l += f * a.part_ml[2 * at + 1];
+    sum += f * *reinterpret_cast<const v4f*>(a.part_out + at * D + 4 * threadIdx.x);
+  }
+  const float inv = inverse_sum(l);
+  V4 x;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] = static_cast<E>(sum[e] * inv);
+  *reinterpret_cast<V4*>(static_cast<E*>(a.out) + r * D + 4 * threadIdx.x) = x;
+  if (threadIdx.x == 0) a.lse[r] = log_sum(m, l);
+}
+
+// How a call is spread. 0 parts: a wave a row.
+struct AttendPlan {
+  int64_t rows;
+  int32_t tiles, parts;
+};
+
+inline AttendPlan attend_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t page, int64_t count) {
+  AttendPlan p;
+  p.tiles = static_cast<int32_t>(cdiv(Hq / Hkv, 16));
+  p.rows = T * Hkv * p.tiles;
+  p.parts = 0;
+  if (p.rows >= 4096) return p;
+  // workgroups of four waves for two on every CU, each wave with a unit of 64 keys at least
+  const int64_t most = cdiv(count * page, 64 * kAttendWaves);
+  const int64_t want = cdiv(512, p.rows > 0 ? p.rows : 1);
+  p.parts = static_cast<int32_t>(want < most ? want : most);
+  if (p.parts < 1) p.parts = 1;
+  return p;
 }
 
 }  // namespace rt
@@ -99,7 +427,9 @@ using namespace rt;
 
 extern "C" size_t rt_kv_attention_workspace(int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
                                             int64_t page, int64_t count) {
-  return 0;
+  if (Hkv < 1 || T < 1) return 0;
+  const AttendPlan p = attend_plan(T, Hq, Hkv, page, count);
+  return p.parts > 1 ? static_cast<size_t>(p.rows) * p.parts * 16 * (D + 2) * sizeof(float) : 0;
 }
 
 extern "C" int rt_kv_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride,
@@ -126,18 +456,33 @@ extern "C" int rt_kv_attention(const void* q, int64_t q_token_stride, int64_t q_
     set_error("workspace too small: %zu < %zu", workspace_bytes, need);
     return kWorkspaceTooSmall;
   }
+  const AttendPlan plan = attend_plan(T, Hq, Hkv, page, count);
   AttendArgs a{};
   a.q = q, a.q_st = q_token_stride, a.q_sh = q_head_stride, a.T = T;
   a.Hq = static_cast<int32_t>(Hq), a.Hkv = static_cast<int32_t>(Hkv);
+  a.G = a.Hq / a.Hkv, a.tiles = plan.tiles;
   a.k_cache = k_cache, a.v_cache = v_cache, a.blocks = blocks;
   a.count = static_cast<int32_t>(count);
   a.tok = {positions, seq_ids, page_table, static_cast<int32_t>(B),
            static_cast<int32_t>(max_pages), static_cast<int32_t>(P), kv_shift(page)};
-  a.scale = scale, a.out = out, a.lse = lse;
+  a.scale = scale * kLog2e, a.out = out, a.lse = lse, a.parts = plan.parts;
+  a.part_out = static_cast<float*>(workspace);
+  a.part_ml = a.part_out + (plan.parts > 1 ? plan.rows * plan.parts * 16 * D : 0);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
   return kv_dispatch(dtype, D, [&](auto e, auto d) -> int {
-    kv_attention_kernel<decltype(e), decltype(d)::value>
-        <<<dim3(static_cast<unsigned>(T * Hq)), dim3(kWave), 0, static_cast<hipStream_t>(stream)>>>(
-            a);
+    using E = decltype(e);
+    constexpr int DD = decltype(d)::value;
+    const dim3 threads(kAttendWaves * kWave);
+    if (plan.parts == 0) {
+      const int64_t grid = cdiv(T, kAttendWaves) * Hkv * plan.tiles;
+      kv_attend_rows_kernel<E, DD><<<dim3(static_cast<unsigned>(grid)), threads, 0, s>>>(a);
+    } else {
+      const int64_t grid = plan.rows * plan.parts;
+      kv_attend_split_kernel<E, DD><<<dim3(static_cast<unsigned>(grid)), threads, 0, s>>>(a);
+      if (plan.parts > 1) {
+        kv_join_kernel<E, DD><<<dim3(static_cast<unsigned>(T * Hq)), dim3(DD / 4), 0, s>>>(a);
+      }
+    }
     RT_CHECK_HIP(hipGetLastError());
     return kOk;
   });
