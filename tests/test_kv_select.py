@@ -59,7 +59,8 @@ def test_selection_by_rationals():
 @pytest.mark.parametrize("kind,heads,heads_kv,d,page", [
     ("bf16", 8, 2, 128, 64), ("fp16", 3, 3, 64, 16), ("bf16", 7, 1, 96, 32), ("fp16", 12, 2, 192, 16),
     ("bf16", 2, 1, 256, 128), ("fp16", 40, 2, 64, 16), ("bf16", 17, 1, 128, 16),
-    ("bf16", 10, 5, 64, 64)])
+    ("bf16", 10, 5, 64, 64), ("bf16", 80, 1, 64, 16), ("fp16", 40, 1, 256, 32),
+    ("bf16", 33, 1, 96, 64), ("fp16", 4, 1, 192, 64), ("bf16", 1, 1, 128, 16)])
 def test_matches_the_oracle(dev, kind, heads, heads_kv, d, page):
     decode = [(n * page + r, 1) for n, r in [(0, 0), (0, page - 1), (1, 0), (3, 5), (9, 0), (20, 7),
                                               (63, 1), (64, page - 1), (65, 0), (130, 3)]]
