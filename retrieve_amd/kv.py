@@ -53,65 +53,86 @@ _lib.define("block_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor bl
 def _check_tokens(t: int, positions: Tensor, seq_ids: Tensor, page_table: Tensor) -> None:
     if positions.shape != (t,) or seq_ids.shape != (t,) or page_table.dim() != 2:
         raise ValueError(f"positions and seq_ids must be [{t}] and page_table [B, max_pages]")
-    if not (positions.dtype == seq_ids.dtype == page_table.dtype == torch.int32):
+    if not (positions.dtype is seq_ids.dtype is page_table.dtype is torch.int32):
         raise TypeError("positions, seq_ids and page_table must be int32")
     if not (positions.is_contiguous() and seq_ids.is_contiguous() and page_table.is_contiguous()):
         raise ValueError("positions, seq_ids and page_table must be contiguous")
 
 
-def _check_heads(q: Tensor, heads_kv: int, dim: int, page: int) -> int:
-    """The dtype's number, after the checks of a ``[T, Hq, D]`` query against the cache's heads."""
-    if q.dim() != 3 or q.shape[2] != dim:
-        raise ValueError(f"q must be [T, Hq, {dim}], got {list(q.shape)}")
-    if q.dtype not in DTYPES:
-        raise TypeError(f"q must be bfloat16 or float16, got {q.dtype}")
+def _check_heads(dtype: torch.dtype, heads: int, heads_kv: int, dim: int, page: int) -> int:
+    """The dtype's number, after the checks of the numbers that every call has."""
+    if dtype not in DTYPES:
+        raise TypeError(f"q must be bfloat16 or float16, got {dtype}")
     if dim not in HEAD_DIMS:
         raise TypeError(f"heads have {HEAD_DIMS} channels, got {dim}")
     if page not in PAGE_SIZES:
         raise ValueError(f"a page holds {PAGE_SIZES} tokens, got {page}")
-    if heads_kv < 1 or q.shape[1] < 1 or q.shape[1] % heads_kv:
-        raise ValueError(f"{q.shape[1]} query heads do not share {heads_kv} key/value heads evenly")
-    return DTYPES[q.dtype]
+    if heads_kv < 1 or heads < 1 or heads % heads_kv:
+        raise ValueError(f"{heads} query heads do not share {heads_kv} key/value heads evenly")
+    return DTYPES[dtype]
 
 
-def _check_caches(q: Tensor, k_cache: Tensor, v_cache: Tensor) -> int:
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
+def _check_caches(q: Tensor, k_cache: Tensor, v_cache: Tensor):
+    """``(T, Hq, P, Hkv, page, D, dtype's number)``"""
+    shape = k_cache.shape
+    if len(shape) != 4 or v_cache.shape != shape:
         raise ValueError("k_cache and v_cache must both be [P, Hkv, page, D]")
-    if k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+    pages, heads_kv, page, dim = shape
+    if q.dim() != 3 or q.shape[2] != dim:
+        raise ValueError(f"q must be [T, Hq, {dim}], got {list(q.shape)}")
+    t, heads, _ = q.shape
+    if not (q.dtype is k_cache.dtype is v_cache.dtype):
         raise TypeError("q and the caches must have one dtype")
     if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         raise ValueError("k_cache and v_cache must be contiguous")
-    return _check_heads(q, k_cache.shape[1], k_cache.shape[3], k_cache.shape[2])
+    return t, heads, pages, heads_kv, page, dim, _check_heads(q.dtype, heads, heads_kv, dim, page)
 
 
-def _check_bounds(bounds: Tensor, bound_scales: Tensor, pages: int | None, dim: int) -> None:
-    if (bounds.dim() != 3 or bounds.shape[2] != 2 * dim or bound_scales.shape != bounds.shape[:2]
-            or (pages is not None and bounds.shape[0] != pages)):
+def _check_bounds(bounds: Tensor, bound_scales: Tensor, dim: int) -> tuple[int, int]:
+    """``(P, Hkv)``"""
+    shape = bounds.shape
+    if len(shape) != 3 or shape[2] != 2 * dim or bound_scales.shape != shape[:2]:
         raise ValueError("bounds must be [P, Hkv, 2 D] and bound_scales [P, Hkv]")
-    if bounds.dtype != torch.int8 or bound_scales.dtype != torch.float32:
+    if bounds.dtype is not torch.int8 or bound_scales.dtype is not torch.float32:
         raise TypeError("bounds must be int8 and bound_scales float32")
     if not (bounds.is_contiguous() and bound_scales.is_contiguous()):
         raise ValueError("bounds and bound_scales must be contiguous")
+    return shape[0], shape[1]
 
 
 def _rows(x: Tensor) -> tuple[Tensor, int, int]:
     """``x [T, H, D]`` with its token and head strides, where its rows lie as the kernels read them
     (16-byte chunks of contiguous channels: the views of a fused projection do), else a copy."""
-    t, h, d = x.shape
     token, head, channel = x.stride()
-    token, head = token if t > 1 else 0, head if h > 1 else 0
     if channel != 1 or token % 8 or head % 8 or x.data_ptr() % 16:
         x = x.clone(memory_format=torch.contiguous_format)
+        _, h, d = x.shape
         token, head = h * d, d
     return x, token, head
 
 
-def _on(dev: torch.device):
+def _device(*tensors: Tensor) -> int:
+    """The GPU that holds all of them."""
+    at = tensors[0].get_device()
+    for t in tensors:
+        if t.get_device() != at or at < 0:
+            nat.require_device(*tensors)
+    return at
+
+
+def _on(device: int):
     """The tensors' GPU as the current one, where it is not already."""
-    return _HERE if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+    return _HERE if device == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 _HERE = contextlib.nullcontext()
+_stream = torch._C._cuda_getCurrentRawStream  # (the current stream's handle, without an object)
+
+
+def _eager(q: Tensor) -> bool:
+    """Whether a call can go straight to its kernels: plain tensors, nothing being traced. Elsewhere it
+    goes through the registered op (the dispatcher's 3 to 5 us a call are a third of a small one)."""
+    return type(q) is Tensor and not torch.compiler.is_compiling()
 
 
 # --- append -----------------------------------------------------------------------------------
@@ -119,41 +140,41 @@ _HERE = contextlib.nullcontext()
 
 def _append(q, k, v, cos_sin, positions, seq_ids, page_table, k_cache, v_cache, bounds,
             bound_scales, interleaved=False):
-    dtype = _check_caches(q, k_cache, v_cache)
-    pages, heads_kv, page, dim = k_cache.shape
-    t, heads = q.shape[:2]
+    t, heads, pages, heads_kv, page, dim, dtype = _check_caches(q, k_cache, v_cache)
     if k.shape != (t, heads_kv, dim) or v.shape != k.shape:
         raise ValueError(f"k and v must be [{t}, {heads_kv}, {dim}]")
-    if k.dtype != q.dtype or v.dtype != q.dtype:
+    if not (k.dtype is v.dtype is q.dtype):
         raise TypeError("q, k and v must have one dtype")
     _check_tokens(t, positions, seq_ids, page_table)
-    _check_bounds(bounds, bound_scales, pages, dim)
-    if bounds.shape[1] != heads_kv:
+    if _check_bounds(bounds, bound_scales, dim) != (pages, heads_kv):
         raise ValueError("bounds must be [P, Hkv, 2 D] and bound_scales [P, Hkv]")
-    rot = length = 0
-    on = [q, k, v, positions, seq_ids, page_table, k_cache, v_cache, bounds, bound_scales]
+    length = rot = 0
     if cos_sin is not None:
         if cos_sin.dim() != 2 or cos_sin.shape[1] % 2 or cos_sin.shape[1] > dim:
             raise ValueError(f"cos_sin must be [length, rot], rot even and at most {dim}")
-        if cos_sin.dtype != torch.float32:
+        if cos_sin.dtype is not torch.float32:
             raise TypeError("cos_sin must be float32")
         if not cos_sin.is_contiguous():
             raise ValueError("cos_sin must be contiguous")
+        if cos_sin.get_device() != q.get_device():
+            nat.require_device(q, cos_sin)
         length, rot = cos_sin.shape
         if cos_sin.data_ptr() % 16:
             cos_sin = cos_sin.clone()
-        on.append(cos_sin)
-    dev = nat.require_device(*on)
-    (q, *q_at), (k, *k_at), (v, *v_at) = _rows(q), _rows(k), _rows(v)
-    out = torch.empty((t, heads, dim), dtype=q.dtype, device=dev)
+    dev = _device(q, k, v, positions, seq_ids, page_table, k_cache, v_cache, bounds, bound_scales)
+    q, q_token, q_head = _rows(q)
+    k, k_token, k_head = _rows(k)
+    v, v_token, v_head = _rows(v)
+    out = q.new_empty((t, heads, dim))
     with _on(dev):
         st = nat.lib().rt_kv_append(
-            q.data_ptr(), *q_at, k.data_ptr(), *k_at, v.data_ptr(), *v_at, t, heads, heads_kv, dim,
-            dtype, nat.ptr(cos_sin), length, rot, bool(interleaved), positions.data_ptr(),
-            seq_ids.data_ptr(), page_table.data_ptr(), *page_table.shape, k_cache.data_ptr(),
-            v_cache.data_ptr(), pages, page, bounds.data_ptr(), bound_scales.data_ptr(),
-            out.data_ptr(), nat.stream(dev))
-    nat.check(st)
+            q.data_ptr(), q_token, q_head, k.data_ptr(), k_token, k_head, v.data_ptr(), v_token,
+            v_head, t, heads, heads_kv, dim, dtype, nat.ptr(cos_sin), length, rot, interleaved,
+            positions.data_ptr(), seq_ids.data_ptr(), page_table.data_ptr(), *page_table.shape,
+            k_cache.data_ptr(), v_cache.data_ptr(), pages, page, bounds.data_ptr(),
+            bound_scales.data_ptr(), out.data_ptr(), _stream(dev))
+    if st:
+        nat.check(st)
     return out
 
 
@@ -171,8 +192,9 @@ def append(q: Tensor, k: Tensor, v: Tensor, cos_sin: Tensor | None, positions: T
     largest values per channel, quantised as ``quantize_int8``'s rows. For that a sequence's
     tokens come in order, side by side. Tokens that are padding (a position below 0, or past the page
     table or ``cos_sin``; a sequence outside it; no page) write nothing and return a zero row."""
-    return _ops_append(q, k, v, cos_sin, positions, seq_ids, page_table, k_cache, v_cache, bounds,
-                       bound_scales, interleaved)
+    call = _append if _eager(q) else torch.ops.retrieve_kv.append
+    return call(q, k, v, cos_sin, positions, seq_ids, page_table, k_cache, v_cache, bounds,
+                bound_scales, interleaved)
 
 
 # --- select -----------------------------------------------------------------------------------
@@ -180,30 +202,31 @@ def append(q: Tensor, k: Tensor, v: Tensor, cos_sin: Tensor | None, positions: T
 
 def _select(q, bounds, bound_scales, positions, seq_ids, page_table, page_size, count, sink=1,
             recent=1):
-    if q.dim() != 3 or bounds.dim() != 3:
-        raise ValueError("q must be [T, Hq, D] and bounds [P, Hkv, 2 D]")
+    if q.dim() != 3:
+        raise ValueError("q must be [T, Hq, D]")
     t, heads, dim = q.shape
-    pages, heads_kv = bounds.shape[:2]
-    dtype = _check_heads(q, heads_kv, dim, page_size)
-    _check_bounds(bounds, bound_scales, None, dim)
+    pages, heads_kv = _check_bounds(bounds, bound_scales, dim)
+    dtype = _check_heads(q.dtype, heads, heads_kv, dim, page_size)
     _check_tokens(t, positions, seq_ids, page_table)
     if not 1 <= count <= MAX_COUNT:
         raise ValueError(f"count must be in [1, {MAX_COUNT}], got {count}")
     if sink < 0 or recent < 1 or sink + recent > count:
         raise ValueError(f"sink >= 0 and recent >= 1 must fit in count, got {sink}, {recent}")
-    dev = nat.require_device(q, bounds, bound_scales, positions, seq_ids, page_table)
-    q, *q_at = _rows(q)
-    out = torch.empty((t, heads_kv, count), dtype=torch.int32, device=dev)
+    dev = _device(q, bounds, bound_scales, positions, seq_ids, page_table)
+    q, q_token, q_head = _rows(q)
+    out = positions.new_empty((t, heads_kv, count))
     lib = nat.lib()
     b, max_pages = page_table.shape
     with _on(dev):
-        ws = nat.workspace(lib.rt_kv_select_workspace(t, heads_kv, max_pages), dev)
+        need = lib.rt_kv_select_workspace(t, heads_kv, max_pages)
+        ws = bounds.new_empty((need,))
         st = lib.rt_kv_select(
-            q.data_ptr(), *q_at, t, heads, heads_kv, dim, dtype,
-            bounds.data_ptr(), bound_scales.data_ptr(), pages, page_size, positions.data_ptr(),
-            seq_ids.data_ptr(), page_table.data_ptr(), b, max_pages, count, sink, recent,
-            out.data_ptr(), ws.data_ptr(), ws.numel(), nat.stream(dev))
-    nat.check(st)
+            q.data_ptr(), q_token, q_head, t, heads, heads_kv, dim, dtype, bounds.data_ptr(),
+            bound_scales.data_ptr(), pages, page_size, positions.data_ptr(), seq_ids.data_ptr(),
+            page_table.data_ptr(), b, max_pages, count, sink, recent, out.data_ptr(),
+            ws.data_ptr(), need, _stream(dev))
+    if st:
+        nat.check(st)
     return out
 
 
@@ -217,40 +240,40 @@ def select_blocks(q: Tensor, bounds: Tensor, bound_scales: Tensor, positions: Te
     ``c`` the rotated query's int8 codes) times the query's and the block's scales: an upper bound on
     what the block's keys can score, up to the codes' rounding. Blocks between without a page are left
     out; padding tokens get -1 throughout."""
-    return _ops_select(q, bounds, bound_scales, positions, seq_ids, page_table, page_size, count,
-                       sink, recent)
+    call = _select if _eager(q) else torch.ops.retrieve_kv.select_blocks
+    return call(q, bounds, bound_scales, positions, seq_ids, page_table, page_size, count, sink,
+                recent)
 
 
 # --- attention ----------------------------------------------------------------------------------
 
 
 def _attention(q, k_cache, v_cache, blocks, positions, seq_ids, page_table, scale=None):
-    dtype = _check_caches(q, k_cache, v_cache)
-    pages, heads_kv, page, dim = k_cache.shape
-    t, heads = q.shape[:2]
+    t, heads, pages, heads_kv, page, dim, dtype = _check_caches(q, k_cache, v_cache)
     _check_tokens(t, positions, seq_ids, page_table)
     if blocks.dim() != 3 or blocks.shape[:2] != (t, heads_kv):
         raise ValueError(f"blocks must be [{t}, {heads_kv}, count]")
-    if blocks.dtype != torch.int32:
+    if blocks.dtype is not torch.int32:
         raise TypeError("blocks must be int32")
     if not blocks.is_contiguous():
         raise ValueError("blocks must be contiguous")
-    dev = nat.require_device(q, k_cache, v_cache, blocks, positions, seq_ids, page_table)
-    q, *q_at = _rows(q)
+    dev = _device(q, k_cache, v_cache, blocks, positions, seq_ids, page_table)
+    q, q_token, q_head = _rows(q)
     count = blocks.shape[2]
-    out = torch.empty((t, heads, dim), dtype=q.dtype, device=dev)
-    lse = torch.empty((t, heads), dtype=torch.float32, device=dev)
+    out = q.new_empty((t, heads, dim))
+    lse = q.new_empty((t, heads), dtype=torch.float32)
     lib = nat.lib()
     with _on(dev):
         need = lib.rt_kv_attention_workspace(t, heads, heads_kv, dim, page, count)
         ws = nat.workspace(need, dev) if need else None
         st = lib.rt_kv_attention(
-            q.data_ptr(), *q_at, t, heads, heads_kv, dim, dtype,
-            k_cache.data_ptr(), v_cache.data_ptr(), pages, page, blocks.data_ptr(), count,
-            positions.data_ptr(), seq_ids.data_ptr(), page_table.data_ptr(), *page_table.shape,
+            q.data_ptr(), q_token, q_head, t, heads, heads_kv, dim, dtype, k_cache.data_ptr(),
+            v_cache.data_ptr(), pages, page, blocks.data_ptr(), count, positions.data_ptr(),
+            seq_ids.data_ptr(), page_table.data_ptr(), *page_table.shape,
             1.0 / math.sqrt(dim) if scale is None else scale, out.data_ptr(), lse.data_ptr(),
-            nat.ptr(ws), need, nat.stream(dev))
-    nat.check(st)
+            nat.ptr(ws), need, _stream(dev))
+    if st:
+        nat.check(st)
     return out, lse
 
 
@@ -263,15 +286,13 @@ def block_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, blocks: Tensor,
     the natural logarithm of the weights' sum. Entries below 0, past the token's block or without a
     page are skipped; a row without a key is zeros and ``-inf``. Slots past a token's position are not
     used, whatever they hold."""
-    return _ops_attention(q, k_cache, v_cache, blocks, positions, seq_ids, page_table, scale)
+    call = _attention if _eager(q) else torch.ops.retrieve_kv.block_attention
+    return call(q, k_cache, v_cache, blocks, positions, seq_ids, page_table, scale)
 
 
 _lib.impl("append", _append, "CUDA")
 _lib.impl("select_blocks", _select, "CUDA")
 _lib.impl("block_attention", _attention, "CUDA")
-_ops_append = torch.ops.retrieve_kv.append.default
-_ops_select = torch.ops.retrieve_kv.select_blocks.default
-_ops_attention = torch.ops.retrieve_kv.block_attention.default
 
 
 @torch.library.register_fake("retrieve_kv::append", lib=_lib)
