@@ -41,6 +41,7 @@ struct AttendArgs {
   KvTokens tok;
   float scale;      // times log2 e
   int32_t parts;    // workgroups that share a row
+  int32_t joined;   // tokens a wave takes together
   void* out;        // [T, Hq, D]
   float* lse;       // [T, Hq]
   float* part_out;  // [rows, parts, 16, D], sums of weights times values
@@ -138,8 +139,8 @@ struct TileList {
   }
 };
 
-// One wave's pass over its tiles: the accumulators (channel 16 i + 4 (lane / 16) + r of head
-// lane % 16), the maximum and this lane's share of the sum.
+// A wave's accumulators (channel 16 i + 4 (lane / 16) + r of column lane % 16), the columns' maxima
+// and this lane's share of their sums; its queries and the step in flight.
 template <class E, int D>
 struct AttendWave {
   using Op = AttendOp<E>;
@@ -147,14 +148,127 @@ struct AttendWave {
   static constexpr int KS = D / 32, DT = D / 16, VL = D / 16;  // VL: 16-byte loads of V a lane
   v4f acc[DT];
   float m, l;
+  V8 qf[KS], kf[2][KS], vf[VL];
 
-  __device__ void run(const AttendArgs& a, int64_t t, int head, int tile, int part, int parts,
-                      char* lds) {
-    const int lane = lane_id(), col = lane & 15, grp = lane >> 4;
+  __device__ void clear() {
 #pragma unroll
     for (int i = 0; i < DT; ++i) acc[i] = v4f{0.f, 0.f, 0.f, 0.f};
     m = -3.402823466e38f;
     l = 0.0f;
+  }
+  // This lane's column is query head `head` of token t (zeros where it is not `real`).
+  __device__ void load_q(const AttendArgs& a, int64_t t, int64_t head, bool real) {
+    const E* q = static_cast<const E*>(a.q) + (real ? t * a.q_st + head * a.q_sh : 0) +
+                 8 * (lane_id() >> 4);
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const V8 x = *reinterpret_cast<const V8*>(q + 32 * s);
+      qf[s] = real ? x : V8{};
+    }
+  }
+  __device__ void load_k(const AttendArgs& a, const Tiles& s) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const E* base = static_cast<const E*>(a.k_cache) + s.row[j] * D;
+#pragma unroll
+      for (int i = 0; i < KS; ++i) {
+        kf[j][i] = *reinterpret_cast<const V8*>(
+            base + ((lane_id() & 15) * D + 8 * (lane_id() >> 4) + 32 * i));
+      }
+    }
+  }
+  __device__ void load_v(const AttendArgs& a, const Tiles& s) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const E* base = static_cast<const E*>(a.v_cache) + s.row[j] * D;
+#pragma unroll
+      for (int i = 0; i < VL / 2; ++i) {
+        vf[j * (VL / 2) + i] = *reinterpret_cast<const V8*>(base + (i * 64 + lane_id()) * 8);
+      }
+    }
+  }
+  // One step on what load_k and load_v brought; `fetch_k` and `fetch_v` start the next one's loads as
+  // soon as the registers are free. A column's keys count up to n[j] in tile j; V's rows from
+  // rows[j] on are read as zeros (slots that may never have been written).
+  template <class FK, class FV>
+  __device__ void step(const AttendArgs& a, char* lds, bool whole, const int (&n)[2],
+                       const int (&rows)[2], FK&& fetch_k, FV&& fetch_v) {
+    const int lane = lane_id(), col = lane & 15, grp = lane >> 4;
+    v4f sc[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      sc[j] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < KS; ++i) sc[j] = Op::mma(kf[j][i], qf[i], sc[j]);
+    }
+    fetch_k();
+    if (rows[0] < 16 || rows[1] < 16) {
+#pragma unroll
+      for (int i = 0; i < VL; ++i) {
+        const int row = ((i % (VL / 2)) * 64 + lane) / (D / 8);
+        if (row >= rows[i / (VL / 2)]) vf[i] = V8{};
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < VL; ++i) {
+      const int at = i * 64 + lane, row = at / (D / 8), c = at % (D / 8);
+      *reinterpret_cast<V8*>(lds + row * (D * 2) + (((c >> 1) ^ granule_swizzle<D>(row)) << 5) +
+                             (c & 1) * 16) = vf[i];
+    }
+    fetch_v();
+    float w[8];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float y = sc[j][r] * a.scale;
+        w[4 * j + r] = whole || 4 * grp + r < n[j] ? y : -INFINITY;
+      }
+    }
+    float top = w[0];
+#pragma unroll
+    for (int r = 1; r < 8; ++r) top = fmaxf(top, w[r]);
+    if (__any(top > m + 8.0f)) {
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float next = fmaxf(m, top);
+      const float keep = __builtin_amdgcn_exp2f(m - next);
+      m = next;
+      l *= keep;
+#pragma unroll
+      for (int i = 0; i < DT; ++i) acc[i] *= keep;
+    }
+    V8 p;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      const float e = __builtin_amdgcn_exp2f(w[r] - m);
+      l += e;
+      p[r] = static_cast<E>(e);
+    }
+    asm volatile("" ::: "memory");  // (the staged rows are read by other lanes of this wave)
+#pragma unroll
+    for (int i = 0; i < DT; ++i) {
+      typename Op::V4 x[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int row = 16 * j + 4 * grp + (col >> 2);
+        x[j] = Op::read_tr(lds + row * (D * 2) + ((i ^ granule_swizzle<D>(row)) << 5) +
+                           (col & 3) * 8);
+      }
+      const V8 v = {x[0][0], x[0][1], x[0][2], x[0][3], x[1][0], x[1][1], x[1][2], x[1][3]};
+      acc[i] = Op::mma(v, p, acc[i]);
+    }
+    asm volatile("" ::: "memory");
+  }
+  __device__ void join_sums() {
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+  }
+
+  // One token's heads (tile `tile` of the group) over part of its list.
+  __device__ void run(const AttendArgs& a, int64_t t, int head, int tile, int part, int parts,
+                      char* lds) {
+    clear();
     TileList tiles;
     tiles.place = kv_place(a.tok, t);
     if (tiles.place.last < 0) return;
@@ -164,117 +278,21 @@ struct AttendWave {
     tiles.parts = parts;
     tiles.chunk = -1;
     tiles.left = 0;
-
-    V8 qf[KS];
-    const bool real = tile * 16 + col < a.G;
-    const E* q = static_cast<const E*>(a.q) + t * a.q_st +
-                 static_cast<int64_t>(head * a.G + (real ? tile * 16 + col : 0)) * a.q_sh + grp * 8;
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const V8 x = *reinterpret_cast<const V8*>(q + 32 * s);
-      qf[s] = real ? x : V8{};
-    }
-
-    V8 kf[2][KS], vf[VL];
-    auto load_k = [&](const Tiles& s) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const E* base = static_cast<const E*>(a.k_cache) + s.row[j] * D;
-#pragma unroll
-        for (int i = 0; i < KS; ++i) {
-          kf[j][i] = *reinterpret_cast<const V8*>(base + (col * D + grp * 8 + 32 * i));
-        }
-      }
-    };
-    auto load_v = [&](const Tiles& s) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const E* base = static_cast<const E*>(a.v_cache) + s.row[j] * D;
-#pragma unroll
-        for (int i = 0; i < VL / 2; ++i) {
-          vf[j * (VL / 2) + i] = *reinterpret_cast<const V8*>(base + (i * 64 + lane) * 8);
-        }
-      }
-    };
-
+    const int g = tile * 16 + (lane_id() & 15);
+    load_q(a, t, head * a.G + g, g < a.G);
     Tiles now, then;
     bool more = tiles.next(a, then);
     if (more) {
-      load_k(then);
-      load_v(then);
+      load_k(a, then);
+      load_v(a, then);
     }
     while (more) {
       now = then;
       more = tiles.next(a, then);
-      v4f sc[2];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        sc[j] = v4f{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < KS; ++i) sc[j] = Op::mma(kf[j][i], qf[i], sc[j]);
-      }
-      if (more) load_k(then);
-      const bool whole = now.n[0] == 16 && now.n[1] == 16;
-      if (!whole) {
-#pragma unroll
-        for (int i = 0; i < VL; ++i) {
-          const int row = ((i % (VL / 2)) * 64 + lane) / (D / 8);
-          if (row >= now.n[i / (VL / 2)]) vf[i] = V8{};
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < VL; ++i) {
-        const int at = i * 64 + lane, row = at / (D / 8), c = at % (D / 8);
-        *reinterpret_cast<V8*>(lds + row * (D * 2) + (((c >> 1) ^ granule_swizzle<D>(row)) << 5) +
-                               (c & 1) * 16) = vf[i];
-      }
-      if (more) load_v(then);
-      float w[8];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float y = sc[j][r] * a.scale;
-          w[4 * j + r] = whole || 4 * grp + r < now.n[j] ? y : -INFINITY;
-        }
-      }
-      float top = w[0];
-#pragma unroll
-      for (int r = 1; r < 8; ++r) top = fmaxf(top, w[r]);
-      if (__any(top > m + 8.0f)) {
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        const float next = fmaxf(m, top);
-        const float keep = __builtin_amdgcn_exp2f(m - next);
-        m = next;
-        l *= keep;
-#pragma unroll
-        for (int i = 0; i < DT; ++i) acc[i] *= keep;
-      }
-      V8 p;
-#pragma unroll
-      for (int r = 0; r < 8; ++r) {
-        const float e = __builtin_amdgcn_exp2f(w[r] - m);
-        l += e;
-        p[r] = static_cast<E>(e);
-      }
-      asm volatile("" ::: "memory");  // (the staged rows are read by other lanes of this wave)
-#pragma unroll
-      for (int i = 0; i < DT; ++i) {
-        typename Op::V4 x[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int row = 16 * j + 4 * grp + (col >> 2);
-          x[j] = Op::read_tr(lds + row * (D * 2) + ((i ^ granule_swizzle<D>(row)) << 5) +
-                             (col & 3) * 8);
-        }
-        const V8 v = {x[0][0], x[0][1], x[0][2], x[0][3], x[1][0], x[1][1], x[1][2], x[1][3]};
-        acc[i] = Op::mma(v, p, acc[i]);
-      }
-      asm volatile("" ::: "memory");
+      step(a, lds, now.n[0] == 16 && now.n[1] == 16, now.n, now.n,
+           [&] { if (more) load_k(a, then); }, [&] { if (more) load_v(a, then); });
     }
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
+    join_sums();
   }
 };
 
@@ -284,23 +302,12 @@ __device__ inline float log_sum(float m, float l) {
   return l == 0.0f ? -INFINITY : (m + __log2f(l)) * kLn2;
 }
 
-// Many rows: a wave a row, four neighbouring tokens of one head a workgroup (they mostly choose the
-// same blocks).
+// This lane's column, query head `head` of token t, to the outputs.
 template <class E, int D>
-__global__ void __launch_bounds__(kAttendWaves* kWave, D <= 128 ? 2 : 1)
-    kv_attend_rows_kernel(AttendArgs a) {
+__device__ inline void emit(const AttendArgs& a, const AttendWave<E, D>& w, int64_t t, int head) {
   typedef E V4 __attribute__((ext_vector_type(4)));
-  __shared__ __attribute__((aligned(16))) char lds[kAttendWaves][64 * D];
-  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
-  const int heads = a.Hkv * a.tiles;
-  const int64_t t = static_cast<int64_t>(blockIdx.x / heads) * kAttendWaves + wave;
-  if (t >= a.T) return;
-  const int head = blockIdx.x % heads / a.tiles, tile = blockIdx.x % heads % a.tiles;
-  AttendWave<E, D> w;
-  w.run(a, t, head, tile, 0, 1, lds[wave]);
-  const int col = lane_id() & 15, grp = lane_id() >> 4, g = tile * 16 + col;
-  if (g >= a.G) return;
-  const int64_t row = t * a.Hq + head * a.G + g;
+  const int grp = lane_id() >> 4;
+  const int64_t row = t * a.Hq + head;
   const float inv = inverse_sum(w.l);
   E* out = static_cast<E*>(a.out) + row * D + 4 * grp;
 #pragma unroll
@@ -311,6 +318,191 @@ __global__ void __launch_bounds__(kAttendWaves* kWave, D <= 128 ? 2 : 1)
     *reinterpret_cast<V4*>(out + 16 * i) = x;
   }
   if (grp == 0) a.lse[row] = log_sum(w.m, w.l);
+}
+
+// Many rows: a wave a row, four neighbouring tokens of one head a workgroup (they mostly choose the
+// same blocks).
+template <class E, int D>
+__global__ void __launch_bounds__(kAttendWaves* kWave, D <= 128 ? 2 : 1)
+    kv_attend_rows_kernel(AttendArgs a) {
+  __shared__ __attribute__((aligned(16))) char lds[kAttendWaves][64 * D];
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int heads = a.Hkv * a.tiles;
+  const int64_t t = static_cast<int64_t>(blockIdx.x / heads) * kAttendWaves + wave;
+  if (t >= a.T) return;
+  const int head = blockIdx.x % heads / a.tiles, tile = blockIdx.x % heads % a.tiles;
+  AttendWave<E, D> w;
+  w.run(a, t, head, tile, 0, 1, lds[wave]);
+  const int g = tile * 16 + (lane_id() & 15);
+  if (g < a.G) emit(a, w, t, head * a.G + g);
+}
+
+// Many tokens whose group has 8 heads or fewer: a wave holds the heads of several neighbouring
+// tokens (16 / G of them: columns that one token would leave empty) and passes once over all the
+// blocks that any of them lists, each column counting its own. Neighbours mostly choose alike, so
+// a block is read and multiplied once for them; where they choose nothing alike the steps are as
+// many as one token a wave takes.
+//
+// The lists are joined by physical page in a hash table: of a page's entries the first (by token,
+// then place) stands for all and holds the tokens' bits, so the order of the blocks depends
+// on the lists alone. A weight of 0 meets every other column's values: where those are not
+// finite the sums are not either, and the wave's tokens are done again one by one.
+constexpr int kJoinMost = 256;  // entries of a wave's lists
+
+template <int D>
+struct JoinLds {
+  static constexpr int kTable = 2 * kJoinMost;
+  union {
+    char stage[64 * D];
+    struct {
+      int32_t page[kTable];
+      uint32_t tokens[kTable];
+      uint32_t first[kTable];
+    };
+  };
+  int2 list[kJoinMost];  // page, tokens
+};
+
+template <class E, int D>
+__global__ void __launch_bounds__(kAttendWaves* kWave, D <= 128 ? 2 : 1)
+    kv_attend_joined_kernel(AttendArgs a) {
+  __shared__ __attribute__((aligned(16))) JoinLds<D> lds_all[kAttendWaves];
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int lane = lane_id(), col = lane & 15;
+  JoinLds<D>& lds = lds_all[wave];
+  const int64_t t0 = (static_cast<int64_t>(blockIdx.x / a.Hkv) * kAttendWaves + wave) * a.joined;
+  if (t0 >= a.T) return;
+  const int head = blockIdx.x % a.Hkv;
+  const int tokens = a.T - t0 < a.joined ? static_cast<int>(a.T - t0) : a.joined;
+
+  // the union of the lists
+  constexpr int kTable = JoinLds<D>::kTable;
+  for (int i = lane; i < kTable; i += kWave) {
+    lds.page[i] = -1;
+    lds.tokens[i] = 0u;
+    lds.first[i] = ~0u;
+  }
+  asm volatile("" ::: "memory");
+  const int entries = tokens * a.count;
+  int32_t page[kJoinMost / kWave];
+  int slot[kJoinMost / kWave];
+#pragma unroll
+  for (int r = 0; r < kJoinMost / kWave; ++r) {
+    const int e = r * kWave + lane;
+    page[r] = -1;
+    slot[r] = 0;
+    if (e >= entries) continue;
+    const int tok = e / a.count;
+    const KvPlace p = kv_place(a.tok, t0 + tok);
+    const int32_t block = a.blocks[((t0 + tok) * a.Hkv + head) * a.count + e % a.count];
+    if (block < 0 || block > p.last) continue;
+    page[r] = kv_page(a.tok, p, block);
+    if (page[r] < 0) continue;
+    int s = static_cast<int>((static_cast<uint32_t>(page[r]) * 0x9E3779B1u) >> 16) & (kTable - 1);
+    for (;;) {  // (at most half full: a free place or the page's own is met)
+      const int32_t old = atomicCAS(&lds.page[s], -1, page[r]);
+      if (old == -1 || old == page[r]) break;
+      s = (s + 1) & (kTable - 1);
+    }
+    slot[r] = s;
+    atomicOr(&lds.tokens[s], 1u << tok);
+    atomicMin(&lds.first[s], static_cast<uint32_t>(e));
+  }
+  asm volatile("" ::: "memory");
+  int listed = 0;
+#pragma unroll
+  for (int r = 0; r < kJoinMost / kWave; ++r) {
+    const bool first = page[r] >= 0 && lds.first[slot[r]] == static_cast<uint32_t>(r * kWave + lane);
+    const uint64_t m = __ballot(first);
+    if (first) {
+      lds.list[listed + __popcll(m & ((uint64_t{1} << lane) - 1))] =
+          int2{page[r], static_cast<int>(lds.tokens[slot[r]])};
+    }
+    listed += __popcll(m);
+  }
+  asm volatile("" ::: "memory");
+
+  // this lane's column: its token's own page ends after `own_keys`
+  const int tok = col / a.G;
+  const bool real = tok < tokens;
+  const int64_t t = t0 + (real ? tok : 0);
+  const int hq = head * a.G + col % a.G;
+  const int size = 1 << a.tok.shift;
+  int32_t own = -1, own_keys = 0;
+  if (real) {
+    const KvPlace p = kv_place(a.tok, t);
+    if (p.last >= 0) own = kv_page(a.tok, p, p.last);
+    own_keys = (p.pos & (size - 1)) + 1;
+  }
+  AttendWave<E, D> w;
+  w.clear();
+  w.load_q(a, t, hq, real);
+
+  const int total = listed << (a.tok.shift - 4);  // tiles of 16 keys
+  int at = 0;
+  auto next = [&](Tiles& s) {  // (s.n: this column's; one without a token counts all keys)
+    for (; at < total; at += 2) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int i = at + j < total ? (at + j) >> (a.tok.shift - 4) : 0;
+        const int32_t pg = __builtin_amdgcn_readfirstlane(lds.list[i].x);
+        const uint32_t who =
+            at + j < total ? __builtin_amdgcn_readfirstlane(lds.list[i].y) : 0u;
+        const int first = ((at + j) << 4) & (size - 1);
+        s.row[j] = ((static_cast<int64_t>(pg) * a.Hkv + head) << a.tok.shift) + first;
+        const int end = (who >> tok) & 1u ? (pg == own ? own_keys : size) : 0;
+        const int n = end - first;
+        s.n[j] = !real ? 16 : n < 0 ? 0 : n > 16 ? 16 : n;
+      }
+      if (__any(real && (s.n[0] > 0 || s.n[1] > 0))) {
+        at += 2;
+        return true;
+      }
+    }
+    return false;
+  };
+  Tiles now, then;
+  bool more = next(then);
+  if (more) {
+    w.load_k(a, then);
+    w.load_v(a, then);
+  }
+  while (more) {
+    now = then;
+    more = next(then);
+    const bool whole = __all(now.n[0] == 16 && now.n[1] == 16);
+    int rows[2];  // slots that some column counts have been written
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      rows[j] = 16;
+      if (!whole && !__any(real && now.n[j] == 16)) {
+        int n = real ? now.n[j] : 0;
+#pragma unroll
+        for (int x = 1; x < 16; x <<= 1) {
+          const int o = __shfl_xor(n, x);
+          n = o > n ? o : n;
+        }
+        rows[j] = __builtin_amdgcn_readfirstlane(n);
+      }
+    }
+    w.step(a, lds.stage, whole, now.n, rows, [&] { if (more) w.load_k(a, then); },
+           [&] { if (more) w.load_v(a, then); });
+  }
+  w.join_sums();
+  float odd = 0.0f;  // 0 times every sum: not a number where one is not finite
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) odd = fmaf(w.acc[i][r], 0.0f, odd);
+  }
+  if (!__any(real && !(odd == 0.0f))) {
+    if (real) emit(a, w, t, hq);
+    return;
+  }
+  for (int i = 0; i < tokens; ++i) {
+    w.run(a, t0 + i, head, 0, 0, 1, lds.stage);
+    if (col < a.G) emit(a, w, t0 + i, head * a.G + col);
+  }
 }
 
 // Few rows: the workgroup's waves (and `parts` workgroups) share a row's list; their sums are joined
@@ -401,17 +593,20 @@ __global__ void __launch_bounds__(D / 4) kv_join_kernel(AttendArgs a) {
   if (threadIdx.x == 0) a.lse[r] = log_sum(m, l);
 }
 
-// How a call is spread. 0 parts: a wave a row.
+// How a call is spread: `parts` workgroups a row; 0: a wave a row, or `joined` tokens a wave.
 struct AttendPlan {
   int64_t rows;
-  int32_t tiles, parts;
+  int32_t tiles, parts, joined;
 };
 
 inline AttendPlan attend_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t page, int64_t count) {
   AttendPlan p;
-  p.tiles = static_cast<int32_t>(cdiv(Hq / Hkv, 16));
+  const int64_t G = Hq / Hkv;
+  p.tiles = static_cast<int32_t>(cdiv(G, 16));
   p.rows = T * Hkv * p.tiles;
   p.parts = 0;
+  const int64_t cols = 16 / (G < 16 ? G : 16), lists = kJoinMost / (count > 0 ? count : 1);
+  p.joined = static_cast<int32_t>(cols < lists ? cols : lists);
   if (p.rows >= 4096) return p;
   // workgroups of four waves for two on every CU, each wave with a unit of 64 keys at least
   const int64_t most = cdiv(count * page, 64 * kAttendWaves);
@@ -466,6 +661,7 @@ extern "C" int rt_kv_attention(const void* q, int64_t q_token_stride, int64_t q_
   a.tok = {positions, seq_ids, page_table, static_cast<int32_t>(B),
            static_cast<int32_t>(max_pages), static_cast<int32_t>(P), kv_shift(page)};
   a.scale = scale * kLog2e, a.out = out, a.lse = lse, a.parts = plan.parts;
+  a.joined = plan.joined;
   a.part_out = static_cast<float*>(workspace);
   a.part_ml = a.part_out + (plan.parts > 1 ? plan.rows * plan.parts * 16 * D : 0);
   const hipStream_t s = static_cast<hipStream_t>(stream);
@@ -473,7 +669,10 @@ extern "C" int rt_kv_attention(const void* q, int64_t q_token_stride, int64_t q_
     using E = decltype(e);
     constexpr int DD = decltype(d)::value;
     const dim3 threads(kAttendWaves * kWave);
-    if (plan.parts == 0) {
+    if (plan.parts == 0 && plan.joined > 1) {
+      const int64_t grid = cdiv(T, kAttendWaves * plan.joined) * Hkv;
+      kv_attend_joined_kernel<E, DD><<<dim3(static_cast<unsigned>(grid)), threads, 0, s>>>(a);
+    } else if (plan.parts == 0) {
       const int64_t grid = cdiv(T, kAttendWaves) * Hkv * plan.tiles;
       kv_attend_rows_kernel<E, DD><<<dim3(static_cast<unsigned>(grid)), threads, 0, s>>>(a);
     } else {

@@ -101,11 +101,74 @@ def test_few_rows_many_blocks(dev, tokens, count):
     _check(_run(dev, "bf16", *case), "bf16", *case)
 
 
+MANY = [("bf16", 1, 1, 64, 16, 9), ("fp16", 2, 1, 128, 64, 5), ("bf16", 3, 1, 96, 32, 16),
+        ("fp16", 4, 1, 128, 16, 7), ("bf16", 7, 1, 64, 128, 4), ("fp16", 8, 1, 192, 64, 6),
+        ("bf16", 12, 1, 128, 32, 5), ("fp16", 20, 1, 64, 64, 4), ("bf16", 4, 1, 256, 64, 70),
+        ("fp16", 4, 1, 64, 16, 300), ("bf16", 8, 2, 128, 64, 16)]
+
+
+def _many(seed, kind, heads, heads_kv, d, page, count):
+    """More rows than the GPU holds waves (a wave then takes a row, or several tokens at once), of three
+    sequences; neighbours choose alike in the first and last, by chance in the second."""
+    had_new = [(3 * page + 5, 2000), (0, 2300 // heads_kv), (40, 7)]
+    case = list(_case(seed, kind, heads, heads_kv, d, page, had_new, count, sparse=0.1))
+    blocks, pos = case[3], case[4]
+    for t in range(1, 2000):
+        if t % 37:
+            blocks[t] = blocks[t - 1]
+            blocks[t, :, t % count] = pos[t] // page if t % 5 == 0 else blocks[t, :, t % count]
+    own = np.sort(blocks, -1)  # (each block once a row)
+    for t, h in np.argwhere((own[:, :, 1:] == own[:, :, :-1]).any(-1)):
+        row = blocks[t, h]
+        _, first = np.unique(row, return_index=True)
+        row[np.setdiff1d(np.arange(count), first)] = -1
+    return case
+
+
+def _some(got, case, pick):
+    q, kc, vc, blocks, pos, seq, tab = case
+    return (got[0][pick], got[1][pick]), (q[pick], kc, vc, blocks[pick], pos[pick], seq[pick], tab)
+
+
 @pytest.mark.gpu
-def test_many_rows(dev):
-    """More rows than the GPU holds at a time."""
-    case = _case(5, "fp16", 4, 2, 64, 16, [(40, 700), (3, 500)], 3)
-    _check(_run(dev, "fp16", *case), "fp16", *case)
+@pytest.mark.parametrize("kind,heads,heads_kv,d,page,count", MANY)
+def test_many_rows(dev, kind, heads, heads_kv, d, page, count):
+    case = _many(heads + count, kind, heads, heads_kv, d, page, count)
+    got = _run(dev, kind, *case)
+    tokens = len(case[4])
+    assert tokens * heads_kv >= 4096
+    pick = np.r_[0:9, 31:45, 1990:2012, rng(5).integers(0, tokens, 60), tokens - 9:tokens]
+    got, case = _some(got, case, pick)
+    _check(got, kind, *case)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads", [1, 4, 8, 16])
+def test_many_rows_and_values_that_are_not_finite(dev, heads):
+    """Neighbours that choose different blocks: a NaN key or an infinite value reaches the tokens whose
+    lists hold it, and no other; slots past every token's are NaN; padding among the tokens."""
+    page, tokens = 16, 4200
+    q, kc, vc, blocks, pos, seq, tab = _case(71, "bf16", heads, 1, 64, page, [(16 * 7 + 3, 1)], 4)
+    q = normal16(72, (tokens, heads, 64), "bf16")
+    pos, seq = np.full(tokens, 16 * 7 + 3, np.int32), np.zeros(tokens, np.int32)
+    odd = np.arange(tokens) % 2 == 1
+    blocks = np.where(odd[:, None, None], [[[6, 5, -1, 7]]], [[[0, 1, 2, 7]]]).astype(np.int32)
+    pos[::50], blocks[::70] = -1, -1
+    kc[tab[0, 7], 0, 4:], vc[tab[0, 7], 0, 4:] = np.nan, np.nan
+    clean = _run(dev, "bf16", q, kc, vc, blocks, pos, seq, tab)
+    kc0, vc0 = np.nan_to_num(kc), np.nan_to_num(vc)
+    pick = np.r_[0:80, 4100:4200]
+    got, case = _some(clean, (q, kc0, vc0, blocks, pos, seq, tab), pick)
+    _check(got, "bf16", *case)
+    kc[tab[0, 1], 0, 3, 5], vc[tab[0, 6], 0, 2, 9] = np.nan, np.inf
+    out, lse = _run(dev, "bf16", q, kc, vc, blocks, pos, seq, tab)
+    full = (pos >= 0) & (blocks[:, 0, 0] >= 0)
+    assert np.isnan(out[full & ~odd]).all() and np.isnan(lse[full & ~odd]).all()
+    assert np.isposinf(out[full & odd][:, :, 9]).all()
+    out[full & odd, :, 9] = clean[0][full & odd, :, 9]
+    rest = pick[(odd | ~full)[pick]]
+    got, case = _some((out, lse), (q, kc0, vc0, blocks, pos, seq, tab), rest)
+    _check(got, "bf16", *case)
 
 
 @pytest.mark.gpu
@@ -144,10 +207,10 @@ def test_slots_past_the_token_hold_anything(dev, page, what):
         vc[row[p // page], :, p % page + 1:] = what
     got = _run(dev, "bf16", q, kc, vc, blocks, pos, seq, tab)
     _check(got, "bf16", q, *clean, blocks, pos, seq, tab)
-    prompt = np.repeat(q, 300, 0), np.repeat(blocks, 300, 0), np.repeat(pos, 300), np.repeat(seq, 300)
-    many = _run(dev, "bf16", prompt[0], kc, vc, prompt[1], prompt[2], prompt[3], tab)
-    _check((many[0][::300], many[1][::300]), "bf16", q, *clean, blocks, pos, seq, tab)
-    assert np.array_equal(many[0].reshape(5, 300, -1), np.repeat(many[0][::300].reshape(5, 1, -1), 300, 1))
+    q, blocks, pos, seq = (np.repeat(x, 500, 0) for x in (q, blocks, pos, seq))
+    many = _run(dev, "bf16", q, kc, vc, blocks, pos, seq, tab)
+    got, case = _some(many, (q, *clean, blocks, pos, seq, tab), np.r_[0:2500:250, 498:503, 2499])
+    _check(got, "bf16", *case)
 
 
 @pytest.mark.gpu
@@ -236,8 +299,9 @@ def test_strided_queries(dev):
 @pytest.mark.gpu
 def test_the_same_bits_every_time(dev):
     """No order that changes from call to call: few rows (split and joined) and many."""
-    for had_new, count in (([(9000, 1)], 200), ([(300, 400)], 6)):
-        case = _case(47, "bf16", 8, 2, 64, 16, had_new, count)
+    for case in (_case(47, "bf16", 8, 2, 64, 16, [(9000, 1)], 200),
+                 _case(47, "bf16", 8, 2, 64, 16, [(300, 400)], 6),
+                 _many(48, "bf16", 4, 1, 64, 16, 9)):
         first = _run(dev, "bf16", *case)
         for _ in range(3):
             again = _run(dev, "bf16", *case)
