@@ -24,6 +24,7 @@
 
 #include "../../include/retrieve_amd.h"
 #include "kv_common.h"
+#include "lds_load.h"
 
 namespace rt {
 
@@ -193,7 +194,7 @@ struct AttendWave {
   template <class FK, class FV>
   __device__ void step(const AttendArgs& a, char* lds, bool whole, const int (&n)[2],
                        const int (&rows)[2], FK&& fetch_k, FV&& fetch_v) {
-    const int lane = lane_id(), col = lane & 15, grp = lane >> 4;
+    const int lane = lane_id();
     v4f sc[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -216,12 +217,21 @@ struct AttendWave {
                              (c & 1) * 16) = vf[i];
     }
     fetch_v();
+    const V8 p = weigh(a.scale, sc, whole, n);
+    asm volatile("" ::: "memory");  // (the staged rows are read by other lanes of this wave)
+    add(lds, p);
+    asm volatile("" ::: "memory");
+  }
+  // The weights of a step's scores, rounded for the second product (keys 4 (lane / 16) + r of tile
+  // j at 4 j + r), the maximum raised and the sum extended.
+  __device__ V8 weigh(float scale, const v4f (&sc)[2], bool whole, const int (&n)[2]) {
+    const int grp = lane_id() >> 4;
     float w[8];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float y = sc[j][r] * a.scale;
+        const float y = sc[j][r] * scale;
         w[4 * j + r] = whole || 4 * grp + r < n[j] ? y : -INFINITY;
       }
     }
@@ -245,7 +255,11 @@ struct AttendWave {
       l += e;
       p[r] = static_cast<E>(e);
     }
-    asm volatile("" ::: "memory");  // (the staged rows are read by other lanes of this wave)
+    return p;
+  }
+  // The second product: 32 staged rows of values, swizzled by granules.
+  __device__ void add(const char* lds, V8 p) {
+    const int col = lane_id() & 15, grp = lane_id() >> 4;
 #pragma unroll
     for (int i = 0; i < DT; ++i) {
       typename Op::V4 x[2];
@@ -258,7 +272,6 @@ struct AttendWave {
       const V8 v = {x[0][0], x[0][1], x[0][2], x[0][3], x[1][0], x[1][1], x[1][2], x[1][3]};
       acc[i] = Op::mma(v, p, acc[i]);
     }
-    asm volatile("" ::: "memory");
   }
   __device__ void join_sums() {
     l += __shfl_xor(l, 16);
@@ -337,158 +350,326 @@ __global__ void __launch_bounds__(kAttendWaves* kWave, D <= 128 ? 2 : 1)
   if (g < a.G) emit(a, w, t, head * a.G + g);
 }
 
+// One query head of one token by a wave, key by key (a lane scores one of 64, then sums its own
+// channels): only for rows beside values that are not finite, so it spares registers, not time.
+template <class E, int D>
+__device__ inline void attend_alone(const AttendArgs& a, int64_t t, int head, int hq, float* qs) {
+  using V8 = typename Kv<E>::V8;
+  constexpr int R = (D + kWave - 1) / kWave;
+  const int lane = lane_id();
+  const KvPlace p = kv_place(a.tok, t);
+  const E* q = static_cast<const E*>(a.q) + t * a.q_st + hq * a.q_sh;
+  for (int d = lane; d < D; d += kWave) qs[d] = static_cast<float>(q[d]) * a.scale;
+  asm volatile("" ::: "memory");
+  const int size = 1 << a.tok.shift;
+  float m = -3.402823466e38f, l = 0.0f, acc[R] = {};
+  for (int i = 0; i < a.count; ++i) {
+    const int32_t block = a.blocks[(t * a.Hkv + head) * a.count + i];
+    if (block < 0 || block > p.last) continue;
+    const int32_t page = kv_page(a.tok, p, block);
+    if (page < 0) continue;
+    const int64_t base = ((static_cast<int64_t>(page) * a.Hkv + head) << a.tok.shift) * D;
+    const int keys = block == p.last ? (p.pos & (size - 1)) + 1 : size;
+    for (int j0 = 0; j0 < keys; j0 += kWave) {
+      const int j = j0 + lane;
+      float x = -INFINITY;
+      if (j < keys) {
+        const E* k = static_cast<const E*>(a.k_cache) + base + j * D;
+        x = 0.0f;
+#pragma unroll 2
+        for (int d = 0; d < D; d += 8) {
+          const V8 kv = *reinterpret_cast<const V8*>(k + d);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x = fmaf(static_cast<float>(kv[e]), qs[d + e], x);
+        }
+      }
+      float top = x;
+      for (int s = 1; s < kWave; s <<= 1) top = fmaxf(top, __shfl_xor(top, s));
+      const float next = fmaxf(m, top), keep = __builtin_amdgcn_exp2f(m - next);
+      const float w = __builtin_amdgcn_exp2f(x - next);
+      float sum = w;
+      for (int s = 1; s < kWave; s <<= 1) sum += __shfl_xor(sum, s);
+      l = l * keep + sum;
+      m = next;
+#pragma unroll
+      for (int r = 0; r < R; ++r) acc[r] *= keep;
+      const int n = keys - j0 < kWave ? keys - j0 : kWave;
+      for (int jj = 0; jj < n; ++jj) {
+        const float wj = __shfl(w, jj);
+        const E* v = static_cast<const E*>(a.v_cache) + base + (j0 + jj) * D;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const int d = r * kWave + lane;
+          if (d < D) acc[r] = fmaf(wj, static_cast<float>(v[d]), acc[r]);
+        }
+      }
+    }
+  }
+  const float inv = inverse_sum(l);
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int d = r * kWave + lane;
+    if (d < D) static_cast<E*>(a.out)[(t * a.Hq + hq) * D + d] = static_cast<E>(acc[r] * inv);
+  }
+  if (lane == 0) a.lse[t * a.Hq + hq] = log_sum(m, l);
+  asm volatile("" ::: "memory");
+}
+
 // Many tokens whose group has 8 heads or fewer: a wave holds the heads of several neighbouring
-// tokens (16 / G of them: columns that one token would leave empty) and passes once over all the
-// blocks that any of them lists, each column counting its own. Neighbours mostly choose alike, so
-// a block is read and multiplied once for them; where they choose nothing alike the steps are as
-// many as one token a wave takes.
+// tokens (columns that one token would leave empty), a workgroup four such waves, and passes once
+// over all the blocks that any of their tokens lists, each column counting its own. Neighbours
+// mostly choose alike, so a block is read once for them; a wave sits out the blocks that none
+// of its tokens lists.
 //
 // The lists are joined by physical page in a hash table: of a page's entries the first (by token,
 // then place) stands for all and holds the tokens' bits, so the order of the blocks depends
-// on the lists alone. A weight of 0 meets every other column's values: where those are not
-// finite the sums are not either, and the wave's tokens are done again one by one.
-constexpr int kJoinMost = 256;  // entries of a wave's lists
+// on the lists alone. Keys and values go straight to LDS, STAGES - 1 steps of 32 keys ahead of the
+// step in work, each wave loading one of a step's four tiles; slots that no token has written
+// read as zeros (past the buffer's range). A weight of 0 meets every other column's values:
+// where those are not finite the sums are not either, and the wave's tokens are done again one
+// by one.
+constexpr int kJoinMost = 512;  // entries of a workgroup's lists
+constexpr int kJoinTokens = 8;  // tokens of a wave (their bits: 32 a workgroup)
 
 template <int D>
 struct JoinLds {
-  static constexpr int kTable = 2 * kJoinMost;
+  static constexpr int kTable = 2 * kJoinMost, kStages = D <= 192 ? 3 : 2;
+  static constexpr int kTile = 16 * D * 2;  // bytes of 16 rows
   union {
-    char stage[64 * D];
+    char stage[kStages][4][kTile];  // a step's K tiles, then its V tiles
+    float q[kAttendWaves][D];  // attend_alone's
     struct {
       int32_t page[kTable];
-      uint32_t tokens[kTable];
-      uint32_t first[kTable];
+      uint32_t tokens[kTable], first[kTable], keys[kTable];
     };
   };
-  int2 list[kJoinMost];  // page, tokens
+  int2 list[kJoinMost];        // page, tokens
+  uint8_t keys_of[kJoinMost];  // slots that hold keys
+  int32_t counts[kAttendWaves];
 };
 
+// The 16-byte chunks of a staged key row are permuted by the row, so that the rows of one chunk
+// lie in different banks.
+template <int D>
+__device__ inline int chunk_swizzle(int row) {
+  return D % 64 == 0 ? row & 7 : (row >> 1) & 3;
+}
+
 template <class E, int D>
-__global__ void __launch_bounds__(kAttendWaves* kWave, D <= 128 ? 2 : 1)
+__global__ void __launch_bounds__(kAttendWaves* kWave, D <= 128 ? 3 : 2)
     kv_attend_joined_kernel(AttendArgs a) {
-  __shared__ __attribute__((aligned(16))) JoinLds<D> lds_all[kAttendWaves];
+  using Wave = AttendWave<E, D>;
+  using V8 = typename Wave::V8;
+  using Lds = JoinLds<D>;
+  constexpr int LOADS = D / 32, STAGES = Lds::kStages;  // LOADS: of a wave in a step
+  __shared__ __attribute__((aligned(16))) Lds lds;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
-  const int lane = lane_id(), col = lane & 15;
-  JoinLds<D>& lds = lds_all[wave];
-  const int64_t t0 = (static_cast<int64_t>(blockIdx.x / a.Hkv) * kAttendWaves + wave) * a.joined;
-  if (t0 >= a.T) return;
+  const int lane = lane_id(), col = lane & 15, grp = lane >> 4;
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x / a.Hkv) * kAttendWaves * a.joined;
   const int head = blockIdx.x % a.Hkv;
-  const int tokens = a.T - t0 < a.joined ? static_cast<int>(a.T - t0) : a.joined;
+  const int most = kAttendWaves * a.joined;
+  const int tokens = a.T - t0 < most ? static_cast<int>(a.T - t0) : most;
+  const int size = 1 << a.tok.shift;
 
   // the union of the lists
-  constexpr int kTable = JoinLds<D>::kTable;
-  for (int i = lane; i < kTable; i += kWave) {
+  for (int i = threadIdx.x; i < Lds::kTable; i += kAttendWaves * kWave) {
     lds.page[i] = -1;
     lds.tokens[i] = 0u;
     lds.first[i] = ~0u;
+    lds.keys[i] = 0u;
   }
-  asm volatile("" ::: "memory");
-  const int entries = tokens * a.count;
-  int32_t page[kJoinMost / kWave];
-  int slot[kJoinMost / kWave];
+  __syncthreads();
+  constexpr int EACH = kJoinMost / (kAttendWaves * kWave);
+  int32_t page[EACH];
+  int slot[EACH];
 #pragma unroll
-  for (int r = 0; r < kJoinMost / kWave; ++r) {
-    const int e = r * kWave + lane;
+  for (int r = 0; r < EACH; ++r) {
+    const int e = (wave * EACH + r) * kWave + lane;
     page[r] = -1;
     slot[r] = 0;
-    if (e >= entries) continue;
+    if (e >= tokens * a.count) continue;
     const int tok = e / a.count;
     const KvPlace p = kv_place(a.tok, t0 + tok);
     const int32_t block = a.blocks[((t0 + tok) * a.Hkv + head) * a.count + e % a.count];
     if (block < 0 || block > p.last) continue;
     page[r] = kv_page(a.tok, p, block);
     if (page[r] < 0) continue;
-    int s = static_cast<int>((static_cast<uint32_t>(page[r]) * 0x9E3779B1u) >> 16) & (kTable - 1);
+    int s = static_cast<int>((static_cast<uint32_t>(page[r]) * 0x9E3779B1u) >> 16) &
+            (Lds::kTable - 1);
     for (;;) {  // (at most half full: a free place or the page's own is met)
       const int32_t old = atomicCAS(&lds.page[s], -1, page[r]);
       if (old == -1 || old == page[r]) break;
-      s = (s + 1) & (kTable - 1);
+      s = (s + 1) & (Lds::kTable - 1);
     }
     slot[r] = s;
-    atomicOr(&lds.tokens[s], 1u << tok);
+    atomicOr(&lds.tokens[s], 1u << (tok / a.joined * kJoinTokens + tok % a.joined));
     atomicMin(&lds.first[s], static_cast<uint32_t>(e));
+    atomicMax(&lds.keys[s],
+              static_cast<uint32_t>(block == p.last ? (p.pos & (size - 1)) + 1 : size));
   }
-  asm volatile("" ::: "memory");
-  int listed = 0;
+  __syncthreads();
+  bool first[EACH];
+  int mine = 0;
 #pragma unroll
-  for (int r = 0; r < kJoinMost / kWave; ++r) {
-    const bool first = page[r] >= 0 && lds.first[slot[r]] == static_cast<uint32_t>(r * kWave + lane);
-    const uint64_t m = __ballot(first);
-    if (first) {
-      lds.list[listed + __popcll(m & ((uint64_t{1} << lane) - 1))] =
-          int2{page[r], static_cast<int>(lds.tokens[slot[r]])};
-    }
-    listed += __popcll(m);
+  for (int r = 0; r < EACH; ++r) {
+    const uint32_t e = (wave * EACH + r) * kWave + lane;
+    first[r] = page[r] >= 0 && lds.first[slot[r]] == e;
+    mine += __popcll(__ballot(first[r]));
   }
-  asm volatile("" ::: "memory");
+  if (lane == 0) lds.counts[wave] = mine;
+  __syncthreads();
+  int listed = 0, at = 0;
+#pragma unroll
+  for (int w = 0; w < kAttendWaves; ++w) {
+    at += w < wave ? lds.counts[w] : 0;
+    listed += lds.counts[w];
+  }
+  listed = __builtin_amdgcn_readfirstlane(listed);
+#pragma unroll
+  for (int r = 0; r < EACH; ++r) {
+    const uint64_t m = __ballot(first[r]);
+    if (first[r]) {
+      const int i = at + __popcll(m & ((uint64_t{1} << lane) - 1));
+      lds.list[i] = int2{page[r], static_cast<int>(lds.tokens[slot[r]])};
+      lds.keys_of[i] = static_cast<uint8_t>(lds.keys[slot[r]]);
+    }
+    at += __popcll(m);
+  }
 
   // this lane's column: its token's own page ends after `own_keys`
   const int tok = col / a.G;
-  const bool real = tok < tokens;
-  const int64_t t = t0 + (real ? tok : 0);
+  const bool real = tok < a.joined && wave * a.joined + tok < tokens;
+  const int64_t t = t0 + (real ? wave * a.joined + tok : 0);
   const int hq = head * a.G + col % a.G;
-  const int size = 1 << a.tok.shift;
   int32_t own = -1, own_keys = 0;
   if (real) {
     const KvPlace p = kv_place(a.tok, t);
     if (p.last >= 0) own = kv_page(a.tok, p, p.last);
     own_keys = (p.pos & (size - 1)) + 1;
   }
-  AttendWave<E, D> w;
+  Wave w;
   w.clear();
   w.load_q(a, t, hq, real);
+  __syncthreads();  // the list is whole, and the table's place free for the stages
 
-  const int total = listed << (a.tok.shift - 4);  // tiles of 16 keys
-  int at = 0;
-  auto next = [&](Tiles& s) {  // (s.n: this column's; one without a token counts all keys)
-    for (; at < total; at += 2) {
+  // A lane's 16-byte chunks of the tile that this wave loads.
+  int offset[LOADS];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int i = at + j < total ? (at + j) >> (a.tok.shift - 4) : 0;
-        const int32_t pg = __builtin_amdgcn_readfirstlane(lds.list[i].x);
-        const uint32_t who =
-            at + j < total ? __builtin_amdgcn_readfirstlane(lds.list[i].y) : 0u;
-        const int first = ((at + j) << 4) & (size - 1);
-        s.row[j] = ((static_cast<int64_t>(pg) * a.Hkv + head) << a.tok.shift) + first;
-        const int end = (who >> tok) & 1u ? (pg == own ? own_keys : size) : 0;
-        const int n = end - first;
-        s.n[j] = !real ? 16 : n < 0 ? 0 : n > 16 ? 16 : n;
-      }
-      if (__any(real && (s.n[0] > 0 || s.n[1] > 0))) {
-        at += 2;
-        return true;
-      }
-    }
-    return false;
-  };
-  Tiles now, then;
-  bool more = next(then);
-  if (more) {
-    w.load_k(a, then);
-    w.load_v(a, then);
+  for (int i = 0; i < LOADS; ++i) {
+    const int x = i * 64 + lane, row = x / (D / 8), c = x % (D / 8);
+    const int from = wave < 2 ? c ^ chunk_swizzle<D>(row)
+                              : (((c >> 1) ^ granule_swizzle<D>(row)) << 1) + (c & 1);
+    offset[i] = row * (D * 2) + from * 16;
   }
-  while (more) {
-    now = then;
-    more = next(then);
-    const bool whole = __all(now.n[0] == 16 && now.n[1] == 16);
-    int rows[2];  // slots that some column counts have been written
+  // Steps of two tiles of 16 keys, those without keys left out. The list is read 64 entries at a
+  // time, one a lane: the compiler waits for every load to LDS before it reads LDS by itself.
+  const int total = listed << (a.tok.shift - 4);
+  int tile = 0, chunk = -1;
+  int32_t my_page = 0, my_tokens = 0, my_keys = 0;
+  struct Tile {
+    int32_t page, from, keys;  // page, first slot, slots that hold keys
+    uint32_t who;
+  };
+  struct Step {
+    Tile a, b;
+  };
+  auto look = [&](int i) {
+    Tile t{0, (i << 4) & (size - 1), 0, 0u};
+    if (i >= total) return t;
+    const int e = i >> (a.tok.shift - 4);
+    if (e >> 6 != chunk) {
+      chunk = e >> 6;
+      const int mine = 64 * chunk + lane < listed ? 64 * chunk + lane : 0;
+      my_page = lds.list[mine].x;
+      my_tokens = lds.list[mine].y;
+      my_keys = lds.keys_of[mine];
+    }
+    t.page = __builtin_amdgcn_readlane(my_page, e & 63);
+    t.who = __builtin_amdgcn_readlane(my_tokens, e & 63);
+    t.keys = __builtin_amdgcn_readlane(my_keys, e & 63) - t.from;
+    return t;
+  };
+  auto next = [&]() {  // a step without keys: the end
+    Step s{look(tile), look(tile + 1)};
+    while (s.a.keys <= 0 && s.b.keys <= 0 && tile < total) {
+      tile += 2;
+      s = Step{look(tile), look(tile + 1)};
+    }
+    tile += 2;
+    return s;
+  };
+  auto issue = [&](const Step& s, char* stage) {
+    const bool odd = (wave & 1) != 0;
+    const Tile t{odd ? s.b.page : s.a.page, odd ? s.b.from : s.a.from, odd ? s.b.keys : s.a.keys, 0u};
+    // (uniform: a range in a vector register would make a loop of every load)
+    const int rows = __builtin_amdgcn_readfirstlane(t.keys < 0 ? 0 : t.keys > 16 ? 16 : t.keys);
+    const char* base =
+        static_cast<const char*>(wave < 2 ? a.k_cache : a.v_cache) +
+        (((static_cast<int64_t>(t.page) * a.Hkv + head) << a.tok.shift) + t.from) * (D * 2);
+#pragma unroll
+    for (int x = 0; x < LOADS; ++x) {
+      buffer_load_lds<16, false>(base, rows * (D * 2), offset[x],
+                                 stage + wave * Lds::kTile + x * (kWave * 16));
+    }
+  };
+  auto keys_here = [&](const Tile& t) {  // of this lane's column
+    const int end = (t.who >> (kJoinTokens * wave + tok)) & 1u ? (t.page == own ? own_keys : size) : 0;
+    const int left = end - t.from;
+    return !real ? 16 : left < 0 ? 0 : left > 16 ? 16 : left;
+  };
+  // One step from `use` while a later one goes into `fill`. (The two stages differ: said by
+  // `restrict`, else every read here would wait for the loads just started.)
+  auto work = [&](char* __restrict fill, const char* __restrict use, bool more, const Step& late,
+                  const Step& s) {
+    if (more) issue(late, fill);
+    if ((((s.a.who | s.b.who) >> (kJoinTokens * wave)) & ((1u << kJoinTokens) - 1u)) == 0) return;
+    const int n[2] = {keys_here(s.a), keys_here(s.b)};
+    v4f sc[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      rows[j] = 16;
-      if (!whole && !__any(real && now.n[j] == 16)) {
-        int n = real ? now.n[j] : 0;
+      sc[j] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int x = 1; x < 16; x <<= 1) {
-          const int o = __shfl_xor(n, x);
-          n = o > n ? o : n;
-        }
-        rows[j] = __builtin_amdgcn_readfirstlane(n);
+      for (int x = 0; x < D / 32; ++x) {
+        const V8 k = *reinterpret_cast<const V8*>(
+            use + j * Lds::kTile + col * (D * 2) + (((grp + 4 * x) ^ chunk_swizzle<D>(col)) << 4));
+        sc[j] = Wave::Op::mma(k, w.qf[x], sc[j]);
       }
     }
-    w.step(a, lds.stage, whole, now.n, rows, [&] { if (more) w.load_k(a, then); },
-           [&] { if (more) w.load_v(a, then); });
+    const V8 p = w.weigh(a.scale, sc, __all(n[0] == 16 && n[1] == 16), n);
+    w.add(use + 2 * Lds::kTile, p);
+  };
+  // `now` is in work, `then` (with three stages) and `late` behind it
+  Step now = next(), then{};
+  int ahead = 0, put = 0, get = 0;
+  auto start = [&](const Step& s) {
+    if (s.a.keys <= 0 && s.b.keys <= 0) return;
+    issue(s, lds.stage[put][0]);
+    put = put + 1 == STAGES ? 0 : put + 1;
+    ++ahead;
+  };
+  start(now);
+  if (STAGES > 2) {
+    then = next();
+    start(then);
+  }
+  while (ahead > 0) {
+    const Step late = next();
+    const bool more = late.a.keys > 0 || late.b.keys > 0;
+    wait_later<LOADS, STAGES - 2>(ahead - 1);
+    tile_barrier();
+    work(lds.stage[put][0], lds.stage[get][0], more, late, now);
+    if (more) put = put + 1 == STAGES ? 0 : put + 1;
+    if (!more) --ahead;
+    get = get + 1 == STAGES ? 0 : get + 1;
+    if constexpr (STAGES > 2) {
+      now = then;
+      then = late;
+    } else {
+      now = late;
+    }
   }
   w.join_sums();
+  __syncthreads();  // (the stages are free)
   float odd = 0.0f;  // 0 times every sum: not a number where one is not finite
 #pragma unroll
   for (int i = 0; i < D / 16; ++i) {
@@ -499,9 +680,9 @@ __global__ void __launch_bounds__(kAttendWaves* kWave, D <= 128 ? 2 : 1)
     if (real) emit(a, w, t, hq);
     return;
   }
-  for (int i = 0; i < tokens; ++i) {
-    w.run(a, t0 + i, head, 0, 0, 1, lds.stage);
-    if (col < a.G) emit(a, w, t0 + i, head * a.G + col);
+  for (int i = 0; i < a.joined && wave * a.joined + i < tokens; ++i) {
+    const int64_t one = t0 + wave * a.joined + i;
+    for (int g = 0; g < a.G; ++g) attend_alone<E, D>(a, one, head, head * a.G + g, lds.q[wave]);
   }
 }
 
@@ -605,8 +786,10 @@ inline AttendPlan attend_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t page, 
   p.tiles = static_cast<int32_t>(cdiv(G, 16));
   p.rows = T * Hkv * p.tiles;
   p.parts = 0;
-  const int64_t cols = 16 / (G < 16 ? G : 16), lists = kJoinMost / (count > 0 ? count : 1);
-  p.joined = static_cast<int32_t>(cols < lists ? cols : lists);
+  int64_t joined = 16 / (G < 16 ? G : 16);
+  if (joined > kJoinTokens) joined = kJoinTokens;
+  const int64_t lists = kJoinMost / (kAttendWaves * (count > 0 ? count : 1));
+  p.joined = static_cast<int32_t>(joined < lists ? joined : lists);
   if (p.rows >= 4096) return p;
   // workgroups of four waves for two on every CU, each wave with a unit of 64 keys at least
   const int64_t most = cdiv(count * page, 64 * kAttendWaves);
