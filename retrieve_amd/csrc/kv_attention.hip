@@ -423,28 +423,27 @@ __device__ inline void attend_alone(const AttendArgs& a, int64_t t, int head, in
 //
 // The lists are joined by physical page in a hash table: of a page's entries the first (by token,
 // then place) stands for all and holds the tokens' bits, so the order of the blocks depends
-// on the lists alone. Keys and values go straight to LDS, STAGES - 1 steps of 32 keys ahead of the
-// step in work, each wave loading one of a step's four tiles; slots that no token has written
-// read as zeros (past the buffer's range). A weight of 0 meets every other column's values:
-// where those are not finite the sums are not either, and the wave's tokens are done again one
-// by one.
+// on the lists alone. Keys and values go straight to LDS, a step of 32 keys ahead of the one in
+// work, each wave loading one of a step's four tiles; slots that no token has written read as
+// zeros (past the buffer's range). A weight of 0 meets every other column's values: where those
+// are not finite the sums are not either, and the wave's tokens are done again one by one.
 constexpr int kJoinMost = 512;  // entries of a workgroup's lists
 constexpr int kJoinTokens = 8;  // tokens of a wave (their bits: 32 a workgroup)
 
 template <int D>
 struct JoinLds {
-  static constexpr int kTable = 2 * kJoinMost, kStages = D <= 192 ? 3 : 2;
+  static constexpr int kTable = 2 * kJoinMost;
   static constexpr int kTile = 16 * D * 2;  // bytes of 16 rows
   union {
-    char stage[kStages][4][kTile];  // a step's K tiles, then its V tiles
+    char stage[2][4][kTile];  // a step's K tiles, then its V tiles
     float q[kAttendWaves][D];  // attend_alone's
     struct {
       int32_t page[kTable];
-      uint32_t tokens[kTable], first[kTable], keys[kTable];
+      uint32_t tokens[kTable], first[kTable], keys[kTable], part[kTable];
     };
   };
   int2 list[kJoinMost];        // page, tokens
-  uint8_t keys_of[kJoinMost];  // slots that hold keys
+  uint8_t keys_of[kJoinMost];  // slots that hold keys, less 1; bit 7: not all of them for every token
   int32_t counts[kAttendWaves];
 };
 
@@ -456,12 +455,12 @@ __device__ inline int chunk_swizzle(int row) {
 }
 
 template <class E, int D>
-__global__ void __launch_bounds__(kAttendWaves* kWave, D <= 128 ? 3 : 2)
+__global__ void __launch_bounds__(kAttendWaves* kWave, D <= 128 ? 4 : 2)
     kv_attend_joined_kernel(AttendArgs a) {
   using Wave = AttendWave<E, D>;
   using V8 = typename Wave::V8;
   using Lds = JoinLds<D>;
-  constexpr int LOADS = D / 32, STAGES = Lds::kStages;  // LOADS: of a wave in a step
+  constexpr int LOADS = D / 32;  // of a wave in a step
   __shared__ __attribute__((aligned(16))) Lds lds;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   const int lane = lane_id(), col = lane & 15, grp = lane >> 4;
@@ -477,6 +476,7 @@ __global__ void __launch_bounds__(kAttendWaves* kWave, D <= 128 ? 3 : 2)
     lds.tokens[i] = 0u;
     lds.first[i] = ~0u;
     lds.keys[i] = 0u;
+    lds.part[i] = 0u;
   }
   __syncthreads();
   constexpr int EACH = kJoinMost / (kAttendWaves * kWave);
@@ -504,8 +504,9 @@ __global__ void __launch_bounds__(kAttendWaves* kWave, D <= 128 ? 3 : 2)
     slot[r] = s;
     atomicOr(&lds.tokens[s], 1u << (tok / a.joined * kJoinTokens + tok % a.joined));
     atomicMin(&lds.first[s], static_cast<uint32_t>(e));
-    atomicMax(&lds.keys[s],
-              static_cast<uint32_t>(block == p.last ? (p.pos & (size - 1)) + 1 : size));
+    const int slots = block == p.last ? (p.pos & (size - 1)) + 1 : size;
+    atomicMax(&lds.keys[s], static_cast<uint32_t>(slots));
+    if (slots < size) lds.part[s] = 1u;
   }
   __syncthreads();
   bool first[EACH];
@@ -531,7 +532,7 @@ __global__ void __launch_bounds__(kAttendWaves* kWave, D <= 128 ? 3 : 2)
     if (first[r]) {
       const int i = at + __popcll(m & ((uint64_t{1} << lane) - 1));
       lds.list[i] = int2{page[r], static_cast<int>(lds.tokens[slot[r]])};
-      lds.keys_of[i] = static_cast<uint8_t>(lds.keys[slot[r]]);
+      lds.keys_of[i] = static_cast<uint8_t>(lds.keys[slot[r]] - 1u + 128u * lds.part[slot[r]]);
     }
     at += __popcll(m);
   }
@@ -547,6 +548,10 @@ __global__ void __launch_bounds__(kAttendWaves* kWave, D <= 128 ? 3 : 2)
     if (p.last >= 0) own = kv_page(a.tok, p, p.last);
     own_keys = (p.pos & (size - 1)) + 1;
   }
+  const uint32_t real_tokens =
+      (1u << (tokens - wave * a.joined < 0          ? 0
+              : tokens - wave * a.joined > a.joined ? a.joined
+                                                    : tokens - wave * a.joined)) - 1u;
   Wave w;
   w.clear();
   w.load_q(a, t, hq, real);
@@ -561,69 +566,91 @@ __global__ void __launch_bounds__(kAttendWaves* kWave, D <= 128 ? 3 : 2)
                               : (((c >> 1) ^ granule_swizzle<D>(row)) << 1) + (c & 1);
     offset[i] = row * (D * 2) + from * 16;
   }
-  // Steps of two tiles of 16 keys, those without keys left out. The list is read 64 entries at a
-  // time, one a lane: the compiler waits for every load to LDS before it reads LDS by itself.
-  const int total = listed << (a.tok.shift - 4);
-  int tile = 0, chunk = -1;
-  int32_t my_page = 0, my_tokens = 0, my_keys = 0;
-  struct Tile {
-    int32_t page, from, keys;  // page, first slot, slots that hold keys
-    uint32_t who;
-  };
+  // Steps of two tiles of 16 keys. 64 at a time are worked out, one a lane: whose columns count
+  // (this wave's tokens, and whether any do; `part`: not all of a page's slots), and what this wave
+  // loads: its tile's first row and rows. Steps without keys are left out.
+  const int total = listed << (a.tok.shift - 4);  // tiles
+  const uint32_t ours = ((1u << kJoinTokens) - 1u) << (kJoinTokens * wave);
+  int64_t my_row = 0;
+  uint32_t my_who[2] = {0u, 0u};
+  int32_t my_rows = 0, base = -kWave;
+  uint64_t left = 0;
   struct Step {
-    Tile a, b;
+    int64_t row;  // to load
+    int32_t rows;
+    int32_t at;  // its first tile; past `total`: none
+    uint32_t who[2];
+    bool part;
   };
-  auto look = [&](int i) {
-    Tile t{0, (i << 4) & (size - 1), 0, 0u};
-    if (i >= total) return t;
-    const int e = i >> (a.tok.shift - 4);
-    if (e >> 6 != chunk) {
-      chunk = e >> 6;
-      const int mine = 64 * chunk + lane < listed ? 64 * chunk + lane : 0;
-      my_page = lds.list[mine].x;
-      my_tokens = lds.list[mine].y;
-      my_keys = lds.keys_of[mine];
+  auto next = [&]() {
+    Step s{0, 0, total, {0u, 0u}, false};
+    while (left == 0) {
+      base += kWave;
+      if (2 * base >= total) return s;
+      int keys[2];
+      bool part = false;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int i = 2 * (base + lane) + j, e = i >> (a.tok.shift - 4);
+        const int2 x = i < total ? lds.list[e] : int2{0, 0};
+        const int about = i < total ? lds.keys_of[e] : 0, from = (i << 4) & (size - 1);
+        const int slots = i < total ? (about & 127) + 1 : 0;
+        keys[j] = slots - from < 0 ? 0 : slots - from > 16 ? 16 : slots - from;
+        part |= about >= 128;
+        my_who[j] = (static_cast<uint32_t>(x.y) & ours) >> (kJoinTokens * wave);
+        if (j == (wave & 1)) {
+          my_row = ((static_cast<int64_t>(x.x) * a.Hkv + head) << a.tok.shift) + from;
+          my_rows = keys[j];
+        }
+      }
+      my_rows |= part ? 32 : 0;
+      left = __ballot(keys[0] > 0 || keys[1] > 0);
     }
-    t.page = __builtin_amdgcn_readlane(my_page, e & 63);
-    t.who = __builtin_amdgcn_readlane(my_tokens, e & 63);
-    t.keys = __builtin_amdgcn_readlane(my_keys, e & 63) - t.from;
-    return t;
-  };
-  auto next = [&]() {  // a step without keys: the end
-    Step s{look(tile), look(tile + 1)};
-    while (s.a.keys <= 0 && s.b.keys <= 0 && tile < total) {
-      tile += 2;
-      s = Step{look(tile), look(tile + 1)};
-    }
-    tile += 2;
+    const int i = __builtin_ctzll(left);
+    left &= left - 1;
+    s.at = 2 * (base + i);
+    s.row = static_cast<int64_t>(
+        static_cast<uint64_t>(static_cast<uint32_t>(
+            __builtin_amdgcn_readlane(static_cast<int32_t>(my_row), i))) |
+        static_cast<uint64_t>(static_cast<uint32_t>(
+            __builtin_amdgcn_readlane(static_cast<int32_t>(my_row >> 32), i))) << 32);
+    const int32_t rows = __builtin_amdgcn_readlane(my_rows, i);
+    s.rows = rows & 31;
+    s.part = rows >= 32;
+    s.who[0] = __builtin_amdgcn_readlane(my_who[0], i);
+    s.who[1] = __builtin_amdgcn_readlane(my_who[1], i);
     return s;
   };
+  const char* cache = static_cast<const char*>(wave < 2 ? a.k_cache : a.v_cache);
   auto issue = [&](const Step& s, char* stage) {
-    const bool odd = (wave & 1) != 0;
-    const Tile t{odd ? s.b.page : s.a.page, odd ? s.b.from : s.a.from, odd ? s.b.keys : s.a.keys, 0u};
-    // (uniform: a range in a vector register would make a loop of every load)
-    const int rows = __builtin_amdgcn_readfirstlane(t.keys < 0 ? 0 : t.keys > 16 ? 16 : t.keys);
-    const char* base =
-        static_cast<const char*>(wave < 2 ? a.k_cache : a.v_cache) +
-        (((static_cast<int64_t>(t.page) * a.Hkv + head) << a.tok.shift) + t.from) * (D * 2);
+    const char* from = cache + s.row * (D * 2);
 #pragma unroll
     for (int x = 0; x < LOADS; ++x) {
-      buffer_load_lds<16, false>(base, rows * (D * 2), offset[x],
+      buffer_load_lds<16, false>(from, s.rows * (D * 2), offset[x],
                                  stage + wave * Lds::kTile + x * (kWave * 16));
     }
   };
-  auto keys_here = [&](const Tile& t) {  // of this lane's column
-    const int end = (t.who >> (kJoinTokens * wave + tok)) & 1u ? (t.page == own ? own_keys : size) : 0;
-    const int left = end - t.from;
-    return !real ? 16 : left < 0 ? 0 : left > 16 ? 16 : left;
+  auto keys_here = [&](int i, uint32_t who) {  // of tile i that this lane's column counts
+    if (!real) return 16;
+    if (((who >> tok) & 1u) == 0) return 0;
+    const int end = lds.list[i >> (a.tok.shift - 4)].x == own ? own_keys : size;
+    const int n = end - ((i << 4) & (size - 1));
+    return n < 0 ? 0 : n > 16 ? 16 : n;
   };
-  // One step from `use` while a later one goes into `fill`. (The two stages differ: said by
+  // One step from `use` while the next goes into `fill`. (The two stages differ: said by
   // `restrict`, else every read here would wait for the loads just started.)
-  auto work = [&](char* __restrict fill, const char* __restrict use, bool more, const Step& late,
+  auto work = [&](char* __restrict fill, const char* __restrict use, const Step& late,
                   const Step& s) {
-    if (more) issue(late, fill);
-    if ((((s.a.who | s.b.who) >> (kJoinTokens * wave)) & ((1u << kJoinTokens) - 1u)) == 0) return;
-    const int n[2] = {keys_here(s.a), keys_here(s.b)};
+    if (late.at < total) issue(late, fill);
+    const bool whole = !s.part && s.who[0] == real_tokens && s.who[1] == real_tokens;
+    int n[2] = {16, 16};
+    if (s.part) {
+      n[0] = keys_here(s.at, s.who[0]);
+      n[1] = keys_here(s.at + 1, s.who[1]);
+    } else if (!whole) {
+      n[0] = !real || ((s.who[0] >> tok) & 1u) != 0 ? 16 : 0;
+      n[1] = !real || ((s.who[1] >> tok) & 1u) != 0 ? 16 : 0;
+    }
     v4f sc[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -635,38 +662,29 @@ __global__ void __launch_bounds__(kAttendWaves* kWave, D <= 128 ? 3 : 2)
         sc[j] = Wave::Op::mma(k, w.qf[x], sc[j]);
       }
     }
-    const V8 p = w.weigh(a.scale, sc, __all(n[0] == 16 && n[1] == 16), n);
+    const V8 p = w.weigh(a.scale, sc, whole, n);
     w.add(use + 2 * Lds::kTile, p);
   };
-  // `now` is in work, `then` (with three stages) and `late` behind it
-  Step now = next(), then{};
-  int ahead = 0, put = 0, get = 0;
-  auto start = [&](const Step& s) {
-    if (s.a.keys <= 0 && s.b.keys <= 0) return;
-    issue(s, lds.stage[put][0]);
-    put = put + 1 == STAGES ? 0 : put + 1;
-    ++ahead;
-  };
-  start(now);
-  if (STAGES > 2) {
-    then = next();
-    start(then);
-  }
-  while (ahead > 0) {
-    const Step late = next();
-    const bool more = late.a.keys > 0 || late.b.keys > 0;
-    wait_later<LOADS, STAGES - 2>(ahead - 1);
+  Step now = next();
+  if (now.at < total) issue(now, lds.stage[0][0]);
+  int get = 0;
+  while (now.at < total) {
+    Step late = next();
+    wait_vmcnt<0>();
     tile_barrier();
-    work(lds.stage[put][0], lds.stage[get][0], more, late, now);
-    if (more) put = put + 1 == STAGES ? 0 : put + 1;
-    if (!more) --ahead;
-    get = get + 1 == STAGES ? 0 : get + 1;
-    if constexpr (STAGES > 2) {
-      now = then;
-      then = late;
-    } else {
+    while ((now.who[0] | now.who[1]) == 0) {  // (nothing here for this wave's tokens)
+      get ^= 1;
       now = late;
+      if (now.at >= total) break;
+      issue(now, lds.stage[get][0]);
+      late = next();
+      wait_vmcnt<0>();
+      tile_barrier();
     }
+    if (now.at >= total) break;
+    work(lds.stage[get ^ 1][0], lds.stage[get][0], late, now);
+    get ^= 1;
+    now = late;
   }
   w.join_sums();
   __syncthreads();  // (the stages are free)
