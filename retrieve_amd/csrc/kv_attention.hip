@@ -422,8 +422,8 @@ __device__ inline void attend_alone(const AttendArgs& a, int64_t t, int head, in
 // of its tokens lists.
 //
 // The lists are joined by physical page in a hash table: of a page's entries the first (by token,
-// then place) stands for all and holds the tokens' bits, so the order of the blocks depends
-// on the lists alone. Keys and values go straight to LDS, a step of 32 keys ahead of the one in
+// then place) stands for all and holds the tokens' bits; they are taken in the order of their
+// blocks, so it depends on the lists alone. Keys and values go straight to LDS, a step of 32 keys ahead of the one in
 // work, each wave loading one of a step's four tiles; slots that no token has written read as
 // zeros (past the buffer's range). A weight of 0 meets every other column's values: where those
 // are not finite the sums are not either, and the wave's tokens are done again one by one.
@@ -481,19 +481,22 @@ __global__ void __launch_bounds__(kAttendWaves* kWave, D <= 128 ? 4 : 2)
   __syncthreads();
   constexpr int EACH = kJoinMost / (kAttendWaves * kWave);
   int32_t page[EACH];
-  int slot[EACH];
+  uint32_t block[EACH];
+  int slot[EACH], rank[EACH];
 #pragma unroll
   for (int r = 0; r < EACH; ++r) {
     const int e = (wave * EACH + r) * kWave + lane;
     page[r] = -1;
+    block[r] = 0u;
     slot[r] = 0;
     if (e >= tokens * a.count) continue;
     const int tok = e / a.count;
     const KvPlace p = kv_place(a.tok, t0 + tok);
-    const int32_t block = a.blocks[((t0 + tok) * a.Hkv + head) * a.count + e % a.count];
-    if (block < 0 || block > p.last) continue;
-    page[r] = kv_page(a.tok, p, block);
+    const int32_t b = a.blocks[((t0 + tok) * a.Hkv + head) * a.count + e % a.count];
+    if (b < 0 || b > p.last) continue;
+    page[r] = kv_page(a.tok, p, b);
     if (page[r] < 0) continue;
+    block[r] = b;
     int s = static_cast<int>((static_cast<uint32_t>(page[r]) * 0x9E3779B1u) >> 16) &
             (Lds::kTable - 1);
     for (;;) {  // (at most half full: a free place or the page's own is met)
@@ -504,7 +507,7 @@ __global__ void __launch_bounds__(kAttendWaves* kWave, D <= 128 ? 4 : 2)
     slot[r] = s;
     atomicOr(&lds.tokens[s], 1u << (tok / a.joined * kJoinTokens + tok % a.joined));
     atomicMin(&lds.first[s], static_cast<uint32_t>(e));
-    const int slots = block == p.last ? (p.pos & (size - 1)) + 1 : size;
+    const int slots = b == p.last ? (p.pos & (size - 1)) + 1 : size;
     atomicMax(&lds.keys[s], static_cast<uint32_t>(slots));
     if (slots < size) lds.part[s] = 1u;
   }
@@ -526,15 +529,25 @@ __global__ void __launch_bounds__(kAttendWaves* kWave, D <= 128 ? 4 : 2)
     listed += lds.counts[w];
   }
   listed = __builtin_amdgcn_readfirstlane(listed);
+  // by block: the workgroups of a head, which sweep the cache side by side, then meet in its L2
 #pragma unroll
   for (int r = 0; r < EACH; ++r) {
     const uint64_t m = __ballot(first[r]);
-    if (first[r]) {
-      const int i = at + __popcll(m & ((uint64_t{1} << lane) - 1));
-      lds.list[i] = int2{page[r], static_cast<int>(lds.tokens[slot[r]])};
-      lds.keys_of[i] = static_cast<uint8_t>(lds.keys[slot[r]] - 1u + 128u * lds.part[slot[r]]);
-    }
+    rank[r] = at + __popcll(m & ((uint64_t{1} << lane) - 1));
+    if (first[r]) lds.first[rank[r]] = block[r];  // (the table's firsts have been read)
     at += __popcll(m);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < EACH; ++r) {
+    if (!first[r]) continue;
+    int to = 0;
+    for (int i = 0; i < listed; ++i) {
+      const uint32_t b = lds.first[i];
+      to += b < block[r] || (b == block[r] && i < rank[r]) ? 1 : 0;
+    }
+    lds.list[to] = int2{page[r], static_cast<int>(lds.tokens[slot[r]])};
+    lds.keys_of[to] = static_cast<uint8_t>(lds.keys[slot[r]] - 1u + 128u * lds.part[slot[r]]);
   }
 
   // this lane's column: its token's own page ends after `own_keys`
