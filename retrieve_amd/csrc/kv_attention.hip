@@ -40,7 +40,8 @@ struct AttendArgs {
   const int32_t* blocks;  // [T, Hkv, count]
   int32_t count;
   KvTokens tok;
-  float scale;      // times log2 e
+  float scale;      // its magnitude (above 0) times log2 e; the queries carry its sign
+  bool minus;
   int32_t parts;    // workgroups that share a row
   int32_t joined;   // tokens a wave takes together
   void* out;        // [T, Hq, D]
@@ -164,7 +165,7 @@ struct AttendWave {
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       const V8 x = *reinterpret_cast<const V8*>(q + 32 * s);
-      qf[s] = real ? x : V8{};
+      qf[s] = real ? (a.minus ? -x : x) : V8{};
     }
   }
   __device__ void load_k(const AttendArgs& a, const Tiles& s) {
@@ -217,60 +218,76 @@ struct AttendWave {
                              (c & 1) * 16) = vf[i];
     }
     fetch_v();
-    const V8 p = weigh(a.scale, sc, whole, n);
+    V8 p[1];
+    weigh(a.scale, sc, whole, n, p);
     asm volatile("" ::: "memory");  // (the staged rows are read by other lanes of this wave)
     add(lds, p);
     asm volatile("" ::: "memory");
   }
-  // The weights of a step's scores, rounded for the second product (keys 4 (lane / 16) + r of tile
-  // j at 4 j + r), the maximum raised and the sum extended.
-  __device__ V8 weigh(float scale, const v4f (&sc)[2], bool whole, const int (&n)[2]) {
-    const int grp = lane_id() >> 4;
-    float w[8];
+  // The weights of the scores of N tiles (key 4 (lane / 16) + r of tile j at 4 (j % 2) + r of p[j / 2]),
+  // rounded for the second product; the maximum raised and the sum extended. A column counts the
+  // first n[j] keys of tile j (all where `whole`).
+  template <int N>
+  __device__ void weigh(float scale, v4f (&sc)[N], bool whole, const int (&n)[N],
+                        V8 (&p)[N / 2]) {
+    if (!whole) {
+      const int at = 4 * (lane_id() >> 4);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < N; ++j) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float y = sc[j][r] * scale;
-        w[4 * j + r] = whole || 4 * grp + r < n[j] ? y : -INFINITY;
+        for (int r = 0; r < 4; ++r) sc[j][r] = at + r < n[j] ? sc[j][r] : -INFINITY;
       }
     }
-    float top = w[0];
+    float top[N];
 #pragma unroll
-    for (int r = 1; r < 8; ++r) top = fmaxf(top, w[r]);
-    if (__any(top > m + 8.0f)) {
-      top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaxf(top, __shfl_xor(top, 32));
-      const float next = fmaxf(m, top);
+    for (int j = 0; j < N; ++j) {
+      top[j] = fmaxf(fmaxf(sc[j][0], sc[j][1]), fmaxf(sc[j][2], sc[j][3]));
+    }
+#pragma unroll
+    for (int j = 1; j < N; ++j) top[0] = fmaxf(top[0], top[j]);
+    const float high = top[0] * scale;
+    if (__any(high > m + 8.0f)) {
+      float next = fmaxf(high, __shfl_xor(high, 16));
+      next = fmaxf(next, __shfl_xor(next, 32));
+      next = fmaxf(next, m);
       const float keep = __builtin_amdgcn_exp2f(m - next);
       m = next;
       l *= keep;
 #pragma unroll
       for (int i = 0; i < DT; ++i) acc[i] *= keep;
     }
-    V8 p;
+    float sum[N];
 #pragma unroll
-    for (int r = 0; r < 8; ++r) {
-      const float e = __builtin_amdgcn_exp2f(w[r] - m);
-      l += e;
-      p[r] = static_cast<E>(e);
+    for (int j = 0; j < N; ++j) {
+      float e[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        e[r] = __builtin_amdgcn_exp2f(fmaf(sc[j][r], scale, -m));
+        p[j / 2][4 * (j % 2) + r] = static_cast<E>(e[r]);
+      }
+      sum[j] = (e[0] + e[1]) + (e[2] + e[3]);
     }
-    return p;
+#pragma unroll
+    for (int j = 0; j < N; j += 2) l += sum[j] + sum[j + 1];
   }
-  // The second product: 32 staged rows of values, swizzled by granules.
-  __device__ void add(const char* lds, V8 p) {
+  // The second product: 32 N staged rows of values, swizzled by granules.
+  template <int N>
+  __device__ void add(const char* lds, const V8 (&p)[N]) {
     const int col = lane_id() & 15, grp = lane_id() >> 4;
 #pragma unroll
     for (int i = 0; i < DT; ++i) {
-      typename Op::V4 x[2];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int row = 16 * j + 4 * grp + (col >> 2);
-        x[j] = Op::read_tr(lds + row * (D * 2) + ((i ^ granule_swizzle<D>(row)) << 5) +
-                           (col & 3) * 8);
+      for (int h = 0; h < N; ++h) {
+        typename Op::V4 x[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int row = 16 * j + 4 * grp + (col >> 2);
+          x[j] = Op::read_tr(lds + (32 * h + row) * (D * 2) +
+                             ((i ^ granule_swizzle<D>(row)) << 5) + (col & 3) * 8);
+        }
+        const V8 v = {x[0][0], x[0][1], x[0][2], x[0][3], x[1][0], x[1][1], x[1][2], x[1][3]};
+        acc[i] = Op::mma(v, p[h], acc[i]);
       }
-      const V8 v = {x[0][0], x[0][1], x[0][2], x[0][3], x[1][0], x[1][1], x[1][2], x[1][3]};
-      acc[i] = Op::mma(v, p, acc[i]);
     }
   }
   __device__ void join_sums() {
@@ -359,7 +376,7 @@ __device__ inline void attend_alone(const AttendArgs& a, int64_t t, int head, in
   const int lane = lane_id();
   const KvPlace p = kv_place(a.tok, t);
   const E* q = static_cast<const E*>(a.q) + t * a.q_st + hq * a.q_sh;
-  for (int d = lane; d < D; d += kWave) qs[d] = static_cast<float>(q[d]) * a.scale;
+  for (int d = lane; d < D; d += kWave) qs[d] = static_cast<float>(q[d]) * (a.minus ? -a.scale : a.scale);
   asm volatile("" ::: "memory");
   const int size = 1 << a.tok.shift;
   float m = -3.402823466e38f, l = 0.0f, acc[R] = {};
@@ -423,28 +440,38 @@ __device__ inline void attend_alone(const AttendArgs& a, int64_t t, int head, in
 //
 // The lists are joined by physical page in a hash table: of a page's entries the first (by token,
 // then place) stands for all and holds the tokens' bits; they are taken in the order of their
-// blocks, so it depends on the lists alone. Keys and values go straight to LDS, a step of 32 keys ahead of the one in
-// work, each wave loading one of a step's four tiles; slots that no token has written read as
-// zeros (past the buffer's range). A weight of 0 meets every other column's values: where those
-// are not finite the sums are not either, and the wave's tokens are done again one by one.
+// blocks, so it depends on the lists alone. Keys and values go straight to LDS, a step of 32 keys
+// ahead of the one in work, each wave loading one of a step's four tiles; slots that no token has
+// written read as zeros (past the buffer's range). A weight of 0 meets every other column's
+// values: where those are not finite the sums are not either, and the wave's tokens are done
+// again one by one.
+//
+// A step is bound by its chain of instructions (loads issued, two products, the weights, the next
+// step's numbers: about 2,300 cycles for 32 keys of 128 channels), hidden by four workgroups a CU.
+// Eight waves and 64 keys a step share more of the loads and have fewer barriers, but wait longer
+// at each: a prompt of 8192 tokens takes 521 us instead of 464.
+constexpr int kJoinWaves = 4;
+constexpr int kJoinTiles = kJoinWaves / 2;  // of a step: a wave loads one of its K or V tiles
 constexpr int kJoinMost = 512;  // entries of a workgroup's lists
-constexpr int kJoinTokens = 8;  // tokens of a wave (their bits: 32 a workgroup)
+constexpr int kJoinTokens = 8;   // tokens of a wave: their bits in a mask
 
 template <int D>
 struct JoinLds {
   static constexpr int kTable = 2 * kJoinMost;
   static constexpr int kTile = 16 * D * 2;  // bytes of 16 rows
   union {
-    char stage[2][4][kTile];  // a step's K tiles, then its V tiles
-    float q[kAttendWaves][D];  // attend_alone's
+    char stage[2][kJoinWaves][kTile];  // a step's K tiles, then its V tiles
+    float q[kJoinWaves][D];            // attend_alone's
     struct {
       int32_t page[kTable];
-      uint32_t tokens[kTable], first[kTable], keys[kTable], part[kTable];
+      uint32_t tokens[kTable];
+      uint32_t first[kTable], keys[kTable], part[kTable];
     };
   };
-  int2 list[kJoinMost];        // page, tokens
-  uint8_t keys_of[kJoinMost];  // slots that hold keys, less 1; bit 7: not all of them for every token
-  int32_t counts[kAttendWaves];
+  int32_t list[kJoinMost];  // pages
+  uint32_t who[kJoinMost];
+  uint8_t keys_of[kJoinMost];  // slots that hold keys, less 1; bit 7: some tokens count fewer
+  int32_t counts[kJoinWaves];
 };
 
 // The 16-byte chunks of a staged key row are permuted by the row, so that the rows of one chunk
@@ -455,7 +482,7 @@ __device__ inline int chunk_swizzle(int row) {
 }
 
 template <class E, int D>
-__global__ void __launch_bounds__(kAttendWaves* kWave, D <= 128 ? 4 : 2)
+__global__ void __launch_bounds__(kJoinWaves* kWave, D <= 128 ? 4 : 2)
     kv_attend_joined_kernel(AttendArgs a) {
   using Wave = AttendWave<E, D>;
   using V8 = typename Wave::V8;
@@ -464,14 +491,14 @@ __global__ void __launch_bounds__(kAttendWaves* kWave, D <= 128 ? 4 : 2)
   __shared__ __attribute__((aligned(16))) Lds lds;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   const int lane = lane_id(), col = lane & 15, grp = lane >> 4;
-  const int64_t t0 = static_cast<int64_t>(blockIdx.x / a.Hkv) * kAttendWaves * a.joined;
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x / a.Hkv) * kJoinWaves * a.joined;
   const int head = blockIdx.x % a.Hkv;
-  const int most = kAttendWaves * a.joined;
+  const int most = kJoinWaves * a.joined;
   const int tokens = a.T - t0 < most ? static_cast<int>(a.T - t0) : most;
   const int size = 1 << a.tok.shift;
 
   // the union of the lists
-  for (int i = threadIdx.x; i < Lds::kTable; i += kAttendWaves * kWave) {
+  for (int i = threadIdx.x; i < Lds::kTable; i += kJoinWaves * kWave) {
     lds.page[i] = -1;
     lds.tokens[i] = 0u;
     lds.first[i] = ~0u;
@@ -479,7 +506,7 @@ __global__ void __launch_bounds__(kAttendWaves* kWave, D <= 128 ? 4 : 2)
     lds.part[i] = 0u;
   }
   __syncthreads();
-  constexpr int EACH = kJoinMost / (kAttendWaves * kWave);
+  constexpr int EACH = kJoinMost / (kJoinWaves * kWave);
   int32_t page[EACH];
   uint32_t block[EACH];
   int slot[EACH], rank[EACH];
@@ -524,7 +551,7 @@ __global__ void __launch_bounds__(kAttendWaves* kWave, D <= 128 ? 4 : 2)
   __syncthreads();
   int listed = 0, at = 0;
 #pragma unroll
-  for (int w = 0; w < kAttendWaves; ++w) {
+  for (int w = 0; w < kJoinWaves; ++w) {
     at += w < wave ? lds.counts[w] : 0;
     listed += lds.counts[w];
   }
@@ -537,16 +564,24 @@ __global__ void __launch_bounds__(kAttendWaves* kWave, D <= 128 ? 4 : 2)
     if (first[r]) lds.first[rank[r]] = block[r];  // (the table's firsts have been read)
     at += __popcll(m);
   }
+  if (threadIdx.x < 8) lds.first[listed + threadIdx.x] = ~0u;
   __syncthreads();
 #pragma unroll
   for (int r = 0; r < EACH; ++r) {
     if (!first[r]) continue;
     int to = 0;
-    for (int i = 0; i < listed; ++i) {
-      const uint32_t b = lds.first[i];
-      to += b < block[r] || (b == block[r] && i < rank[r]) ? 1 : 0;
+    for (int i = 0; i < listed; i += 8) {
+      v4i b[2];
+      b[0] = *reinterpret_cast<const v4i*>(&lds.first[i]);
+      b[1] = *reinterpret_cast<const v4i*>(&lds.first[i + 4]);
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        const uint32_t o = static_cast<uint32_t>(b[x >> 2][x & 3]);
+        to += o < block[r] || (o == block[r] && i + x < rank[r]) ? 1 : 0;
+      }
     }
-    lds.list[to] = int2{page[r], static_cast<int>(lds.tokens[slot[r]])};
+    lds.list[to] = page[r];
+    lds.who[to] = lds.tokens[slot[r]];
     lds.keys_of[to] = static_cast<uint8_t>(lds.keys[slot[r]] - 1u + 128u * lds.part[slot[r]]);
   }
 
@@ -561,10 +596,9 @@ __global__ void __launch_bounds__(kAttendWaves* kWave, D <= 128 ? 4 : 2)
     if (p.last >= 0) own = kv_page(a.tok, p, p.last);
     own_keys = (p.pos & (size - 1)) + 1;
   }
-  const uint32_t real_tokens =
-      (1u << (tokens - wave * a.joined < 0          ? 0
-              : tokens - wave * a.joined > a.joined ? a.joined
-                                                    : tokens - wave * a.joined)) - 1u;
+  const int here = tokens - wave * a.joined;  // this wave's tokens, their bits for both tiles
+  const uint32_t all =
+      ((1u << (here < 0 ? 0 : here > a.joined ? a.joined : here)) - 1u) * 0x0101u;
   Wave w;
   w.clear();
   w.load_q(a, t, hq, real);
@@ -575,108 +609,103 @@ __global__ void __launch_bounds__(kAttendWaves* kWave, D <= 128 ? 4 : 2)
 #pragma unroll
   for (int i = 0; i < LOADS; ++i) {
     const int x = i * 64 + lane, row = x / (D / 8), c = x % (D / 8);
-    const int from = wave < 2 ? c ^ chunk_swizzle<D>(row)
+    const int from = wave < kJoinTiles ? c ^ chunk_swizzle<D>(row)
                               : (((c >> 1) ^ granule_swizzle<D>(row)) << 1) + (c & 1);
     offset[i] = row * (D * 2) + from * 16;
   }
   // Steps of two tiles of 16 keys. 64 at a time are worked out, one a lane: whose columns count
-  // (this wave's tokens, and whether any do; `part`: not all of a page's slots), and what this wave
+  // (the wave's tokens, a byte a tile; `part`: some not all of a page's slots), and what this wave
   // loads: its tile's first row and rows. Steps without keys are left out.
   const int total = listed << (a.tok.shift - 4);  // tiles
-  const uint32_t ours = ((1u << kJoinTokens) - 1u) << (kJoinTokens * wave);
   int64_t my_row = 0;
-  uint32_t my_who[2] = {0u, 0u};
+  uint32_t my_who = 0u;
   int32_t my_rows = 0, base = -kWave;
   uint64_t left = 0;
   struct Step {
-    int64_t row;  // to load
-    int32_t rows;
-    int32_t at;  // its first tile; past `total`: none
-    uint32_t who[2];
-    bool part;
+    int64_t row;   // to load
+    int32_t rows;  // 32: `part`
+    int32_t at;    // its first tile; `total`: there is none
+    uint32_t who;
   };
   auto next = [&]() {
-    Step s{0, 0, total, {0u, 0u}, false};
+    Step s{0, 0, total, 0u};
     while (left == 0) {
       base += kWave;
-      if (2 * base >= total) return s;
-      int keys[2];
-      bool part = false;
+      if (kJoinTiles * base >= total) return s;
+      bool any = false, part = false;
+      my_who = 0u;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int i = 2 * (base + lane) + j, e = i >> (a.tok.shift - 4);
-        const int2 x = i < total ? lds.list[e] : int2{0, 0};
+      for (int j = 0; j < kJoinTiles; ++j) {
+        const int i = kJoinTiles * (base + lane) + j, e = i < total ? i >> (a.tok.shift - 4) : 0;
         const int about = i < total ? lds.keys_of[e] : 0, from = (i << 4) & (size - 1);
-        const int slots = i < total ? (about & 127) + 1 : 0;
-        keys[j] = slots - from < 0 ? 0 : slots - from > 16 ? 16 : slots - from;
+        const int n = i < total ? (about & 127) + 1 - from : 0;
+        any |= n > 0;
         part |= about >= 128;
-        my_who[j] = (static_cast<uint32_t>(x.y) & ours) >> (kJoinTokens * wave);
-        if (j == (wave & 1)) {
-          my_row = ((static_cast<int64_t>(x.x) * a.Hkv + head) << a.tok.shift) + from;
-          my_rows = keys[j];
+        if (i < total) {
+          my_who |= ((lds.who[e] >> (wave * kJoinTokens)) & 255u) << (8 * j);
+        }
+        if (j == wave % kJoinTiles) {
+          my_row = ((static_cast<int64_t>(lds.list[e]) * a.Hkv + head) << a.tok.shift) + from;
+          my_rows = n < 0 ? 0 : n > 16 ? 16 : n;
         }
       }
-      my_rows |= part ? 32 : 0;
-      left = __ballot(keys[0] > 0 || keys[1] > 0);
+      my_rows += part ? 32 : 0;
+      left = __ballot(any);
     }
     const int i = __builtin_ctzll(left);
     left &= left - 1;
-    s.at = 2 * (base + i);
-    s.row = static_cast<int64_t>(
-        static_cast<uint64_t>(static_cast<uint32_t>(
-            __builtin_amdgcn_readlane(static_cast<int32_t>(my_row), i))) |
-        static_cast<uint64_t>(static_cast<uint32_t>(
-            __builtin_amdgcn_readlane(static_cast<int32_t>(my_row >> 32), i))) << 32);
-    const int32_t rows = __builtin_amdgcn_readlane(my_rows, i);
-    s.rows = rows & 31;
-    s.part = rows >= 32;
-    s.who[0] = __builtin_amdgcn_readlane(my_who[0], i);
-    s.who[1] = __builtin_amdgcn_readlane(my_who[1], i);
+    s.at = kJoinTiles * (base + i);
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int32_t>(my_row), i);
+    s.row = static_cast<int64_t>(__builtin_amdgcn_readlane(static_cast<int32_t>(my_row >> 32), i))
+                << 32 | lo;
+    s.rows = __builtin_amdgcn_readlane(my_rows, i);
+    s.who = __builtin_amdgcn_readlane(static_cast<int32_t>(my_who), i);
     return s;
   };
-  const char* cache = static_cast<const char*>(wave < 2 ? a.k_cache : a.v_cache);
+  const char* cache = static_cast<const char*>(wave < kJoinTiles ? a.k_cache : a.v_cache);
   auto issue = [&](const Step& s, char* stage) {
     const char* from = cache + s.row * (D * 2);
+    const int bytes = (s.rows & 31) * (D * 2);
 #pragma unroll
     for (int x = 0; x < LOADS; ++x) {
-      buffer_load_lds<16, false>(from, s.rows * (D * 2), offset[x],
+      buffer_load_lds<16, false>(from, bytes, offset[x],
                                  stage + wave * Lds::kTile + x * (kWave * 16));
     }
-  };
-  auto keys_here = [&](int i, uint32_t who) {  // of tile i that this lane's column counts
-    if (!real) return 16;
-    if (((who >> tok) & 1u) == 0) return 0;
-    const int end = lds.list[i >> (a.tok.shift - 4)].x == own ? own_keys : size;
-    const int n = end - ((i << 4) & (size - 1));
-    return n < 0 ? 0 : n > 16 ? 16 : n;
   };
   // One step from `use` while the next goes into `fill`. (The two stages differ: said by
   // `restrict`, else every read here would wait for the loads just started.)
   auto work = [&](char* __restrict fill, const char* __restrict use, const Step& late,
                   const Step& s) {
     if (late.at < total) issue(late, fill);
-    const bool whole = !s.part && s.who[0] == real_tokens && s.who[1] == real_tokens;
-    int n[2] = {16, 16};
-    if (s.part) {
-      n[0] = keys_here(s.at, s.who[0]);
-      n[1] = keys_here(s.at + 1, s.who[1]);
-    } else if (!whole) {
-      n[0] = !real || ((s.who[0] >> tok) & 1u) != 0 ? 16 : 0;
-      n[1] = !real || ((s.who[1] >> tok) & 1u) != 0 ? 16 : 0;
-    }
-    v4f sc[2];
+    v4f sc[kJoinTiles];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      sc[j] = v4f{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < kJoinTiles; ++j) sc[j] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int x = 0; x < D / 32; ++x) {
+    for (int x = 0; x < D / 32; ++x) {
+#pragma unroll
+      for (int j = 0; j < kJoinTiles; ++j) {
         const V8 k = *reinterpret_cast<const V8*>(
             use + j * Lds::kTile + col * (D * 2) + (((grp + 4 * x) ^ chunk_swizzle<D>(col)) << 4));
         sc[j] = Wave::Op::mma(k, w.qf[x], sc[j]);
       }
     }
-    const V8 p = w.weigh(a.scale, sc, whole, n);
-    w.add(use + 2 * Lds::kTile, p);
+    const bool whole = s.rows < 32 && s.who == all;
+    int n[kJoinTiles];
+    if (!whole) {
+#pragma unroll
+      for (int j = 0; j < kJoinTiles; ++j) {
+        const bool counts = ((s.who >> (8 * j + tok)) & 1u) != 0;
+        n[j] = !real || counts ? 16 : 0;
+        if (s.rows >= 32 && real && counts) {
+          const int i = s.at + j;
+          const int end = lds.list[i >> (a.tok.shift - 4)] == own ? own_keys : size;
+          n[j] = end - ((i << 4) & (size - 1));
+        }
+      }
+    }
+    V8 p[kJoinTiles / 2];
+    w.weigh(a.scale, sc, whole, n, p);
+    w.add(use + kJoinTiles * Lds::kTile, p);
   };
   Step now = next();
   if (now.at < total) issue(now, lds.stage[0][0]);
@@ -685,7 +714,7 @@ __global__ void __launch_bounds__(kAttendWaves* kWave, D <= 128 ? 4 : 2)
     Step late = next();
     wait_vmcnt<0>();
     tile_barrier();
-    while ((now.who[0] | now.who[1]) == 0) {  // (nothing here for this wave's tokens)
+    while (now.who == 0) {  // (nothing here for this wave's tokens)
       get ^= 1;
       now = late;
       if (now.at >= total) break;
@@ -819,7 +848,7 @@ inline AttendPlan attend_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t page, 
   p.parts = 0;
   int64_t joined = 16 / (G < 16 ? G : 16);
   if (joined > kJoinTokens) joined = kJoinTokens;
-  const int64_t lists = kJoinMost / (kAttendWaves * (count > 0 ? count : 1));
+  const int64_t lists = kJoinMost / (kJoinWaves * (count > 0 ? count : 1));
   p.joined = static_cast<int32_t>(joined < lists ? joined : lists);
   if (p.rows >= 4096) return p;
   // workgroups of four waves for two on every CU, each wave with a unit of 64 keys at least
@@ -874,7 +903,9 @@ extern "C" int rt_kv_attention(const void* q, int64_t q_token_stride, int64_t q_
   a.count = static_cast<int32_t>(count);
   a.tok = {positions, seq_ids, page_table, static_cast<int32_t>(B),
            static_cast<int32_t>(max_pages), static_cast<int32_t>(P), kv_shift(page)};
-  a.scale = scale * kLog2e, a.out = out, a.lse = lse, a.parts = plan.parts;
+  // (a scale of 0 becomes the least number: the scores are 0 all the same, and -inf stays -inf)
+  a.scale = fmaxf(fabsf(scale * kLog2e), 1.17549435e-38f), a.minus = scale < 0.0f;
+  a.out = out, a.lse = lse, a.parts = plan.parts;
   a.joined = plan.joined;
   a.part_out = static_cast<float*>(workspace);
   a.part_ml = a.part_out + (plan.parts > 1 ? plan.rows * plan.parts * 16 * D : 0);
@@ -884,8 +915,9 @@ extern "C" int rt_kv_attention(const void* q, int64_t q_token_stride, int64_t q_
     constexpr int DD = decltype(d)::value;
     const dim3 threads(kAttendWaves * kWave);
     if (plan.parts == 0 && plan.joined > 1) {
-      const int64_t grid = cdiv(T, kAttendWaves * plan.joined) * Hkv;
-      kv_attend_joined_kernel<E, DD><<<dim3(static_cast<unsigned>(grid)), threads, 0, s>>>(a);
+      const int64_t grid = cdiv(T, kJoinWaves * plan.joined) * Hkv;
+      kv_attend_joined_kernel<E, DD>
+          <<<dim3(static_cast<unsigned>(grid)), dim3(kJoinWaves * kWave), 0, s>>>(a);
     } else if (plan.parts == 0) {
       const int64_t grid = cdiv(T, kAttendWaves) * Hkv * plan.tiles;
       kv_attend_rows_kernel<E, DD><<<dim3(static_cast<unsigned>(grid)), threads, 0, s>>>(a);
