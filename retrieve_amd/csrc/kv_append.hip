@@ -11,10 +11,11 @@
 // most that any key of the block can score with q. Minimum and maximum do not depend on the
 // order, so the codes are the same in any split.
 //
-// One launch. The first workgroups move rows: a lane holds one 16-byte chunk (8 channels) of a
-// token's rows and its cosines and sines, and walks over heads. The others look for tokens
-// that complete a block: the block's keys that are part of this call are rotated again from the
-// input (no wait on the workgroups that store them), the earlier ones come from the cache.
+// One launch. Some workgroups look for tokens that complete a block: the block's keys that are part
+// of this call are rotated again from the input (no wait on the waves that store them), the
+// earlier ones come from the cache. In the others a wave moves a token's rows (or some of them, where
+// there are few tokens): a lane holds two 16-byte chunks of a row, which in the split layout are
+// partners, with their cosines and sines, and walks over the heads, several rows in flight.
 #include <type_traits>
 
 #include "../../include/retrieve_amd.h"
@@ -36,9 +37,9 @@ struct AppendArgs {
   int8_t* bounds;
   float* scales;
   void* q_out;
-  int32_t head_groups;  // workgroups a token's rows are split over
-  int64_t row_groups;   // workgroups that move rows
-  int32_t tile;         // tokens a bounds workgroup looks at
+  int32_t row_parts;      // waves a token's rows are split over
+  uint32_t bound_groups;  // workgroups that look for full blocks
+  int32_t tile;           // tokens that one of them looks at
 };
 
 // How channel i meets its partner: halves of the rotated part with every half on whole chunks,
@@ -75,6 +76,16 @@ struct Turn {
       }
       return;
     }
+    if (MODE == kRotPairs && a.rot % 8 == 0 && 8 * chunk < a.rot) {
+      const v4f cv = *reinterpret_cast<const v4f*>(row + 4 * chunk);
+      const v4f sv = *reinterpret_cast<const v4f*>(row + half + 4 * chunk);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        c[e] = cv[e >> 1];
+        s[e] = sv[e >> 1];
+      }
+      return;
+    }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int i = 8 * chunk + e;
@@ -85,12 +96,11 @@ struct Turn {
   }
 };
 
-// Chunk `chunk` of a row after the rotation.
+// Chunk `chunk` of a row, read as x, after the rotation.
 template <class E, int MODE>
-__device__ inline typename Kv<E>::V8 rotated(const E* row, int chunk, const Turn<MODE>& t,
-                                             int rot) {
+__device__ inline typename Kv<E>::V8 rotated_chunk(const E* row, typename Kv<E>::V8 x, int chunk,
+                                                   const Turn<MODE>& t, int rot) {
   using V8 = typename Kv<E>::V8;
-  const V8 x = *reinterpret_cast<const V8*>(row + 8 * chunk);
   if (8 * chunk >= rot) return x;
   const int half = rot >> 1;
   V8 y;
@@ -126,39 +136,94 @@ __device__ inline int64_t cache_row(const AppendArgs& a, int32_t page, int head,
   return ((block << a.tok.shift) + (pos & ((1 << a.tok.shift) - 1))) * D;
 }
 
+// A lane's two chunks of a row and what turns them. Split halves: partners in the rotated part,
+// neighbours' distance apart in the rest; otherwise the same place in either half of the row.
 template <class E, int D, int MODE>
-__device__ inline void move_rows(const AppendArgs& a) {
+struct Pair {
   using V8 = typename Kv<E>::V8;
-  constexpr int C = D / 8, SLOTS = kAppendThreads / C;
-  const int chunk = threadIdx.x % C, slot = threadIdx.x / C;
-  const int64_t t = blockIdx.x / a.head_groups;
-  const int group = blockIdx.x % a.head_groups;
-  if (slot >= SLOTS) return;
+  static constexpr int C = D / 16;
+  int chunk[2];
+  Turn<MODE> turn[MODE == kRotHalf ? 1 : 2];
+  bool turned;  // split halves: in the rotated part
+
+  __device__ Pair(const AppendArgs& a, int lane) {
+    const int r = a.rot / 16;
+    turned = lane < r;
+    if (MODE == kRotHalf) {
+      chunk[0] = turned ? lane : lane + r;
+      chunk[1] = turned ? lane + r : lane + C;
+    } else {
+      chunk[0] = lane;
+      chunk[1] = lane + C;
+    }
+  }
+  __device__ void load(const AppendArgs& a, int32_t pos) {
+    turn[0].load(a, pos, chunk[0]);
+    if constexpr (MODE != kRotHalf) turn[1].load(a, pos, chunk[1]);
+  }
+  // x: the two chunks as read; `row` for partners elsewhere
+  __device__ void rotate(const E* row, int rot, V8 (&x)[2]) const {
+    if constexpr (MODE == kRotHalf) {
+      if (!turned) return;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float f = static_cast<float>(x[0][e]), s = static_cast<float>(x[1][e]);
+        x[0][e] = static_cast<E>(rot_first(f, s, turn[0].c[e], turn[0].s[e]));
+        x[1][e] = static_cast<E>(rot_second(s, f, turn[0].c[e], turn[0].s[e]));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) x[i] = rotated_chunk<E, MODE>(row, x[i], chunk[i], turn[i], rot);
+    }
+  }
+};
+
+template <class E, int D, int MODE>
+__device__ inline void move_rows(const AppendArgs& a, int64_t unit) {
+  using V8 = typename Kv<E>::V8;
+  constexpr int C = D / 16, SLOTS = kWave / C, FLIGHT = 4;
+  const int lane = lane_id() % C, slot = lane_id() / C;
+  const int64_t t = unit / a.row_parts;
+  if (t >= a.T || slot >= SLOTS) return;
   const KvPlace p = kv_place(a.tok, t);
   const int32_t page = p.last >= 0 ? kv_page(a.tok, p, p.last) : -1;
   const bool valid = page >= 0 && (a.rot == 0 || p.pos < a.table_len);
-  Turn<MODE> turn;
-  if (valid && a.rot > 0) turn.load(a, p.pos, chunk);
-  const int rows = a.Hq + 2 * a.Hkv;
-  for (int r = group * SLOTS + slot; r < rows; r += a.head_groups * SLOTS) {
-    if (r < a.Hq) {
-      V8 out = {};
-      if (valid) {
-        out = rotated<E, MODE>(static_cast<const E*>(a.q) + t * a.q_st + r * a.q_sh, chunk, turn,
-                               a.rot);
+  Pair<E, D, MODE> pair(a, lane);
+  if (valid && a.rot > 0) pair.load(a, p.pos);
+  const int rows = a.Hq + 2 * a.Hkv, step = a.row_parts * SLOTS;
+  const E* q = static_cast<const E*>(a.q) + t * a.q_st;
+  const E* k = static_cast<const E*>(a.k) + t * a.k_st;
+  const E* v = static_cast<const E*>(a.v) + t * a.v_st;
+  E* to_q = static_cast<E*>(a.q_out) + t * a.Hq * D;
+  const int64_t at = valid ? cache_row<D>(a, page, 0, p.pos) : 0;
+  const int64_t head = static_cast<int64_t>(D) << a.tok.shift;  // from head to head of a page
+  for (int r0 = static_cast<int>(unit % a.row_parts) * SLOTS + slot; r0 < rows;
+       r0 += FLIGHT * step) {
+    V8 x[FLIGHT][2];
+    const E* from[FLIGHT];
+#pragma unroll
+    for (int i = 0; i < FLIGHT; ++i) {
+      const int r = r0 + i * step;
+      from[i] = r < a.Hq           ? q + r * a.q_sh
+                : r < a.Hq + a.Hkv ? k + (r - a.Hq) * a.k_sh
+                                   : v + (r - a.Hq - a.Hkv) * a.v_sh;
+      x[i][0] = V8{};
+      x[i][1] = V8{};
+      if (valid && r < rows) {
+        x[i][0] = __builtin_nontemporal_load(reinterpret_cast<const V8*>(from[i]) + pair.chunk[0]);
+        x[i][1] = __builtin_nontemporal_load(reinterpret_cast<const V8*>(from[i]) + pair.chunk[1]);
       }
-      *reinterpret_cast<V8*>(static_cast<E*>(a.q_out) + (t * a.Hq + r) * D + 8 * chunk) = out;
-    } else if (valid && r < a.Hq + a.Hkv) {
-      const int h = r - a.Hq;
-      *reinterpret_cast<V8*>(static_cast<E*>(a.k_cache) + cache_row<D>(a, page, h, p.pos) +
-                             8 * chunk) =
-          rotated<E, MODE>(static_cast<const E*>(a.k) + t * a.k_st + h * a.k_sh, chunk, turn, a.rot);
-    } else if (valid) {
-      const int h = r - a.Hq - a.Hkv;
-      *reinterpret_cast<V8*>(static_cast<E*>(a.v_cache) + cache_row<D>(a, page, h, p.pos) +
-                             8 * chunk) =
-          *reinterpret_cast<const V8*>(static_cast<const E*>(a.v) + t * a.v_st + h * a.v_sh +
-                                       8 * chunk);
+    }
+#pragma unroll
+    for (int i = 0; i < FLIGHT; ++i) {
+      const int r = r0 + i * step;
+      if (r >= rows || (r >= a.Hq && !valid)) continue;
+      if (valid && r < a.Hq + a.Hkv && a.rot > 0) pair.rotate(from[i], a.rot, x[i]);
+      E* to = r < a.Hq           ? to_q + r * D
+              : r < a.Hq + a.Hkv ? static_cast<E*>(a.k_cache) + at + (r - a.Hq) * head
+                                 : static_cast<E*>(a.v_cache) + at + (r - a.Hq - a.Hkv) * head;
+      reinterpret_cast<V8*>(to)[pair.chunk[0]] = x[i][0];
+      reinterpret_cast<V8*>(to)[pair.chunk[1]] = x[i][1];
     }
   }
 }
@@ -169,17 +234,23 @@ __device__ inline void fill_bounds(const AppendArgs& a) {
   constexpr int C = D / 8, SLOTS = kAppendThreads / C;
   __shared__ float lows[SLOTS][D], highs[SLOTS][D];
   __shared__ float tops[kAppendThreads / kWave];
-  const int64_t wg = blockIdx.x - a.row_groups;
-  const int head = static_cast<int>(wg % a.Hkv);
-  const int64_t t0 = wg / a.Hkv * a.tile;
+  const int head = static_cast<int>(blockIdx.x % a.Hkv);
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x / a.Hkv) * a.tile;
   const int size = 1 << a.tok.shift;
   const int chunk = threadIdx.x % C, slot = threadIdx.x / C;
   const E* k = static_cast<const E*>(a.k) + head * a.k_sh;
-  for (int64_t t = t0; t < t0 + a.tile && t < a.T; ++t) {
-    const KvPlace p = kv_place(a.tok, t);  // (the same for the whole workgroup)
-    if (p.last < 0 || (p.pos & (size - 1)) != size - 1) continue;
+  // which of the tile's tokens complete a block: one a lane (the same in every wave)
+  const int64_t mine = t0 + lane_id();
+  bool full = false;
+  if (lane_id() < a.tile && mine < a.T) {
+    const KvPlace p = kv_place(a.tok, mine);
+    full = p.last >= 0 && (p.pos & (size - 1)) == size - 1 && kv_page(a.tok, p, p.last) >= 0 &&
+           (a.rot == 0 || p.pos < a.table_len);
+  }
+  for (uint64_t left = __ballot(full); left != 0; left &= left - 1) {
+    const int64_t t = t0 + __builtin_ctzll(left);
+    const KvPlace p = kv_place(a.tok, t);
     const int32_t page = kv_page(a.tok, p, p.last);
-    if (page < 0 || (a.rot > 0 && p.pos >= a.table_len)) continue;
     const int32_t seq = a.tok.seq_ids[t];
     float lo[8], hi[8];
 #pragma unroll
@@ -195,7 +266,8 @@ __device__ inline void fill_bounds(const AppendArgs& a) {
         if (from >= 0 && a.tok.positions[from] == pos && a.tok.seq_ids[from] == seq) {
           Turn<MODE> turn;
           if (a.rot > 0) turn.load(a, pos, chunk);
-          x = rotated<E, MODE>(k + from * a.k_st, chunk, turn, a.rot);
+          const E* row = k + from * a.k_st;
+          x = rotated_chunk<E, MODE>(row, reinterpret_cast<const V8*>(row)[chunk], chunk, turn, a.rot);
         } else {
           x = *reinterpret_cast<const V8*>(static_cast<const E*>(a.k_cache) +
                                            cache_row<D>(a, page, head, pos) + 8 * chunk);
@@ -242,10 +314,12 @@ __device__ inline void fill_bounds(const AppendArgs& a) {
 
 template <class E, int D, int MODE>
 __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(AppendArgs a) {
-  if (blockIdx.x < a.row_groups) {
-    move_rows<E, D, MODE>(a);
-  } else {
+  if (blockIdx.x < a.bound_groups) {
     fill_bounds<E, D, MODE>(a);
+  } else {
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+    move_rows<E, D, MODE>(
+        a, (blockIdx.x - a.bound_groups) * (kAppendThreads / kWave) + wave);
   }
 }
 
@@ -289,16 +363,20 @@ extern "C" int rt_kv_append(const void* q, int64_t q_token_stride, int64_t q_hea
            static_cast<int32_t>(max_pages), static_cast<int32_t>(P), kv_shift(page)};
   a.k_cache = k_cache, a.v_cache = v_cache, a.bounds = bounds, a.scales = bound_scales;
   a.q_out = q_out;
-  const int slots = static_cast<int>(kAppendThreads / (D / 8));
+  const int slots = static_cast<int>(kWave / (D / 16));
   const int64_t all = cdiv(Hq + 2 * Hkv, slots);
-  // Few tokens: every pass over a token's heads a workgroup of its own. Many: one workgroup a token.
-  a.head_groups = static_cast<int32_t>(T * all <= 4096 ? all : 1);
-  a.row_groups = T * a.head_groups;
-  // Few tokens may all complete a block in one step (sequences of one length): one workgroup a
-  // token and head. In prompts one in `page` does.
-  a.tile = T * Hkv <= 4096 ? 1 : 64;
-  const int64_t grid = a.row_groups + cdiv(T, a.tile) * Hkv;
+  // Few tokens: a token's rows over as many waves as have one each. Many: one wave a token.
+  const int64_t parts = cdiv(4096, T);
+  a.row_parts = static_cast<int32_t>(parts < all ? parts : all);
+  // Few tokens may all complete a block in one step (sequences of one length): a workgroup for each
+  // and every head, up to 1024 of them (more would cost their launch). In prompts one token in
+  // `page` does: 64 tokens a workgroup.
+  const int64_t tile = next_pow2(cdiv(T * Hkv, 1024));
+  a.tile = static_cast<int32_t>(tile < 64 ? tile : 64);
+  const int64_t bound_groups = cdiv(T, a.tile) * Hkv;
+  const int64_t grid = bound_groups + cdiv(T * a.row_parts, kAppendThreads / kWave);
   RT_CHECK_ARG(grid <= INT32_MAX, "too many tokens");
+  a.bound_groups = static_cast<uint32_t>(bound_groups);
   const int mode = interleaved ? kRotPairs : rot % 16 == 0 ? kRotHalf : kRotHalfOdd;
   return kv_dispatch(dtype, D, [&](auto e, auto d) -> int {
     using E = decltype(e);
