@@ -230,6 +230,7 @@ struct AttendWave {
   template <int N>
   __device__ void weigh(float scale, v4f (&sc)[N], bool whole, const int (&n)[N],
                         V8 (&p)[N / 2]) {
+    settle(sc);
     if (!whole) {
       const int at = 4 * (lane_id() >> 4);
 #pragma unroll

@@ -64,6 +64,36 @@ __device__ inline int kv_code(float x, float top) {
   return static_cast<int>(fminf(fmaxf(v, -127.0f), 127.0f));
 }
 
+// The same code by a reciprocal r = 1 / top (rounded to nearest): q = x r, then q + r (x - q top) is the
+// quotient rounded to nearest wherever |x| <= top, top is normal and its significand is not all
+// ones (Markstein's theorem; queries of 16 bits have neither), in 3 instructions instead of about
+// ten. For a top above 2^100, whose reciprocal may lose bits, x and top come in scaled by 2^-64.
+__device__ inline float kv_code_value(float x, float top, float r) {
+#pragma clang fp contract(off)
+  const float q = x * r;
+  const float quotient = __builtin_fmaf(__builtin_fmaf(-q, top, x), r, q);
+  return fmaxf(rintf(quotient * 127.0f), -127.0f);  // (NaN: -127)
+}
+
+// Eight wait states behind matrix products, before x is read. The compiler counts them itself within a
+// block, but not where a branch comes between a product and its first use: the path that takes
+// the branch then reads the old registers.
+template <class V, int N>
+__device__ inline void settle(V (&x)[N]) {
+  if constexpr (N == 1) {
+    asm volatile("s_nop 7" : "+v"(x[0]));
+  } else if constexpr (N == 2) {
+    asm volatile("s_nop 7" : "+v"(x[0]), "+v"(x[1]));
+  } else if constexpr (N == 4) {
+    asm volatile("s_nop 7" : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]));
+  } else {
+    static_assert(N == 8, "1, 2, 4 or 8 results");
+    asm volatile("s_nop 7"
+                 : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]), "+v"(x[4]), "+v"(x[5]),
+                   "+v"(x[6]), "+v"(x[7]));
+  }
+}
+
 // Host: the checks every entry point makes of the shared arguments.
 inline int kv_check(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int dtype, int64_t B,
                     int64_t max_pages, int64_t P, int64_t page) {

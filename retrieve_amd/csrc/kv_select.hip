@@ -6,13 +6,18 @@
 // 2 * 256 * 127^2 < 2^23, so exact as fp32 too); the two products are rounded once each, in this
 // order, and rounding is monotone, so the largest over the heads is taken before the block's scale.
 //
-// Two launches. Scores: [blocks x columns] = bounds [c | |c|]^T on the int8 matrix cores, 16 blocks
-// by 16 columns an instruction, a column being one query head of one token; the columns stay in
-// registers (quantised there by the wave that needs them), the bounds come from memory in the
-// operand's layout with a chunk of 64 blocks in flight; the largest of a token's neighbouring
-// columns by lane exchange, then one key a (token, head, block). Keep: the cut by bisection over the
-// keys' bits, from the highest bit in which they differ until the count is exact, then the kept
-// blocks in order.
+// Two launches.
+//
+// Scores: [blocks x columns] = bounds [c | |c|]^T on the int8 matrix cores, 16 blocks by 16 columns
+// an instruction; the columns stay in registers (quantised by the wave that needs them), the bounds
+// come from memory in the operand's layout. Decode: a column is a query head of the wave's one
+// token, the largest of them found by lane exchange. Prompts: a column is a token, a tile one
+// head of 16 tokens, the largest over the heads found within the lane; the tokens of one sequence
+// share the pass over its blocks. One key a (token, head, block) is left behind.
+//
+// Keep: few blocks by a wave, which bisects over the keys' bits from the highest in which they differ
+// until the count is exact. Many by a workgroup: the want-th largest of the lanes' largest keys is
+// a bound that at least `want` keys reach and few more; those are ranked against each other.
 #include <type_traits>
 
 #include "../../include/retrieve_amd.h"
@@ -35,9 +40,7 @@ struct SelectArgs {
   int32_t* out;       // [T, Hkv, count]
   uint32_t* keys;     // [T * Hkv, stride]
   int64_t stride;
-  int32_t cols;       // columns of a token in a tile of 16: a power of two
-  int32_t per_wave;   // tokens a wave holds
-  int32_t splits;     // waves that share a token tile's blocks
+  int32_t splits;     // waves that share a wave's tokens' blocks
   int32_t head_groups;
 };
 
@@ -46,241 +49,19 @@ __device__ inline uint32_t score_key(float s) {
   return key_of_f32(s == s ? s : -INFINITY);
 }
 
-// The largest over aligned groups of `n` lanes (a power of two up to 16), in every lane.
-__device__ inline float group_max(float x, int n) {
+// The largest over aligned groups of 16 lanes, in every lane.
+__device__ inline float group_max16(float x) {
   auto step = [&](auto ctrl) {
     const int y = __builtin_amdgcn_update_dpp(0, __float_as_int(x), decltype(ctrl)::value, 0xf, 0xf,
                                               true);
     x = fmaxf(x, __int_as_float(y));
   };
-  if (n > 1) step(std::integral_constant<int, 0xB1>{});   // lane ^ 1
-  if (n > 2) step(std::integral_constant<int, 0x4E>{});   // lane ^ 2
-  if (n > 4) step(std::integral_constant<int, 0x141>{});  // the other four of eight
-  if (n > 8) step(std::integral_constant<int, 0x140>{});  // the other eight of sixteen
+  step(std::integral_constant<int, 0xB1>{});   // lane ^ 1
+  step(std::integral_constant<int, 0x4E>{});   // lane ^ 2
+  step(std::integral_constant<int, 0x141>{});  // the other four of eight
+  step(std::integral_constant<int, 0x140>{});  // the other eight of sixteen
   return x;
 }
-
-// A wave holds NT tiles of 16 columns: `per_wave` tokens of `cols` columns each (heads past the
-// group's repeat its last), or one token of 16 NT heads, its further heads in later passes. The
-// tokens of one sequence share a pass over its blocks.
-template <class E, int D, int NT>
-__global__ void __launch_bounds__(kScoreWaves* kWave, D == 256 && NT == 2 ? 1 : 2)
-    kv_score_kernel(SelectArgs a) {
-  using V8 = typename Kv<E>::V8;
-  constexpr int KS = D / 32;  // steps of 64 of a row's 2 D bytes
-  __shared__ __attribute__((aligned(16))) int32_t pages[kScoreWaves][2][kChunk];
-  __shared__ __attribute__((aligned(16))) float block_scales[kScoreWaves][2][kChunk];
-  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
-  const int lane = lane_id(), col = lane & 15, grp = lane >> 4;
-  const int head = static_cast<int>(blockIdx.x % a.head_groups) * kScoreWaves + wave;
-  if (head >= a.Hkv) return;
-  const int split = static_cast<int>(blockIdx.x / a.head_groups % a.splits);
-  const int64_t t0 = static_cast<int64_t>(blockIdx.x / a.head_groups / a.splits) * a.per_wave;
-  const bool wide = a.G > 16;
-  const int passes = wide ? (a.G + 16 * NT - 1) / (16 * NT) : 1;
-
-  // the lane's token in each tile, and where its candidates end (0: none)
-  int64_t token[NT];
-  int32_t seq[NT], end[NT];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int i = wide ? 0 : (n * 16 + col) / a.cols;
-    token[n] = t0 + i;
-    end[n] = 0;
-    seq[n] = -1;
-    if (i < a.per_wave && token[n] < a.T) {
-      const KvPlace p = kv_place(a.tok, token[n]);
-      const int32_t e = p.last - a.recent + 1;
-      if (p.last >= 0 && e > a.sink) {
-        end[n] = e;
-        seq[n] = a.tok.seq_ids[token[n]];
-      }
-    }
-  }
-  bool any = false;
-#pragma unroll
-  for (int n = 0; n < NT; ++n) any |= end[n] > 0;
-  if (!__any(any)) return;
-
-  for (int pass = 0; pass < passes; ++pass) {
-    // columns: bytes [64 s + 16 grp, +16) of [c | |c|]
-    v4i cf[NT][KS];
-    float scale[NT];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      int g = wide ? (pass * NT + n) * 16 + col : col & (a.cols - 1);
-      if (g >= a.G) g = a.G - 1;
-      const int64_t t = end[n] > 0 ? token[n] : t0;
-      const E* q = static_cast<const E*>(a.q) + t * a.q_st +
-                   static_cast<int64_t>(head * a.G + g) * a.q_sh;
-      constexpr int LOADS = D % 64 == 0 ? KS / 2 : KS;
-      V8 x[LOADS][2];
-      float top = 0.0f;
-#pragma unroll
-      for (int s = 0; s < LOADS; ++s) {
-        const int at = 64 * s + 16 * grp, d = at < D ? at : at - D;
-        x[s][0] = *reinterpret_cast<const V8*>(q + d);
-        x[s][1] = *reinterpret_cast<const V8*>(q + d + 8);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(static_cast<float>(x[s][e >> 3][e & 7])));
-      }
-      top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaxf(top, __shfl_xor(top, 32));
-      top = fmaxf(top, kKvTopFloor);
-      scale[n] = top / 127.0f;
-#pragma unroll
-      for (int s = 0; s < LOADS; ++s) {
-        const bool size = 64 * s + 16 * grp >= D;
-        v4i codes, sizes;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          uint32_t c4 = 0, s4 = 0;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int i = 4 * w + e;
-            const int c = kv_code(static_cast<float>(x[s][i >> 3][i & 7]), top);
-            c4 |= static_cast<uint32_t>(c & 255) << (8 * e);
-            s4 |= static_cast<uint32_t>(c < 0 ? -c : c) << (8 * e);
-          }
-          codes[w] = static_cast<int>(c4);
-          sizes[w] = static_cast<int>(s4);
-        }
-        if constexpr (D % 64 == 0) {
-          cf[n][s] = codes;
-          cf[n][s + LOADS] = sizes;
-        } else {
-          cf[n][s] = size ? sizes : codes;
-        }
-      }
-    }
-
-    bool todo[NT];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) todo[n] = end[n] > 0;
-    for (;;) {  // the sequences among the tokens
-      int32_t of = -1;
-#pragma unroll
-      for (int n = NT - 1; n >= 0; --n) {
-        const uint64_t m = __ballot(todo[n]);
-        if (m != 0) {
-          const int l = __builtin_ctzll(m);
-          of = __builtin_amdgcn_readlane(seq[n], l);
-        }
-      }
-      if (of < 0) break;
-      int32_t last = 0;
-      bool mine[NT];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        mine[n] = todo[n] && seq[n] == of;
-        todo[n] = todo[n] && !mine[n];
-        if (mine[n] && end[n] > last) last = end[n];
-      }
-      for (int i = 1; i < kWave; i <<= 1) {
-        const int32_t o = __shfl_xor(last, i);
-        last = o > last ? o : last;
-      }
-      last = __builtin_amdgcn_readfirstlane(last);
-      const int32_t* row = a.tok.page_table + static_cast<int64_t>(of) * a.tok.max_pages;
-
-      auto look_up = [&](int64_t chunk) {
-        const int64_t b = chunk * kChunk + lane;
-        if (b >= last) return -1;
-        const int32_t p = row[b];
-        return p >= 0 && p < a.tok.P ? p : -1;
-      };
-      auto scale_of = [&](int32_t page) {
-        return page >= 0 ? a.scales[static_cast<int64_t>(page) * a.Hkv + head] : 0.0f;
-      };
-      v4i bf[4][KS];
-      auto load_tile = [&](int buf, int tile) {
-        const int32_t p = pages[wave][buf][16 * tile + col];
-        const int8_t* from = a.bounds +
-                             (static_cast<int64_t>(p < 0 ? 0 : p) * a.Hkv + head) * (2 * D) +
-                             16 * grp;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          bf[tile][s] = p < 0 ? v4i{0, 0, 0, 0} : *reinterpret_cast<const v4i*>(from + 64 * s);
-        }
-      };
-
-      int64_t chunk = a.sink / kChunk + split;
-      const int64_t stop = cdiv(last, kChunk);
-      if (chunk >= stop) continue;
-      int buf = 0;
-      int32_t page = look_up(chunk), page_next = look_up(chunk + a.splits);
-      pages[wave][0][lane] = page;
-      block_scales[wave][0][lane] = scale_of(page);
-      asm volatile("" ::: "memory");  // (read by other lanes of this wave)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) load_tile(0, i);
-      for (; chunk < stop; chunk += a.splits, buf ^= 1) {
-        const bool more = chunk + a.splits < stop;
-        float next_scale = 0.0f;
-        if (more) {
-          pages[wave][buf ^ 1][lane] = page_next;
-          next_scale = scale_of(page_next);
-          page_next = look_up(chunk + 2 * static_cast<int64_t>(a.splits));
-        }
-        asm volatile("" ::: "memory");
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          v4i acc[NT];
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            acc[n] = v4i{0, 0, 0, 0};
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-              acc[n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bf[i][s], cf[n][s], acc[n], 0, 0, 0);
-            }
-          }
-          if (more) load_tile(buf ^ 1, i);
-          const v4i pg = *reinterpret_cast<const v4i*>(&pages[wave][buf][16 * i + 4 * grp]);
-          const v4f bs = *reinterpret_cast<const v4f*>(&block_scales[wave][buf][16 * i + 4 * grp]);
-          const int64_t b = chunk * kChunk + 16 * i + 4 * grp;
-          float best[NT][4];
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) best[n][r] = static_cast<float>(acc[n][r]) * scale[n];
-          }
-          if (wide) {
-#pragma unroll
-            for (int n = 1; n < NT; ++n) {
-#pragma unroll
-              for (int r = 0; r < 4; ++r) best[0][r] = fmaxf(best[0][r], best[n][r]);
-            }
-          }
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            if (wide && n > 0) break;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) best[n][r] = group_max(best[n][r], wide ? 16 : a.cols);
-            if (!mine[n] || (wide ? col != 0 : (col & (a.cols - 1)) != 0)) continue;
-            v4i* to = reinterpret_cast<v4i*>(a.keys + (token[n] * a.Hkv + head) * a.stride + b);
-            if (pass > 0) {
-              const v4i old = *to;
-#pragma unroll
-              for (int r = 0; r < 4; ++r) best[n][r] = fmaxf(best[n][r], __int_as_float(old[r]));
-            }
-            v4i key;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              key[r] = pass + 1 < passes ? __float_as_int(best[n][r])
-                       : pg[r] < 0       ? 0
-                                         : static_cast<int>(score_key(best[n][r] * bs[r]));
-            }
-            *to = key;
-          }
-        }
-        if (more) block_scales[wave][buf ^ 1][lane] = next_scale;
-        asm volatile("" ::: "memory");
-      }
-    }
-  }
-}
-
-// --- keep ---------------------------------------------------------------------------------------
 
 // The largest (or least) over the wave, in every lane.
 template <bool MAX>
@@ -300,15 +81,280 @@ __device__ inline uint32_t wave_extreme(uint32_t x) {
   return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(x), 63));
 }
 
-// Candidates of a row as a wave or a workgroup of WAVES waves holds them: R keys a lane, in block
-// order (a wave has 64 R neighbours). R = 0: any number, read again where they are needed.
+// 16 channels of a query row as codes (or their sizes): the bytes of one operand step.
+template <class V8>
+__device__ inline void pack_codes(const V8 (&x)[2], float top, float r, float small, v4i& codes,
+                                  v4i& sizes) {
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    uint32_t c4 = 0, s4 = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int i = 4 * w + e;
+      const float v = kv_code_value(static_cast<float>(x[i >> 3][i & 7]) * small, top, r);
+      c4 = __builtin_amdgcn_cvt_pk_u8_f32(v + 128.0f, e, c4);
+      s4 = __builtin_amdgcn_cvt_pk_u8_f32(fabsf(v), e, s4);
+    }
+    codes[w] = static_cast<int>(c4 ^ 0x80808080u);
+    sizes[w] = static_cast<int>(s4);
+  }
+}
+
+// A wave holds NT tiles of 16 columns. GH = 0 (decode): one token, column = query head, 16 NT heads a
+// pass. GH > 0 (prompts): column = token, tile n = head n % GH of token group n / GH, GH heads a
+// pass (heads past the group's repeat its last).
+template <class E, int D, int NT, int GH>
+__global__ void __launch_bounds__(kScoreWaves* kWave, D > 128 && NT == 4 ? 1 : 2)
+    kv_score_kernel(SelectArgs a) {
+  using V8 = typename Kv<E>::V8;
+  constexpr int KS = D / 32;  // steps of 64 of a row's 2 D bytes
+  constexpr int TG = GH > 0 ? NT / GH : 1, HEADS = GH > 0 ? GH : 16 * NT;
+  constexpr int FLIGHT = D * NT > 512 || D > 128 ? 2 : 4;  // tiles of bounds in flight
+  __shared__ __attribute__((aligned(16))) int32_t pages[kScoreWaves][2][kChunk];
+  __shared__ __attribute__((aligned(16))) float block_scales[kScoreWaves][2][kChunk];
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int lane = lane_id(), col = lane & 15, grp = lane >> 4;
+  const int head = static_cast<int>(blockIdx.x % a.head_groups) * kScoreWaves + wave;
+  if (head >= a.Hkv) return;
+  const int split = static_cast<int>(blockIdx.x / a.head_groups % a.splits);
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x / a.head_groups / a.splits) *
+                     (GH > 0 ? 16 * TG : 1);
+  const int passes = (a.G + HEADS - 1) / HEADS;
+
+  // the lane's token of each group, and where its candidates end (0: none)
+  int64_t token[TG];
+  int32_t seq[TG], end[TG];
+  bool any = false;
+#pragma unroll
+  for (int g = 0; g < TG; ++g) {
+    token[g] = t0 + (GH > 0 ? 16 * g + col : 0);
+    end[g] = 0;
+    seq[g] = -1;
+    if (token[g] < a.T) {
+      const KvPlace p = kv_place(a.tok, token[g]);
+      const int32_t e = p.last - a.recent + 1;
+      if (p.last >= 0 && e > a.sink) {
+        end[g] = e;
+        seq[g] = a.tok.seq_ids[token[g]];
+      }
+    }
+    any |= end[g] > 0;
+  }
+  if (!__any(any)) return;
+
+  for (int pass = 0; pass < passes; ++pass) {
+    // columns: bytes [64 s + 16 grp, +16) of [c | |c|]
+    v4i cf[NT][KS];
+    float scale[NT];
+    auto quantise = [&]() {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        int h = GH > 0 ? pass * GH + n % GH : (pass * NT + n) * 16 + col;
+        if (h >= a.G) h = a.G - 1;
+        const int g = GH > 0 ? n / GH : 0;
+        const E* q = static_cast<const E*>(a.q) + (end[g] > 0 ? token[g] : t0) * a.q_st +
+                     static_cast<int64_t>(head * a.G + h) * a.q_sh;
+        constexpr int LOADS = D % 64 == 0 ? KS / 2 : KS;
+        V8 x[LOADS][2];
+        float top = 0.0f;
+#pragma unroll
+        for (int s = 0; s < LOADS; ++s) {
+          const int at = 64 * s + 16 * grp, d = at < D ? at : at - D;
+          x[s][0] = *reinterpret_cast<const V8*>(q + d);
+          x[s][1] = *reinterpret_cast<const V8*>(q + d + 8);
+        }
+#pragma unroll
+        for (int s = 0; s < LOADS; ++s) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            top = fmaxf(top, fabsf(static_cast<float>(x[s][e >> 3][e & 7])));
+          }
+        }
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        top = fmaxf(top, kKvTopFloor);
+        scale[n] = top / 127.0f;
+        const float small = top > 0x1p100f ? 0x1p-64f : 1.0f;
+        top *= small;
+        const float r = 1.0f / top;
+#pragma unroll
+        for (int s = 0; s < LOADS; ++s) {
+          v4i codes, sizes;
+          pack_codes(x[s], top, r, small, codes, sizes);
+          if constexpr (D % 64 == 0) {
+            cf[n][s] = codes;
+            cf[n][s + LOADS] = sizes;
+          } else {
+            const bool second = 64 * s + 16 * grp >= D;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) cf[n][s][w] = second ? sizes[w] : codes[w];
+          }
+        }
+      }
+    };
+    bool quantised = false;
+    bool todo[TG];
+#pragma unroll
+    for (int g = 0; g < TG; ++g) todo[g] = end[g] > 0;
+    for (;;) {  // the sequences among the tokens
+      int32_t of = -1;
+#pragma unroll
+      for (int g = TG - 1; g >= 0; --g) {
+        const uint64_t m = __ballot(todo[g]);
+        if (m != 0) of = __builtin_amdgcn_readlane(seq[g], __builtin_ctzll(m));
+      }
+      if (of < 0) break;
+      int32_t last = 0;
+      bool mine[TG];
+#pragma unroll
+      for (int g = 0; g < TG; ++g) {
+        mine[g] = todo[g] && seq[g] == of;
+        todo[g] = todo[g] && !mine[g];
+        if (mine[g] && end[g] > last) last = end[g];
+      }
+      last = static_cast<int32_t>(wave_extreme<true>(static_cast<uint32_t>(last)));
+      const int32_t* row = a.tok.page_table + static_cast<int64_t>(of) * a.tok.max_pages;
+
+      auto look_up = [&](int64_t chunk) {
+        const int64_t b = chunk * kChunk + lane;
+        if (b >= last) return -1;
+        const int32_t p = row[b];
+        return p >= 0 && p < a.tok.P ? p : -1;
+      };
+      auto scale_of = [&](int32_t page) {
+        return page >= 0 ? a.scales[static_cast<int64_t>(page) * a.Hkv + head] : 0.0f;
+      };
+      v4i bf[FLIGHT][KS];
+      auto load_tile = [&](int buf, int tile) {
+        const int32_t p = pages[wave][buf][16 * tile + col];
+        const int8_t* from = a.bounds +
+                             (static_cast<int64_t>(p < 0 ? 0 : p) * a.Hkv + head) * (2 * D) +
+                             16 * grp;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          bf[tile % FLIGHT][s] = *reinterpret_cast<const v4i*>(from + 64 * s);
+        }
+      };
+
+      int64_t chunk = a.sink / kChunk + split;
+      const int64_t stop = cdiv(last, kChunk);
+      if (chunk >= stop) continue;
+      int buf = 0;
+      int32_t page = look_up(chunk), page_next = look_up(chunk + a.splits);
+      pages[wave][0][lane] = page;
+      asm volatile("" ::: "memory");  // (read by other lanes of this wave)
+#pragma unroll
+      for (int i = 0; i < FLIGHT; ++i) load_tile(0, i);
+      block_scales[wave][0][lane] = scale_of(page);
+      if (!quantised) quantise();
+      quantised = true;
+      for (; chunk < stop; chunk += a.splits, buf ^= 1) {
+        const bool more = chunk + a.splits < stop;
+        float next_scale = 0.0f;
+        if (more) {
+          pages[wave][buf ^ 1][lane] = page_next;
+          next_scale = scale_of(page_next);
+          page_next = look_up(chunk + 2 * static_cast<int64_t>(a.splits));
+        }
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v4i acc[NT];
+#pragma unroll
+          for (int n = 0; n < NT; ++n) acc[n] = v4i{0, 0, 0, 0};
+#pragma unroll
+          for (int s = 0; s < KS; ++s) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              acc[n] =
+                  __builtin_amdgcn_mfma_i32_16x16x64_i8(bf[i % FLIGHT][s], cf[n][s], acc[n], 0, 0, 0);
+            }
+          }
+          settle(acc);
+          float best[TG][4];
+#pragma unroll
+          for (int g = 0; g < TG; ++g) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              best[g][r] = static_cast<float>(acc[g * (NT / TG)][r]) * scale[g * (NT / TG)];
+#pragma unroll
+              for (int n = 1; n < NT / TG; ++n) {
+                best[g][r] = fmaxf(best[g][r], static_cast<float>(acc[g * (NT / TG) + n][r]) *
+                                                   scale[g * (NT / TG) + n]);
+              }
+              if (GH == 0) best[g][r] = group_max16(best[g][r]);
+            }
+          }
+          if (i + FLIGHT < 4) {
+            load_tile(buf, i + FLIGHT);
+          } else if (more) {
+            load_tile(buf ^ 1, (i + FLIGHT) % 4);
+          }
+          const v4i pg = *reinterpret_cast<const v4i*>(&pages[wave][buf][16 * i + 4 * grp]);
+          const v4f bs = *reinterpret_cast<const v4f*>(&block_scales[wave][buf][16 * i + 4 * grp]);
+          const int64_t b = chunk * kChunk + 16 * i + 4 * grp;
+#pragma unroll
+          for (int g = 0; g < TG; ++g) {
+            if (!mine[g] || (GH == 0 && col != 0)) continue;
+            v4i* to = reinterpret_cast<v4i*>(a.keys + (token[g] * a.Hkv + head) * a.stride + b);
+            if (pass > 0) {
+              const v4i old = *to;
+#pragma unroll
+              for (int r = 0; r < 4; ++r) best[g][r] = fmaxf(best[g][r], __int_as_float(old[r]));
+            }
+            v4i key;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              key[r] = pass + 1 < passes ? __float_as_int(best[g][r])
+                       : pg[r] < 0       ? 0
+                                         : static_cast<int>(score_key(best[g][r] * bs[r]));
+            }
+            *to = key;
+          }
+        }
+        if (more) block_scales[wave][buf ^ 1][lane] = next_scale;
+        asm volatile("" ::: "memory");
+      }
+    }
+  }
+}
+
+// --- keep ---------------------------------------------------------------------------------------
+
+// A row's blocks: `lead` forced ones, n candidates, `tail` forced ones; `want` places for candidates.
+struct Span {
+  int32_t* out;
+  int32_t lead, n, end, tail;
+  uint32_t want;
+  __device__ Span(const SelectArgs& a, int64_t row) {
+    const KvPlace p = kv_place(a.tok, row / a.Hkv);
+    const int32_t blocks = p.last + 1;
+    out = a.out + row * a.count;
+    lead = a.sink < blocks ? a.sink : blocks;
+    end = blocks - a.recent > lead ? blocks - a.recent : lead;
+    n = end - lead;
+    tail = blocks - end;
+    want = static_cast<uint32_t>(a.count - a.sink - a.recent);
+  }
+  // The forced blocks around `kept` candidates, and -1 behind them.
+  __device__ void rest(const SelectArgs& a, uint32_t kept, int thread, int threads) const {
+    for (int32_t i = thread; i < lead; i += threads) out[i] = i;
+    const int32_t from = lead + static_cast<int32_t>(kept);
+    for (int32_t i = thread; from + i < a.count; i += threads) {
+      out[from + i] = i < tail ? end + i : -1;
+    }
+  }
+};
+
+// A row's candidates as a workgroup of WAVES waves holds them: even shares of neighbours, up to R keys
+// a lane. R = 0: any number, read again where they are needed.
 template <int WAVES, int R>
 struct Row {
   uint32_t k[R > 0 ? R : 1];
   const uint32_t* keys;
   int32_t first, n;  // this wave's first candidate (from the row's first) and how many
   __device__ void load(const uint32_t* row, int32_t candidates, int wave) {
-    const int32_t each = R > 0 ? 64 * R : (candidates + 64 * WAVES - 1) / (64 * WAVES) * 64;
+    const int32_t each = (candidates + 64 * WAVES - 1) / (64 * WAVES) * 64;  // at most 64 R
     first = wave * each;
     n = candidates - first < each ? candidates - first : each;
     keys = row + first;
@@ -324,7 +370,9 @@ struct Row {
   __device__ void each(F&& f) const {  // f(key, candidate in the row), 64 neighbours at a time
     if constexpr (R > 0) {
 #pragma unroll
-      for (int i = 0; i < R; ++i) f(k[i], first + 64 * i + lane_id());
+      for (int i = 0; i < R; ++i) {
+        if (64 * i < n) f(k[i], first + 64 * i + lane_id());
+      }
     } else {
       for (int32_t i = 0; i < n; i += 64) {
         f(i + lane_id() < n ? keys[i + lane_id()] : 0u, first + i + lane_id());
@@ -333,135 +381,277 @@ struct Row {
   }
 };
 
-template <int WAVES, int R>
-__global__ void __launch_bounds__(WAVES == 1 ? 4 * kWave : WAVES * kWave)
-    kv_keep_kernel(SelectArgs a) {
-  __shared__ uint32_t sums[WAVES > 1 ? 40 : 1];
-  __shared__ uint32_t part[2][WAVES];
-  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
-  const int64_t row = WAVES == 1 ? static_cast<int64_t>(blockIdx.x) * 4 + wave : blockIdx.x;
-  const int lane = lane_id(), me = WAVES == 1 ? 0 : wave;
-  const uint64_t below = (uint64_t{1} << lane) - 1;
-  if (row >= a.T * a.Hkv) return;  // (whole waves, and none where a workgroup has one row)
-  const KvPlace p = kv_place(a.tok, row / a.Hkv);
-  int32_t* out = a.out + row * a.count;
-  const int32_t blocks = p.last + 1;
-  const int32_t lead = a.sink < blocks ? a.sink : blocks;
-  const int32_t end = blocks - a.recent > lead ? blocks - a.recent : lead;
-  const int32_t tail = blocks - end;  // of the last `recent`
-  const uint32_t want = a.count - a.sink - a.recent;
-  Row<WAVES, R> r;
-  r.load(a.keys + row * a.stride + lead, end - lead, me);
-
-  if (WAVES > 1) {
-    for (int i = threadIdx.x; i < 40; i += WAVES * kWave) sums[i] = 0;
-  }
-  // candidates and their extreme keys
-  uint32_t least = ~0u, most = 0u, total = 0u;
-  r.each([&](uint32_t k, int32_t) {
-    total += static_cast<uint32_t>(__popcll(__ballot(k != 0)));
-    most = k > most ? k : most;
-    least = k != 0 && k < least ? k : least;
-  });
-  most = wave_extreme<true>(most);
-  least = wave_extreme<false>(least);
-  if (WAVES > 1) {
-    __shared__ uint32_t ends[2][WAVES];
-    if (lane == 0) {
-      ends[0][wave] = most;
-      ends[1][wave] = least;
-      part[0][wave] = total;
-    }
-    __syncthreads();
-    total = 0;
-    for (int w = 0; w < WAVES; ++w) {
-      most = ends[0][w] > most ? ends[0][w] : most;
-      least = ends[1][w] < least ? ends[1][w] : least;
-      total += part[0][w];
+// The largest cut that at least `want` of a wave's keys reach (1 where fewer are above 0), and how
+// many do. `count(probe)`: how many reach a key, the same in every lane.
+template <class F>
+__device__ inline uint32_t bisect(uint32_t most, uint32_t least, uint32_t total, uint32_t want,
+                                  F&& count, uint32_t& reach) {
+  reach = total;
+  if (total <= want) return 1u;
+  const uint32_t differ = most ^ least;
+  if (differ == 0) return most;
+  int bit = 31 - __builtin_clz(differ);
+  uint32_t cut = most & ~((2u << bit) - 1u);
+  for (; bit >= 0 && reach != want; --bit) {
+    const uint32_t probe = cut | (1u << bit);
+    const uint32_t n = count(probe);
+    if (n >= want) {
+      cut = probe;
+      reach = n;
     }
   }
-  // the largest cut that at least `want` keys reach
-  uint32_t cut = 1u, reach = total;
-  if (total > want && want > 0) {
-    const uint32_t differ = most ^ least;
-    int bit = differ != 0 ? 31 - __builtin_clz(differ) : -1;
-    cut = bit >= 0 ? most & ~((2u << bit) - 1u) : most;
-    int step = 0;
-    for (; bit >= 0 && reach != want; --bit, ++step) {
-      const uint32_t probe = cut | (1u << bit);
-      uint32_t n = 0;
-      r.each([&](uint32_t k, int32_t) {
-        n += static_cast<uint32_t>(__popcll(__ballot(k >= probe)));
-      });
-      if (WAVES > 1) {
-        if (lane == 0) atomicAdd(&sums[step], n);
-        __syncthreads();
-        n = sums[step];
-      }
-      if (n >= want) {
-        cut = probe;
-        reach = n;
-      }
-    }
-  } else if (want == 0) {
-    cut = ~0u;
-    reach = 0;
-  }
-  // more keys than places reach the cut: the lowest blocks of the cut's own key
-  uint32_t ties = ~0u;
-  uint32_t above = 0, equal = 0;  // this wave's
-  const bool tied = reach > want;
-  if (want == 0) {
-    ties = 0;
-  } else if (tied || WAVES > 1) {
-    r.each([&](uint32_t k, int32_t) {
-      above += static_cast<uint32_t>(__popcll(__ballot(k > cut)));
-      equal += static_cast<uint32_t>(__popcll(__ballot(k == cut)));
-    });
-  }
-  uint32_t place = 0;  // kept before this wave's first
-  if (WAVES > 1) {
-    __syncthreads();  // (every wave has read `part`)
-    if (lane == 0) {
-      part[0][wave] = above;
-      part[1][wave] = equal;
-    }
-    __syncthreads();
-    uint32_t all = 0, ties_before = 0;
-    for (int w = 0; w < WAVES; ++w) all += part[0][w];
-    if (want > 0) ties = want - all;
-    for (int w = 0; w < WAVES; ++w) {
-      if (w < wave) {
-        const uint32_t left = ties > ties_before ? ties - ties_before : 0;
-        place += part[0][w] + (part[1][w] < left ? part[1][w] : left);
-        ties_before += part[1][w];
-      }
-    }
-    ties = ties > ties_before ? ties - ties_before : 0;
-  } else if (tied) {
-    ties = want - above;
-  }
-  r.each([&](uint32_t k, int32_t at) {
-    const uint64_t same = __ballot(k == cut);
-    const bool keep = k > cut || (k == cut && static_cast<uint32_t>(__popcll(same & below)) < ties);
-    const uint64_t kept = __ballot(keep);
-    if (keep) out[lead + place + __popcll(kept & below)] = lead + at;
-    place += static_cast<uint32_t>(__popcll(kept));
-    const uint32_t seen = static_cast<uint32_t>(__popcll(same));
-    ties = ties > seen ? ties - seen : 0;
-  });
-  // the forced blocks and the padding, by the last wave, which knows how many were kept
-  if (me == WAVES - 1) {
-    for (int32_t i = lane; i < lead; i += kWave) out[i] = i;
-    for (int32_t i = lane; i < a.count - lead - static_cast<int32_t>(place); i += kWave) {
-      out[lead + place + i] = i < tail ? end + i : -1;
-    }
-  }
+  return cut;
 }
 
+// The kept of up to N keys a lane, in order (index(i): the candidate of key i): how many.
+template <int N, class F>
+__device__ inline uint32_t keep_in_order(const Span& p, const uint32_t (&k)[N], int32_t n,
+                                         F&& index) {
+  const int lane = lane_id();
+  const uint64_t below = (uint64_t{1} << lane) - 1;
+  uint32_t most = 0u, least = ~0u, total = 0u;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (64 * i < n) {
+      total += static_cast<uint32_t>(__popcll(__ballot(k[i] != 0)));
+      most = k[i] > most ? k[i] : most;
+      least = k[i] != 0 && k[i] < least ? k[i] : least;
+    }
+  }
+  uint32_t reach;
+  const uint32_t cut = bisect(
+      wave_extreme<true>(most), wave_extreme<false>(least), total, p.want,
+      [&](uint32_t probe) {
+        uint32_t c = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          if (64 * i < n) c += static_cast<uint32_t>(__popcll(__ballot(k[i] >= probe)));
+        }
+        return c;
+      },
+      reach);
+  // more keys than places reach the cut: the lowest blocks of the cut's own key
+  uint32_t ties = ~0u;
+  if (reach > p.want) {
+    ties = p.want;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (64 * i < n) ties -= static_cast<uint32_t>(__popcll(__ballot(k[i] > cut)));
+    }
+  }
+  uint32_t kept = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (64 * i >= n) continue;
+    const uint64_t same = __ballot(k[i] == cut);
+    const bool keep =
+        k[i] > cut || (k[i] == cut && static_cast<uint32_t>(__popcll(same & below)) < ties);
+    const uint64_t m = __ballot(keep);
+    if (keep) p.out[p.lead + kept + __popcll(m & below)] = p.lead + index(i);
+    kept += static_cast<uint32_t>(__popcll(m));
+    const uint32_t seen = static_cast<uint32_t>(__popcll(same));
+    ties = ties > seen ? ties - seen : 0;
+  }
+  return kept;
+}
+
+// A wave a row, R keys a lane. Where few are wanted of many: the want-th largest of the lanes' largest
+// keys bounds the cut; the keys that reach it, one a lane if they are 64 or fewer, hold the kept.
+template <int R>
+__global__ void __launch_bounds__(4 * kWave) kv_keep_few_kernel(SelectArgs a) {
+  __shared__ uint32_t near[4][kWave];
+  __shared__ int32_t near_at[4][kWave];
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + wave;
+  if (row >= a.T * a.Hkv) return;
+  const Span p(a, row);
+  const uint32_t* keys = a.keys + row * a.stride + p.lead;
+  const int lane = lane_id();
+  uint32_t k[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) k[i] = 64 * i + lane < p.n ? keys[64 * i + lane] : 0u;
+  uint32_t kept = 0;
+  bool done = p.want == 0;
+  if (R > 1 && !done && p.n > 2 * kWave && p.want <= 40) {
+    uint32_t top = k[0], reach;
+#pragma unroll
+    for (int i = 1; i < R; ++i) top = k[i] > top ? k[i] : top;
+    const uint32_t floor = bisect(
+        wave_extreme<true>(top), wave_extreme<false>(top != 0 ? top : ~0u),
+        static_cast<uint32_t>(__popcll(__ballot(top != 0))), p.want,
+        [&](uint32_t probe) { return static_cast<uint32_t>(__popcll(__ballot(top >= probe))); },
+        reach);
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      if (64 * i < p.n) {
+        const uint64_t m = __ballot(k[i] >= floor);
+        const int at = n + __popcll(m & ((uint64_t{1} << lane) - 1));
+        if (k[i] >= floor && at < kWave) {
+          near[wave][at] = k[i];
+          near_at[wave][at] = 64 * i + lane;
+        }
+        n += __popcll(m);
+      }
+    }
+    asm volatile("" ::: "memory");  // (read by other lanes of this wave)
+    if (n <= kWave) {
+      const uint32_t one[1] = {lane < n ? near[wave][lane] : 0u};
+      const int32_t at = lane < n ? near_at[wave][lane] : 0;
+      kept = keep_in_order(p, one, kWave, [&](int) { return at; });
+      done = true;
+    }
+  }
+  if (!done) kept = keep_in_order(p, k, p.n, [&](int i) { return 64 * i + lane; });
+  p.rest(a, kept, lane, kWave);
+}
+
+// A workgroup of WAVES waves a row, R keys a lane (0: read again where they are needed).
+constexpr int kRankMost = 2048;  // keys that are ranked against each other
+
+template <int WAVES, int R>
+__global__ void __launch_bounds__(WAVES* kWave) kv_keep_many_kernel(SelectArgs a) {
+  constexpr int LANES = WAVES * kWave;
+  __shared__ __attribute__((aligned(16))) uint32_t tops[LANES];
+  __shared__ uint64_t near[kRankMost];  // key << 32 | ~candidate: the order of (key desc, block asc)
+  __shared__ int32_t winners[1024];
+  __shared__ uint32_t shared_cut, listed, sums[WAVES];
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int lane = lane_id();
+  const int64_t row = blockIdx.x;
+  const Span p(a, row);
+  Row<WAVES, R> r;
+  r.load(a.keys + row * a.stride + p.lead, p.n, wave);
+  uint32_t top = 0u;
+  r.each([&](uint32_t k, int32_t) { top = k > top ? k : top; });
+  tops[threadIdx.x] = top;
+  if (threadIdx.x == 0) listed = 0u;
+  __syncthreads();
+  if (wave == 0) {
+    // Groups of lanes, some more than places: the want-th largest of their largest keys.
+    auto cut_of = [&](auto groups, auto load) {
+      constexpr int N = decltype(groups)::value;
+      uint32_t g[N], most = 0u, least = ~0u, total = 0u, reach;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        g[i] = load(i);
+        total += static_cast<uint32_t>(__popcll(__ballot(g[i] != 0)));
+        most = g[i] > most ? g[i] : most;
+        least = g[i] != 0 && g[i] < least ? g[i] : least;
+      }
+      return bisect(
+          wave_extreme<true>(most), wave_extreme<false>(least), total, p.want,
+          [&](uint32_t probe) {
+            uint32_t n = 0;
+#pragma unroll
+            for (int i = 0; i < N; ++i) n += static_cast<uint32_t>(__popcll(__ballot(g[i] >= probe)));
+            return n;
+          },
+          reach);
+    };
+    uint32_t cut = ~0u;
+    if (p.want == 0) {
+    } else if (WAVES > 4 && p.want <= 192) {
+      cut = cut_of(std::integral_constant<int, WAVES / 4>{}, [&](int i) {
+        const v4i x = *reinterpret_cast<const v4i*>(&tops[4 * (64 * i + lane)]);
+        const uint32_t u = static_cast<uint32_t>(x[0]), v = static_cast<uint32_t>(x[1]);
+        const uint32_t y = static_cast<uint32_t>(x[2]), z = static_cast<uint32_t>(x[3]);
+        const uint32_t f = u > v ? u : v, t = y > z ? y : z;
+        return f > t ? f : t;
+      });
+    } else {
+      cut = cut_of(std::integral_constant<int, WAVES>{}, [&](int i) { return tops[64 * i + lane]; });
+    }
+    if (lane == 0) shared_cut = cut;
+  }
+  __syncthreads();
+  const uint32_t floor = shared_cut;
+  if (p.want > 0) {
+    r.each([&](uint32_t k, int32_t at) {
+      const uint64_t m = __ballot(k >= floor);
+      if (m == 0) return;
+      uint32_t first = 0;
+      if (lane == 0) first = atomicAdd(&listed, static_cast<uint32_t>(__popcll(m)));
+      first = __builtin_amdgcn_readfirstlane(first) + __popcll(m & ((uint64_t{1} << lane) - 1));
+      if (k >= floor && first < kRankMost) {
+        near[first] = static_cast<uint64_t>(k) << 32 | (0xffffffffu - static_cast<uint32_t>(at));
+      }
+    });
+  }
+  __syncthreads();
+  const uint32_t n = listed;
+  uint32_t kept = n < p.want ? n : p.want;
+  if (n <= kRankMost) {
+    for (uint32_t i = threadIdx.x; i < n; i += LANES) {
+      const uint64_t x = near[i];
+      uint32_t rank = 0;
+#pragma unroll 8
+      for (uint32_t j = 0; j < n; ++j) rank += near[j] > x ? 1u : 0u;
+      if (rank < p.want) winners[rank] = static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(x));
+    }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < kept; i += LANES) {
+      const int32_t x = winners[i];
+      int32_t at = 0;
+#pragma unroll 8
+      for (uint32_t j = 0; j < kept; ++j) at += winners[j] < x ? 1 : 0;
+      p.out[p.lead + at] = p.lead + x;
+    }
+  } else {
+    // (keys that mostly tie) the cut over all of them, then the kept in order, ties from the lowest
+    auto count = [&](auto pred) {
+      uint32_t c = 0;
+      r.each([&](uint32_t k, int32_t) { c += static_cast<uint32_t>(__popcll(__ballot(pred(k)))); });
+      __syncthreads();
+      if (lane == 0) sums[wave] = c;
+      __syncthreads();
+      c = 0;
+      for (int w = 0; w < WAVES; ++w) c += sums[w];
+      return c;
+    };
+    uint32_t cut = 0u;
+    for (int bit = 31; bit >= 0; --bit) {
+      const uint32_t probe = cut | (1u << bit);
+      if (count([&](uint32_t k) { return k >= probe; }) >= p.want) cut = probe;
+    }
+    const uint32_t above = count([&](uint32_t k) { return k > cut; });
+    uint32_t mine_above = 0, mine_same = 0;
+    r.each([&](uint32_t k, int32_t) {
+      mine_above += static_cast<uint32_t>(__popcll(__ballot(k > cut)));
+      mine_same += static_cast<uint32_t>(__popcll(__ballot(k == cut)));
+    });
+    __syncthreads();
+    if (lane == 0) {
+      tops[wave] = mine_above;
+      tops[WAVES + wave] = mine_same;
+    }
+    __syncthreads();
+    uint32_t ties = p.want - above, place = 0, same_before = 0;
+    for (int w = 0; w < wave; ++w) {
+      const uint32_t left = ties > same_before ? ties - same_before : 0;
+      place += tops[w] + (tops[WAVES + w] < left ? tops[WAVES + w] : left);
+      same_before += tops[WAVES + w];
+    }
+    ties = ties > same_before ? ties - same_before : 0;
+    const uint64_t below = (uint64_t{1} << lane) - 1;
+    r.each([&](uint32_t k, int32_t at) {
+      const uint64_t same = __ballot(k == cut);
+      const bool keep =
+          k > cut || (k == cut && static_cast<uint32_t>(__popcll(same & below)) < ties);
+      const uint64_t m = __ballot(keep);
+      if (keep) p.out[p.lead + place + __popcll(m & below)] = p.lead + at;
+      place += static_cast<uint32_t>(__popcll(m));
+      const uint32_t seen = static_cast<uint32_t>(__popcll(same));
+      ties = ties > seen ? ties - seen : 0;
+    });
+  }
+  p.rest(a, kept, static_cast<int>(threadIdx.x), LANES);
+}
+
+// gh = 0: a token a wave, its heads across `tiles` tiles. gh > 0: tokens across the lanes, gh heads a pass.
 struct SelectPlan {
   int64_t stride;
-  int32_t tiles, cols, per_wave, splits, head_groups;
+  int32_t tiles, gh, per_wave, splits, head_groups;
 };
 
 inline SelectPlan select_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t B,
@@ -469,18 +659,19 @@ inline SelectPlan select_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int
   SelectPlan p;
   const int64_t G = Hq / Hkv;
   p.stride = align_up(static_cast<size_t>(max_pages), kChunk);
-  p.cols = static_cast<int32_t>(next_pow2(G < 16 ? G : 16));
   p.head_groups = static_cast<int32_t>(cdiv(Hkv, kScoreWaves));
-  const int32_t most = D <= 128 ? 4 : 2;  // tiles whose columns fit in registers beside a chunk
-  if (G > 16) {
-    p.tiles = G <= 32 ? 2 : most;
-    p.per_wave = 1;
+  // Tokens that mostly are of one sequence share a pass over its blocks; a wave with tokens of
+  // several passes over each one's.
+  if (B > 0 && T >= 4 * B) {
+    const int64_t most = D <= 128 ? 8 : 4;  // heads whose columns fit in registers beside the bounds
+    const int64_t gh = next_pow2(G);
+    p.gh = static_cast<int32_t>(gh < most ? gh : most);
+    p.tiles = p.gh < 4 ? 4 : p.gh;
+    p.per_wave = 16 * p.tiles / p.gh;
   } else {
-    // A wave's tokens should mostly be of one sequence: each sequence among them is a pass of all
-    // its tiles over that sequence's blocks.
-    const int64_t same = B > 0 ? T / B : 0, tile = 16 / p.cols;
-    p.tiles = same >= 2 * most * tile ? most : 1;
-    p.per_wave = static_cast<int32_t>(same >= 2 ? p.tiles * tile : 1);
+    p.gh = 0;
+    p.tiles = G <= 16 ? 1 : G <= 32 || D > 128 ? 2 : 4;
+    p.per_wave = 1;
   }
   const int64_t waves = cdiv(T, p.per_wave) * Hkv;
   const int64_t chunks = cdiv(max_pages > sink ? max_pages - sink : 1, kChunk);
@@ -532,8 +723,7 @@ extern "C" int rt_kv_select(const void* q, int64_t q_token_stride, int64_t q_hea
            static_cast<int32_t>(max_pages), static_cast<int32_t>(P), kv_shift(page)};
   a.count = static_cast<int32_t>(count), a.sink = static_cast<int32_t>(sink);
   a.recent = static_cast<int32_t>(recent), a.out = out, a.keys = static_cast<uint32_t*>(workspace);
-  a.stride = plan.stride, a.cols = plan.cols, a.per_wave = plan.per_wave;
-  a.splits = plan.splits, a.head_groups = plan.head_groups;
+  a.stride = plan.stride, a.splits = plan.splits, a.head_groups = plan.head_groups;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const int64_t grid = cdiv(T, plan.per_wave) * plan.splits * plan.head_groups;
   RT_CHECK_ARG(grid <= INT32_MAX, "too many tokens");
@@ -542,31 +732,43 @@ extern "C" int rt_kv_select(const void* q, int64_t q_token_stride, int64_t q_hea
       using E = decltype(e);
       constexpr int DD = decltype(d)::value;
       const dim3 g(static_cast<unsigned>(grid)), b(kScoreWaves * kWave);
-      if (plan.tiles == 1) {
-        kv_score_kernel<E, DD, 1><<<g, b, 0, s>>>(a);
-      } else if (plan.tiles == 2) {
-        kv_score_kernel<E, DD, 2><<<g, b, 0, s>>>(a);
+      constexpr int W = DD <= 128 ? 4 : 2;  // the widest decode form
+      if (plan.gh == 0) {
+        if (plan.tiles == 1) {
+          kv_score_kernel<E, DD, 1, 0><<<g, b, 0, s>>>(a);
+        } else if (plan.tiles == 2) {
+          kv_score_kernel<E, DD, 2, 0><<<g, b, 0, s>>>(a);
+        } else {
+          kv_score_kernel<E, DD, W, 0><<<g, b, 0, s>>>(a);
+        }
+      } else if (plan.gh == 1) {
+        kv_score_kernel<E, DD, 4, 1><<<g, b, 0, s>>>(a);
+      } else if (plan.gh == 2) {
+        kv_score_kernel<E, DD, 4, 2><<<g, b, 0, s>>>(a);
+      } else if (plan.gh == 4) {
+        kv_score_kernel<E, DD, 4, 4><<<g, b, 0, s>>>(a);
       } else if constexpr (DD <= 128) {
-        kv_score_kernel<E, DD, 4><<<g, b, 0, s>>>(a);
+        kv_score_kernel<E, DD, 8, 8><<<g, b, 0, s>>>(a);
       }
       RT_CHECK_HIP(hipGetLastError());
       return kOk;
     });
     if (st != kOk) return st;
   }
-  // One wave a row while its keys fit in a few registers a lane, else a workgroup of 16 waves.
+  // A wave a row while its keys fit in 16 registers a lane; then four waves, unless more places are
+  // wanted than their lanes bound well; then sixteen.
   const int64_t rows = T * Hkv;
   const dim3 one(static_cast<unsigned>(rows)), four(static_cast<unsigned>(cdiv(rows, 4)));
   if (max_pages <= 64 * 4) {
-    kv_keep_kernel<1, 4><<<four, 4 * kWave, 0, s>>>(a);
+    kv_keep_few_kernel<4><<<four, 4 * kWave, 0, s>>>(a);
   } else if (max_pages <= 64 * 16) {
-    kv_keep_kernel<1, 16><<<four, 4 * kWave, 0, s>>>(a);
-  } else if (max_pages <= 64 * 16 * 4) {
-    kv_keep_kernel<16, 4><<<one, 16 * kWave, 0, s>>>(a);
-  } else if (max_pages <= 64 * 16 * 16) {
-    kv_keep_kernel<16, 16><<<one, 16 * kWave, 0, s>>>(a);
+    kv_keep_few_kernel<16><<<four, 4 * kWave, 0, s>>>(a);
+  } else if (max_pages <= 4 * 64 * 16 && count - sink - recent <= 128) {
+    kv_keep_many_kernel<4, 16><<<one, 4 * kWave, 0, s>>>(a);
+  } else if (max_pages <= 16 * 64 * 16) {
+    kv_keep_many_kernel<16, 16><<<one, 16 * kWave, 0, s>>>(a);
   } else {
-    kv_keep_kernel<16, 0><<<one, 16 * kWave, 0, s>>>(a);
+    kv_keep_many_kernel<16, 0><<<one, 16 * kWave, 0, s>>>(a);
   }
   RT_CHECK_HIP(hipGetLastError());
   return kOk;

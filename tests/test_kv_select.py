@@ -205,3 +205,40 @@ def test_refusals(dev):
     ]:
         with pytest.raises(error):
             kv.select_blocks(**{**good, **wrong})
+
+
+def test_codes_by_reciprocal():
+    """The kernels' quotient (reciprocal, product, one correction) is the division's, rounded to nearest, for
+    every pair of bf16 significands, a spread of fp16's, and the floor: codes equal bit for bit. (The
+    correction's product and sum are exact in 64 bits up to their last rounding.)"""
+    def quotient(x, top):
+        r = (np.float32(1) / top).astype(np.float32)
+        q = (x * r).astype(np.float32)
+        rest = (x.astype(np.float64) - q.astype(np.float64) * top).astype(np.float32)
+        return (rest.astype(np.float64) * r + q).astype(np.float32)
+
+    for bits, step in ((8, 1), (11, 13)):
+        m = np.arange(1 << (bits - 1), 1 << bits, dtype=np.float32)
+        for top in m[::step]:
+            for e in range(9):
+                x = (m * 2.0**-e).astype(np.float32)
+                x = x[x <= top]
+                assert np.array_equal(quotient(x, np.float32(top)), x / np.float32(top))
+    x = (np.arange(0, 129, dtype=np.float32) * np.float32(2.0**-34)).astype(np.float32)
+    x = x[x <= np.float32(1e-8)]
+    assert np.array_equal(quotient(x, np.float32(1e-8)), x / np.float32(1e-8))
+
+
+@pytest.mark.gpu
+def test_queries_of_extreme_sizes(dev):
+    """Largest magnitudes from below the floor to the ends of bf16's range."""
+    pos, seq, tab, pages = layout(121, 16, [(16 * 60, 1)] * 8)
+    q = normal16(122, (8, 4, 64), "bf16")
+    q *= np.float32(2.0)**np.array([-120, -40, -27, -20, 0, 60, 101, 120], np.float32)[:, None, None]
+    q[7, 2] = 0.0
+    codes, scales = _bounds(123, pages, 1, 64)
+    got = _select(dev, q, "bf16", codes, scales, pos, seq, tab, 16, 12, 1, 2)
+    assert np.array_equal(got, okv.select(q, codes, scales, pos, seq, tab, 16, 12, 1, 2))
+    prompt = [np.repeat(x, 5, 0) for x in (q, pos, seq)]
+    got = _select(dev, prompt[0], "bf16", codes, scales, prompt[1], prompt[2], tab, 16, 12, 1, 2)
+    assert np.array_equal(got[::5], okv.select(q, codes, scales, pos, seq, tab, 16, 12, 1, 2))
