@@ -597,7 +597,8 @@ int rt_kv_append(const void* q, int64_t q_token_stride, int64_t q_head_stride, c
  * query head's row is quantised as bounds are (codes c, scale s); score(b) = max over the group's
  * heads of float(c . mid_b + |c| . half_b) * s, times the block's scale (the sum exact in int32,
  * two float products); not a number ranks last. Blocks without a page are not candidates. */
-size_t rt_kv_select_workspace(int64_t T, int64_t Hkv, int64_t max_pages);
+size_t rt_kv_select_workspace(int64_t T, int64_t Hkv, int64_t B, int64_t max_pages, int64_t count,
+                              int64_t sink, int64_t recent);
 int rt_kv_select(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t T,
                  int64_t Hq, int64_t Hkv, int64_t D, int dtype, const int8_t* bounds,
                  const float* bound_scales, int64_t P, int64_t page, const int32_t* positions,

@@ -161,7 +161,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [*[_c_p, _c_i64, _c_i64] * 3, *[_c_i64] * 4, _c_int, _c_p, _c_i64, _c_i64, _c_int, _c_p,
          _c_p, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_p],
     ),
-    "rt_kv_select_workspace": (_c_sz, [_c_i64] * 3),
+    "rt_kv_select_workspace": (_c_sz, [_c_i64] * 7),
     "rt_kv_select": (
         _c_int,
         [_c_p, *[_c_i64] * 6, _c_int, _c_p, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_p, *[_c_i64] * 5,

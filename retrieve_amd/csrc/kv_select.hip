@@ -103,23 +103,32 @@ __device__ inline void pack_codes(const V8 (&x)[2], float top, float r, float sm
 // A wave holds NT tiles of 16 columns. GH = 0 (decode): one token, column = query head, 16 NT heads a
 // pass. GH > 0 (prompts): column = token, tile n = head n % GH of token group n / GH, GH heads a
 // pass (heads past the group's repeat its last).
-template <class E, int D, int NT, int GH>
-__global__ void __launch_bounds__(kScoreWaves* kWave, D > 128 && NT == 4 ? 1 : 2)
-    kv_score_kernel(SelectArgs a) {
+// Chunks first, first + step, ... of 64 blocks are scored; `put(token, block)` is where the keys of
+// four blocks go.
+struct ScoreLds {
+  __attribute__((aligned(16))) int32_t pages[2][kChunk];
+  __attribute__((aligned(16))) float scales[2][kChunk];
+};
+
+template <class E, int D, int NT, int GH, int FLIGHT, class Put>
+__device__ inline void score_blocks(const SelectArgs& a, int64_t t0, int head, int first, int step,
+                                    ScoreLds& lds, Put&& put) {
   using V8 = typename Kv<E>::V8;
   constexpr int KS = D / 32;  // steps of 64 of a row's 2 D bytes
   constexpr int TG = GH > 0 ? NT / GH : 1, HEADS = GH > 0 ? GH : 16 * NT;
-  constexpr int FLIGHT = D * NT > 512 || D > 128 ? 2 : 4;  // tiles of bounds in flight
-  __shared__ __attribute__((aligned(16))) int32_t pages[kScoreWaves][2][kChunk];
-  __shared__ __attribute__((aligned(16))) float block_scales[kScoreWaves][2][kChunk];
-  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   const int lane = lane_id(), col = lane & 15, grp = lane >> 4;
-  const int head = static_cast<int>(blockIdx.x % a.head_groups) * kScoreWaves + wave;
-  if (head >= a.Hkv) return;
-  const int split = static_cast<int>(blockIdx.x / a.head_groups % a.splits);
-  const int64_t t0 = static_cast<int64_t>(blockIdx.x / a.head_groups / a.splits) *
-                     (GH > 0 ? 16 * TG : 1);
   const int passes = (a.G + HEADS - 1) / HEADS;
+  constexpr int LOADS = D % 64 == 0 ? KS / 2 : KS;  // 16 channels of a query row a lane
+  auto load_q = [&](int64_t t, int h, V8 (&x)[LOADS][2]) {
+    const E* q = static_cast<const E*>(a.q) + t * a.q_st +
+                 static_cast<int64_t>(head * a.G + (h < a.G ? h : a.G - 1)) * a.q_sh;
+#pragma unroll
+    for (int s = 0; s < LOADS; ++s) {
+      const int at = 64 * s + 16 * grp, d = at < D ? at : at - D;
+      x[s][0] = *reinterpret_cast<const V8*>(q + d);
+      x[s][1] = *reinterpret_cast<const V8*>(q + d + 8);
+    }
+  };
 
   // the lane's token of each group, and where its candidates end (0: none)
   int64_t token[TG];
@@ -149,20 +158,11 @@ __global__ void __launch_bounds__(kScoreWaves* kWave, D > 128 && NT == 4 ? 1 : 2
     auto quantise = [&]() {
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        int h = GH > 0 ? pass * GH + n % GH : (pass * NT + n) * 16 + col;
-        if (h >= a.G) h = a.G - 1;
         const int g = GH > 0 ? n / GH : 0;
-        const E* q = static_cast<const E*>(a.q) + (end[g] > 0 ? token[g] : t0) * a.q_st +
-                     static_cast<int64_t>(head * a.G + h) * a.q_sh;
-        constexpr int LOADS = D % 64 == 0 ? KS / 2 : KS;
         V8 x[LOADS][2];
+        load_q(end[g] > 0 ? token[g] : t0,
+               GH > 0 ? pass * GH + n % GH : (pass * NT + n) * 16 + col, x);
         float top = 0.0f;
-#pragma unroll
-        for (int s = 0; s < LOADS; ++s) {
-          const int at = 64 * s + 16 * grp, d = at < D ? at : at - D;
-          x[s][0] = *reinterpret_cast<const V8*>(q + d);
-          x[s][1] = *reinterpret_cast<const V8*>(q + d + 8);
-        }
 #pragma unroll
         for (int s = 0; s < LOADS; ++s) {
 #pragma unroll
@@ -226,7 +226,7 @@ __global__ void __launch_bounds__(kScoreWaves* kWave, D > 128 && NT == 4 ? 1 : 2
       };
       v4i bf[FLIGHT][KS];
       auto load_tile = [&](int buf, int tile) {
-        const int32_t p = pages[wave][buf][16 * tile + col];
+        const int32_t p = lds.pages[buf][16 * tile + col];
         const int8_t* from = a.bounds +
                              (static_cast<int64_t>(p < 0 ? 0 : p) * a.Hkv + head) * (2 * D) +
                              16 * grp;
@@ -236,25 +236,25 @@ __global__ void __launch_bounds__(kScoreWaves* kWave, D > 128 && NT == 4 ? 1 : 2
         }
       };
 
-      int64_t chunk = a.sink / kChunk + split;
+      int64_t chunk = a.sink / kChunk + first;
       const int64_t stop = cdiv(last, kChunk);
       if (chunk >= stop) continue;
       int buf = 0;
-      int32_t page = look_up(chunk), page_next = look_up(chunk + a.splits);
-      pages[wave][0][lane] = page;
+      int32_t page = look_up(chunk), page_next = look_up(chunk + step);
+      lds.pages[0][lane] = page;
       asm volatile("" ::: "memory");  // (read by other lanes of this wave)
 #pragma unroll
       for (int i = 0; i < FLIGHT; ++i) load_tile(0, i);
-      block_scales[wave][0][lane] = scale_of(page);
+      lds.scales[0][lane] = scale_of(page);
       if (!quantised) quantise();
       quantised = true;
-      for (; chunk < stop; chunk += a.splits, buf ^= 1) {
-        const bool more = chunk + a.splits < stop;
+      for (; chunk < stop; chunk += step, buf ^= 1) {
+        const bool more = chunk + step < stop;
         float next_scale = 0.0f;
         if (more) {
-          pages[wave][buf ^ 1][lane] = page_next;
+          lds.pages[buf ^ 1][lane] = page_next;
           next_scale = scale_of(page_next);
-          page_next = look_up(chunk + 2 * static_cast<int64_t>(a.splits));
+          page_next = look_up(chunk + 2 * static_cast<int64_t>(step));
         }
         asm volatile("" ::: "memory");
 #pragma unroll
@@ -290,13 +290,13 @@ __global__ void __launch_bounds__(kScoreWaves* kWave, D > 128 && NT == 4 ? 1 : 2
           } else if (more) {
             load_tile(buf ^ 1, (i + FLIGHT) % 4);
           }
-          const v4i pg = *reinterpret_cast<const v4i*>(&pages[wave][buf][16 * i + 4 * grp]);
-          const v4f bs = *reinterpret_cast<const v4f*>(&block_scales[wave][buf][16 * i + 4 * grp]);
+          const v4i pg = *reinterpret_cast<const v4i*>(&lds.pages[buf][16 * i + 4 * grp]);
+          const v4f bs = *reinterpret_cast<const v4f*>(&lds.scales[buf][16 * i + 4 * grp]);
           const int64_t b = chunk * kChunk + 16 * i + 4 * grp;
 #pragma unroll
           for (int g = 0; g < TG; ++g) {
             if (!mine[g] || (GH == 0 && col != 0)) continue;
-            v4i* to = reinterpret_cast<v4i*>(a.keys + (token[g] * a.Hkv + head) * a.stride + b);
+            auto* to = put(token[g], b);
             if (pass > 0) {
               const v4i old = *to;
 #pragma unroll
@@ -312,11 +312,29 @@ __global__ void __launch_bounds__(kScoreWaves* kWave, D > 128 && NT == 4 ? 1 : 2
             *to = key;
           }
         }
-        if (more) block_scales[wave][buf ^ 1][lane] = next_scale;
+        if (more) lds.scales[buf ^ 1][lane] = next_scale;
         asm volatile("" ::: "memory");
       }
     }
   }
+}
+
+template <class E, int D, int NT, int GH>
+__global__ void __launch_bounds__(kScoreWaves* kWave, D > 128 && NT == 4 ? 1 : 2)
+    kv_score_kernel(SelectArgs a) {
+  __shared__ ScoreLds lds[kScoreWaves];
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int head = static_cast<int>(blockIdx.x % a.head_groups) * kScoreWaves + wave;
+  if (head >= a.Hkv) return;
+  const int split = static_cast<int>(blockIdx.x / a.head_groups % a.splits);
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x / a.head_groups / a.splits) *
+                     (GH > 0 ? 16 * (NT / (GH > 0 ? GH : 1)) : 1);
+  constexpr int FLIGHT = D * NT > 512 || D > 128 ? 2 : 4;  // tiles of bounds in flight
+  score_blocks<E, D, NT, GH, FLIGHT>(a, t0, head, split, a.splits, lds[wave],
+                                     [&](int64_t token, int64_t b) {
+                                       return reinterpret_cast<v4i*>(
+                                           a.keys + (token * a.Hkv + head) * a.stride + b);
+                                     });
 }
 
 // --- keep ---------------------------------------------------------------------------------------
@@ -458,14 +476,8 @@ __device__ inline uint32_t keep_in_order(const Span& p, const uint32_t (&k)[N], 
 // A wave a row, R keys a lane. Where few are wanted of many: the want-th largest of the lanes' largest
 // keys bounds the cut; the keys that reach it, one a lane if they are 64 or fewer, hold the kept.
 template <int R>
-__global__ void __launch_bounds__(4 * kWave) kv_keep_few_kernel(SelectArgs a) {
-  __shared__ uint32_t near[4][kWave];
-  __shared__ int32_t near_at[4][kWave];
-  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + wave;
-  if (row >= a.T * a.Hkv) return;
-  const Span p(a, row);
-  const uint32_t* keys = a.keys + row * a.stride + p.lead;
+__device__ inline void keep_few(const SelectArgs& a, const Span& p, const uint32_t* keys,
+                                uint32_t* near, int32_t* near_at) {
   const int lane = lane_id();
   uint32_t k[R];
 #pragma unroll
@@ -488,16 +500,16 @@ __global__ void __launch_bounds__(4 * kWave) kv_keep_few_kernel(SelectArgs a) {
         const uint64_t m = __ballot(k[i] >= floor);
         const int at = n + __popcll(m & ((uint64_t{1} << lane) - 1));
         if (k[i] >= floor && at < kWave) {
-          near[wave][at] = k[i];
-          near_at[wave][at] = 64 * i + lane;
+          near[at] = k[i];
+          near_at[at] = 64 * i + lane;
         }
         n += __popcll(m);
       }
     }
     asm volatile("" ::: "memory");  // (read by other lanes of this wave)
     if (n <= kWave) {
-      const uint32_t one[1] = {lane < n ? near[wave][lane] : 0u};
-      const int32_t at = lane < n ? near_at[wave][lane] : 0;
+      const uint32_t one[1] = {lane < n ? near[lane] : 0u};
+      const int32_t at = lane < n ? near_at[lane] : 0;
       kept = keep_in_order(p, one, kWave, [&](int) { return at; });
       done = true;
     }
@@ -506,22 +518,41 @@ __global__ void __launch_bounds__(4 * kWave) kv_keep_few_kernel(SelectArgs a) {
   p.rest(a, kept, lane, kWave);
 }
 
+template <int R>
+__global__ void __launch_bounds__(4 * kWave) kv_keep_few_kernel(SelectArgs a) {
+  __shared__ uint32_t near[4][kWave];
+  __shared__ int32_t near_at[4][kWave];
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + wave;
+  if (row >= a.T * a.Hkv) return;
+  const Span p(a, row);
+  keep_few<R>(a, p, a.keys + row * a.stride + p.lead, near[wave], near_at[wave]);
+}
+
 // A workgroup of WAVES waves a row, R keys a lane (0: read again where they are needed).
 constexpr int kRankMost = 2048;  // keys that are ranked against each other
 
+template <int WAVES>
+struct KeepLds {
+  __attribute__((aligned(16))) uint32_t tops[WAVES * kWave];
+  uint64_t near[kRankMost];  // key << 32 | ~candidate: the order of (key desc, block asc)
+  int32_t winners[1024];
+  uint32_t cut, listed, sums[WAVES];
+};
+
 template <int WAVES, int R>
-__global__ void __launch_bounds__(WAVES* kWave) kv_keep_many_kernel(SelectArgs a) {
+__device__ inline void keep_many(const SelectArgs& a, const Span& p, const uint32_t* keys,
+                                 KeepLds<WAVES>& lds) {
   constexpr int LANES = WAVES * kWave;
-  __shared__ __attribute__((aligned(16))) uint32_t tops[LANES];
-  __shared__ uint64_t near[kRankMost];  // key << 32 | ~candidate: the order of (key desc, block asc)
-  __shared__ int32_t winners[1024];
-  __shared__ uint32_t shared_cut, listed, sums[WAVES];
+  auto& tops = lds.tops;
+  auto& near = lds.near;
+  auto& winners = lds.winners;
+  auto& sums = lds.sums;
+  auto& listed = lds.listed;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   const int lane = lane_id();
-  const int64_t row = blockIdx.x;
-  const Span p(a, row);
   Row<WAVES, R> r;
-  r.load(a.keys + row * a.stride + p.lead, p.n, wave);
+  r.load(keys, p.n, wave);
   uint32_t top = 0u;
   r.each([&](uint32_t k, int32_t) { top = k > top ? k : top; });
   tops[threadIdx.x] = top;
@@ -551,7 +582,7 @@ __global__ void __launch_bounds__(WAVES* kWave) kv_keep_many_kernel(SelectArgs a
     };
     uint32_t cut = ~0u;
     if (p.want == 0) {
-    } else if (WAVES > 4 && p.want <= 192) {
+    } else if (WAVES == 16 && p.want <= 96) {
       cut = cut_of(std::integral_constant<int, WAVES / 4>{}, [&](int i) {
         const v4i x = *reinterpret_cast<const v4i*>(&tops[4 * (64 * i + lane)]);
         const uint32_t u = static_cast<uint32_t>(x[0]), v = static_cast<uint32_t>(x[1]);
@@ -562,10 +593,10 @@ __global__ void __launch_bounds__(WAVES* kWave) kv_keep_many_kernel(SelectArgs a
     } else {
       cut = cut_of(std::integral_constant<int, WAVES>{}, [&](int i) { return tops[64 * i + lane]; });
     }
-    if (lane == 0) shared_cut = cut;
+    if (lane == 0) lds.cut = cut;
   }
   __syncthreads();
-  const uint32_t floor = shared_cut;
+  const uint32_t floor = lds.cut;
   if (p.want > 0) {
     r.each([&](uint32_t k, int32_t at) {
       const uint64_t m = __ballot(k >= floor);
@@ -648,7 +679,51 @@ __global__ void __launch_bounds__(WAVES* kWave) kv_keep_many_kernel(SelectArgs a
   p.rest(a, kept, static_cast<int>(threadIdx.x), LANES);
 }
 
-// gh = 0: a token a wave, its heads across `tiles` tiles. gh > 0: tokens across the lanes, gh heads a pass.
+template <int WAVES, int R>
+__global__ void __launch_bounds__(WAVES* kWave) kv_keep_many_kernel(SelectArgs a) {
+  __shared__ KeepLds<WAVES> lds;
+  const int64_t row = blockIdx.x;
+  const Span p(a, row);
+  keep_many<WAVES, R>(a, p, a.keys + row * a.stride + p.lead, lds);
+}
+
+// Both in one launch, a workgroup a (token, key/value head): decode over page tables of up to
+// kFusedMost blocks. The keys stay in LDS.
+constexpr int kFusedWaves = 8;
+constexpr int kFusedMost = 4096;
+
+template <class E, int D, int NT>
+__global__ void __launch_bounds__(kFusedWaves* kWave, D <= 128 && NT == 1 ? 4 : 2)
+    kv_select_kernel(SelectArgs a) {
+  __shared__ __attribute__((aligned(16))) uint32_t keys[kFusedMost];
+  __shared__ ScoreLds score_lds[kFusedWaves];
+  __shared__ KeepLds<kFusedWaves> keep_lds;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int64_t row = blockIdx.x;
+  score_blocks<E, D, NT, 0, 2>(
+      a, row / a.Hkv, static_cast<int>(row % a.Hkv), wave, kFusedWaves, score_lds[wave],
+      [&](int64_t, int64_t b) { return reinterpret_cast<v4i*>(&keys[b]); });
+  __syncthreads();
+  const Span p(a, row);
+  if (p.n <= 8 * kWave) {
+    if (wave == 0) keep_few<8>(a, p, keys + p.lead, keep_lds.tops, keep_lds.winners);
+  } else {
+    keep_many<kFusedWaves, kFusedMost / (kFusedWaves * kWave)>(a, p, keys + p.lead, keep_lds);
+  }
+}
+
+
+// Whether tokens mostly share their sequences (their scores are then taken several tokens a wave), and
+// whether a call is one launch: few enough places for 512 lanes to bound well, and two chunks a
+// wave or rows enough to fill the GPU (one row of 1258 blocks: 13 us in two launches, 16 in one).
+inline bool select_prompt(int64_t T, int64_t B) { return B > 0 && T >= 4 * B; }
+inline bool select_fused(int64_t T, int64_t Hkv, int64_t B, int64_t max_pages, int64_t want) {
+  return !select_prompt(T, B) && want <= 256 &&
+         max_pages <= (T * Hkv >= 128 ? kFusedMost : 2 * kFusedWaves * kChunk);
+}
+
+// gh = 0: a token a wave, its heads across `tiles` tiles. gh > 0: tokens across the lanes, gh heads
+// a pass.
 struct SelectPlan {
   int64_t stride;
   int32_t tiles, gh, per_wave, splits, head_groups;
@@ -660,9 +735,8 @@ inline SelectPlan select_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int
   const int64_t G = Hq / Hkv;
   p.stride = align_up(static_cast<size_t>(max_pages), kChunk);
   p.head_groups = static_cast<int32_t>(cdiv(Hkv, kScoreWaves));
-  // Tokens that mostly are of one sequence share a pass over its blocks; a wave with tokens of
-  // several passes over each one's.
-  if (B > 0 && T >= 4 * B) {
+  // (a wave with tokens of several sequences passes over each one's blocks)
+  if (select_prompt(T, B)) {
     const int64_t most = D <= 128 ? 8 : 4;  // heads whose columns fit in registers beside the bounds
     const int64_t gh = next_pow2(G);
     p.gh = static_cast<int32_t>(gh < most ? gh : most);
@@ -684,8 +758,10 @@ inline SelectPlan select_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int
 
 using namespace rt;
 
-extern "C" size_t rt_kv_select_workspace(int64_t T, int64_t Hkv, int64_t max_pages) {
+extern "C" size_t rt_kv_select_workspace(int64_t T, int64_t Hkv, int64_t B, int64_t max_pages,
+                                         int64_t count, int64_t sink, int64_t recent) {
   if (T < 1 || Hkv < 1 || max_pages < 1) return 0;
+  if (select_fused(T, Hkv, B, max_pages, count - sink - recent)) return 0;
   return static_cast<size_t>(T) * Hkv * align_up(static_cast<size_t>(max_pages), kChunk) *
          sizeof(uint32_t);
 }
@@ -709,7 +785,7 @@ extern "C" int rt_kv_select(const void* q, int64_t q_token_stride, int64_t q_hea
   RT_CHECK_ARG(kv_rows_aligned(q, q_token_stride, q_head_stride) && kv_rows_aligned(bounds, 0, 0),
                "rows must start on 16 bytes");
   RT_CHECK_ARG(T * Hkv <= INT32_MAX, "too many tokens");
-  const size_t need = rt_kv_select_workspace(T, Hkv, max_pages);
+  const size_t need = rt_kv_select_workspace(T, Hkv, B, max_pages, count, sink, recent);
   if (workspace_bytes < need || (need > 0 && workspace == nullptr)) {
     set_error("workspace too small: %zu < %zu", workspace_bytes, need);
     return kWorkspaceTooSmall;
@@ -725,6 +801,20 @@ extern "C" int rt_kv_select(const void* q, int64_t q_token_stride, int64_t q_hea
   a.recent = static_cast<int32_t>(recent), a.out = out, a.keys = static_cast<uint32_t*>(workspace);
   a.stride = plan.stride, a.splits = plan.splits, a.head_groups = plan.head_groups;
   const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (select_fused(T, Hkv, B, max_pages, count - sink - recent)) {
+    return kv_dispatch(dtype, D, [&](auto e, auto d) -> int {
+      using E = decltype(e);
+      constexpr int DD = decltype(d)::value;
+      const dim3 g(static_cast<unsigned>(T * Hkv)), b(kFusedWaves * kWave);
+      if (plan.tiles == 1) {
+        kv_select_kernel<E, DD, 1><<<g, b, 0, s>>>(a);
+      } else {
+        kv_select_kernel<E, DD, 2><<<g, b, 0, s>>>(a);
+      }
+      RT_CHECK_HIP(hipGetLastError());
+      return kOk;
+    });
+  }
   const int64_t grid = cdiv(T, plan.per_wave) * plan.splits * plan.head_groups;
   RT_CHECK_ARG(grid <= INT32_MAX, "too many tokens");
   if (max_pages > sink && count > sink + recent) {  // else no block is chosen by its score

@@ -218,13 +218,13 @@ def _select(q, bounds, bound_scales, positions, seq_ids, page_table, page_size, 
     lib = nat.lib()
     b, max_pages = page_table.shape
     with _on(dev):
-        need = lib.rt_kv_select_workspace(t, heads_kv, max_pages)
-        ws = bounds.new_empty((need,))
+        need = lib.rt_kv_select_workspace(t, heads_kv, b, max_pages, count, sink, recent)
+        ws = bounds.new_empty((need,)) if need else None
         st = lib.rt_kv_select(
             q.data_ptr(), q_token, q_head, t, heads, heads_kv, dim, dtype, bounds.data_ptr(),
             bound_scales.data_ptr(), pages, page_size, positions.data_ptr(), seq_ids.data_ptr(),
-            page_table.data_ptr(), b, max_pages, count, sink, recent, out.data_ptr(),
-            ws.data_ptr(), need, _stream(dev))
+            page_table.data_ptr(), b, max_pages, count, sink, recent, out.data_ptr(), nat.ptr(ws),
+            need, _stream(dev))
     if st:
         nat.check(st)
     return out

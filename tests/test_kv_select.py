@@ -102,11 +102,25 @@ def test_ties_go_to_the_lower_block(dev):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("blocks,count", [(2047, 64), (2048, 64), (4097, 100), (20000, 64),
-                                          (70001, 1000)])
-def test_long_contexts(dev, blocks, count):
-    """One token over so many blocks that their scores take several workgroups."""
-    _check(dev, blocks, "bf16", 4, 1, 64, 16, [(16 * blocks + 5, 1), (16 * 333, 1)], (count, 1, 2))
+@pytest.mark.parametrize("heads,d,blocks,count", [
+    (4, 64, 511, 64), (4, 64, 513, 64), (4, 64, 2047, 64), (4, 96, 2048, 260), (4, 64, 4095, 250),
+    (4, 64, 4096, 100), (40, 64, 4200, 300), (20, 256, 5000, 64), (4, 128, 20000, 64),
+    (4, 64, 70001, 1000)])
+def test_long_contexts(dev, heads, d, blocks, count):
+    """Single tokens around the sizes where the kernels change: one launch up to 4096 blocks, keys in
+    registers or read again."""
+    had = [(16 * blocks - 5, 1), (16 * 333, 1)]
+    _check(dev, blocks, "bf16", heads, 1, d, 16, had, (count, 1, 2))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,d,blocks,count", [(4, 64, 200, 30), (2, 128, 900, 30), (2, 64, 1000, 60),
+                                                  (1, 96, 1100, 64), (8, 64, 3000, 300),
+                                                  (16, 64, 4500, 64), (3, 192, 300, 20)])
+def test_prompts_behind_long_contexts(dev, heads, d, blocks, count):
+    """A few tokens of each sequence, over blocks that take a wave's registers, four waves' or more."""
+    had = [(16 * blocks + 9, 9), (16 * (blocks // 2), 3), (40, 5)]
+    _check(dev, blocks + 1, "fp16", heads, 1, d, 16, had, (count, 1, 2))
 
 
 @pytest.mark.gpu
