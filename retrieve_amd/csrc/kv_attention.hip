@@ -141,6 +141,13 @@ struct TileList {
   }
 };
 
+// Sixteen bytes of a cache; STREAM: of rows that are read once (not kept in L2 before others).
+template <bool STREAM, class V>
+__device__ inline V load_row(const V* p) {
+  if constexpr (STREAM) return __builtin_nontemporal_load(p);
+  return *p;
+}
+
 // A wave's accumulators (channel 16 i + 4 (lane / 16) + r of column lane % 16), the columns' maxima
 // and this lane's share of their sums; its queries and the step in flight.
 template <class E, int D>
@@ -168,24 +175,27 @@ struct AttendWave {
       qf[s] = real ? (a.minus ? -x : x) : V8{};
     }
   }
+  template <bool STREAM>
   __device__ void load_k(const AttendArgs& a, const Tiles& s) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const E* base = static_cast<const E*>(a.k_cache) + s.row[j] * D;
 #pragma unroll
       for (int i = 0; i < KS; ++i) {
-        kf[j][i] = *reinterpret_cast<const V8*>(
-            base + ((lane_id() & 15) * D + 8 * (lane_id() >> 4) + 32 * i));
+        kf[j][i] = load_row<STREAM>(reinterpret_cast<const V8*>(
+            base + ((lane_id() & 15) * D + 8 * (lane_id() >> 4) + 32 * i)));
       }
     }
   }
+  template <bool STREAM>
   __device__ void load_v(const AttendArgs& a, const Tiles& s) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const E* base = static_cast<const E*>(a.v_cache) + s.row[j] * D;
 #pragma unroll
       for (int i = 0; i < VL / 2; ++i) {
-        vf[j * (VL / 2) + i] = *reinterpret_cast<const V8*>(base + (i * 64 + lane_id()) * 8);
+        vf[j * (VL / 2) + i] =
+            load_row<STREAM>(reinterpret_cast<const V8*>(base + (i * 64 + lane_id()) * 8));
       }
     }
   }
@@ -297,6 +307,7 @@ struct AttendWave {
   }
 
   // One token's heads (tile `tile` of the group) over part of its list.
+  template <bool STREAM>
   __device__ void run(const AttendArgs& a, int64_t t, int head, int tile, int part, int parts,
                       char* lds) {
     clear();
@@ -314,14 +325,15 @@ struct AttendWave {
     Tiles now, then;
     bool more = tiles.next(a, then);
     if (more) {
-      load_k(a, then);
-      load_v(a, then);
+      load_k<STREAM>(a, then);
+      load_v<STREAM>(a, then);
     }
     while (more) {
       now = then;
       more = tiles.next(a, then);
       step(a, lds, now.n[0] == 16 && now.n[1] == 16, now.n, now.n,
-           [&] { if (more) load_k(a, then); }, [&] { if (more) load_v(a, then); });
+           [&] { if (more) load_k<STREAM>(a, then); },
+           [&] { if (more) load_v<STREAM>(a, then); });
     }
     join_sums();
   }
@@ -363,7 +375,7 @@ __global__ void __launch_bounds__(kAttendWaves* kWave, D <= 128 ? 2 : 1)
   if (t >= a.T) return;
   const int head = blockIdx.x % heads / a.tiles, tile = blockIdx.x % heads % a.tiles;
   AttendWave<E, D> w;
-  w.run(a, t, head, tile, 0, 1, lds[wave]);
+  w.template run<false>(a, t, head, tile, 0, 1, lds[wave]);
   const int g = tile * 16 + (lane_id() & 15);
   if (g < a.G) emit(a, w, t, head * a.G + g);
 }
@@ -761,7 +773,17 @@ __global__ void __launch_bounds__(kAttendWaves* kWave, D <= 128 ? 2 : 1)
   const int head = static_cast<int>(row / a.tiles % a.Hkv);
   const int64_t t = row / a.tiles / a.Hkv;
   AttendWave<E, D> w;
-  w.run(a, t, head, tile, part * kAttendWaves + wave, a.parts * kAttendWaves, lds[wave]);
+  // A token beside one of its own sequence chooses mostly its blocks: these stay in L2. Others' rows
+  // are read once.
+  const int32_t seq = a.tok.seq_ids[t];
+  const bool beside = (t > 0 && a.tok.seq_ids[t - 1] == seq) ||
+                      (t + 1 < a.T && a.tok.seq_ids[t + 1] == seq);
+  const int first = part * kAttendWaves + wave, parts = a.parts * kAttendWaves;
+  if (beside) {
+    w.template run<false>(a, t, head, tile, first, parts, lds[wave]);
+  } else {
+    w.template run<true>(a, t, head, tile, first, parts, lds[wave]);
+  }
   // the sums as fp32 rows of a head, 16-byte chunks permuted by the head (bank conflicts)
   const int col = lane_id() & 15, grp = lane_id() >> 4;
 #pragma unroll
@@ -818,9 +840,11 @@ __global__ void __launch_bounds__(D / 4) kv_join_kernel(AttendArgs a) {
   const int64_t row = (t * a.Hkv + head) * a.tiles + g / 16;
   const int64_t first = row * a.parts * 16 + g % 16;
   float m = a.part_ml[2 * first];
+#pragma unroll 8
   for (int p = 1; p < a.parts; ++p) m = fmaxf(m, a.part_ml[2 * (first + 16 * p)]);
   float l = 0.0f;
   v4f sum{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
   for (int p = 0; p < a.parts; ++p) {
     const int64_t at = first + 16 * p;
     const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * at] - m);
@@ -841,7 +865,8 @@ struct AttendPlan {
   int32_t tiles, parts, joined;
 };
 
-inline AttendPlan attend_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t page, int64_t count) {
+inline AttendPlan attend_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t page,
+                              int64_t count) {
   AttendPlan p;
   const int64_t G = Hq / Hkv;
   p.tiles = static_cast<int32_t>(cdiv(G, 16));
@@ -851,7 +876,10 @@ inline AttendPlan attend_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t page, 
   if (joined > kJoinTokens) joined = kJoinTokens;
   const int64_t lists = kJoinMost / (kJoinWaves * (count > 0 ? count : 1));
   p.joined = static_cast<int32_t>(joined < lists ? joined : lists);
-  if (p.rows >= 4096) return p;
+  // A joined workgroup's chain of steps takes as long for few tokens as for many: us for lists of 16
+  // blocks of 64 keys, 32 heads of 8 key/value heads, split and joined, at 400 and 511 tokens:
+  // D 64: 63 and 105, 76 and 97; D 128: 120 and 121, 148 and 113; D 256: 321 and 193, 395 and 168.
+  if (p.joined > 1 ? p.rows * D >= 400 << 10 : p.rows >= 4096) return p;
   // workgroups of four waves for two on every CU, each wave with a unit of 64 keys at least
   const int64_t most = cdiv(count * page, 64 * kAttendWaves);
   const int64_t want = cdiv(512, p.rows > 0 ? p.rows : 1);
@@ -867,7 +895,7 @@ using namespace rt;
 extern "C" size_t rt_kv_attention_workspace(int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
                                             int64_t page, int64_t count) {
   if (Hkv < 1 || T < 1) return 0;
-  const AttendPlan p = attend_plan(T, Hq, Hkv, page, count);
+  const AttendPlan p = attend_plan(T, Hq, Hkv, D, page, count);
   return p.parts > 1 ? static_cast<size_t>(p.rows) * p.parts * 16 * (D + 2) * sizeof(float) : 0;
 }
 
@@ -895,7 +923,7 @@ extern "C" int rt_kv_attention(const void* q, int64_t q_token_stride, int64_t q_
     set_error("workspace too small: %zu < %zu", workspace_bytes, need);
     return kWorkspaceTooSmall;
   }
-  const AttendPlan plan = attend_plan(T, Hq, Hkv, page, count);
+  const AttendPlan plan = attend_plan(T, Hq, Hkv, D, page, count);
   AttendArgs a{};
   a.q = q, a.q_st = q_token_stride, a.q_sh = q_head_stride, a.T = T;
   a.Hq = static_cast<int32_t>(Hq), a.Hkv = static_cast<int32_t>(Hkv);

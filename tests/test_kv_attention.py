@@ -110,7 +110,7 @@ MANY = [("bf16", 1, 1, 64, 16, 9), ("fp16", 2, 1, 128, 64, 5), ("bf16", 3, 1, 96
 def _many(seed, kind, heads, heads_kv, d, page, count):
     """More rows than the GPU holds waves (a wave then takes a row, or several tokens at once), of three
     sequences; neighbours choose alike in the first and last, by chance in the second."""
-    had_new = [(3 * page + 5, 2000), (0, 2300 // heads_kv), (40, 7)]
+    had_new = [(3 * page + 5, 2000), (0, 5000 // heads_kv), (40, 7)]
     case = list(_case(seed, kind, heads, heads_kv, d, page, had_new, count, sparse=0.1))
     blocks, pos = case[3], case[4]
     for t in range(1, 2000):
@@ -136,7 +136,7 @@ def test_many_rows(dev, kind, heads, heads_kv, d, page, count):
     case = _many(heads + count, kind, heads, heads_kv, d, page, count)
     got = _run(dev, kind, *case)
     tokens = len(case[4])
-    assert tokens * heads_kv >= 4096
+    assert tokens * heads_kv >= 4096 and tokens * heads_kv * d >= 400 << 10
     pick = np.r_[0:9, 31:45, 1990:2012, rng(5).integers(0, tokens, 60), tokens - 9:tokens]
     got, case = _some(got, case, pick)
     _check(got, kind, *case)
@@ -147,7 +147,7 @@ def test_many_rows(dev, kind, heads, heads_kv, d, page, count):
 def test_many_rows_and_values_that_are_not_finite(dev, heads):
     """Neighbours that choose different blocks: a NaN key or an infinite value reaches the tokens whose
     lists hold it, and no other; slots past every token's are NaN; padding among the tokens."""
-    page, tokens = 16, 4200
+    page, tokens = 16, 6700
     q, kc, vc, blocks, pos, seq, tab = _case(71, "bf16", heads, 1, 64, page, [(16 * 7 + 3, 1)], 4)
     q = normal16(72, (tokens, heads, 64), "bf16")
     pos, seq = np.full(tokens, 16 * 7 + 3, np.int32), np.zeros(tokens, np.int32)
@@ -157,7 +157,7 @@ def test_many_rows_and_values_that_are_not_finite(dev, heads):
     kc[tab[0, 7], 0, 4:], vc[tab[0, 7], 0, 4:] = np.nan, np.nan
     clean = _run(dev, "bf16", q, kc, vc, blocks, pos, seq, tab)
     kc0, vc0 = np.nan_to_num(kc), np.nan_to_num(vc)
-    pick = np.r_[0:80, 4100:4200]
+    pick = np.r_[0:80, 6600:6700]
     got, case = _some(clean, (q, kc0, vc0, blocks, pos, seq, tab), pick)
     _check(got, "bf16", *case)
     kc[tab[0, 1], 0, 3, 5], vc[tab[0, 6], 0, 2, 9] = np.nan, np.inf
