@@ -25,7 +25,8 @@ PAGE = 64
 class Layer(torch.nn.Module):
     """Projections around the cache's three calls."""
 
-    def __init__(self, heads: int, heads_kv: int, dim: int, cache: PagedCache, cos_sin, chosen: int):
+    def __init__(self, heads: int, heads_kv: int, dim: int, cache: PagedCache, cos_sin,
+                 chosen: int):
         super().__init__()
         width = heads * dim
         self.heads, self.heads_kv, self.dim, self.chosen = heads, heads_kv, dim, chosen

@@ -1,7 +1,8 @@
 """The paged cache's operators in numpy (test infrastructure; see ``oracle/__init__``).
 
-Values of 16-bit types are held as float32 arrays; ``round16`` rounds to them. ``append`` follows the
-kernels' single fp32 roundings (bit-exact), ``append64`` and ``attention`` the formulas in 64 bits,
+Values of 16-bit types are held as float32 arrays; ``round16`` rounds to them. ``append`` follows
+the kernels' single fp32 roundings (bit-exact), ``append64`` and ``attention`` the formulas in 64
+bits,
 ``select`` integers. ``blocks_by_bounds`` states the selection a second time, over exact rationals.
 """
 
@@ -15,7 +16,8 @@ from oracle import quantize as oq
 
 
 def round16(x: np.ndarray, kind: str) -> np.ndarray:
-    """float32 or float64 values to the nearest ``"bf16"`` or ``"fp16"`` (ties to even), as float32."""
+    """float32 or float64 values to the nearest ``"bf16"`` or ``"fp16"`` (ties to even), as
+    float32."""
     if kind == "fp16":
         with np.errstate(over="ignore"):
             return np.asarray(x).astype(np.float16).astype(np.float32)
@@ -121,8 +123,9 @@ def most_a_block_can_score(q, stored) -> np.ndarray:
 
 
 def attention(q, k_cache, v_cache, blocks, positions, seq_ids, page_table, scale):
-    """``(out, lse, spread, slack)`` in 64 bits: ``spread`` = the weights' sum over ``|v|`` (what a relative
-    error of every weight can move an output by), ``slack [T, Hq]`` = the largest ``|scale| sum |q k|``."""
+    """``(out, lse, spread, slack)`` in 64 bits: ``spread`` = the weights' sum over ``|v|`` (what a
+    relative error of every weight can move an output by), ``slack [T, Hq]`` = the largest ``|scale|
+    sum |q k|``."""
     pages, heads_kv, page, d = k_cache.shape
     t, heads, _ = q.shape
     out, spread = np.zeros((t, heads, d)), np.zeros((t, heads, d))
@@ -153,8 +156,8 @@ def attention(q, k_cache, v_cache, blocks, positions, seq_ids, page_table, scale
 
 
 def blocks_by_bounds(q_codes, q_scales, codes, scale, want):
-    """The ``want`` best blocks of one head group over exact rationals (no fp32 rounding), ties to the
-    lower block: what ``select`` gives wherever no two scores are within fp32 rounding."""
+    """The ``want`` best blocks of one head group over exact rationals (no fp32 rounding), ties to
+    the lower block: what ``select`` gives wherever no two scores are within fp32 rounding."""
     def score(b):
         return max(Fraction(int(sum(int(c) * int(m) for c, m in zip(row, codes[b][:len(row)]))
                                 + sum(abs(int(c)) * int(m)

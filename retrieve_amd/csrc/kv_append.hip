@@ -6,16 +6,16 @@
 // multiply-add), then to the cache's 16 bits: the same bits whichever tile a token falls in, so
 // a block's bounds do not depend on how its tokens were split over calls.
 //
-// Bounds of a full block: per channel lo and hi over its stored keys, mid = (lo + hi) / 2 and half =
-// (hi - lo) / 2, the row [mid | half] as int8 codes of one scale. q . mid + |q| . half is then the
-// most that any key of the block can score with q. Minimum and maximum do not depend on the
+// Bounds of a full block: per channel lo and hi over its stored keys, mid = (lo + hi) / 2 and half
+// = (hi - lo) / 2, the row [mid | half] as int8 codes of one scale. q . mid + |q| . half is then
+// the most that any key of the block can score with q. Minimum and maximum do not depend on the
 // order, so the codes are the same in any split.
 //
 // One launch. Some workgroups look for tokens that complete a block: the block's keys that are part
 // of this call are rotated again from the input (no wait on the waves that store them), the
-// earlier ones come from the cache. In the others a wave moves a token's rows (or some of them, where
-// there are few tokens): a lane holds two 16-byte chunks of a row, which in the split layout are
-// partners, with their cosines and sines, and walks over the heads, two rows in flight.
+// earlier ones come from the cache. In the others a wave moves a token's rows (or some of them,
+// where there are few tokens): a lane holds two 16-byte chunks of a row, which in the split layout
+// are partners, with their cosines and sines, and walks over the heads, two rows in flight.
 //
 // Bound by memory: every row is read and written once. 32768 tokens of 32 rows of 256 channels
 // take 238 us (4.7 TB/s, what a large copy reaches) with nontemporal loads and stores, 283 us with
@@ -112,7 +112,8 @@ __device__ inline typename Kv<E>::V8 rotated_chunk(const E* row, typename Kv<E>:
 #pragma unroll
     for (int e = 0; e < 8; ++e) y[e] = x[e ^ 1];
   } else if (MODE == kRotHalf) {
-    y = *reinterpret_cast<const V8*>(row + (8 * chunk < half ? 8 * chunk + half : 8 * chunk - half));
+    const int other = 8 * chunk < half ? 8 * chunk + half : 8 * chunk - half;
+    y = *reinterpret_cast<const V8*>(row + other);
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -271,7 +272,8 @@ __device__ inline void fill_bounds(const AppendArgs& a) {
           Turn<MODE> turn;
           if (a.rot > 0) turn.load(a, pos, chunk);
           const E* row = k + from * a.k_st;
-          x = rotated_chunk<E, MODE>(row, reinterpret_cast<const V8*>(row)[chunk], chunk, turn, a.rot);
+          x = rotated_chunk<E, MODE>(row, reinterpret_cast<const V8*>(row)[chunk], chunk, turn,
+                                     a.rot);
         } else {
           x = *reinterpret_cast<const V8*>(static_cast<const E*>(a.k_cache) +
                                            cache_row<D>(a, page, head, pos) + 8 * chunk);

@@ -20,6 +20,9 @@
 //
 // Memory: a wave keeps the next step's keys and values in flight (registers) while it works on
 // this one. Slots past the token's position are read but replaced: scores by -inf, values by 0.
+// Single tokens are bound by the cache's bytes: 64 sequences of lists of 64 blocks, 64 keys of 128
+// channels a block, 8 key/value heads take 168 us (6.3 TB/s). Prompts read most blocks from L2 and
+// are bound by the steps' instructions (2053 tokens of 32 heads over 16 blocks: 141 us).
 #include <type_traits>
 
 #include "../../include/retrieve_amd.h"
@@ -141,7 +144,9 @@ struct TileList {
   }
 };
 
-// Sixteen bytes of a cache; STREAM: of rows that are read once (not kept in L2 before others).
+// Sixteen bytes of a cache; STREAM: of rows that are read once (not kept in L2 before others: 64
+// sequences of 64 blocks 168 us, 187 with ordinary loads; 400 tokens of prompts, which share
+// blocks, 157 us streamed and 121 with ordinary loads).
 template <bool STREAM, class V>
 __device__ inline V load_row(const V* p) {
   if constexpr (STREAM) return __builtin_nontemporal_load(p);
@@ -199,8 +204,8 @@ struct AttendWave {
       }
     }
   }
-  // One step on what load_k and load_v brought; `fetch_k` and `fetch_v` start the next one's loads as
-  // soon as the registers are free. A column's keys count up to n[j] in tile j; V's rows from
+  // One step on what load_k and load_v brought; `fetch_k` and `fetch_v` start the next one's loads
+  // as soon as the registers are free. A column's keys count up to n[j] in tile j; V's rows from
   // rows[j] on are read as zeros (slots that may never have been written).
   template <class FK, class FV>
   __device__ void step(const AttendArgs& a, char* lds, bool whole, const int (&n)[2],
@@ -234,9 +239,9 @@ struct AttendWave {
     add(lds, p);
     asm volatile("" ::: "memory");
   }
-  // The weights of the scores of N tiles (key 4 (lane / 16) + r of tile j at 4 (j % 2) + r of p[j / 2]),
-  // rounded for the second product; the maximum raised and the sum extended. A column counts the
-  // first n[j] keys of tile j (all where `whole`).
+  // The weights of the scores of N tiles (key 4 (lane / 16) + r of tile j at 4 (j % 2) + r of p[j /
+  // 2]), rounded for the second product; the maximum raised and the sum extended. A column counts
+  // the first n[j] keys of tile j (all where `whole`).
   template <int N>
   __device__ void weigh(float scale, v4f (&sc)[N], bool whole, const int (&n)[N],
                         V8 (&p)[N / 2]) {
@@ -363,8 +368,9 @@ __device__ inline void emit(const AttendArgs& a, const AttendWave<E, D>& w, int6
   if (grp == 0) a.lse[row] = log_sum(w.m, w.l);
 }
 
-// Many rows: a wave a row, four neighbouring tokens of one head a workgroup (they mostly choose the
-// same blocks).
+// Many rows (from 4096, when the GPU holds no more waves): a wave a row, four neighbouring tokens
+// of one head a workgroup (they mostly choose the same blocks). For groups of more than 8 heads,
+// which fill the columns of a wave by themselves, and lists too long to be joined.
 template <class E, int D>
 __global__ void __launch_bounds__(kAttendWaves* kWave, D <= 128 ? 2 : 1)
     kv_attend_rows_kernel(AttendArgs a) {
@@ -389,7 +395,8 @@ __device__ inline void attend_alone(const AttendArgs& a, int64_t t, int head, in
   const int lane = lane_id();
   const KvPlace p = kv_place(a.tok, t);
   const E* q = static_cast<const E*>(a.q) + t * a.q_st + hq * a.q_sh;
-  for (int d = lane; d < D; d += kWave) qs[d] = static_cast<float>(q[d]) * (a.minus ? -a.scale : a.scale);
+  const float scale = a.minus ? -a.scale : a.scale;
+  for (int d = lane; d < D; d += kWave) qs[d] = static_cast<float>(q[d]) * scale;
   asm volatile("" ::: "memory");
   const int size = 1 << a.tok.shift;
   float m = -3.402823466e38f, l = 0.0f, acc[R] = {};
@@ -759,8 +766,9 @@ __global__ void __launch_bounds__(kJoinWaves* kWave, D <= 128 ? 4 : 2)
   }
 }
 
-// Few rows: the workgroup's waves (and `parts` workgroups) share a row's list; their sums are joined
-// at the largest maximum, here where one workgroup has the whole row, else by kv_join_kernel.
+// Few rows: the workgroup's waves (and `parts` workgroups) share a row's list; their sums are
+// joined at the largest maximum, here where one workgroup has the whole row, else by
+// kv_join_kernel.
 template <class E, int D>
 __global__ void __launch_bounds__(kAttendWaves* kWave, D <= 128 ? 2 : 1)
     kv_attend_split_kernel(AttendArgs a) {
@@ -773,8 +781,8 @@ __global__ void __launch_bounds__(kAttendWaves* kWave, D <= 128 ? 2 : 1)
   const int head = static_cast<int>(row / a.tiles % a.Hkv);
   const int64_t t = row / a.tiles / a.Hkv;
   AttendWave<E, D> w;
-  // A token beside one of its own sequence chooses mostly its blocks: these stay in L2. Others' rows
-  // are read once.
+  // A token beside one of its own sequence chooses mostly its blocks: these stay in L2. Others'
+  // rows are read once.
   const int32_t seq = a.tok.seq_ids[t];
   const bool beside = (t > 0 && a.tok.seq_ids[t - 1] == seq) ||
                       (t + 1 < a.T && a.tok.seq_ids[t + 1] == seq);
@@ -876,11 +884,13 @@ inline AttendPlan attend_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int
   if (joined > kJoinTokens) joined = kJoinTokens;
   const int64_t lists = kJoinMost / (kJoinWaves * (count > 0 ? count : 1));
   p.joined = static_cast<int32_t>(joined < lists ? joined : lists);
-  // A joined workgroup's chain of steps takes as long for few tokens as for many: us for lists of 16
-  // blocks of 64 keys, 32 heads of 8 key/value heads, split and joined, at 400 and 511 tokens:
+  // A joined workgroup's chain of steps takes as long for few tokens as for many: us for lists of
+  // 16 blocks of 64 keys, 32 heads of 8 key/value heads, split and joined, at 400 and 511 tokens:
   // D 64: 63 and 105, 76 and 97; D 128: 120 and 121, 148 and 113; D 256: 321 and 193, 395 and 168.
   if (p.joined > 1 ? p.rows * D >= 400 << 10 : p.rows >= 4096) return p;
-  // workgroups of four waves for two on every CU, each wave with a unit of 64 keys at least
+  // Workgroups of four waves for two on every CU, each wave with a unit of 64 keys at least. A
+  // second launch that joins the parts costs 4 us, a row in one workgroup more: one token of 8
+  // heads over 32 blocks of 64 keys takes 12 us in 8 parts a row, 23 in one workgroup of 8 waves.
   const int64_t most = cdiv(count * page, 64 * kAttendWaves);
   const int64_t want = cdiv(512, p.rows > 0 ? p.rows : 1);
   p.parts = static_cast<int32_t>(want < most ? want : most);

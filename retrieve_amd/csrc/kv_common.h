@@ -64,10 +64,11 @@ __device__ inline int kv_code(float x, float top) {
   return static_cast<int>(fminf(fmaxf(v, -127.0f), 127.0f));
 }
 
-// The same code by a reciprocal r = 1 / top (rounded to nearest): q = x r, then q + r (x - q top) is the
-// quotient rounded to nearest wherever |x| <= top, top is normal and its significand is not all
-// ones (Markstein's theorem; queries of 16 bits have neither), in 3 instructions instead of about
-// ten. For a top above 2^100, whose reciprocal may lose bits, x and top come in scaled by 2^-64.
+// The same code by a reciprocal r = 1 / top (rounded to nearest): q = x r, then q + r (x - q top)
+// is the quotient rounded to nearest wherever |x| <= top, top is normal and its significand is not
+// all ones (Markstein's theorem; queries of 16 bits have neither), in 3 instructions instead of
+// about ten. For a top above 2^100, whose reciprocal may lose bits, x and top come in scaled by
+// 2^-64.
 __device__ inline float kv_code_value(float x, float top, float r) {
 #pragma clang fp contract(off)
   const float q = x * r;
@@ -75,9 +76,9 @@ __device__ inline float kv_code_value(float x, float top, float r) {
   return fmaxf(rintf(quotient * 127.0f), -127.0f);  // (NaN: -127)
 }
 
-// Eight wait states behind matrix products, before x is read. The compiler counts them itself within a
-// block, but not where a branch comes between a product and its first use: the path that takes
-// the branch then reads the old registers.
+// Eight wait states behind matrix products, before x is read. The compiler counts them itself
+// within a block, but not where a branch comes between a product and its first use: the path that
+// takes the branch then reads the old registers.
 template <class V, int N>
 __device__ inline void settle(V (&x)[N]) {
   if constexpr (N == 1) {

@@ -15,9 +15,17 @@
 // head of 16 tokens, the largest over the heads found within the lane; the tokens of one sequence
 // share the pass over its blocks. One key a (token, head, block) is left behind.
 //
-// Keep: few blocks by a wave, which bisects over the keys' bits from the highest in which they differ
-// until the count is exact. Many by a workgroup: the want-th largest of the lanes' largest keys is
-// a bound that at least `want` keys reach and few more; those are ranked against each other.
+// Bound: single tokens by the bounds' bytes, 2 D a (block, head) in scattered pieces (64 sequences
+// of 16K to 131K tokens in blocks of 64, 8 heads of 128 channels: 53 us, 2.9 TB/s, the longest
+// row's chain behind the others), one launch for up to 4096 blocks; a million tokens of one
+// sequence take 13 us of scores and 8 of keeping. Prompts by the vector instructions: a column's
+// codes (ten instructions a channel) and a block's key (about seven a head): 4099 tokens over 9K
+// to 30K take 77 us.
+//
+// Keep: few blocks by a wave, which bisects over the keys' bits from the highest in which they
+// differ until the count is exact. Many by a workgroup: the want-th largest of the lanes' largest
+// keys is a bound that at least `want` keys reach and few more; those are ranked against each
+// other.
 #include <type_traits>
 
 #include "../../include/retrieve_amd.h"
@@ -100,8 +108,8 @@ __device__ inline void pack_codes(const V8 (&x)[2], float top, float r, float sm
   }
 }
 
-// A wave holds NT tiles of 16 columns. GH = 0 (decode): one token, column = query head, 16 NT heads a
-// pass. GH > 0 (prompts): column = token, tile n = head n % GH of token group n / GH, GH heads a
+// A wave holds NT tiles of 16 columns. GH = 0 (decode): one token, column = query head, 16 NT heads
+// a pass. GH > 0 (prompts): column = token, tile n = head n % GH of token group n / GH, GH heads a
 // pass (heads past the group's repeat its last).
 // Chunks first, first + step, ... of 64 blocks are scored; `put(token, block)` is where the keys of
 // four blocks go.
@@ -266,8 +274,8 @@ __device__ inline void score_blocks(const SelectArgs& a, int64_t t0, int head, i
           for (int s = 0; s < KS; ++s) {
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              acc[n] =
-                  __builtin_amdgcn_mfma_i32_16x16x64_i8(bf[i % FLIGHT][s], cf[n][s], acc[n], 0, 0, 0);
+              acc[n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bf[i % FLIGHT][s], cf[n][s],
+                                                             acc[n], 0, 0, 0);
             }
           }
           settle(acc);
@@ -319,8 +327,9 @@ __device__ inline void score_blocks(const SelectArgs& a, int64_t t0, int head, i
   }
 }
 
-// Four heads of 128 channels are worth three waves a SIMD with half the tiles in flight (prompts of 4099
-// tokens: 78 us with the kept, 84 with two waves and four tiles); wider columns take two waves or one.
+// Four heads of 128 channels are worth three waves a SIMD with half the tiles in flight (prompts of
+// 4099 tokens: 78 us with the kept, 84 with two waves and four tiles); wider columns take two waves
+// or one.
 template <int D, int NT, int GH>
 constexpr int kScoreOccupancy = D == 128 && GH == 4 ? 3 : D > 128 && NT == 4 ? 1 : 2;
 
@@ -345,7 +354,8 @@ __global__ void __launch_bounds__(kScoreWaves* kWave, (kScoreOccupancy<D, NT, GH
 
 // --- keep ---------------------------------------------------------------------------------------
 
-// A row's blocks: `lead` forced ones, n candidates, `tail` forced ones; `want` places for candidates.
+// A row's blocks: `lead` forced ones, n candidates, `tail` forced ones; `want` places for
+// candidates.
 struct Span {
   int32_t* out;
   int32_t lead, n, end, tail;
@@ -370,8 +380,8 @@ struct Span {
   }
 };
 
-// A row's candidates as a workgroup of WAVES waves holds them: even shares of neighbours, up to R keys
-// a lane. R = 0: any number, read again where they are needed.
+// A row's candidates as a workgroup of WAVES waves holds them: even shares of neighbours, up to R
+// keys a lane. R = 0: any number, read again where they are needed.
 template <int WAVES, int R>
 struct Row {
   uint32_t k[R > 0 ? R : 1];
@@ -479,8 +489,9 @@ __device__ inline uint32_t keep_in_order(const Span& p, const uint32_t (&k)[N], 
   return kept;
 }
 
-// A wave a row, R keys a lane. Where few are wanted of many: the want-th largest of the lanes' largest
-// keys bounds the cut; the keys that reach it, one a lane if they are 64 or fewer, hold the kept.
+// A wave a row, R keys a lane. Where few are wanted of many: the want-th largest of the lanes'
+// largest keys bounds the cut; the keys that reach it, one a lane if they are 64 or fewer, hold the
+// kept.
 template <int R>
 __device__ inline void keep_few(const SelectArgs& a, const Span& p, const uint32_t* keys,
                                 uint32_t* near, int32_t* near_at) {
@@ -581,7 +592,9 @@ __device__ inline void keep_many(const SelectArgs& a, const Span& p, const uint3
           [&](uint32_t probe) {
             uint32_t n = 0;
 #pragma unroll
-            for (int i = 0; i < N; ++i) n += static_cast<uint32_t>(__popcll(__ballot(g[i] >= probe)));
+            for (int i = 0; i < N; ++i) {
+              n += static_cast<uint32_t>(__popcll(__ballot(g[i] >= probe)));
+            }
             return n;
           },
           reach);
@@ -597,7 +610,8 @@ __device__ inline void keep_many(const SelectArgs& a, const Span& p, const uint3
         return f > t ? f : t;
       });
     } else {
-      cut = cut_of(std::integral_constant<int, WAVES>{}, [&](int i) { return tops[64 * i + lane]; });
+      cut = cut_of(std::integral_constant<int, WAVES>{},
+                   [&](int i) { return tops[64 * i + lane]; });
     }
     if (lane == 0) lds.cut = cut;
   }
@@ -624,7 +638,9 @@ __device__ inline void keep_many(const SelectArgs& a, const Span& p, const uint3
       uint32_t rank = 0;
 #pragma unroll 8
       for (uint32_t j = 0; j < n; ++j) rank += near[j] > x ? 1u : 0u;
-      if (rank < p.want) winners[rank] = static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(x));
+      if (rank < p.want) {
+        winners[rank] = static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(x));
+      }
     }
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < kept; i += LANES) {
@@ -694,9 +710,9 @@ __global__ void __launch_bounds__(WAVES* kWave) kv_keep_many_kernel(SelectArgs a
 }
 
 // Both in one launch, a workgroup a (token, key/value head): decode over page tables of up to
-// kFusedMost blocks. The keys stay in LDS. Workgroups go to the eight XCDs in turn: each takes rows side
-// by side, as the heads of a token share lines of the page table and of the scales (64 sequences, 8
-// heads: 53 us, 57 with the heads spread).
+// kFusedMost blocks. The keys stay in LDS. Workgroups go to the eight XCDs in turn: each takes rows
+// side by side, as the heads of a token share lines of the page table and of the scales (64
+// sequences, 8 heads: 53 us, 57 with the heads spread).
 constexpr int kFusedWaves = 8;
 constexpr int kFusedMost = 4096;
 
@@ -723,8 +739,8 @@ __global__ void __launch_bounds__(kFusedWaves* kWave, D <= 128 && NT == 1 ? 4 : 
 }
 
 
-// Whether tokens mostly share their sequences (their scores are then taken several tokens a wave), and
-// whether a call is one launch: few enough places for 512 lanes to bound well, and two chunks a
+// Whether tokens mostly share their sequences (their scores are then taken several tokens a wave),
+// and whether a call is one launch: few enough places for 512 lanes to bound well, and two chunks a
 // wave or rows enough to fill the GPU (one row of 1258 blocks: 13 us in two launches, 16 in one).
 inline bool select_prompt(int64_t T, int64_t B) { return B > 0 && T >= 4 * B; }
 inline bool select_fused(int64_t T, int64_t Hkv, int64_t B, int64_t max_pages, int64_t want) {
@@ -747,7 +763,8 @@ inline SelectPlan select_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int
   p.head_groups = static_cast<int32_t>(cdiv(Hkv, kScoreWaves));
   // (a wave with tokens of several sequences passes over each one's blocks)
   if (select_prompt(T, B)) {
-    const int64_t most = D <= 128 ? 8 : 4;  // heads whose columns fit in registers beside the bounds
+    // heads whose columns fit in registers beside the bounds
+    const int64_t most = D <= 128 ? 8 : 4;
     const int64_t gh = next_pow2(G);
     p.gh = static_cast<int32_t>(gh < most ? gh : most);
     p.tiles = p.gh < 4 ? 4 : p.gh;

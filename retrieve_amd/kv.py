@@ -1,7 +1,7 @@
 """A language model's paged key/value cache searched by block, as ``torch.ops.retrieve_kv.*``.
 
-At long contexts a token attends to the few blocks of the cache whose keys can score highest with its
-query, found the way the scans find items: int8 codes, int32 sums, exact selection with ties
+At long contexts a token attends to the few blocks of the cache whose keys can score highest with
+its query, found the way the scans find items: int8 codes, int32 sums, exact selection with ties
 to the lower index. Three ops over one layer's cache, in the order a model's layer calls them:
 
 - :func:`append`: new tokens' queries, keys and values rotated, keys and values written to their
@@ -9,15 +9,18 @@ to the lower index. Three ops over one layer's cache, in the order a model's lay
 - :func:`select_blocks`: the best blocks of each token and key/value head by those bounds;
 - :func:`block_attention`: softmax attention over the chosen blocks.
 
-Tokens are packed: token ``t`` is at ``positions[t]`` of sequence ``seq_ids[t]``, a row of ``page_table``
+Tokens are packed: token ``t`` is at ``positions[t]`` of sequence ``seq_ids[t]``, a row of
+``page_table``
 ``[B, max_pages]`` (the physical page of each block of ``page`` tokens, -1 for none), all int32. One
 token a sequence is a decode step, many a prompt; a call may mix them. Caches are ``[P, Hkv, page,
-D]`` (a block of one head is contiguous), bounds int8 ``[P, Hkv, 2 D]`` with scales fp32 ``[P, Hkv]``.
+D]`` (a block of one head is contiguous), bounds int8 ``[P, Hkv, 2 D]`` with scales fp32 ``[P,
+Hkv]``.
 :class:`PagedCache` holds them and makes the three calls; :func:`rotary_table` builds the table of
 cosines and sines. No counterpart in the reference; serving only (no gradients).
 
-The ops check their arguments here (``ValueError`` on shapes, ``TypeError`` on dtypes), allocate from
-torch's caching allocator and enqueue on torch's current stream, without a host synchronization.
+The ops check their arguments here (``ValueError`` on shapes, ``TypeError`` on dtypes), allocate
+from torch's caching allocator and enqueue on torch's current stream, without a host
+synchronization.
 """
 
 from __future__ import annotations
@@ -36,8 +39,8 @@ PAGE_SIZES = (16, 32, 64, 128)
 MAX_COUNT = 1024
 
 _lib = torch.library.Library("retrieve_kv", "DEF")
-_lib.define("append(Tensor q, Tensor k, Tensor v, Tensor? cos_sin, Tensor positions, Tensor seq_ids, "
-            "Tensor page_table, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!) bounds, "
+_lib.define("append(Tensor q, Tensor k, Tensor v, Tensor? cos_sin, Tensor positions, "
+            "Tensor seq_ids, Tensor page_table, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!) bounds, "
             "Tensor(d!) bound_scales, bool interleaved=False) -> Tensor")
 _lib.define("select_blocks(Tensor q, Tensor bounds, Tensor bound_scales, Tensor positions, "
             "Tensor seq_ids, Tensor page_table, int page_size, int count, int sink=1, "
@@ -130,8 +133,9 @@ _stream = torch._C._cuda_getCurrentRawStream  # (the current stream's handle, wi
 
 
 def _eager(q: Tensor) -> bool:
-    """Whether a call can go straight to its kernels: plain tensors, nothing being traced. Elsewhere it
-    goes through the registered op (the dispatcher's 3 to 5 us a call are a third of a small one)."""
+    """Whether a call can go straight to its kernels: plain tensors, nothing being traced. Elsewhere
+    it goes through the registered op (the dispatcher's 3 to 5 us a call are a third of a small
+    one)."""
     return type(q) is Tensor and not torch.compiler.is_compiling()
 
 
@@ -181,17 +185,18 @@ def _append(q, k, v, cos_sin, positions, seq_ids, page_table, k_cache, v_cache, 
 def append(q: Tensor, k: Tensor, v: Tensor, cos_sin: Tensor | None, positions: Tensor,
            seq_ids: Tensor, page_table: Tensor, k_cache: Tensor, v_cache: Tensor, bounds: Tensor,
            bound_scales: Tensor, interleaved: bool = False) -> Tensor:
-    """Rotates the new tokens' queries ``q [T, Hq, D]`` and keys ``k [T, Hkv, D]`` and writes keys and
-    values ``v [T, Hkv, D]`` to their slots; returns the rotated queries. Any token and head strides (the
-    views of a fused projection are read where they lie).
+    """Rotates the new tokens' queries ``q [T, Hq, D]`` and keys ``k [T, Hkv, D]`` and writes keys
+    and values ``v [T, Hkv, D]`` to their slots; returns the rotated queries. Any token and head
+    strides (the views of a fused projection are read where they lie).
 
     ``cos_sin [length, rot]`` fp32 holds a position's ``rot / 2`` cosines, then its sines
     (:func:`rotary_table`); channels ``(i, i + rot / 2)`` turn together, ``(2 i, 2 i + 1)`` with
-    ``interleaved``; channels from ``rot`` on stay as they are; None rotates nothing. A token at the last
-    slot of its block fills the block's ``bounds``: ``[mid | half]`` of its stored keys' least and
-    largest values per channel, quantised as ``quantize_int8``'s rows. For that a sequence's
-    tokens come in order, side by side. Tokens that are padding (a position below 0, or past the page
-    table or ``cos_sin``; a sequence outside it; no page) write nothing and return a zero row."""
+    ``interleaved``; channels from ``rot`` on stay as they are; None rotates nothing. A token at the
+    last slot of its block fills the block's ``bounds``: ``[mid | half]`` of its stored keys' least
+    and largest values per channel, quantised as ``quantize_int8``'s rows. For that a sequence's
+    tokens come in order, side by side. Tokens that are padding (a position below 0, or past the
+    page table or ``cos_sin``; a sequence outside it; no page) write nothing and return a zero
+    row."""
     call = _append if _eager(q) else torch.ops.retrieve_kv.append
     return call(q, k, v, cos_sin, positions, seq_ids, page_table, k_cache, v_cache, bounds,
                 bound_scales, interleaved)
@@ -233,13 +238,15 @@ def _select(q, bounds, bound_scales, positions, seq_ids, page_table, page_size, 
 def select_blocks(q: Tensor, bounds: Tensor, bound_scales: Tensor, positions: Tensor,
                   seq_ids: Tensor, page_table: Tensor, page_size: int, count: int, sink: int = 1,
                   recent: int = 1) -> Tensor:
-    """The blocks that each token and key/value head attends to, int32 ``[T, Hkv, count]``, ascending,
-    -1 at the end. The first ``sink`` blocks and the last ``recent`` ones up to the token's own are always
-    among them; the other places go to the best blocks between by ``(score desc, block asc)``. A score
-    is the largest, over the heads that share the key/value head, of ``c . mid + |c| . half`` (int32;
-    ``c`` the rotated query's int8 codes) times the query's and the block's scales: an upper bound on
-    what the block's keys can score, up to the codes' rounding. Blocks between without a page are left
-    out; padding tokens get -1 throughout."""
+    """The blocks that each token and key/value head attends to, int32 ``[T, Hkv, count]``,
+    ascending,
+    -1 at the end. The first ``sink`` blocks and the last ``recent`` ones up to the token's own are
+    always among them; the other places go to the best blocks between by ``(score desc, block
+    asc)``. A score is the largest, over the heads that share the key/value head, of ``c . mid + |c|
+    . half`` (int32;
+    ``c`` the rotated query's int8 codes) times the query's and the block's scales: an upper bound
+    on what the block's keys can score, up to the codes' rounding. Blocks between without a page are
+    left out; padding tokens get -1 throughout."""
     call = _select if _eager(q) else torch.ops.retrieve_kv.select_blocks
     return call(q, bounds, bound_scales, positions, seq_ids, page_table, page_size, count, sink,
                 recent)
@@ -281,11 +288,11 @@ def block_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, blocks: Tensor,
                     seq_ids: Tensor, page_table: Tensor, scale: float | None = None
                     ) -> tuple[Tensor, Tensor]:
     """Softmax attention of ``q [T, Hq, D]`` (rotated) over the keys of the listed ``blocks`` (int32
-    ``[T, Hkv, count]``, each at most once a row, in any order) at positions up to the token's own, with
-    scores ``scale * q . k`` (``1 / sqrt(D)`` by default): ``(out [T, Hq, D], lse fp32 [T, Hq])``, ``lse``
-    the natural logarithm of the weights' sum. Entries below 0, past the token's block or without a
-    page are skipped; a row without a key is zeros and ``-inf``. Slots past a token's position are not
-    used, whatever they hold."""
+    ``[T, Hkv, count]``, each at most once a row, in any order) at positions up to the token's own,
+    with scores ``scale * q . k`` (``1 / sqrt(D)`` by default): ``(out [T, Hq, D], lse fp32 [T,
+    Hq])``, ``lse`` the natural logarithm of the weights' sum. Entries below 0, past the token's
+    block or without a page are skipped; a row without a key is zeros and ``-inf``. Slots past a
+    token's position are not used, whatever they hold."""
     call = _attention if _eager(q) else torch.ops.retrieve_kv.block_attention
     return call(q, k_cache, v_cache, blocks, positions, seq_ids, page_table, scale)
 
@@ -325,14 +332,17 @@ for _name in ("append", "select_blocks", "block_attention"):
 def rotary_table(length: int, rot: int, *, base: float = 10000.0, scaling: str | None = None,
                  factor: float = 1.0, original: int | None = None, beta_fast: float = 32.0,
                  beta_slow: float = 1.0, device: str | torch.device = "cuda") -> Tensor:
-    """``cos_sin [length, rot]`` fp32 for :func:`append`, computed in 64 bits: position ``p`` turns pair ``i``
-    by ``p * base ** (-2 i / rot)``. ``scaling`` stretches a model trained on ``original`` positions to
+    """``cos_sin [length, rot]`` fp32 for :func:`append`, computed in 64 bits: position ``p`` turns
+    pair ``i`` by ``p * base ** (-2 i / rot)``. ``scaling`` stretches a model trained on
+    ``original`` positions to
     ``factor`` times as many:
 
     - ``"linear"``: every position divided by ``factor``;
-    - ``"base"``: a larger base, ``base * factor ** (rot / (rot - 2))``: the fastest pair as it was, the
+    - ``"base"``: a larger base, ``base * factor ** (rot / (rot - 2))``: the fastest pair as it was,
+    the
       slowest slowed by ``factor``;
-    - ``"ramp"``: pairs that turn more than ``beta_fast`` times over ``original`` as they were, those
+    - ``"ramp"``: pairs that turn more than ``beta_fast`` times over ``original`` as they were,
+    those
       below ``beta_slow`` divided by ``factor``, a linear ramp over the pairs between (from the pair
       where the turns pass ``beta_fast``, rounded down, to the one where they pass ``beta_slow``,
       rounded up), cosines and sines scaled by ``0.1 ln(factor) + 1``.
@@ -401,7 +411,8 @@ class PagedCache:
         self._held: list[list[int]] = [[] for _ in range(sequences)]
 
     def reserve(self, seq: int, tokens: int) -> None:
-        """Pages for the sequence's first ``tokens`` tokens, those that it has already among them."""
+        """Pages for the sequence's first ``tokens`` tokens, those that it has already among
+        them."""
         held, need = self._held[seq], -(-tokens // self.page)
         if need > self.page_table.shape[1]:
             raise ValueError(f"{need} pages: a sequence has at most {self.page_table.shape[1]}")

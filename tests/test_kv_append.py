@@ -1,4 +1,5 @@
-"""Appending to the paged cache: slots, rotations, bounds and padding, bit for bit against the oracle."""
+"""Appending to the paged cache: slots, rotations, bounds and padding, bit for bit against the
+oracle."""
 
 from __future__ import annotations
 
@@ -9,7 +10,8 @@ from oracle import kv as okv
 from tests.conftest import rng
 from tests.kv_cases import back, layout, normal16, table, to
 
-# one token a sequence at every place of a page, prompts that start and end inside pages, an empty call
+# one token a sequence at every place of a page, prompts that start and end inside pages, an empty
+# call
 DECODE = [(p, 1) for p in (0, 1, 14, 15, 16, 31, 47, 63, 64, 127, 128, 255)]
 PROMPTS = [(0, 16), (5, 60), (0, 1), (130, 200), (127, 1), (1, 127)]
 
@@ -103,8 +105,8 @@ def test_matches_the_oracle(dev, had_new, kind, heads, heads_kv, d, page, rot, i
 
 @pytest.mark.gpu
 def test_many_tokens_share_a_workgroup(dev):
-    """More tokens and heads than are given a workgroup each: the bounds' tiles of 64 tokens, with blocks
-    that begin in one tile and end in the next."""
+    """More tokens and heads than are given a workgroup each: the bounds' tiles of 64 tokens, with
+    blocks that begin in one tile and end in the next."""
     had_new = [(3, 700), (0, 65), (60, 1)] + [(i, 1) for i in range(7, 200, 16)]
     pos, seq, tab, qkv, *state = _state(7, 16, had_new, 12, 6, 64, "bf16")
     args = (qkv, 12, 6, table(800, 64), pos, seq, tab, *state, False)
@@ -122,7 +124,8 @@ def test_without_rotation(dev):
 
 @pytest.mark.gpu
 def test_padding_writes_nothing(dev):
-    """Negative and too large positions, sequences and pages out of range, positions past the table."""
+    """Negative and too large positions, sequences and pages out of range, positions past the
+    table."""
     pos, seq, tab, qkv, *state = _state(11, 16, [(0, 40), (15, 1), (30, 20)], 4, 2, 64, "bf16")
     pos, seq, tab = pos.copy(), seq.copy(), tab.copy()
     pos[3], pos[20], seq[5], seq[41] = -1, 2**31 - 1, -2, 3
@@ -137,7 +140,8 @@ def test_padding_writes_nothing(dev):
 @pytest.mark.gpu
 @pytest.mark.parametrize("cuts", [[40], [1] * 40, [15, 1, 1, 7, 16]])
 def test_split_calls_leave_the_same_cache(dev, cuts):
-    """The same 40 tokens in one call, token by token, or in pieces: one cache, one set of bounds."""
+    """The same 40 tokens in one call, token by token, or in pieces: one cache, one set of
+    bounds."""
     import torch
 
     from retrieve_amd import kv

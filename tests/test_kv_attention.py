@@ -1,10 +1,10 @@
 """Attention over chosen blocks against softmax in 64 bits.
 
-Tolerances, from the arithmetic: with ``u`` the 16-bit type's unit roundoff, an output is rounded once
-(``u |out|``) and every weight once before its product with ``v`` (``u`` relative; for fp16 also its
-least step, 2^-25 of a weight of 1), so a sum moves by ``u sum w |v|``; scores are fp32 sums of ``D``
-exact products, off by ``(D + 8) 2^-24 scale sum |q k|`` at most, which moves a weight by twice that,
-relative, and the log-sum by once.
+Tolerances, from the arithmetic: with ``u`` the 16-bit type's unit roundoff, an output is rounded
+once (``u |out|``) and every weight once before its product with ``v`` (``u`` relative; for fp16
+also its least step, 2^-25 of a weight of 1), so a sum moves by ``u sum w |v|``; scores are fp32
+sums of ``D`` exact products, off by ``(D + 8) 2^-24 scale sum |q k|`` at most, which moves a weight
+by twice that, relative, and the log-sum by once.
 """
 
 from __future__ import annotations
@@ -108,8 +108,8 @@ MANY = [("bf16", 1, 1, 64, 16, 9), ("fp16", 2, 1, 128, 64, 5), ("bf16", 3, 1, 96
 
 
 def _many(seed, kind, heads, heads_kv, d, page, count):
-    """More rows than the GPU holds waves (a wave then takes a row, or several tokens at once), of three
-    sequences; neighbours choose alike in the first and last, by chance in the second."""
+    """More rows than the GPU holds waves (a wave then takes a row, or several tokens at once), of
+    three sequences; neighbours choose alike in the first and last, by chance in the second."""
     had_new = [(3 * page + 5, 2000), (0, 5000 // heads_kv), (40, 7)]
     case = list(_case(seed, kind, heads, heads_kv, d, page, had_new, count, sparse=0.1))
     blocks, pos = case[3], case[4]
@@ -145,8 +145,9 @@ def test_many_rows(dev, kind, heads, heads_kv, d, page, count):
 @pytest.mark.gpu
 @pytest.mark.parametrize("heads", [1, 4, 8, 16])
 def test_many_rows_and_values_that_are_not_finite(dev, heads):
-    """Neighbours that choose different blocks: a NaN key or an infinite value reaches the tokens whose
-    lists hold it, and no other; slots past every token's are NaN; padding among the tokens."""
+    """Neighbours that choose different blocks: a NaN key or an infinite value reaches the tokens
+    whose lists hold it, and no other; slots past every token's are NaN; padding among the
+    tokens."""
     page, tokens = 16, 6700
     q, kc, vc, blocks, pos, seq, tab = _case(71, "bf16", heads, 1, 64, page, [(16 * 7 + 3, 1)], 4)
     q = normal16(72, (tokens, heads, 64), "bf16")
@@ -173,7 +174,8 @@ def test_many_rows_and_values_that_are_not_finite(dev, heads):
 
 @pytest.mark.gpu
 def test_rows_without_keys(dev):
-    """All -1, padding tokens, blocks past the token's own, pages that are missing: zeros and -inf."""
+    """All -1, padding tokens, blocks past the token's own, pages that are missing: zeros and
+    -inf."""
     q, kc, vc, blocks, pos, seq, tab = _case(23, "bf16", 4, 2, 64, 16,
                                              [(100, 2), (50, 2), (30, 1), (3, 1)], 4)
     pos, seq, tab = pos.copy(), seq.copy(), tab.copy()
@@ -216,8 +218,8 @@ def test_slots_past_the_token_hold_anything(dev, page, what):
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["bf16", "fp16"])
 def test_large_scores(dev, kind):
-    """Scores of hundreds to thousands, both signs: the running maximum jumps; a scale of its own; equal
-    keys; zero queries."""
+    """Scores of hundreds to thousands, both signs: the running maximum jumps; a scale of its own;
+    equal keys; zero queries."""
     case = _case(33, kind, 4, 2, 128, 16, [(400, 1), (37, 9), (16 * 40, 1)], 8, size=60.0)
     _check(_run(dev, kind, *case), kind, *case)
     _check(_run(dev, kind, *case, 3.7), kind, *case, 3.7)

@@ -1,5 +1,5 @@
-"""The paged cache as a layer uses it: the rotary tables, the page book-keeping, the three calls together,
-their schemas, graph capture, other streams."""
+"""The paged cache as a layer uses it: the rotary tables, the page book-keeping, the three calls
+together, their schemas, graph capture, other streams."""
 
 from __future__ import annotations
 
@@ -168,8 +168,8 @@ def _layer(dev, kind="bf16", steps=70, heads=8, heads_kv=2, d=64, page=16):
 
 @pytest.mark.gpu
 def test_prompt_then_tokens(dev):
-    """Prompt, then decode steps, each step held to the oracle on the oracle's own cache: chosen blocks
-    equal, outputs within the attention's tolerance, over pages that start as NaN."""
+    """Prompt, then decode steps, each step held to the oracle on the oracle's own cache: chosen
+    blocks equal, outputs within the attention's tolerance, over pages that start as NaN."""
     from tests.test_kv_attention import _check
 
     kind = "bf16"
@@ -225,8 +225,8 @@ def test_every_block_kept_is_full_attention(dev):
 @pytest.mark.gpu
 @pytest.mark.parametrize("sequences,blocks", [(1, 300), (2, 12)])
 def test_graph_replays(dev, sequences, blocks):
-    """A captured decode step, replayed with new inputs and positions between eager work, gives the eager
-    step's results every time (the split forms' scratch among them)."""
+    """A captured decode step, replayed with new inputs and positions between eager work, gives the
+    eager step's results every time (the split forms' scratch among them)."""
     import torch
 
     from retrieve_amd import kv
@@ -327,8 +327,8 @@ def test_opcheck(dev):
 
 @pytest.mark.gpu
 def test_recall_of_the_heaviest_blocks(dev):
-    """On keys with structure (each block around its own centre) the chosen blocks hold nearly all the
-    attention's weight: log-sums over 16 of 128 blocks close to those over all."""
+    """On keys with structure (each block around its own centre) the chosen blocks hold nearly all
+    the attention's weight: log-sums over 16 of 128 blocks close to those over all."""
     import torch
 
     from retrieve_amd import kv

@@ -1,4 +1,5 @@
-"""Choosing blocks by their int8 bounds: every index equal to the oracle's, whose sums are integers."""
+"""Choosing blocks by their int8 bounds: every index equal to the oracle's, whose sums are
+integers."""
 
 from __future__ import annotations
 
@@ -39,8 +40,8 @@ def _check(dev, seed, kind, heads, heads_kv, d, page, had_new, how, ties=False, 
 
 
 def test_selection_by_rationals():
-    """The oracle's order is that of the exact scores (random scores are no fp32 rounding apart), and ties
-    go to the lower block."""
+    """The oracle's order is that of the exact scores (random scores are no fp32 rounding apart),
+    and ties go to the lower block."""
     g = rng(31)
     q = normal16(32, (4, 64), "bf16")
     for ties in (False, True):
@@ -107,8 +108,8 @@ def test_ties_go_to_the_lower_block(dev):
     (4, 64, 4096, 100), (40, 64, 4200, 300), (20, 256, 5000, 64), (4, 128, 20000, 64),
     (4, 64, 70001, 1000)])
 def test_long_contexts(dev, heads, d, blocks, count):
-    """Single tokens around the sizes where the kernels change: one launch up to 4096 blocks, keys in
-    registers or read again."""
+    """Single tokens around the sizes where the kernels change: one launch up to 4096 blocks, keys
+    in registers or read again."""
     had = [(16 * blocks - 5, 1), (16 * 333, 1)]
     _check(dev, blocks, "bf16", heads, 1, d, 16, had, (count, 1, 2))
 
@@ -118,7 +119,8 @@ def test_long_contexts(dev, heads, d, blocks, count):
                                                   (1, 96, 1100, 64), (8, 64, 3000, 300),
                                                   (16, 64, 4500, 64), (3, 192, 300, 20)])
 def test_prompts_behind_long_contexts(dev, heads, d, blocks, count):
-    """A few tokens of each sequence, over blocks that take a wave's registers, four waves' or more."""
+    """A few tokens of each sequence, over blocks that take a wave's registers, four waves' or
+    more."""
     had = [(16 * blocks + 9, 9), (16 * (blocks // 2), 3), (40, 5)]
     _check(dev, blocks + 1, "fp16", heads, 1, d, 16, had, (count, 1, 2))
 
@@ -222,9 +224,9 @@ def test_refusals(dev):
 
 
 def test_codes_by_reciprocal():
-    """The kernels' quotient (reciprocal, product, one correction) is the division's, rounded to nearest, for
-    every pair of bf16 significands, a spread of fp16's, and the floor: codes equal bit for bit. (The
-    correction's product and sum are exact in 64 bits up to their last rounding.)"""
+    """The kernels' quotient (reciprocal, product, one correction) is the division's, rounded to
+    nearest, for every pair of bf16 significands, a spread of fp16's, and the floor: codes equal bit
+    for bit. (The correction's product and sum are exact in 64 bits up to their last rounding.)"""
     def quotient(x, top):
         r = (np.float32(1) / top).astype(np.float32)
         q = (x * r).astype(np.float32)
