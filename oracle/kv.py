@@ -2,8 +2,7 @@
 
 Values of 16-bit types are held as float32 arrays; ``round16`` rounds to them. ``append`` follows
 the kernels' single fp32 roundings (bit-exact), ``append64`` and ``attention`` the formulas in 64
-bits,
-``select`` integers. ``blocks_by_bounds`` states the selection a second time, over exact rationals.
+bits, ``select`` integers. ``blocks_by_bounds`` states the selection a second time, over exact rationals.
 """
 
 from __future__ import annotations

@@ -10,13 +10,11 @@ to the lower index. Three ops over one layer's cache, in the order a model's lay
 - :func:`block_attention`: softmax attention over the chosen blocks.
 
 Tokens are packed: token ``t`` is at ``positions[t]`` of sequence ``seq_ids[t]``, a row of
-``page_table``
-``[B, max_pages]`` (the physical page of each block of ``page`` tokens, -1 for none), all int32. One
-token a sequence is a decode step, many a prompt; a call may mix them. Caches are ``[P, Hkv, page,
-D]`` (a block of one head is contiguous), bounds int8 ``[P, Hkv, 2 D]`` with scales fp32 ``[P,
-Hkv]``.
-:class:`PagedCache` holds them and makes the three calls; :func:`rotary_table` builds the table of
-cosines and sines. No counterpart in the reference; serving only (no gradients).
+``page_table [B, max_pages]`` (the physical page of each block of ``page`` tokens, -1 for none), all
+int32. One token a sequence is a decode step, many a prompt; a call may mix them. Caches are ``[P,
+Hkv, page, D]`` (a block of one head is contiguous), bounds int8 ``[P, Hkv, 2 D]`` with scales fp32
+``[P, Hkv]``. :class:`PagedCache` holds them and makes the three calls; :func:`rotary_table` builds
+the table of cosines and sines. No counterpart in the reference; serving only (no gradients).
 
 The ops check their arguments here (``ValueError`` on shapes, ``TypeError`` on dtypes), allocate
 from torch's caching allocator and enqueue on torch's current stream, without a host
@@ -40,8 +38,8 @@ MAX_COUNT = 1024
 
 _lib = torch.library.Library("retrieve_kv", "DEF")
 _lib.define("append(Tensor q, Tensor k, Tensor v, Tensor? cos_sin, Tensor positions, "
-            "Tensor seq_ids, Tensor page_table, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!) bounds, "
-            "Tensor(d!) bound_scales, bool interleaved=False) -> Tensor")
+            "Tensor seq_ids, Tensor page_table, Tensor(a!) k_cache, Tensor(b!) v_cache, "
+            "Tensor(c!) bounds, Tensor(d!) bound_scales, bool interleaved=False) -> Tensor")
 _lib.define("select_blocks(Tensor q, Tensor bounds, Tensor bound_scales, Tensor positions, "
             "Tensor seq_ids, Tensor page_table, int page_size, int count, int sink=1, "
             "int recent=1) -> Tensor")
@@ -239,14 +237,12 @@ def select_blocks(q: Tensor, bounds: Tensor, bound_scales: Tensor, positions: Te
                   seq_ids: Tensor, page_table: Tensor, page_size: int, count: int, sink: int = 1,
                   recent: int = 1) -> Tensor:
     """The blocks that each token and key/value head attends to, int32 ``[T, Hkv, count]``,
-    ascending,
-    -1 at the end. The first ``sink`` blocks and the last ``recent`` ones up to the token's own are
-    always among them; the other places go to the best blocks between by ``(score desc, block
-    asc)``. A score is the largest, over the heads that share the key/value head, of ``c . mid + |c|
-    . half`` (int32;
-    ``c`` the rotated query's int8 codes) times the query's and the block's scales: an upper bound
-    on what the block's keys can score, up to the codes' rounding. Blocks between without a page are
-    left out; padding tokens get -1 throughout."""
+    ascending, -1 at the end. The first ``sink`` blocks and the last ``recent`` ones up to the
+    token's own are always among them; the other places go to the best blocks between by ``(score
+    desc, block asc)``. A score is the largest, over the heads that share the key/value head, of
+    ``c . mid + |c| . half`` (int32; ``c`` the rotated query's int8 codes) times the query's and the
+    block's scales: an upper bound on what the block's keys can score, up to the codes' rounding.
+    Blocks between without a page are left out; padding tokens get -1 throughout."""
     call = _select if _eager(q) else torch.ops.retrieve_kv.select_blocks
     return call(q, bounds, bound_scales, positions, seq_ids, page_table, page_size, count, sink,
                 recent)
@@ -334,18 +330,15 @@ def rotary_table(length: int, rot: int, *, base: float = 10000.0, scaling: str |
                  beta_slow: float = 1.0, device: str | torch.device = "cuda") -> Tensor:
     """``cos_sin [length, rot]`` fp32 for :func:`append`, computed in 64 bits: position ``p`` turns
     pair ``i`` by ``p * base ** (-2 i / rot)``. ``scaling`` stretches a model trained on
-    ``original`` positions to
-    ``factor`` times as many:
+    ``original`` positions to ``factor`` times as many:
 
     - ``"linear"``: every position divided by ``factor``;
     - ``"base"``: a larger base, ``base * factor ** (rot / (rot - 2))``: the fastest pair as it was,
-    the
-      slowest slowed by ``factor``;
+      the slowest slowed by ``factor``;
     - ``"ramp"``: pairs that turn more than ``beta_fast`` times over ``original`` as they were,
-    those
-      below ``beta_slow`` divided by ``factor``, a linear ramp over the pairs between (from the pair
-      where the turns pass ``beta_fast``, rounded down, to the one where they pass ``beta_slow``,
-      rounded up), cosines and sines scaled by ``0.1 ln(factor) + 1``.
+      those below ``beta_slow`` divided by ``factor``, a linear ramp over the pairs between (from
+      the pair where the turns pass ``beta_fast``, rounded down, to the one where they pass
+      ``beta_slow``, rounded up), cosines and sines scaled by ``0.1 ln(factor) + 1``.
     """
     if rot < 2 or rot % 2 or length < 0:
         raise ValueError(f"rot must be even and at least 2, length at least 0: {rot}, {length}")
