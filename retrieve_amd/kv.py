@@ -123,10 +123,16 @@ def _device(*tensors: Tensor) -> int:
 
 def _on(device: int):
     """The tensors' GPU as the current one, where it is not already."""
-    return _HERE if device == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if device == _current() else torch.cuda.device(device)
+
+
+def _out(q: Tensor, t: int, heads: int, dim: int) -> Tensor:
+    """A contiguous tensor of the queries' shape."""
+    return torch.empty_like(q) if q.is_contiguous() else q.new_empty((t, heads, dim))
 
 
 _HERE = contextlib.nullcontext()
+_current = torch._C._cuda_getDevice  # (torch is initialised there: the tensors are on a GPU)
 _stream = torch._C._cuda_getCurrentRawStream  # (the current stream's handle, without an object)
 
 
@@ -167,7 +173,7 @@ def _append(q, k, v, cos_sin, positions, seq_ids, page_table, k_cache, v_cache, 
     q, q_token, q_head = _rows(q)
     k, k_token, k_head = _rows(k)
     v, v_token, v_head = _rows(v)
-    out = q.new_empty((t, heads, dim))
+    out = _out(q, t, heads, dim)
     with _on(dev):
         st = nat.lib().rt_kv_append(
             q.data_ptr(), q_token, q_head, k.data_ptr(), k_token, k_head, v.data_ptr(), v_token,
@@ -263,12 +269,12 @@ def _attention(q, k_cache, v_cache, blocks, positions, seq_ids, page_table, scal
     dev = _device(q, k_cache, v_cache, blocks, positions, seq_ids, page_table)
     q, q_token, q_head = _rows(q)
     count = blocks.shape[2]
-    out = q.new_empty((t, heads, dim))
+    out = _out(q, t, heads, dim)
     lse = q.new_empty((t, heads), dtype=torch.float32)
     lib = nat.lib()
     with _on(dev):
         need = lib.rt_kv_attention_workspace(t, heads, heads_kv, dim, page, count)
-        ws = nat.workspace(need, dev) if need else None
+        ws = blocks.new_empty((need // 4,)) if need else None  # (floats)
         st = lib.rt_kv_attention(
             q.data_ptr(), q_token, q_head, t, heads, heads_kv, dim, dtype, k_cache.data_ptr(),
             v_cache.data_ptr(), pages, page, blocks.data_ptr(), count, positions.data_ptr(),

@@ -260,8 +260,9 @@ def test_keys_of_minus_infinity_weigh_nothing(dev):
 
 
 @pytest.mark.gpu
-def test_offsets_past_32_bits(dev):
-    """Caches of 2.4 G elements: blocks on their first and last pages."""
+@pytest.mark.parametrize("tokens", [2, 600])
+def test_offsets_past_32_bits(dev, tokens):
+    """Caches of 2.4 G elements: blocks on their first and last pages, few rows and many."""
     import torch
 
     from retrieve_amd import kv
@@ -273,13 +274,15 @@ def test_offsets_past_32_bits(dev):
     small_v = normal16(42, (4, 8, page, d), "bf16")
     where = [0, pages // 2, pages - 2, pages - 1]
     kc[where], vc[where] = to(dev, small_k, "bf16"), to(dev, small_v, "bf16")
-    q = normal16(43, (2, 16, d), "bf16")
-    pos, seq = np.array([4 * page - 1, 3 * page + 9], np.int32), np.zeros(2, np.int32)
-    blocks = np.broadcast_to(np.arange(4, dtype=np.int32), (2, 8, 4))
+    q = normal16(43, (tokens, 16, d), "bf16")
+    pos = np.array([4 * page - 1, 3 * page + 9] * (tokens // 2), np.int32)
+    seq = np.zeros(tokens, np.int32)
+    blocks = np.broadcast_to(np.arange(4, dtype=np.int32), (tokens, 8, 4))
     got = kv.block_attention(to(dev, q, "bf16"), kc, vc, to(dev, blocks), to(dev, pos), to(dev, seq),
                              torch.tensor([where], dtype=torch.int32, device=dev))
-    _check([back(x) for x in got], "bf16", q, small_k, small_v, blocks, pos, seq,
-           np.arange(4, dtype=np.int32)[None])
+    last = slice(-20, None)
+    _check([back(x)[last] for x in got], "bf16", q[last], small_k, small_v, blocks[last], pos[last],
+           seq[last], np.arange(4, dtype=np.int32)[None])
 
 
 @pytest.mark.gpu
