@@ -867,14 +867,15 @@ __global__ void __launch_bounds__(D / 4) kv_join_kernel(AttendArgs a) {
   if (threadIdx.x == 0) a.lse[r] = log_sum(m, l);
 }
 
-// How a call is spread: `parts` workgroups a row; 0: a wave a row, or `joined` tokens a wave.
+// How a call is spread: `parts` workgroups a row; 0: `joined` tokens a wave, or (0) a wave a row.
 struct AttendPlan {
   int64_t rows;
   int32_t tiles, parts, joined;
 };
 
-inline AttendPlan attend_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t page,
-                              int64_t count) {
+// Times in us are of lists of 16 blocks of 64 keys, 32 heads of 8 key/value heads.
+inline AttendPlan attend_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t B,
+                              int64_t page, int64_t count) {
   AttendPlan p;
   const int64_t G = Hq / Hkv;
   p.tiles = static_cast<int32_t>(cdiv(G, 16));
@@ -883,14 +884,23 @@ inline AttendPlan attend_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int
   int64_t joined = 16 / (G < 16 ? G : 16);
   if (joined > kJoinTokens) joined = kJoinTokens;
   const int64_t lists = kJoinMost / (kJoinWaves * (count > 0 ? count : 1));
-  p.joined = static_cast<int32_t>(joined < lists ? joined : lists);
-  // A joined workgroup's chain of steps takes as long for few tokens as for many: us for lists of
-  // 16 blocks of 64 keys, 32 heads of 8 key/value heads, split and joined, at 400 and 511 tokens:
-  // D 64: 63 and 105, 76 and 97; D 128: 120 and 121, 148 and 113; D 256: 321 and 193, 395 and 168.
-  if (p.joined > 1 ? p.rows * D >= 400 << 10 : p.rows >= 4096) return p;
+  if (joined > lists) joined = lists;
+  p.joined = joined > 1 ? static_cast<int32_t>(joined) : 0;
+  // A joined workgroup's time is its chain of steps, whether it has a CU for itself or shares it, so
+  // while the GPU holds them all there are twice as many with half the tokens (and a shorter
+  // union): 1024 tokens of 128 channels 103 for 127, 511 tokens 73 for 114.
+  const int64_t held = D <= 128 ? 1024 : 512;
+  while (p.joined > 1 && cdiv(T, kJoinWaves * (p.joined / 2)) * Hkv <= held) p.joined /= 2;
+  // Prompts are joined where the chain is shorter than the split form's reads of every row's blocks
+  // (split and joined: 64 channels, 300 tokens 50 and 50, 400 tokens 63 and 52; 128 channels, 200
+  // tokens 67 and 53; 256 channels, 100 tokens 100 and 99, 200 tokens 176 and 85). No more tokens
+  // than sequences are taken for single tokens, which share nothing: 500 of 128 channels take 328
+  // split and 365 joined, 2000 take 1246 and 1434.
+  if (T > B && (p.joined > 0 ? p.rows * D >= 200 << 10 : p.rows >= 4096)) return p;
   // Workgroups of four waves for two on every CU, each wave with a unit of 64 keys at least. A
   // second launch that joins the parts costs 4 us, a row in one workgroup more: one token of 8
   // heads over 32 blocks of 64 keys takes 12 us in 8 parts a row, 23 in one workgroup of 8 waves.
+  // (Rows whose parts are several are too few to be joined: the workspace does not depend on B.)
   const int64_t most = cdiv(count * page, 64 * kAttendWaves);
   const int64_t want = cdiv(512, p.rows > 0 ? p.rows : 1);
   p.parts = static_cast<int32_t>(want < most ? want : most);
@@ -905,7 +915,7 @@ using namespace rt;
 extern "C" size_t rt_kv_attention_workspace(int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
                                             int64_t page, int64_t count) {
   if (Hkv < 1 || T < 1) return 0;
-  const AttendPlan p = attend_plan(T, Hq, Hkv, D, page, count);
+  const AttendPlan p = attend_plan(T, Hq, Hkv, D, 0, page, count);
   return p.parts > 1 ? static_cast<size_t>(p.rows) * p.parts * 16 * (D + 2) * sizeof(float) : 0;
 }
 
@@ -933,7 +943,7 @@ extern "C" int rt_kv_attention(const void* q, int64_t q_token_stride, int64_t q_
     set_error("workspace too small: %zu < %zu", workspace_bytes, need);
     return kWorkspaceTooSmall;
   }
-  const AttendPlan plan = attend_plan(T, Hq, Hkv, D, page, count);
+  const AttendPlan plan = attend_plan(T, Hq, Hkv, D, B, page, count);
   AttendArgs a{};
   a.q = q, a.q_st = q_token_stride, a.q_sh = q_head_stride, a.T = T;
   a.Hq = static_cast<int32_t>(Hq), a.Hkv = static_cast<int32_t>(Hkv);
@@ -953,7 +963,7 @@ extern "C" int rt_kv_attention(const void* q, int64_t q_token_stride, int64_t q_
     using E = decltype(e);
     constexpr int DD = decltype(d)::value;
     const dim3 threads(kAttendWaves * kWave);
-    if (plan.parts == 0 && plan.joined > 1) {
+    if (plan.parts == 0 && plan.joined > 0) {
       const int64_t grid = cdiv(T, kJoinWaves * plan.joined) * Hkv;
       kv_attend_joined_kernel<E, DD>
           <<<dim3(static_cast<unsigned>(grid)), dim3(kJoinWaves * kWave), 0, s>>>(a);

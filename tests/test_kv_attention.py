@@ -104,7 +104,8 @@ def test_few_rows_many_blocks(dev, tokens, count):
 MANY = [("bf16", 1, 1, 64, 16, 9), ("fp16", 2, 1, 128, 64, 5), ("bf16", 3, 1, 96, 32, 16),
         ("fp16", 4, 1, 128, 16, 7), ("bf16", 7, 1, 64, 128, 4), ("fp16", 8, 1, 192, 64, 6),
         ("bf16", 12, 1, 128, 32, 5), ("fp16", 20, 1, 64, 64, 4), ("bf16", 4, 1, 256, 64, 70),
-        ("fp16", 4, 1, 64, 16, 300), ("bf16", 8, 2, 128, 64, 16)]
+        ("fp16", 4, 1, 64, 16, 300), ("bf16", 8, 2, 128, 64, 16), ("fp16", 8, 8, 64, 16, 9),
+        ("bf16", 16, 8, 128, 32, 5), ("fp16", 32, 8, 128, 64, 7), ("bf16", 8, 4, 256, 16, 6)]
 
 
 def _many(seed, kind, heads, heads_kv, d, page, count):
@@ -140,6 +141,27 @@ def test_many_rows(dev, kind, heads, heads_kv, d, page, count):
     pick = np.r_[0:9, 31:45, 1990:2012, rng(5).integers(0, tokens, 60), tokens - 9:tokens]
     got, case = _some(got, case, pick)
     _check(got, kind, *case)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,heads,heads_kv,d,page,count,tokens",
+                         [("bf16", 32, 8, 128, 64, 6, 230), ("fp16", 8, 8, 64, 16, 12, 430),
+                          ("bf16", 6, 2, 256, 32, 5, 500), ("fp16", 8, 8, 128, 16, 20, 300),
+                          ("bf16", 24, 3, 96, 128, 3, 777), ("bf16", 10, 10, 192, 16, 4, 201)])
+def test_hundreds_of_tokens(dev, kind, heads, heads_kv, d, page, count, tokens):
+    """Prompts between few rows and many: a wave joins fewer tokens than its columns would hold."""
+    had_new = [(5 * page + 3, tokens - tokens // 3 - 9), (0, tokens // 3), (33, 9)]
+    case = _case(tokens + d, kind, heads, heads_kv, d, page, had_new, count, sparse=0.1)
+    _check(_run(dev, kind, *case), kind, *case)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sequences", [600, 1100])
+def test_hundreds_of_sequences(dev, sequences):
+    """Single tokens of many sequences."""
+    case = _case(sequences, "bf16", 16, 4, 64, 16, [(3 + 7 * i % 90, 1) for i in range(sequences)],
+                 3)
+    _check(_run(dev, "bf16", *case), "bf16", *case)
 
 
 @pytest.mark.gpu
