@@ -16,11 +16,11 @@
 // share the pass over its blocks. One key a (token, head, block) is left behind.
 //
 // Bound: single tokens by the bounds' bytes, 2 D a (block, head) in scattered pieces (64 sequences
-// of 16K to 131K tokens in blocks of 64, 8 heads of 128 channels: 53 us, 2.9 TB/s, the longest
+// of 16K to 131K tokens in blocks of 64, 8 heads of 128 channels: 51 us, 3.0 TB/s, the longest
 // row's chain behind the others), one launch for up to 4096 blocks; a million tokens of one
 // sequence take 13 us of scores and 8 of keeping. Prompts by the vector instructions: a column's
 // codes (ten instructions a channel) and a block's key (about seven a head): 4099 tokens over 9K
-// to 30K take 77 us.
+// to 30K take 76 us.
 //
 // Keep: few blocks by a wave, which bisects over the keys' bits from the highest in which they
 // differ until the count is exact. Many by a workgroup: the want-th largest of the lanes' largest
@@ -45,6 +45,7 @@ struct SelectArgs {
   const float* scales;
   KvTokens tok;
   int32_t count, sink, recent;
+  int32_t want;       // places for blocks chosen by their score (of a cache without pages: none)
   int32_t* out;       // [T, Hkv, count]
   uint32_t* keys;     // [T * Hkv, stride]
   int64_t stride;
@@ -368,7 +369,7 @@ struct Span {
     end = blocks - a.recent > lead ? blocks - a.recent : lead;
     n = end - lead;
     tail = blocks - end;
-    want = static_cast<uint32_t>(a.count - a.sink - a.recent);
+    want = static_cast<uint32_t>(a.want);
   }
   // The forced blocks around `kept` candidates, and -1 behind them.
   __device__ void rest(const SelectArgs& a, uint32_t kept, int thread, int threads) const {
@@ -726,9 +727,11 @@ __global__ void __launch_bounds__(kFusedWaves* kWave, D <= 128 && NT == 1 ? 4 : 
   const unsigned share = gridDim.x / 8;
   const int64_t row = static_cast<int64_t>(blockIdx.x % 8) * share + blockIdx.x / 8;
   if (row >= a.T * a.Hkv) return;
-  score_blocks<E, D, NT, 0, 2>(
-      a, row / a.Hkv, static_cast<int>(row % a.Hkv), wave, kFusedWaves, score_lds[wave],
-      [&](int64_t, int64_t b) { return reinterpret_cast<v4i*>(&keys[b]); });
+  if (a.want > 0) {
+    score_blocks<E, D, NT, 0, 2>(
+        a, row / a.Hkv, static_cast<int>(row % a.Hkv), wave, kFusedWaves, score_lds[wave],
+        [&](int64_t, int64_t b) { return reinterpret_cast<v4i*>(&keys[b]); });
+  }
   __syncthreads();
   const Span p(a, row);
   if (p.n <= 8 * kWave) {
@@ -826,6 +829,8 @@ extern "C" int rt_kv_select(const void* q, int64_t q_token_stride, int64_t q_hea
            static_cast<int32_t>(max_pages), static_cast<int32_t>(P), kv_shift(page)};
   a.count = static_cast<int32_t>(count), a.sink = static_cast<int32_t>(sink);
   a.recent = static_cast<int32_t>(recent), a.out = out, a.keys = static_cast<uint32_t*>(workspace);
+  // (blocks without a page read page 0's bounds, so there has to be one)
+  a.want = P > 0 ? static_cast<int32_t>(count - sink - recent) : 0;
   a.stride = plan.stride, a.splits = plan.splits, a.head_groups = plan.head_groups;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (select_fused(T, Hkv, B, max_pages, count - sink - recent)) {
@@ -844,7 +849,7 @@ extern "C" int rt_kv_select(const void* q, int64_t q_token_stride, int64_t q_hea
   }
   const int64_t grid = cdiv(T, plan.per_wave) * plan.splits * plan.head_groups;
   RT_CHECK_ARG(grid <= INT32_MAX, "too many tokens");
-  if (max_pages > sink && count > sink + recent) {  // else no block is chosen by its score
+  if (max_pages > sink && a.want > 0) {  // else no block is chosen by its score
     const int st = kv_dispatch(dtype, D, [&](auto e, auto d) -> int {
       using E = decltype(e);
       constexpr int DD = decltype(d)::value;

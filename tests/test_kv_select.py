@@ -258,3 +258,18 @@ def test_queries_of_extreme_sizes(dev):
     prompt = [np.repeat(x, 5, 0) for x in (q, pos, seq)]
     got = _select(dev, prompt[0], "bf16", codes, scales, prompt[1], prompt[2], tab, 16, 12, 1, 2)
     assert np.array_equal(got[::5], okv.select(q, codes, scales, pos, seq, tab, 16, 12, 1, 2))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,blocks", [(1, 40), (9, 40), (2, 5000)])
+def test_a_cache_without_pages(dev, tokens, blocks):
+    """One launch, prompts and long page tables: the forced blocks only."""
+    print(f"no pages, {tokens} tokens, {blocks} blocks", flush=True)
+    pos = np.arange(16 * blocks - tokens, 16 * blocks, dtype=np.int32)
+    seq, tab = np.zeros(tokens, np.int32), np.full((1, blocks), -1, np.int32)
+    tab[0, ::3] = 0
+    codes, scales = _bounds(131, 0, 2, 64)
+    got = _select(dev, normal16(132, (tokens, 4, 64), "bf16"), "bf16", codes, scales, pos, seq, tab,
+                  16, 10, 1, 2)
+    forced = [[0, p // 16 - 1, p // 16] + [-1] * 7 for p in pos]
+    assert np.array_equal(got, np.repeat(np.array(forced, np.int32)[:, None], 2, 1))
