@@ -610,7 +610,7 @@ int rt_kv_select(const void* q, int64_t q_token_stride, int64_t q_head_stride, i
  * any order; entries below 0, past the token's block or without a page are skipped), the keys at
  * positions up to the token's, scores scale * q . k -> out [T, Hq, D], lse float [T, Hq] (natural
  * log of the weights' sum). A row without a key: zeros and -inf. Cache slots past a token's
- * position are never used, whatever they hold. */
+ * position are never used, whatever they hold. scale has to be finite (also times log2 e). */
 size_t rt_kv_attention_workspace(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t page,
                                  int64_t count);
 int rt_kv_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t T,

@@ -21,8 +21,9 @@
 // Memory: a wave keeps the next step's keys and values in flight (registers) while it works on
 // this one. Slots past the token's position are read but replaced: scores by -inf, values by 0.
 // Single tokens are bound by the cache's bytes: 64 sequences of lists of 64 blocks, 64 keys of 128
-// channels a block, 8 key/value heads take 168 us (6.3 TB/s). Prompts read most blocks from L2 and
-// are bound by the steps' instructions (2053 tokens of 32 heads over 16 blocks: 141 us).
+// channels a block, 8 key/value heads take 162 us (6.5 TB/s). Prompts read most blocks from L2 and
+// are bound by the steps' instructions (2053 tokens of 32 heads over 16 blocks: 136 us).
+#include <cmath>
 #include <type_traits>
 
 #include "../../include/retrieve_amd.h"
@@ -145,7 +146,7 @@ struct TileList {
 };
 
 // Sixteen bytes of a cache; STREAM: of rows that are read once (not kept in L2 before others: 64
-// sequences of 64 blocks 168 us, 187 with ordinary loads; 400 tokens of prompts, which share
+// sequences of 64 blocks 168 us, 187 with ordinary loads; 400 tokens of prompts, split, which share
 // blocks, 157 us streamed and 121 with ordinary loads).
 template <bool STREAM, class V>
 __device__ inline V load_row(const V* p) {
@@ -886,8 +887,8 @@ inline AttendPlan attend_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int
   const int64_t lists = kJoinMost / (kJoinWaves * (count > 0 ? count : 1));
   if (joined > lists) joined = lists;
   p.joined = joined > 1 ? static_cast<int32_t>(joined) : 0;
-  // A joined workgroup's time is its chain of steps, whether it has a CU for itself or shares it, so
-  // while the GPU holds them all there are twice as many with half the tokens (and a shorter
+  // A joined workgroup's time is its chain of steps, whether it has a CU for itself or shares it,
+  // so while the GPU holds them all there are twice as many with half the tokens (and a shorter
   // union): 1024 tokens of 128 channels 103 for 127, 511 tokens 73 for 114.
   const int64_t held = D <= 128 ? 1024 : 512;
   while (p.joined > 1 && cdiv(T, kJoinWaves * (p.joined / 2)) * Hkv <= held) p.joined /= 2;
@@ -938,6 +939,8 @@ extern "C" int rt_kv_attention(const void* q, int64_t q_token_stride, int64_t q_
                    kv_rows_aligned(out, 0, 0),
                "rows must start on 16 bytes");
   RT_CHECK_ARG(T * Hq <= INT32_MAX, "too many tokens");
+  RT_CHECK_ARG(std::isfinite(scale * kLog2e), "the scale must be finite, got %g",
+               static_cast<double>(scale));
   const size_t need = rt_kv_attention_workspace(T, Hq, Hkv, D, page, count);
   if (workspace_bytes < need || (need > 0 && workspace == nullptr)) {
     set_error("workspace too small: %zu < %zu", workspace_bytes, need);

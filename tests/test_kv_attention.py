@@ -357,3 +357,15 @@ def test_refusals(dev):
     ]:
         with pytest.raises(error):
             kv.block_attention(**{**good, **wrong})
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf"), 3e38])
+def test_scales_that_are_not_finite_are_refused(dev, scale):
+    """(3e38 is not finite in the kernels' powers of two.)"""
+    from retrieve_amd import kv
+
+    q, kc, vc, blocks, pos, seq, tab = _case(51, "bf16", 4, 2, 64, 16, [(60, 2)], 3)
+    with pytest.raises(ValueError, match="scale"):
+        kv.block_attention(to(dev, q, "bf16"), to(dev, kc, "bf16"), to(dev, vc, "bf16"),
+                           to(dev, blocks), to(dev, pos), to(dev, seq), to(dev, tab), scale)
