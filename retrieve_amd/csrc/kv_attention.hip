@@ -886,7 +886,9 @@ inline AttendPlan attend_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int
   if (joined > kJoinTokens) joined = kJoinTokens;
   const int64_t lists = kJoinMost / (kJoinWaves * (count > 0 ? count : 1));
   if (joined > lists) joined = lists;
-  p.joined = joined > 1 ? static_cast<int32_t>(joined) : 0;
+  // (one token a wave still shares a workgroup's loads: 460 tokens of 10 heads of 128, lists of 96
+  // blocks of 32 keys, 260 us for 532 with a wave a row)
+  p.joined = G <= 8 ? static_cast<int32_t>(joined) : 0;
   // A joined workgroup's time is its chain of steps, whether it has a CU for itself or shares it,
   // so while the GPU holds them all there are twice as many with half the tokens (and a shorter
   // union): 1024 tokens of 128 channels 103 for 127, 511 tokens 73 for 114.
