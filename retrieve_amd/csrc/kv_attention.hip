@@ -473,12 +473,14 @@ __device__ inline void attend_alone(const AttendArgs& a, int64_t t, int head, in
 // at each: a prompt of 8192 tokens takes 521 us instead of 464.
 constexpr int kJoinWaves = 4;
 constexpr int kJoinTiles = kJoinWaves / 2;  // of a step: a wave loads one of its K or V tiles
-constexpr int kJoinMost = 512;  // entries of a workgroup's lists
+// Entries of a workgroup's lists: of the first, the table is no larger than the stages of 128
+// channels; the second costs the narrower ones a workgroup a CU.
+constexpr int kJoinMost = 512, kJoinMore = 1024;
 constexpr int kJoinTokens = 8;   // tokens of a wave: their bits in a mask
 
-template <int D>
+template <int D, int MOST>
 struct JoinLds {
-  static constexpr int kTable = 2 * kJoinMost;
+  static constexpr int kTable = 2 * MOST;
   static constexpr int kTile = 16 * D * 2;  // bytes of 16 rows
   union {
     char stage[2][kJoinWaves][kTile];  // a step's K tiles, then its V tiles
@@ -489,9 +491,9 @@ struct JoinLds {
       uint32_t first[kTable], keys[kTable], part[kTable];
     };
   };
-  int32_t list[kJoinMost];  // pages
-  uint32_t who[kJoinMost];
-  uint8_t keys_of[kJoinMost];  // slots that hold keys, less 1; bit 7: some tokens count fewer
+  int32_t list[MOST];  // pages
+  uint32_t who[MOST];
+  uint8_t keys_of[MOST];  // slots that hold keys, less 1; bit 7: some tokens count fewer
   int32_t counts[kJoinWaves];
 };
 
@@ -502,12 +504,12 @@ __device__ inline int chunk_swizzle(int row) {
   return D % 64 == 0 ? row & 7 : (row >> 1) & 3;
 }
 
-template <class E, int D>
-__global__ void __launch_bounds__(kJoinWaves* kWave, D <= 128 ? 4 : 2)
+template <class E, int D, int MOST>
+__global__ void __launch_bounds__(kJoinWaves* kWave, D > 128 ? 2 : MOST > kJoinMost ? 3 : 4)
     kv_attend_joined_kernel(AttendArgs a) {
   using Wave = AttendWave<E, D>;
   using V8 = typename Wave::V8;
-  using Lds = JoinLds<D>;
+  using Lds = JoinLds<D, MOST>;
   constexpr int LOADS = D / 32;  // of a wave in a step
   __shared__ __attribute__((aligned(16))) Lds lds;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
@@ -527,7 +529,7 @@ __global__ void __launch_bounds__(kJoinWaves* kWave, D <= 128 ? 4 : 2)
     lds.part[i] = 0u;
   }
   __syncthreads();
-  constexpr int EACH = kJoinMost / (kJoinWaves * kWave);
+  constexpr int EACH = MOST / (kJoinWaves * kWave);
   int32_t page[EACH];
   uint32_t block[EACH];
   int slot[EACH], rank[EACH];
@@ -872,6 +874,7 @@ __global__ void __launch_bounds__(D / 4) kv_join_kernel(AttendArgs a) {
 struct AttendPlan {
   int64_t rows;
   int32_t tiles, parts, joined;
+  bool more;  // joined lists of up to kJoinMore entries
 };
 
 // Times in us are of lists of 16 blocks of 64 keys, 32 heads of 8 key/value heads.
@@ -884,7 +887,18 @@ inline AttendPlan attend_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int
   p.parts = 0;
   int64_t joined = 16 / (G < 16 ? G : 16);
   if (joined > kJoinTokens) joined = kJoinTokens;
-  const int64_t lists = kJoinMost / (kJoinWaves * (count > 0 ? count : 1));
+  const int64_t entries = kJoinWaves * (count > 0 ? count : 1);
+  const int64_t held = D <= 128 ? 1024 : 512;
+  // Lists of which kJoinMost holds one token a wave: two of them by the larger table, where there
+  // are more workgroups than the GPU holds and a block's work outweighs its entries' in the table
+  // (1000 tokens of 10 heads of 128, 96 blocks of 32 keys: 376 for 488; of 20 heads of 64: 573 for
+  // 519, but 551 for 650 with 70 blocks of 64). Lists of which it holds none: one, against a wave a
+  // row (1000 tokens of 10 heads of 128, 200 blocks of 16: 747 for 1105; of 20 heads of 96: 1243
+  // for 1103, but 1599 for 3035 with 160 blocks of 64).
+  p.more = kJoinMost / entries < 1 ? D > 96 || page >= 64
+                                   : kJoinMost / entries < 2 && (D > 64 || page >= 64) &&
+                                         cdiv(T, kJoinWaves) * Hkv > held;
+  const int64_t lists = (p.more ? kJoinMore : kJoinMost) / entries;
   if (joined > lists) joined = lists;
   // (one token a wave still shares a workgroup's loads: 460 tokens of 10 heads of 128, lists of 96
   // blocks of 32 keys, 260 us for 532 with a wave a row)
@@ -892,7 +906,6 @@ inline AttendPlan attend_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int
   // A joined workgroup's time is its chain of steps, whether it has a CU for itself or shares it,
   // so while the GPU holds them all there are twice as many with half the tokens (and a shorter
   // union): 1024 tokens of 128 channels 103 for 127, 511 tokens 73 for 114.
-  const int64_t held = D <= 128 ? 1024 : 512;
   while (p.joined > 1 && cdiv(T, kJoinWaves * (p.joined / 2)) * Hkv <= held) p.joined /= 2;
   // Prompts are joined where the chain is shorter than the split form's reads of every row's blocks
   // (split and joined: 64 channels, 300 tokens 50 and 50, 400 tokens 63 and 52; 128 channels, 200
@@ -970,8 +983,12 @@ extern "C" int rt_kv_attention(const void* q, int64_t q_token_stride, int64_t q_
     const dim3 threads(kAttendWaves * kWave);
     if (plan.parts == 0 && plan.joined > 0) {
       const int64_t grid = cdiv(T, kJoinWaves * plan.joined) * Hkv;
-      kv_attend_joined_kernel<E, DD>
-          <<<dim3(static_cast<unsigned>(grid)), dim3(kJoinWaves * kWave), 0, s>>>(a);
+      const dim3 g(static_cast<unsigned>(grid)), b(kJoinWaves * kWave);
+      if (plan.more) {
+        kv_attend_joined_kernel<E, DD, kJoinMore><<<g, b, 0, s>>>(a);
+      } else {
+        kv_attend_joined_kernel<E, DD, kJoinMost><<<g, b, 0, s>>>(a);
+      }
     } else if (plan.parts == 0) {
       const int64_t grid = cdiv(T, kAttendWaves) * Hkv * plan.tiles;
       kv_attend_rows_kernel<E, DD><<<dim3(static_cast<unsigned>(grid)), threads, 0, s>>>(a);

@@ -369,3 +369,18 @@ def test_scales_that_are_not_finite_are_refused(dev, scale):
     with pytest.raises(ValueError, match="scale"):
         kv.block_attention(to(dev, q, "bf16"), to(dev, kc, "bf16"), to(dev, vc, "bf16"),
                            to(dev, blocks), to(dev, pos), to(dev, seq), to(dev, tab), scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,heads,heads_kv,d,page,count,tokens",
+                         [("fp16", 8, 4, 128, 16, 128, 410), ("bf16", 14, 7, 96, 32, 65, 460),
+                          ("bf16", 4, 2, 256, 16, 96, 520), ("fp16", 8, 8, 64, 16, 129, 420),
+                          ("bf16", 32, 8, 128, 16, 256, 211), ("fp16", 16, 8, 192, 64, 70, 150)])
+def test_prompts_of_long_lists(dev, kind, heads, heads_kv, d, page, count, tokens):
+    """A workgroup's lists are joined though few of its tokens' fit."""
+    had_new = [(150 * page + 3, tokens - tokens // 3 - 9), (0, tokens // 3), (300 * page, 9)]
+    case = _case(tokens + d, kind, heads, heads_kv, d, page, had_new, count, sparse=0.1)
+    got = _run(dev, kind, *case)
+    pick = np.r_[0:12, rng(7).integers(0, tokens, 40), tokens - 12:tokens]
+    got, case = _some(got, case, pick)
+    _check(got, kind, *case)
