@@ -742,12 +742,19 @@ __global__ void __launch_bounds__(kFusedWaves* kWave, D <= 128 && NT == 1 ? 4 : 
 }
 
 
-// Whether tokens mostly share their sequences (their scores are then taken several tokens a wave),
-// and whether a call is one launch: few enough places for 512 lanes to bound well, and two chunks a
-// wave or rows enough to fill the GPU (one row of 1258 blocks: 13 us in two launches, 16 in one).
-inline bool select_prompt(int64_t T, int64_t B) { return B > 0 && T >= 4 * B; }
+// Whether tokens mostly share their sequences and there are keys enough (their scores are then
+// taken several tokens a wave), and whether a call is one launch: few enough places for 512 lanes
+// to bound well, and two chunks a wave or rows enough to fill the GPU (one row of 1258 blocks: 13 us
+// in two launches, 16 in one). A few tokens of one sequence take less as single tokens do, whose
+// workgroups are more (32 tokens of 8 heads of 128 over 470 blocks: 15 us for 21, 128 tokens 32 for
+// 22; 4 heads of 256: 64 tokens 19 for 41, 256 tokens 52 for 43; over 2032 blocks, two launches
+// where rows are few, 8 tokens of 4 heads of 256 18 for 36, 16 of 8 heads of 128 27 for 19).
+inline bool select_prompt(int64_t T, int64_t Hkv, int64_t B, int64_t max_pages) {
+  const double keys = static_cast<double>(T) * static_cast<double>(Hkv * max_pages);
+  return B > 0 && T >= 4 * B && keys > (max_pages <= 2 * kFusedWaves * kChunk ? 1 << 18 : 1 << 17);
+}
 inline bool select_fused(int64_t T, int64_t Hkv, int64_t B, int64_t max_pages, int64_t want) {
-  return !select_prompt(T, B) && want <= 256 &&
+  return !select_prompt(T, Hkv, B, max_pages) && want <= 256 &&
          max_pages <= (T * Hkv >= 128 ? kFusedMost : 2 * kFusedWaves * kChunk);
 }
 
@@ -765,7 +772,7 @@ inline SelectPlan select_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int
   p.stride = align_up(static_cast<size_t>(max_pages), kChunk);
   p.head_groups = static_cast<int32_t>(cdiv(Hkv, kScoreWaves));
   // (a wave with tokens of several sequences passes over each one's blocks)
-  if (select_prompt(T, B)) {
+  if (select_prompt(T, Hkv, B, max_pages)) {
     // heads whose columns fit in registers beside the bounds
     const int64_t most = D <= 128 ? 8 : 4;
     const int64_t gh = next_pow2(G);

@@ -273,3 +273,15 @@ def test_a_cache_without_pages(dev, tokens, blocks):
                   16, 10, 1, 2)
     forced = [[0, p // 16 - 1, p // 16] + [-1] * 7 for p in pos]
     assert np.array_equal(got, np.repeat(np.array(forced, np.int32)[:, None], 2, 1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_pages", [200, 2000])
+@pytest.mark.parametrize("kind,heads,heads_kv,d,page", [
+    ("bf16", 2, 2, 64, 16), ("fp16", 4, 2, 128, 64), ("bf16", 6, 2, 96, 32), ("fp16", 8, 2, 128, 16),
+    ("bf16", 14, 2, 256, 32), ("fp16", 16, 2, 64, 128), ("bf16", 24, 2, 192, 16),
+    ("fp16", 40, 2, 96, 16)])
+def test_prompts_by_the_table_s_width(dev, kind, heads, heads_kv, d, page, max_pages):
+    """The same ragged prompts as few keys (scored as single tokens are) and as many."""
+    had_new = [(90 * page + 3, 37), (0, 2 * page + 1), (150 * page, 11)]
+    _check(dev, heads + d, kind, heads, heads_kv, d, page, had_new, (24, 1, 2), max_pages=max_pages)
