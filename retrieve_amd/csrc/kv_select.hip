@@ -742,16 +742,18 @@ __global__ void __launch_bounds__(kFusedWaves* kWave, D <= 128 && NT == 1 ? 4 : 
 }
 
 
-// Whether tokens mostly share their sequences and there are keys enough (their scores are then
-// taken several tokens a wave), and whether a call is one launch: few enough places for 512 lanes
-// to bound well, and two chunks a wave or rows enough to fill the GPU (one row of 1258 blocks: 13 us
-// in two launches, 16 in one). A few tokens of one sequence take less as single tokens do, whose
-// workgroups are more (32 tokens of 8 heads of 128 over 470 blocks: 15 us for 21, 128 tokens 32 for
-// 22; 4 heads of 256: 64 tokens 19 for 41, 256 tokens 52 for 43; over 2032 blocks, two launches
-// where rows are few, 8 tokens of 4 heads of 256 18 for 36, 16 of 8 heads of 128 27 for 19).
+// Whether tokens mostly share their sequences and there are rows and keys enough (their scores are
+// then taken several tokens a wave), and whether a call is one launch: few enough places for 512
+// lanes to bound well, and two chunks a wave or rows enough to fill the GPU (one row of 1258
+// blocks: 13 us in two launches, 16 in one). Rows for little more than a workgroup a CU take less
+// as single tokens do (32 tokens of 8 heads of 128 over 470 blocks: 15 us for 21, 128 tokens 32 for
+// 22; 4 heads of 256: 64 tokens 19 for 41; 6 of 256 over 403: 93 tokens 36 for 26; over 2032
+// blocks, two launches where rows are few, 8 tokens of 4 heads of 256 18 for 36, 16 of 8 heads of
+// 128 27 for 19).
 inline bool select_prompt(int64_t T, int64_t Hkv, int64_t B, int64_t max_pages) {
-  const double keys = static_cast<double>(T) * static_cast<double>(Hkv * max_pages);
-  return B > 0 && T >= 4 * B && keys > (max_pages <= 2 * kFusedWaves * kChunk ? 1 << 18 : 1 << 17);
+  if (B <= 0 || T < 4 * B) return false;
+  if (T > 320 / Hkv) return true;
+  return max_pages > 2 * kFusedWaves * kChunk && T * Hkv * max_pages > 1 << 17;
 }
 inline bool select_fused(int64_t T, int64_t Hkv, int64_t B, int64_t max_pages, int64_t want) {
   return !select_prompt(T, Hkv, B, max_pages) && want <= 256 &&
