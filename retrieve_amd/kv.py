@@ -14,7 +14,8 @@ Tokens are packed: token ``t`` is at ``positions[t]`` of sequence ``seq_ids[t]``
 int32. One token a sequence is a decode step, many a prompt; a call may mix them. Caches are ``[P,
 Hkv, page, D]`` (a block of one head is contiguous), bounds int8 ``[P, Hkv, 2 D]`` with scales fp32
 ``[P, Hkv]``. :class:`PagedCache` holds them and makes the three calls; :func:`rotary_table` builds
-the table of cosines and sines. No counterpart in the reference; serving only (no gradients).
+the table of cosines and sines. No counterpart in the reference; serving only: the ops have no
+gradients (a backward pass through one warns and stops there, a forward-mode tangent is refused).
 
 The ops check their arguments here (``ValueError`` on shapes, ``TypeError`` on dtypes), allocate
 from torch's caching allocator and enqueue on torch's current stream, without a host
@@ -28,6 +29,7 @@ import math
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from retrieve_amd import _native as nat
 
@@ -136,11 +138,31 @@ _current = torch._C._cuda_getDevice  # (torch is initialised there: the tensors 
 _stream = torch._C._cuda_getCurrentRawStream  # (the current stream's handle, without an object)
 
 
-def _eager(q: Tensor) -> bool:
-    """Whether a call can go straight to its kernels: plain tensors, nothing being traced. Elsewhere
-    it goes through the registered op (the dispatcher's 3 to 5 us a call are a third of a small
-    one)."""
-    return type(q) is Tensor and not torch.compiler.is_compiling()
+# What a thread that traces nothing and transforms nothing has among the dispatcher's included keys.
+# The modes that see or rewrite calls (make_fx, torch.jit.trace, dispatch modes, vmap, grad, jvp)
+# each add their own.
+_included = torch._C._dispatch_tls_local_include_set
+_PLAIN_KEYS = (torch._C.DispatchKeySet(torch._C.DispatchKey.BackendSelect)
+               | torch._C.DispatchKeySet(torch._C.DispatchKey.ADInplaceOrView)).raw_repr()
+
+
+def _eager(*tensors: Tensor | None) -> bool:
+    """Whether a call can go straight to its kernels: plain tensors that carry no gradients, nothing
+    being traced or transformed. Elsewhere it goes through the registered op (the dispatcher's 3 to
+    5 us a call are a third of a small one)."""
+    if torch.compiler.is_compiling():
+        return False
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError("retrieve_kv ops have no derivatives: an input has a tangent")
+    if _included().raw_repr() & ~_PLAIN_KEYS:
+        return False
+    grad = torch.is_grad_enabled()
+    for t in tensors:
+        if t is not None and (type(t) is not Tensor or grad and t.requires_grad):
+            return False
+    return True
 
 
 # --- append -----------------------------------------------------------------------------------
@@ -201,9 +223,9 @@ def append(q: Tensor, k: Tensor, v: Tensor, cos_sin: Tensor | None, positions: T
     tokens come in order, side by side. Tokens that are padding (a position below 0, or past the
     page table or ``cos_sin``; a sequence outside it; no page) write nothing and return a zero
     row."""
-    call = _append if _eager(q) else torch.ops.retrieve_kv.append
-    return call(q, k, v, cos_sin, positions, seq_ids, page_table, k_cache, v_cache, bounds,
-                bound_scales, interleaved)
+    args = (q, k, v, cos_sin, positions, seq_ids, page_table, k_cache, v_cache, bounds, bound_scales)
+    call = _append if _eager(*args) else torch.ops.retrieve_kv.append
+    return call(*args, interleaved)
 
 
 # --- select -----------------------------------------------------------------------------------
@@ -249,9 +271,9 @@ def select_blocks(q: Tensor, bounds: Tensor, bound_scales: Tensor, positions: Te
     ``c . mid + |c| . half`` (int32; ``c`` the rotated query's int8 codes) times the query's and the
     block's scales: an upper bound on what the block's keys can score, up to the codes' rounding.
     Blocks between without a page are left out; padding tokens get -1 throughout."""
-    call = _select if _eager(q) else torch.ops.retrieve_kv.select_blocks
-    return call(q, bounds, bound_scales, positions, seq_ids, page_table, page_size, count, sink,
-                recent)
+    args = (q, bounds, bound_scales, positions, seq_ids, page_table)
+    call = _select if _eager(*args) else torch.ops.retrieve_kv.select_blocks
+    return call(*args, page_size, count, sink, recent)
 
 
 # --- attention ----------------------------------------------------------------------------------
@@ -295,8 +317,9 @@ def block_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, blocks: Tensor,
     Hq])``, ``lse`` the natural logarithm of the weights' sum. Entries below 0, past the token's
     block or without a page are skipped; a row without a key is zeros and ``-inf``. Slots past a
     token's position are not used, whatever they hold."""
-    call = _attention if _eager(q) else torch.ops.retrieve_kv.block_attention
-    return call(q, k_cache, v_cache, blocks, positions, seq_ids, page_table, scale)
+    args = (q, k_cache, v_cache, blocks, positions, seq_ids, page_table)
+    call = _attention if _eager(*args) else torch.ops.retrieve_kv.block_attention
+    return call(*args, scale)
 
 
 _lib.impl("append", _append, "CUDA")
