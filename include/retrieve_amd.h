@@ -594,9 +594,10 @@ int rt_kv_append(const void* q, int64_t q_token_stride, int64_t q_head_stride, c
  * the end. The token's own block is last = position / page. Blocks below `sink` and the `recent`
  * ones up to last are always kept (recent >= 1: the own block may have no bounds yet; sink +
  * recent <= count <= 1024); the other places go to the blocks between, by (score desc, block asc). A
- * query head's row is quantised as bounds are (codes c, scale s); score(b) = max over the group's
- * heads of float(c . mid_b + |c| . half_b) * s, times the block's scale (the sum exact in int32,
- * two float products); not a number ranks last. Blocks without a page are not candidates. */
+ * query head's row is quantised as bounds are (codes c, scale s; a quotient that is not a number has
+ * the code -127); score(b) = max over the group's heads of float(c . mid_b + |c| . half_b) * s (heads
+ * that give no number are passed over), times the block's scale (the sum exact in int32, two float
+ * products); not a number ranks last. Blocks without a page are not candidates. */
 size_t rt_kv_select_workspace(int64_t T, int64_t Hkv, int64_t B, int64_t max_pages, int64_t count,
                               int64_t sink, int64_t recent);
 int rt_kv_select(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t T,

@@ -68,7 +68,7 @@ __device__ inline int kv_code(float x, float top) {
 // is the quotient rounded to nearest wherever |x| <= top, top is normal and its significand is not
 // all ones (Markstein's theorem; queries of 16 bits have neither), in 3 instructions instead of
 // about ten. For a top above 2^100, whose reciprocal may lose bits, x and top come in scaled by
-// 2^-64.
+// 2^-64; for an infinite one (r = 0) as 1, since 0 times the infinity would not be a number.
 __device__ inline float kv_code_value(float x, float top, float r) {
 #pragma clang fp contract(off)
   const float q = x * r;

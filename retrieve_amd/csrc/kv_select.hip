@@ -186,6 +186,8 @@ __device__ inline void score_blocks(const SelectArgs& a, int64_t t0, int head, i
         const float small = top > 0x1p100f ? 0x1p-64f : 1.0f;
         top *= small;
         const float r = 1.0f / top;
+        // (an infinite row: by 1 and r = 0 a finite channel is 0 and an infinite one NaN, as divided)
+        if (r == 0.0f) top = 1.0f;
 #pragma unroll
         for (int s = 0; s < LOADS; ++s) {
           v4i codes, sizes;
