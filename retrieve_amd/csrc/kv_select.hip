@@ -53,9 +53,11 @@ struct SelectArgs {
   int32_t head_groups;
 };
 
-// The key of a candidate's score (0: not a candidate). A score that is not a number is the least.
-__device__ inline uint32_t score_key(float s) {
-  return key_of_f32(fmaxf(s, -INFINITY));
+// The key of a candidate's score, the group's times the block's scale (0: not a candidate). A score
+// that is not a number is the least. (The sum with 0 makes -0, of a block of scale 0, the other zero's
+// equal.)
+__device__ inline uint32_t score_key(float group, float scale) {
+  return key_of_f32(fmaxf(fmaf(group, scale, 0.0f), -INFINITY));
 }
 
 // The largest over aligned groups of 16 lanes, in every lane.
@@ -318,7 +320,7 @@ __device__ inline void score_blocks(const SelectArgs& a, int64_t t0, int head, i
             for (int r = 0; r < 4; ++r) {
               key[r] = pass + 1 < passes ? __float_as_int(best[g][r])
                        : pg[r] < 0       ? 0
-                                         : static_cast<int>(score_key(best[g][r] * bs[r]));
+                                         : static_cast<int>(score_key(best[g][r], bs[r]));
             }
             *to = key;
           }

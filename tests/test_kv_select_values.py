@@ -1,4 +1,4 @@
-"""Choosing blocks by scores at the ends of the range: infinite queries."""
+"""Choosing blocks by scores at the ends of the range: infinite queries, scores of either zero."""
 
 from __future__ import annotations
 
@@ -53,3 +53,20 @@ def test_infinite_queries(dev, tokens, d):
         assert len(set(np.sign(score[~np.isnan(score)]))) == 2 and np.isnan(score).any()
         got = _run(dev, q, codes, scales, tab, blocks, 20, tokens)
         assert got.tolist() == _order(score, 19) + [blocks - 1]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", FORMS)
+@pytest.mark.parametrize("blocks", [60, 5000])
+def test_either_zero_is_one_score(dev, tokens, blocks):
+    """Blocks of scale 0 score zero whichever the sign of their sums: ties, to the lower block."""
+    _, _, tab, pages = layout(11, 16, [(16 * blocks - 1, 1)])
+    q = normal16(12, (1, 2, 64), "bf16")
+    codes = rng(13).integers(-127, 128, (pages, 1, 128), dtype=np.int8)
+    scales = np.zeros((pages, 1), np.float32)
+    best = [11, 29, blocks - 3]
+    codes[tab[0, best]] = 0
+    codes[tab[0, best], :, 64:] = 1
+    scales[tab[0, best]] = 1.0
+    got = _run(dev, q, codes, scales, tab, blocks, 20, tokens)
+    assert got.tolist() == sorted(set(range(17)) | set(best)) + [blocks - 1]
