@@ -15,8 +15,10 @@
 // A lane's column is one head in both products: maxima, sums and rescaling stay in the lane. The
 // maximum is raised only where a score passes it by 8 (in powers of two: weights reach 256 at
 // most, far inside both types), so most steps do not touch the accumulators or exchange lanes.
-// Weights are rounded to the values' 16 bits for the matrix cores (l sums them unrounded):
-// relative 2^-9 / 2^-12 a weight, the size of the output's own rounding.
+// Weights are rounded to the values' 16 bits for the matrix cores (l sums them unrounded): relative
+// 2^-9 / 2^-12 a weight, the size of the output's own rounding. fp16's step is absolute below 2^-14, so
+// its weights are held 2^5 times as large (m is 5 below the maximum; they reach 2^13): at most 2^-30
+// of the row's largest weight a key, half an output's rounding over 2^17 keys.
 //
 // Memory: a wave keeps the next step's keys and values in flight (registers) while it works on
 // this one. Slots past the token's position are read but replaced: scores by -inf, values by 0.
@@ -155,12 +157,13 @@ __device__ inline V load_row(const V* p) {
 }
 
 // A wave's accumulators (channel 16 i + 4 (lane / 16) + r of column lane % 16), the columns' maxima
-// and this lane's share of their sums; its queries and the step in flight.
+// (less kLift) and this lane's share of their sums; its queries and the step in flight.
 template <class E, int D>
 struct AttendWave {
   using Op = AttendOp<E>;
   using V8 = typename Op::V8;
   static constexpr int KS = D / 32, DT = D / 16, VL = D / 16;  // VL: 16-byte loads of V a lane
+  static constexpr float kLift = std::is_same<E, _Float16>::value ? 5.0f : 0.0f;  // maximum - m
   v4f acc[DT];
   float m, l;
   V8 qf[KS], kf[2][KS], vf[VL];
@@ -263,10 +266,10 @@ struct AttendWave {
 #pragma unroll
     for (int j = 1; j < N; ++j) top[0] = fmaxf(top[0], top[j]);
     const float high = top[0] * scale;
-    if (__any(high > m + 8.0f)) {
+    if (__any(high - m > 8.0f + kLift)) {
       float next = fmaxf(high, __shfl_xor(high, 16));
       next = fmaxf(next, __shfl_xor(next, 32));
-      next = fmaxf(next, m);
+      next = fmaxf(next - kLift, m);
       const float keep = __builtin_amdgcn_exp2f(m - next);
       m = next;
       l *= keep;
