@@ -51,6 +51,7 @@ struct SelectArgs {
   int64_t stride;
   int32_t splits;     // waves that share a wave's tokens' blocks
   int32_t head_groups;
+  int32_t above;      // rows of so many candidates or fewer are another launch's (-1: none)
 };
 
 // The key of a candidate's score, the group's times the block's scale (0: not a candidate). A score
@@ -548,6 +549,7 @@ __global__ void __launch_bounds__(4 * kWave) kv_keep_few_kernel(SelectArgs a) {
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + wave;
   if (row >= a.T * a.Hkv) return;
   const Span p(a, row);
+  if (p.n > R * kWave) return;  // (kv_keep_many_kernel's)
   keep_few<R>(a, p, a.keys + row * a.stride + p.lead, near[wave], near_at[wave]);
 }
 
@@ -711,6 +713,7 @@ __global__ void __launch_bounds__(WAVES* kWave) kv_keep_many_kernel(SelectArgs a
   __shared__ KeepLds<WAVES> lds;
   const int64_t row = blockIdx.x;
   const Span p(a, row);
+  if (p.n <= a.above) return;
   keep_many<WAVES, R>(a, p, a.keys + row * a.stride + p.lead, lds);
 }
 
@@ -763,6 +766,8 @@ inline bool select_fused(int64_t T, int64_t Hkv, int64_t B, int64_t max_pages, i
   return !select_prompt(T, Hkv, B, max_pages) && want <= 256 &&
          max_pages <= (T * Hkv >= 128 ? kFusedMost : 2 * kFusedWaves * kChunk);
 }
+
+constexpr int64_t kKeepRows = 2048;  // rows whose short ones are cut in a launch of their own
 
 // gh = 0: a token a wave, its heads across `tiles` tiles. gh > 0: tokens across the lanes, gh heads
 // a pass.
@@ -891,13 +896,21 @@ extern "C" int rt_kv_select(const void* q, int64_t q_token_stride, int64_t q_hea
     if (st != kOk) return st;
   }
   // A wave a row while its keys fit in 16 registers a lane; then four waves, unless more places are
-  // wanted than their lanes bound well; then sixteen.
+  // wanted than their lanes bound well; then sixteen. Of many rows each is cut by its own number of
+  // candidates, not by the table's width: the short ones a wave a row in a launch before (4099 tokens
+  // of 8 heads behind 313 blocks of a table of 16384 columns: 168 for 616 us). With fewer rows that
+  // launch costs what it saves (1024 rows behind 313 blocks of 2048 columns: 28 us for 23.5).
   const int64_t rows = T * Hkv;
   const dim3 one(static_cast<unsigned>(rows)), four(static_cast<unsigned>(cdiv(rows, 4)));
+  const bool few = max_pages <= 64 * 16;
+  a.above = -1;
   if (max_pages <= 64 * 4) {
     kv_keep_few_kernel<4><<<four, 4 * kWave, 0, s>>>(a);
-  } else if (max_pages <= 64 * 16) {
+  } else if (few || rows >= kKeepRows) {
     kv_keep_few_kernel<16><<<four, 4 * kWave, 0, s>>>(a);
+    a.above = 64 * 16;
+  }
+  if (few) {
   } else if (max_pages <= 4 * 64 * 16 && count - sink - recent <= 128) {
     kv_keep_many_kernel<4, 16><<<one, 4 * kWave, 0, s>>>(a);
   } else if (max_pages <= 16 * 64 * 16) {
