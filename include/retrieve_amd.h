@@ -597,7 +597,9 @@ int rt_kv_append(const void* q, int64_t q_token_stride, int64_t q_head_stride, c
  * query head's row is quantised as bounds are (codes c, scale s; a quotient that is not a number has
  * the code -127); score(b) = max over the group's heads of float(c . mid_b + |c| . half_b) * s (heads
  * that give no number are passed over), times the block's scale (the sum exact in int32, two float
- * products); not a number ranks last. Blocks without a page are not candidates. */
+ * products); not a number ranks last. Blocks without a page are not candidates. The workspace is at
+ * most 512 MiB, or one token's keys (4 Hkv max_pages bytes) where these are more: longer calls take
+ * their tokens in pieces. */
 size_t rt_kv_select_workspace(int64_t T, int64_t Hkv, int64_t B, int64_t max_pages, int64_t count,
                               int64_t sink, int64_t recent);
 int rt_kv_select(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t T,

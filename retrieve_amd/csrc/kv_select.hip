@@ -776,14 +776,14 @@ struct SelectPlan {
   int32_t tiles, gh, per_wave, splits, head_groups;
 };
 
-inline SelectPlan select_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t B,
+inline SelectPlan select_plan(bool prompt, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
                               int64_t max_pages, int64_t sink) {
   SelectPlan p;
   const int64_t G = Hq / Hkv;
   p.stride = align_up(static_cast<size_t>(max_pages), kChunk);
   p.head_groups = static_cast<int32_t>(cdiv(Hkv, kScoreWaves));
   // (a wave with tokens of several sequences passes over each one's blocks)
-  if (select_prompt(T, Hkv, B, max_pages)) {
+  if (prompt) {
     // heads whose columns fit in registers beside the bounds
     const int64_t most = D <= 128 ? 8 : 4;
     const int64_t gh = next_pow2(G);
@@ -802,72 +802,27 @@ inline SelectPlan select_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int
   return p;
 }
 
-}  // namespace rt
-
-using namespace rt;
-
-extern "C" size_t rt_kv_select_workspace(int64_t T, int64_t Hkv, int64_t B, int64_t max_pages,
-                                         int64_t count, int64_t sink, int64_t recent) {
-  if (T < 1 || Hkv < 1 || max_pages < 1) return 0;
-  if (select_fused(T, Hkv, B, max_pages, count - sink - recent)) return 0;
-  return static_cast<size_t>(T) * Hkv * align_up(static_cast<size_t>(max_pages), kChunk) *
-         sizeof(uint32_t);
+// In two launches a call's tokens are taken in slabs whose keys fit in kSlabBytes (of 64s of tokens,
+// whole waves of either form, where that many fit), one after the other over the same workspace, so
+// it grows neither with a prompt's length nor, but for a token's own rows, with the page table. A slab
+// has to fill the GPU: 4099 tokens of 8 heads behind 313 blocks of a table of 16384 columns take
+// 602 us in slabs of 128 MiB, 403 of 256, 269 of 512 and 168 in one of 2.1 GiB; 8192 tokens in a
+// table of 2048 columns 303, 232, and 202 in the one of 512.
+constexpr int64_t kSlabBytes = int64_t{512} << 20;
+inline int64_t select_slab(int64_t T, int64_t Hkv, int64_t max_pages) {
+  const size_t row = align_up(static_cast<size_t>(max_pages > 0 ? max_pages : 1), kChunk);
+  int64_t n = kSlabBytes / static_cast<int64_t>(Hkv * row * sizeof(uint32_t));
+  if (n >= 64) n &= ~int64_t{63};
+  if (n < 1) n = 1;
+  return n < T ? n : T;
 }
 
-extern "C" int rt_kv_select(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t T,
-                            int64_t Hq, int64_t Hkv, int64_t D, int dtype, const int8_t* bounds,
-                            const float* bound_scales, int64_t P, int64_t page,
-                            const int32_t* positions, const int32_t* seq_ids,
-                            const int32_t* page_table, int64_t B, int64_t max_pages, int64_t count,
-                            int64_t sink, int64_t recent, int32_t* out, void* workspace,
-                            size_t workspace_bytes, rt_stream_t stream) {
-  if (const int st = kv_check(T, Hq, Hkv, D, dtype, B, max_pages, P, page)) return st;
-  RT_CHECK_ARG(count >= 1 && count <= 1024, "count must be in [1, 1024], got %lld",
-               static_cast<long long>(count));
-  RT_CHECK_ARG(sink >= 0 && recent >= 1 && sink + recent <= count,
-               "sink >= 0 and recent >= 1 must fit in count");
-  if (T == 0) return kOk;
-  RT_CHECK_ARG(q && positions && seq_ids && out, "null pointer");
-  RT_CHECK_ARG(B * max_pages == 0 || page_table, "null page table");
-  RT_CHECK_ARG(P == 0 || (bounds && bound_scales), "null bounds");
-  RT_CHECK_ARG(kv_rows_aligned(q, q_token_stride, q_head_stride) && kv_rows_aligned(bounds, 0, 0),
-               "rows must start on 16 bytes");
-  RT_CHECK_ARG(T * Hkv <= INT32_MAX - 8, "too many tokens");
-  const size_t need = rt_kv_select_workspace(T, Hkv, B, max_pages, count, sink, recent);
-  if (workspace_bytes < need || (need > 0 && workspace == nullptr)) {
-    set_error("workspace too small: %zu < %zu", workspace_bytes, need);
-    return kWorkspaceTooSmall;
-  }
-  const SelectPlan plan = select_plan(T, Hq, Hkv, D, B, max_pages, sink);
-  SelectArgs a{};
-  a.q = q, a.q_st = q_token_stride, a.q_sh = q_head_stride, a.T = T;
-  a.Hq = static_cast<int32_t>(Hq), a.Hkv = static_cast<int32_t>(Hkv), a.G = a.Hq / a.Hkv;
-  a.bounds = bounds, a.scales = bound_scales;
-  a.tok = {positions, seq_ids, page_table, static_cast<int32_t>(B),
-           static_cast<int32_t>(max_pages), static_cast<int32_t>(P), kv_shift(page)};
-  a.count = static_cast<int32_t>(count), a.sink = static_cast<int32_t>(sink);
-  a.recent = static_cast<int32_t>(recent), a.out = out, a.keys = static_cast<uint32_t*>(workspace);
-  // (blocks without a page read page 0's bounds, so there has to be one)
-  a.want = P > 0 ? static_cast<int32_t>(count - sink - recent) : 0;
-  a.stride = plan.stride, a.splits = plan.splits, a.head_groups = plan.head_groups;
-  const hipStream_t s = static_cast<hipStream_t>(stream);
-  if (select_fused(T, Hkv, B, max_pages, count - sink - recent)) {
-    return kv_dispatch(dtype, D, [&](auto e, auto d) -> int {
-      using E = decltype(e);
-      constexpr int DD = decltype(d)::value;
-      const dim3 g(static_cast<unsigned>(cdiv(T * Hkv, 8) * 8)), b(kFusedWaves * kWave);
-      if (plan.tiles == 1) {
-        kv_select_kernel<E, DD, 1><<<g, b, 0, s>>>(a);
-      } else {
-        kv_select_kernel<E, DD, 2><<<g, b, 0, s>>>(a);
-      }
-      RT_CHECK_HIP(hipGetLastError());
-      return kOk;
-    });
-  }
-  const int64_t grid = cdiv(T, plan.per_wave) * plan.splits * plan.head_groups;
+// The launches of a slab: scores, then the cut.
+inline int select_slab_blocks(SelectArgs a, const SelectPlan& plan, int dtype, int64_t D,
+                              int64_t max_pages, hipStream_t s) {
+  const int64_t grid = cdiv(a.T, plan.per_wave) * plan.splits * plan.head_groups;
   RT_CHECK_ARG(grid <= INT32_MAX, "too many tokens");
-  if (max_pages > sink && a.want > 0) {  // else no block is chosen by its score
+  if (max_pages > a.sink && a.want > 0) {  // else no block is chosen by its score
     const int st = kv_dispatch(dtype, D, [&](auto e, auto d) -> int {
       using E = decltype(e);
       constexpr int DD = decltype(d)::value;
@@ -900,7 +855,7 @@ extern "C" int rt_kv_select(const void* q, int64_t q_token_stride, int64_t q_hea
   // candidates, not by the table's width: the short ones a wave a row in a launch before (4099 tokens
   // of 8 heads behind 313 blocks of a table of 16384 columns: 168 for 616 us). With fewer rows that
   // launch costs what it saves (1024 rows behind 313 blocks of 2048 columns: 28 us for 23.5).
-  const int64_t rows = T * Hkv;
+  const int64_t rows = a.T * a.Hkv;
   const dim3 one(static_cast<unsigned>(rows)), four(static_cast<unsigned>(cdiv(rows, 4)));
   const bool few = max_pages <= 64 * 16;
   a.above = -1;
@@ -911,7 +866,7 @@ extern "C" int rt_kv_select(const void* q, int64_t q_token_stride, int64_t q_hea
     a.above = 64 * 16;
   }
   if (few) {
-  } else if (max_pages <= 4 * 64 * 16 && count - sink - recent <= 128) {
+  } else if (max_pages <= 4 * 64 * 16 && a.count - a.sink - a.recent <= 128) {
     kv_keep_many_kernel<4, 16><<<one, 4 * kWave, 0, s>>>(a);
   } else if (max_pages <= 16 * 64 * 16) {
     kv_keep_many_kernel<16, 16><<<one, 16 * kWave, 0, s>>>(a);
@@ -919,5 +874,81 @@ extern "C" int rt_kv_select(const void* q, int64_t q_token_stride, int64_t q_hea
     kv_keep_many_kernel<16, 0><<<one, 16 * kWave, 0, s>>>(a);
   }
   RT_CHECK_HIP(hipGetLastError());
+  return kOk;
+}
+
+}  // namespace rt
+
+using namespace rt;
+
+extern "C" size_t rt_kv_select_workspace(int64_t T, int64_t Hkv, int64_t B, int64_t max_pages,
+                                         int64_t count, int64_t sink, int64_t recent) {
+  if (T < 1 || Hkv < 1 || max_pages < 1) return 0;
+  if (select_fused(T, Hkv, B, max_pages, count - sink - recent)) return 0;
+  return static_cast<size_t>(select_slab(T, Hkv, max_pages)) * Hkv *
+         align_up(static_cast<size_t>(max_pages), kChunk) * sizeof(uint32_t);
+}
+
+extern "C" int rt_kv_select(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t T,
+                            int64_t Hq, int64_t Hkv, int64_t D, int dtype, const int8_t* bounds,
+                            const float* bound_scales, int64_t P, int64_t page,
+                            const int32_t* positions, const int32_t* seq_ids,
+                            const int32_t* page_table, int64_t B, int64_t max_pages, int64_t count,
+                            int64_t sink, int64_t recent, int32_t* out, void* workspace,
+                            size_t workspace_bytes, rt_stream_t stream) {
+  if (const int st = kv_check(T, Hq, Hkv, D, dtype, B, max_pages, P, page)) return st;
+  RT_CHECK_ARG(count >= 1 && count <= 1024, "count must be in [1, 1024], got %lld",
+               static_cast<long long>(count));
+  RT_CHECK_ARG(sink >= 0 && recent >= 1 && sink + recent <= count,
+               "sink >= 0 and recent >= 1 must fit in count");
+  if (T == 0) return kOk;
+  RT_CHECK_ARG(q && positions && seq_ids && out, "null pointer");
+  RT_CHECK_ARG(B * max_pages == 0 || page_table, "null page table");
+  RT_CHECK_ARG(P == 0 || (bounds && bound_scales), "null bounds");
+  RT_CHECK_ARG(kv_rows_aligned(q, q_token_stride, q_head_stride) && kv_rows_aligned(bounds, 0, 0),
+               "rows must start on 16 bytes");
+  RT_CHECK_ARG(T * Hkv <= INT32_MAX - 8, "too many tokens");
+  const size_t need = rt_kv_select_workspace(T, Hkv, B, max_pages, count, sink, recent);
+  if (workspace_bytes < need || (need > 0 && workspace == nullptr)) {
+    set_error("workspace too small: %zu < %zu", workspace_bytes, need);
+    return kWorkspaceTooSmall;
+  }
+  SelectArgs a{};
+  a.q = q, a.q_st = q_token_stride, a.q_sh = q_head_stride, a.T = T;
+  a.Hq = static_cast<int32_t>(Hq), a.Hkv = static_cast<int32_t>(Hkv), a.G = a.Hq / a.Hkv;
+  a.bounds = bounds, a.scales = bound_scales;
+  a.tok = {positions, seq_ids, page_table, static_cast<int32_t>(B),
+           static_cast<int32_t>(max_pages), static_cast<int32_t>(P), kv_shift(page)};
+  a.count = static_cast<int32_t>(count), a.sink = static_cast<int32_t>(sink);
+  a.recent = static_cast<int32_t>(recent), a.out = out, a.keys = static_cast<uint32_t*>(workspace);
+  // (blocks without a page read page 0's bounds, so there has to be one)
+  a.want = P > 0 ? static_cast<int32_t>(count - sink - recent) : 0;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (select_fused(T, Hkv, B, max_pages, count - sink - recent)) {
+    return kv_dispatch(dtype, D, [&](auto e, auto d) -> int {
+      using E = decltype(e);
+      constexpr int DD = decltype(d)::value;
+      const dim3 g(static_cast<unsigned>(cdiv(T * Hkv, 8) * 8)), b(kFusedWaves * kWave);
+      if (a.G <= 16) {
+        kv_select_kernel<E, DD, 1><<<g, b, 0, s>>>(a);
+      } else {
+        kv_select_kernel<E, DD, 2><<<g, b, 0, s>>>(a);
+      }
+      RT_CHECK_HIP(hipGetLastError());
+      return kOk;
+    });
+  }
+  const bool prompt = select_prompt(T, Hkv, B, max_pages);
+  const int64_t slab = select_slab(T, Hkv, max_pages);
+  for (int64_t t0 = 0; t0 < T; t0 += slab) {
+    SelectArgs part = a;
+    part.T = T - t0 < slab ? T - t0 : slab;
+    part.q = static_cast<const uint16_t*>(q) + t0 * q_token_stride;  // (16 bits an element)
+    part.tok.positions += t0, part.tok.seq_ids += t0;
+    part.out += t0 * Hkv * count;
+    const SelectPlan plan = select_plan(prompt, part.T, Hq, Hkv, D, max_pages, sink);
+    part.stride = plan.stride, part.splits = plan.splits, part.head_groups = plan.head_groups;
+    if (const int st = select_slab_blocks(part, plan, dtype, D, max_pages, s)) return st;
+  }
   return kOk;
 }
