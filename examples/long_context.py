@@ -34,11 +34,12 @@ class Layer(torch.nn.Module):
         self.out = torch.nn.Linear(width, width, bias=False)
         self.cache, self.cos_sin = cache, cos_sin
 
-    def forward(self, x, positions, seq_ids):
+    def forward(self, x, positions, seq_ids, sequences):
         rows = self.qkv(x).view(len(x), -1, self.dim)
         q, k, v = rows.split([self.heads, self.heads_kv, self.heads_kv], 1)  # (strided views)
         q = self.cache.append(q, k, v, self.cos_sin, positions, seq_ids)
-        out, lse = self.cache.attend(q, positions, seq_ids, self.chosen, sink=1, recent=2)
+        out, lse = self.cache.attend(q, positions, seq_ids, self.chosen, sink=1, recent=2,
+                                     sequences=sequences)
         return self.out(out.view(len(x), -1)), q, lse
 
 
@@ -64,7 +65,7 @@ def run(sequences: int, context: int, chosen: int, steps: int, heads: int = 32, 
         for s in range(sequences):
             x = torch.randn(n, heads * dim, device=dev, dtype=torch.bfloat16)
             seq_ids = torch.full((n,), s, dtype=torch.int32, device=dev)
-            layer(x, positions[first:first + n], seq_ids)
+            layer(x, positions[first:first + n], seq_ids, 1)
     mid.record()
 
     # single tokens: one graph, replayed with its inputs rewritten in place
@@ -74,11 +75,11 @@ def run(sequences: int, context: int, chosen: int, steps: int, heads: int = 32, 
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
-        layer(x, pos, seq_ids)
+        layer(x, pos, seq_ids, sequences)
     torch.cuda.current_stream().wait_stream(side)
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
-        y, q, lse = layer(x, pos, seq_ids)
+        y, q, lse = layer(x, pos, seq_ids, sequences)
     graph.replay()  # (the first replay sends the graph to the GPU)
     decode = torch.cuda.Event(enable_timing=True)
     decode.record()

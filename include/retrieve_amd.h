@@ -600,14 +600,24 @@ int rt_kv_append(const void* q, int64_t q_token_stride, int64_t q_head_stride, c
  * products); not a number ranks last. Blocks without a page are not candidates. The workspace is at
  * most 512 MiB, or one token's keys (4 Hkv max_pages bytes) where these are more: longer calls take
  * their tokens in pieces. */
-size_t rt_kv_select_workspace(int64_t T, int64_t Hkv, int64_t B, int64_t max_pages, int64_t count,
-                              int64_t sink, int64_t recent);
+size_t rt_kv_select_workspace(int64_t T, int64_t Hkv, int64_t sequences, int64_t max_pages,
+                              int64_t count, int64_t sink, int64_t recent);
 int rt_kv_select(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t T,
                  int64_t Hq, int64_t Hkv, int64_t D, int dtype, const int8_t* bounds,
                  const float* bound_scales, int64_t P, int64_t page, const int32_t* positions,
                  const int32_t* seq_ids, const int32_t* page_table, int64_t B, int64_t max_pages,
                  int64_t count, int64_t sink, int64_t recent, int32_t* out, void* workspace,
                  size_t workspace_bytes, rt_stream_t stream);
+
+/* rt_kv_select for a call whose tokens belong to at most `sequences` sequences (the plain call takes
+ * B, the rows of the page table, which may have many idle ones). The number chooses among kernels
+ * only: the results are the same whatever it is. The workspace is asked for with the same number. */
+int rt_kv_select_of(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t T,
+                    int64_t Hq, int64_t Hkv, int64_t D, int dtype, const int8_t* bounds,
+                    const float* bound_scales, int64_t P, int64_t page, const int32_t* positions,
+                    const int32_t* seq_ids, const int32_t* page_table, int64_t B, int64_t max_pages,
+                    int64_t count, int64_t sink, int64_t recent, int64_t sequences, int32_t* out,
+                    void* workspace, size_t workspace_bytes, rt_stream_t stream);
 
 /* Softmax attention over listed blocks: blocks int32 [T, Hkv, count] (each block at most once a row,
  * any order; entries below 0, past the token's block or without a page are skipped), the keys at
@@ -622,6 +632,17 @@ int rt_kv_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride
                     int64_t count, const int32_t* positions, const int32_t* seq_ids,
                     const int32_t* page_table, int64_t B, int64_t max_pages, float scale, void* out,
                     float* lse, void* workspace, size_t workspace_bytes, rt_stream_t stream);
+
+/* rt_kv_attention with the number of sequences, as rt_kv_select_of has it. Either form's outputs are
+ * within the roundings of the weights and sums; their order, and so the last bits, may differ. The
+ * workspace does not depend on the number. */
+int rt_kv_attention_of(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t T,
+                       int64_t Hq, int64_t Hkv, int64_t D, int dtype, const void* k_cache,
+                       const void* v_cache, int64_t P, int64_t page, const int32_t* blocks,
+                       int64_t count, const int32_t* positions, const int32_t* seq_ids,
+                       const int32_t* page_table, int64_t B, int64_t max_pages, float scale,
+                       int64_t sequences, void* out, float* lse, void* workspace,
+                       size_t workspace_bytes, rt_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -167,11 +167,21 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_c_p, *[_c_i64] * 6, _c_int, _c_p, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_p, *[_c_i64] * 5,
          _c_p, _c_p, _c_sz, _c_p],
     ),
+    "rt_kv_select_of": (
+        _c_int,
+        [_c_p, *[_c_i64] * 6, _c_int, _c_p, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_p, *[_c_i64] * 6,
+         _c_p, _c_p, _c_sz, _c_p],
+    ),
     "rt_kv_attention_workspace": (_c_sz, [_c_i64] * 6),
     "rt_kv_attention": (
         _c_int,
         [_c_p, *[_c_i64] * 6, _c_int, _c_p, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_p, _c_p, _c_p,
          _c_i64, _c_i64, ctypes.c_float, _c_p, _c_p, _c_p, _c_sz, _c_p],
+    ),
+    "rt_kv_attention_of": (
+        _c_int,
+        [_c_p, *[_c_i64] * 6, _c_int, _c_p, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_p, _c_p, _c_p,
+         _c_i64, _c_i64, ctypes.c_float, _c_i64, _c_p, _c_p, _c_p, _c_sz, _c_p],
     ),
     "rt_int8_scan_topk_noalloc": (
         _c_int, [_c_p, _c_i64, _c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_p, _c_p, _c_p],

@@ -873,7 +873,8 @@ __global__ void __launch_bounds__(D / 4) kv_join_kernel(AttendArgs a) {
   if (threadIdx.x == 0) a.lse[r] = log_sum(m, l);
 }
 
-// How a call is spread: `parts` workgroups a row; 0: `joined` tokens a wave, or (0) a wave a row.
+// How a call of `seqs` sequences at most is spread: `parts` workgroups a row; 0: `joined` tokens a
+// wave, or (0) a wave a row.
 struct AttendPlan {
   int64_t rows;
   int32_t tiles, parts, joined;
@@ -881,7 +882,7 @@ struct AttendPlan {
 };
 
 // Times in us are of lists of 16 blocks of 64 keys, 32 heads of 8 key/value heads.
-inline AttendPlan attend_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t B,
+inline AttendPlan attend_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t seqs,
                               int64_t page, int64_t count) {
   AttendPlan p;
   const int64_t G = Hq / Hkv;
@@ -915,11 +916,11 @@ inline AttendPlan attend_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int
   // tokens 67 and 53; 256 channels, 100 tokens 100 and 99, 200 tokens 176 and 85). No more tokens
   // than sequences are taken for single tokens, which share nothing: 500 of 128 channels take 328
   // split and 365 joined, 2000 take 1246 and 1434.
-  if (T > B && (p.joined > 0 ? p.rows * D >= 200 << 10 : p.rows >= 4096)) return p;
+  if (T > seqs && (p.joined > 0 ? p.rows * D >= 200 << 10 : p.rows >= 4096)) return p;
   // Workgroups of four waves for two on every CU, each wave with a unit of 64 keys at least. A
   // second launch that joins the parts costs 4 us, a row in one workgroup more: one token of 8
   // heads over 32 blocks of 64 keys takes 12 us in 8 parts a row, 23 in one workgroup of 8 waves.
-  // (Rows whose parts are several are too few to be joined: the workspace does not depend on B.)
+  // (Rows whose parts are several are too few to be joined: the workspace does not depend on seqs.)
   const int64_t most = cdiv(count * page, 64 * kAttendWaves);
   const int64_t want = cdiv(512, p.rows > 0 ? p.rows : 1);
   p.parts = static_cast<int32_t>(want < most ? want : most);
@@ -945,6 +946,19 @@ extern "C" int rt_kv_attention(const void* q, int64_t q_token_stride, int64_t q_
                                const int32_t* seq_ids, const int32_t* page_table, int64_t B,
                                int64_t max_pages, float scale, void* out, float* lse,
                                void* workspace, size_t workspace_bytes, rt_stream_t stream) {
+  return rt_kv_attention_of(q, q_token_stride, q_head_stride, T, Hq, Hkv, D, dtype, k_cache, v_cache,
+                            P, page, blocks, count, positions, seq_ids, page_table, B, max_pages,
+                            scale, B, out, lse, workspace, workspace_bytes, stream);
+}
+
+extern "C" int rt_kv_attention_of(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                                  int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int dtype,
+                                  const void* k_cache, const void* v_cache, int64_t P, int64_t page,
+                                  const int32_t* blocks, int64_t count, const int32_t* positions,
+                                  const int32_t* seq_ids, const int32_t* page_table, int64_t B,
+                                  int64_t max_pages, float scale, int64_t sequences, void* out,
+                                  float* lse, void* workspace, size_t workspace_bytes,
+                                  rt_stream_t stream) {
   if (const int st = kv_check(T, Hq, Hkv, D, dtype, B, max_pages, P, page)) return st;
   RT_CHECK_ARG(count >= 0 && count <= (1 << 20), "count must be in [0, 2^20], got %lld",
                static_cast<long long>(count));
@@ -959,12 +973,14 @@ extern "C" int rt_kv_attention(const void* q, int64_t q_token_stride, int64_t q_
   RT_CHECK_ARG(T * Hq <= INT32_MAX, "too many tokens");
   RT_CHECK_ARG(std::isfinite(scale * kLog2e), "the scale must be finite, got %g",
                static_cast<double>(scale));
+  RT_CHECK_ARG(sequences >= 0, "sequences must not be negative, got %lld",
+               static_cast<long long>(sequences));
   const size_t need = rt_kv_attention_workspace(T, Hq, Hkv, D, page, count);
   if (workspace_bytes < need || (need > 0 && workspace == nullptr)) {
     set_error("workspace too small: %zu < %zu", workspace_bytes, need);
     return kWorkspaceTooSmall;
   }
-  const AttendPlan plan = attend_plan(T, Hq, Hkv, D, B, page, count);
+  const AttendPlan plan = attend_plan(T, Hq, Hkv, D, sequences, page, count);
   AttendArgs a{};
   a.q = q, a.q_st = q_token_stride, a.q_sh = q_head_stride, a.T = T;
   a.Hq = static_cast<int32_t>(Hq), a.Hkv = static_cast<int32_t>(Hkv);

@@ -749,21 +749,21 @@ __global__ void __launch_bounds__(kFusedWaves* kWave, D <= 128 && NT == 1 ? 4 : 
 }
 
 
-// Whether tokens mostly share their sequences and there are rows and keys enough (their scores are
-// then taken several tokens a wave), and whether a call is one launch: few enough places for 512
+// Whether tokens mostly share their sequences (`seqs` of them at most) and there are rows and keys
+// enough (their scores are then taken several tokens a wave), and whether a call is one launch: few enough places for 512
 // lanes to bound well, and two chunks a wave or rows enough to fill the GPU (one row of 1258
 // blocks: 13 us in two launches, 16 in one). Rows for little more than a workgroup a CU take less
 // as single tokens do (32 tokens of 8 heads of 128 over 470 blocks: 15 us for 21, 128 tokens 32 for
 // 22; 4 heads of 256: 64 tokens 19 for 41; 6 of 256 over 403: 93 tokens 36 for 26; over 2032
 // blocks, two launches where rows are few, 8 tokens of 4 heads of 256 18 for 36, 16 of 8 heads of
 // 128 27 for 19).
-inline bool select_prompt(int64_t T, int64_t Hkv, int64_t B, int64_t max_pages) {
-  if (B <= 0 || T < 4 * B) return false;
+inline bool select_prompt(int64_t T, int64_t Hkv, int64_t seqs, int64_t max_pages) {
+  if (seqs <= 0 || T < 4 * seqs) return false;
   if (T > 320 / Hkv) return true;
   return max_pages > 2 * kFusedWaves * kChunk && T * Hkv * max_pages > 1 << 17;
 }
-inline bool select_fused(int64_t T, int64_t Hkv, int64_t B, int64_t max_pages, int64_t want) {
-  return !select_prompt(T, Hkv, B, max_pages) && want <= 256 &&
+inline bool select_fused(int64_t T, int64_t Hkv, int64_t seqs, int64_t max_pages, int64_t want) {
+  return !select_prompt(T, Hkv, seqs, max_pages) && want <= 256 &&
          max_pages <= (T * Hkv >= 128 ? kFusedMost : 2 * kFusedWaves * kChunk);
 }
 
@@ -881,10 +881,11 @@ inline int select_slab_blocks(SelectArgs a, const SelectPlan& plan, int dtype, i
 
 using namespace rt;
 
-extern "C" size_t rt_kv_select_workspace(int64_t T, int64_t Hkv, int64_t B, int64_t max_pages,
-                                         int64_t count, int64_t sink, int64_t recent) {
+extern "C" size_t rt_kv_select_workspace(int64_t T, int64_t Hkv, int64_t sequences,
+                                         int64_t max_pages, int64_t count, int64_t sink,
+                                         int64_t recent) {
   if (T < 1 || Hkv < 1 || max_pages < 1) return 0;
-  if (select_fused(T, Hkv, B, max_pages, count - sink - recent)) return 0;
+  if (select_fused(T, Hkv, sequences, max_pages, count - sink - recent)) return 0;
   return static_cast<size_t>(select_slab(T, Hkv, max_pages)) * Hkv *
          align_up(static_cast<size_t>(max_pages), kChunk) * sizeof(uint32_t);
 }
@@ -896,6 +897,19 @@ extern "C" int rt_kv_select(const void* q, int64_t q_token_stride, int64_t q_hea
                             const int32_t* page_table, int64_t B, int64_t max_pages, int64_t count,
                             int64_t sink, int64_t recent, int32_t* out, void* workspace,
                             size_t workspace_bytes, rt_stream_t stream) {
+  return rt_kv_select_of(q, q_token_stride, q_head_stride, T, Hq, Hkv, D, dtype, bounds,
+                         bound_scales, P, page, positions, seq_ids, page_table, B, max_pages, count,
+                         sink, recent, B, out, workspace, workspace_bytes, stream);
+}
+
+extern "C" int rt_kv_select_of(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                               int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int dtype,
+                               const int8_t* bounds, const float* bound_scales, int64_t P,
+                               int64_t page, const int32_t* positions, const int32_t* seq_ids,
+                               const int32_t* page_table, int64_t B, int64_t max_pages,
+                               int64_t count, int64_t sink, int64_t recent, int64_t sequences,
+                               int32_t* out, void* workspace, size_t workspace_bytes,
+                               rt_stream_t stream) {
   if (const int st = kv_check(T, Hq, Hkv, D, dtype, B, max_pages, P, page)) return st;
   RT_CHECK_ARG(count >= 1 && count <= 1024, "count must be in [1, 1024], got %lld",
                static_cast<long long>(count));
@@ -908,7 +922,9 @@ extern "C" int rt_kv_select(const void* q, int64_t q_token_stride, int64_t q_hea
   RT_CHECK_ARG(kv_rows_aligned(q, q_token_stride, q_head_stride) && kv_rows_aligned(bounds, 0, 0),
                "rows must start on 16 bytes");
   RT_CHECK_ARG(T * Hkv <= INT32_MAX - 8, "too many tokens");
-  const size_t need = rt_kv_select_workspace(T, Hkv, B, max_pages, count, sink, recent);
+  RT_CHECK_ARG(sequences >= 0, "sequences must not be negative, got %lld",
+               static_cast<long long>(sequences));
+  const size_t need = rt_kv_select_workspace(T, Hkv, sequences, max_pages, count, sink, recent);
   if (workspace_bytes < need || (need > 0 && workspace == nullptr)) {
     set_error("workspace too small: %zu < %zu", workspace_bytes, need);
     return kWorkspaceTooSmall;
@@ -924,7 +940,7 @@ extern "C" int rt_kv_select(const void* q, int64_t q_token_stride, int64_t q_hea
   // (blocks without a page read page 0's bounds, so there has to be one)
   a.want = P > 0 ? static_cast<int32_t>(count - sink - recent) : 0;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  if (select_fused(T, Hkv, B, max_pages, count - sink - recent)) {
+  if (select_fused(T, Hkv, sequences, max_pages, count - sink - recent)) {
     return kv_dispatch(dtype, D, [&](auto e, auto d) -> int {
       using E = decltype(e);
       constexpr int DD = decltype(d)::value;
@@ -938,7 +954,7 @@ extern "C" int rt_kv_select(const void* q, int64_t q_token_stride, int64_t q_hea
       return kOk;
     });
   }
-  const bool prompt = select_prompt(T, Hkv, B, max_pages);
+  const bool prompt = select_prompt(T, Hkv, sequences, max_pages);
   const int64_t slab = select_slab(T, Hkv, max_pages);
   for (int64_t t0 = 0; t0 < T; t0 += slab) {
     SelectArgs part = a;

@@ -44,10 +44,10 @@ _lib.define("append(Tensor q, Tensor k, Tensor v, Tensor? cos_sin, Tensor positi
             "Tensor(c!) bounds, Tensor(d!) bound_scales, bool interleaved=False) -> Tensor")
 _lib.define("select_blocks(Tensor q, Tensor bounds, Tensor bound_scales, Tensor positions, "
             "Tensor seq_ids, Tensor page_table, int page_size, int count, int sink=1, "
-            "int recent=1) -> Tensor")
+            "int recent=1, int? sequences=None) -> Tensor")
 _lib.define("block_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor blocks, "
-            "Tensor positions, Tensor seq_ids, Tensor page_table, float? scale=None) "
-            "-> (Tensor, Tensor)")
+            "Tensor positions, Tensor seq_ids, Tensor page_table, float? scale=None, "
+            "int? sequences=None) -> (Tensor, Tensor)")
 
 
 # --- checks -----------------------------------------------------------------------------------
@@ -101,6 +101,15 @@ def _check_bounds(bounds: Tensor, bound_scales: Tensor, dim: int) -> tuple[int, 
     if not (bounds.is_contiguous() and bound_scales.is_contiguous()):
         raise ValueError("bounds and bound_scales must be contiguous")
     return shape[0], shape[1]
+
+
+def _sequences(sequences: int | None, page_table: Tensor) -> int:
+    """How many sequences a call's tokens belong to at most."""
+    if sequences is None:
+        return page_table.shape[0]
+    if sequences < 1:
+        raise ValueError(f"sequences must be at least 1, got {sequences}")
+    return sequences
 
 
 def _rows(x: Tensor) -> tuple[Tensor, int, int]:
@@ -223,7 +232,8 @@ def append(q: Tensor, k: Tensor, v: Tensor, cos_sin: Tensor | None, positions: T
     tokens come in order, side by side. Tokens that are padding (a position below 0, or past the
     page table or ``cos_sin``; a sequence outside it; no page) write nothing and return a zero
     row."""
-    args = (q, k, v, cos_sin, positions, seq_ids, page_table, k_cache, v_cache, bounds, bound_scales)
+    args = (q, k, v, cos_sin, positions, seq_ids, page_table, k_cache, v_cache, bounds,
+            bound_scales)
     call = _append if _eager(*args) else torch.ops.retrieve_kv.append
     return call(*args, interleaved)
 
@@ -232,7 +242,7 @@ def append(q: Tensor, k: Tensor, v: Tensor, cos_sin: Tensor | None, positions: T
 
 
 def _select(q, bounds, bound_scales, positions, seq_ids, page_table, page_size, count, sink=1,
-            recent=1):
+            recent=1, sequences=None):
     if q.dim() != 3:
         raise ValueError("q must be [T, Hq, D]")
     t, heads, dim = q.shape
@@ -243,19 +253,20 @@ def _select(q, bounds, bound_scales, positions, seq_ids, page_table, page_size, 
         raise ValueError(f"count must be in [1, {MAX_COUNT}], got {count}")
     if sink < 0 or recent < 1 or sink + recent > count:
         raise ValueError(f"sink >= 0 and recent >= 1 must fit in count, got {sink}, {recent}")
+    sequences = _sequences(sequences, page_table)
     dev = _device(q, bounds, bound_scales, positions, seq_ids, page_table)
     q, q_token, q_head = _rows(q)
     out = positions.new_empty((t, heads_kv, count))
     lib = nat.lib()
     b, max_pages = page_table.shape
     with _on(dev):
-        need = lib.rt_kv_select_workspace(t, heads_kv, b, max_pages, count, sink, recent)
+        need = lib.rt_kv_select_workspace(t, heads_kv, sequences, max_pages, count, sink, recent)
         ws = bounds.new_empty((need,)) if need else None
-        st = lib.rt_kv_select(
+        st = lib.rt_kv_select_of(
             q.data_ptr(), q_token, q_head, t, heads, heads_kv, dim, dtype, bounds.data_ptr(),
             bound_scales.data_ptr(), pages, page_size, positions.data_ptr(), seq_ids.data_ptr(),
-            page_table.data_ptr(), b, max_pages, count, sink, recent, out.data_ptr(), nat.ptr(ws),
-            need, _stream(dev))
+            page_table.data_ptr(), b, max_pages, count, sink, recent, sequences, out.data_ptr(),
+            nat.ptr(ws), need, _stream(dev))
     if st:
         nat.check(st)
     return out
@@ -263,23 +274,28 @@ def _select(q, bounds, bound_scales, positions, seq_ids, page_table, page_size, 
 
 def select_blocks(q: Tensor, bounds: Tensor, bound_scales: Tensor, positions: Tensor,
                   seq_ids: Tensor, page_table: Tensor, page_size: int, count: int, sink: int = 1,
-                  recent: int = 1) -> Tensor:
+                  recent: int = 1, sequences: int | None = None) -> Tensor:
     """The blocks that each token and key/value head attends to, int32 ``[T, Hkv, count]``,
     ascending, -1 at the end. The first ``sink`` blocks and the last ``recent`` ones up to the
     token's own are always among them; the other places go to the best blocks between by ``(score
     desc, block asc)``. A score is the largest, over the heads that share the key/value head, of
     ``c . mid + |c| . half`` (int32; ``c`` the rotated query's int8 codes) times the query's and the
     block's scales: an upper bound on what the block's keys can score, up to the codes' rounding.
-    Blocks between without a page are left out; padding tokens get -1 throughout."""
+    Blocks between without a page are left out; padding tokens get -1 throughout.
+
+    ``sequences``: how many sequences the tokens belong to at most, where that is known to be fewer
+    than the page table has rows. It chooses among kernels (prompts share a pass over their
+    sequence's blocks), never what is chosen."""
     args = (q, bounds, bound_scales, positions, seq_ids, page_table)
     call = _select if _eager(*args) else torch.ops.retrieve_kv.select_blocks
-    return call(*args, page_size, count, sink, recent)
+    return call(*args, page_size, count, sink, recent, sequences)
 
 
 # --- attention ----------------------------------------------------------------------------------
 
 
-def _attention(q, k_cache, v_cache, blocks, positions, seq_ids, page_table, scale=None):
+def _attention(q, k_cache, v_cache, blocks, positions, seq_ids, page_table, scale=None,
+               sequences=None):
     t, heads, pages, heads_kv, page, dim, dtype = _check_caches(q, k_cache, v_cache)
     _check_tokens(t, positions, seq_ids, page_table)
     if blocks.dim() != 3 or blocks.shape[:2] != (t, heads_kv):
@@ -288,6 +304,7 @@ def _attention(q, k_cache, v_cache, blocks, positions, seq_ids, page_table, scal
         raise TypeError("blocks must be int32")
     if not blocks.is_contiguous():
         raise ValueError("blocks must be contiguous")
+    sequences = _sequences(sequences, page_table)
     dev = _device(q, k_cache, v_cache, blocks, positions, seq_ids, page_table)
     q, q_token, q_head = _rows(q)
     count = blocks.shape[2]
@@ -297,29 +314,29 @@ def _attention(q, k_cache, v_cache, blocks, positions, seq_ids, page_table, scal
     with _on(dev):
         need = lib.rt_kv_attention_workspace(t, heads, heads_kv, dim, page, count)
         ws = blocks.new_empty((need // 4,)) if need else None  # (floats)
-        st = lib.rt_kv_attention(
+        st = lib.rt_kv_attention_of(
             q.data_ptr(), q_token, q_head, t, heads, heads_kv, dim, dtype, k_cache.data_ptr(),
             v_cache.data_ptr(), pages, page, blocks.data_ptr(), count, positions.data_ptr(),
             seq_ids.data_ptr(), page_table.data_ptr(), *page_table.shape,
-            1.0 / math.sqrt(dim) if scale is None else scale, out.data_ptr(), lse.data_ptr(),
-            nat.ptr(ws), need, _stream(dev))
+            1.0 / math.sqrt(dim) if scale is None else scale, sequences, out.data_ptr(),
+            lse.data_ptr(), nat.ptr(ws), need, _stream(dev))
     if st:
         nat.check(st)
     return out, lse
 
 
 def block_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, blocks: Tensor, positions: Tensor,
-                    seq_ids: Tensor, page_table: Tensor, scale: float | None = None
-                    ) -> tuple[Tensor, Tensor]:
+                    seq_ids: Tensor, page_table: Tensor, scale: float | None = None,
+                    sequences: int | None = None) -> tuple[Tensor, Tensor]:
     """Softmax attention of ``q [T, Hq, D]`` (rotated) over the keys of the listed ``blocks`` (int32
     ``[T, Hkv, count]``, each at most once a row, in any order) at positions up to the token's own,
     with scores ``scale * q . k`` (``1 / sqrt(D)`` by default): ``(out [T, Hq, D], lse fp32 [T,
     Hq])``, ``lse`` the natural logarithm of the weights' sum. Entries below 0, past the token's
     block or without a page are skipped; a row without a key is zeros and ``-inf``. Slots past a
-    token's position are not used, whatever they hold."""
+    token's position are not used, whatever they hold. ``sequences`` as in :func:`select_blocks`."""
     args = (q, k_cache, v_cache, blocks, positions, seq_ids, page_table)
     call = _attention if _eager(*args) else torch.ops.retrieve_kv.block_attention
-    return call(*args, scale)
+    return call(*args, scale, sequences)
 
 
 _lib.impl("append", _append, "CUDA")
@@ -334,12 +351,13 @@ def _(q, k, v, cos_sin, positions, seq_ids, page_table, k_cache, v_cache, bounds
 
 
 @torch.library.register_fake("retrieve_kv::select_blocks", lib=_lib)
-def _(q, bounds, bound_scales, positions, seq_ids, page_table, page_size, count, sink=1, recent=1):
+def _(q, bounds, bound_scales, positions, seq_ids, page_table, page_size, count, sink=1, recent=1,
+      sequences=None):
     return q.new_empty((q.shape[0], bounds.shape[1], count), dtype=torch.int32)
 
 
 @torch.library.register_fake("retrieve_kv::block_attention", lib=_lib)
-def _(q, k_cache, v_cache, blocks, positions, seq_ids, page_table, scale=None):
+def _(q, k_cache, v_cache, blocks, positions, seq_ids, page_table, scale=None, sequences=None):
     return q.new_empty(q.shape), q.new_empty(q.shape[:2], dtype=torch.float32)
 
 
@@ -412,7 +430,9 @@ class PagedCache:
     >>> out, lse = cache.attend(q, positions, seq_ids, count=64)
 
     ``reserve`` and ``free`` keep the page table on the host and send a sequence's row to the GPU;
-    ``append`` and ``attend`` only launch kernels."""
+    ``append`` and ``attend`` only launch kernels. These are chosen by how many sequences a call's
+    tokens belong to: ``sequences``, or the slots that hold pages where it is not said (say it for a
+    prompt beside many held slots)."""
 
     def __init__(self, pages: int, heads: int, dim: int, page: int = 64, sequences: int = 1,
                  max_pages: int | None = None, dtype: torch.dtype = torch.bfloat16,
@@ -431,6 +451,7 @@ class PagedCache:
         self.page_table = torch.full((sequences, max_pages), -1, dtype=torch.int32, device=device)
         self._free = list(range(pages - 1, -1, -1))
         self._held: list[list[int]] = [[] for _ in range(sequences)]
+        self._active = 0  # slots that hold pages
 
     def reserve(self, seq: int, tokens: int) -> None:
         """Pages for the sequence's first ``tokens`` tokens, those that it has already among
@@ -444,11 +465,13 @@ class PagedCache:
         if more > 0:
             new = [self._free.pop() for _ in range(more)]
             self.page_table[seq, len(held):need] = torch.tensor(new, dtype=torch.int32)
+            self._active += not held
             held += new
 
     def free(self, seq: int) -> None:
         """Returns the sequence's pages."""
         self._free += reversed(self._held[seq])
+        self._active -= bool(self._held[seq])
         self._held[seq] = []
         self.page_table[seq] = -1
 
@@ -458,18 +481,23 @@ class PagedCache:
         return append(q, k, v, cos_sin, positions, seq_ids, self.page_table, self.k, self.v,
                       self.bounds, self.bound_scales, interleaved)
 
+    def _sequences(self, sequences: int | None) -> int | None:
+        return self._active or None if sequences is None else sequences
+
     def select(self, q: Tensor, positions: Tensor, seq_ids: Tensor, count: int, sink: int = 1,
-               recent: int = 1) -> Tensor:
+               recent: int = 1, sequences: int | None = None) -> Tensor:
         """:func:`select_blocks` over this cache."""
         return select_blocks(q, self.bounds, self.bound_scales, positions, seq_ids,
-                             self.page_table, self.page, count, sink, recent)
+                             self.page_table, self.page, count, sink, recent,
+                             self._sequences(sequences))
 
     def attend(self, q: Tensor, positions: Tensor, seq_ids: Tensor, count: int, sink: int = 1,
-               recent: int = 1, scale: float | None = None) -> tuple[Tensor, Tensor]:
+               recent: int = 1, scale: float | None = None, sequences: int | None = None
+               ) -> tuple[Tensor, Tensor]:
         """The selection and the attention over what it chose: ``(out, lse)``."""
-        blocks = self.select(q, positions, seq_ids, count, sink, recent)
+        blocks = self.select(q, positions, seq_ids, count, sink, recent, sequences)
         return block_attention(q, self.k, self.v, blocks, positions, seq_ids, self.page_table,
-                               scale)
+                               scale, self._sequences(sequences))
 
 
 __all__ = ["PagedCache", "append", "block_attention", "rotary_table", "select_blocks"]
