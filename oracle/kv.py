@@ -1,8 +1,8 @@
 """The paged cache's operators in numpy (test infrastructure; see ``oracle/__init__``).
 
 Values of 16-bit types are held as float32 arrays; ``round16`` rounds to them. ``append`` follows
-the kernels' single fp32 roundings (bit-exact), ``append64`` and ``attention`` the formulas in 64
-bits, ``select`` integers. ``blocks_by_bounds`` states the selection a second time, over exact rationals.
+the kernels' single fp32 roundings (bit-exact), ``append64``, ``bounds64`` and ``attention`` the
+formulas in 64 bits, ``select`` integers. ``blocks_by_bounds`` states the selection a second time, over exact rationals.
 """
 
 from __future__ import annotations
@@ -63,6 +63,26 @@ def bounds_of(stored: np.ndarray) -> tuple[np.ndarray, np.float32]:
     row = np.concatenate([(low + high) * half, (high - low) * half]).astype(np.float32)
     codes, scales = oq.quantize_int8(row[None], divide=True)
     return codes[0], scales[0]
+
+
+def append64(x, cos_sin, positions, interleaved=False):
+    """Queries or keys ``[T, H, D]`` turned by their positions' angles, nothing rounded to fewer than
+    64 bits: each pair as a complex number times ``c + i s``."""
+    out = np.array(x, np.float64)
+    rot = cos_sin.shape[1]
+    a, b = _pairs(rot, interleaved)
+    row = cos_sin[positions].astype(np.float64)[:, None]
+    z = (out[..., a] + 1j * out[..., b]) * (row[..., :rot // 2] + 1j * row[..., rot // 2:])
+    out[..., a], out[..., b] = z.real, z.imag
+    return out
+
+
+def bounds64(stored):
+    """``(row [2 D], scale)`` of a block's stored keys ``[page, D]``: the middle and half the width of
+    each channel's range, and what one code of the row stands for."""
+    low, high = stored.astype(np.float64).min(0), stored.astype(np.float64).max(0)
+    row = np.concatenate([low + (high - low) / 2, (high - low) / 2])
+    return row, max(np.abs(row).max(), 1e-8) / 127
 
 
 def append(q, k, v, cos_sin, positions, seq_ids, page_table, k_cache, v_cache, bounds, scales, kind,
