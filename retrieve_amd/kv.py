@@ -153,25 +153,22 @@ _stream = torch._C._cuda_getCurrentRawStream  # (the current stream's handle, wi
 _included = torch._C._dispatch_tls_local_include_set
 _PLAIN_KEYS = (torch._C.DispatchKeySet(torch._C.DispatchKey.BackendSelect)
                | torch._C.DispatchKeySet(torch._C.DispatchKey.ADInplaceOrView)).raw_repr()
+_PLAIN_TYPES = frozenset((Tensor, type(None)))
 
 
 def _eager(*tensors: Tensor | None) -> bool:
     """Whether a call can go straight to its kernels: plain tensors that carry no gradients, nothing
     being traced or transformed. Elsewhere it goes through the registered op (the dispatcher's 3 to
-    5 us a call are a third of a small one)."""
+    5 us a call are a third of a small one; these checks take 1)."""
     if torch.compiler.is_compiling():
         return False
     if forward_ad._current_level >= 0:
         for t in tensors:
             if t is not None and forward_ad.unpack_dual(t).tangent is not None:
                 raise ValueError("retrieve_kv ops have no derivatives: an input has a tangent")
-    if _included().raw_repr() & ~_PLAIN_KEYS:
+    if _included().raw_repr() & ~_PLAIN_KEYS or not _PLAIN_TYPES.issuperset(map(type, tensors)):
         return False
-    grad = torch.is_grad_enabled()
-    for t in tensors:
-        if t is not None and (type(t) is not Tensor or grad and t.requires_grad):
-            return False
-    return True
+    return not (torch.is_grad_enabled() and torch._C._any_requires_grad(*tensors))
 
 
 # --- append -----------------------------------------------------------------------------------
