@@ -563,7 +563,8 @@ int rt_search_epilogue(int64_t* ids, const int32_t* raw_dots, float* out_scores,
  * No counterpart in the reference: the scoring-and-selection path applied to a language model's
  * cache. Conventions of the three calls: T packed tokens, token t at positions[t] of sequence
  * seq_ids[t] (a row of page_table int32 [B, max_pages]: the physical page of each block of `page`
- * tokens; an entry outside [0, P) is absent). A token whose position is negative or past the page
+ * tokens; an entry outside [0, P) is absent; sequences may share pages, one sequence's blocks have
+ * different ones). A token whose position is negative or past the page
  * table, or whose sequence is outside [0, B), is padding. Hq query heads, Hq / Hkv of them to a
  * key/value head. dtype 0 = bf16, 1 = fp16 (queries, keys, values, outputs). D in {64, 96, 128, 192,
  * 256}; page in {16, 32, 64, 128}. k_cache, v_cache [P, Hkv, page, D]; bounds int8 [P, Hkv, 2 D];

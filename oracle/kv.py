@@ -2,7 +2,8 @@
 
 Values of 16-bit types are held as float32 arrays; ``round16`` rounds to them. ``append`` follows
 the kernels' single fp32 roundings (bit-exact), ``append64``, ``bounds64`` and ``attention`` the
-formulas in 64 bits, ``select`` integers. ``blocks_by_bounds`` states the selection a second time, over exact rationals.
+formulas in 64 bits, ``select`` integers. ``blocks_by_bounds`` states the selection a second time,
+over exact rationals.
 """
 
 from __future__ import annotations
@@ -66,8 +67,8 @@ def bounds_of(stored: np.ndarray) -> tuple[np.ndarray, np.float32]:
 
 
 def append64(x, cos_sin, positions, interleaved=False):
-    """Queries or keys ``[T, H, D]`` turned by their positions' angles, nothing rounded to fewer than
-    64 bits: each pair as a complex number times ``c + i s``."""
+    """Queries or keys ``[T, H, D]`` turned by their positions' angles in 64 bits: each pair as a
+    complex number times ``c + i s``."""
     out = np.array(x, np.float64)
     rot = cos_sin.shape[1]
     a, b = _pairs(rot, interleaved)
@@ -78,8 +79,8 @@ def append64(x, cos_sin, positions, interleaved=False):
 
 
 def bounds64(stored):
-    """``(row [2 D], scale)`` of a block's stored keys ``[page, D]``: the middle and half the width of
-    each channel's range, and what one code of the row stands for."""
+    """``(row [2 D], scale)`` of a block's stored keys ``[page, D]``: the middle and half the width
+    of each channel's range, and what one code of the row stands for."""
     low, high = stored.astype(np.float64).min(0), stored.astype(np.float64).max(0)
     row = np.concatenate([low + (high - low) / 2, (high - low) / 2])
     return row, max(np.abs(row).max(), 1e-8) / 127

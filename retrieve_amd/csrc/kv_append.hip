@@ -17,8 +17,8 @@
 // where there are few tokens): a lane holds two 16-byte chunks of a row, which in the split layout
 // are partners, with their cosines and sines, and walks over the heads, two rows in flight.
 //
-// Bound by memory: every row is read and written once. 32768 tokens of 32 rows of 256 channels
-// take 229 to 234 us (4.8 TB/s, what a large copy reaches) with nontemporal loads and stores (when they
+// Bound by memory: every row is read and written once. 32768 tokens of 32 rows of 256 channels take
+// 229 to 234 us (4.8 TB/s, what a large copy reaches) with nontemporal loads and stores (when they
 // were taken 238, 283 with ordinary stores; four rows in flight instead of two 250). A decode step
 // is bound by its launch (3 us).
 #include <type_traits>

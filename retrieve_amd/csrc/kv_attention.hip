@@ -15,15 +15,17 @@
 // A lane's column is one head in both products: maxima, sums and rescaling stay in the lane. The
 // maximum is raised only where a score passes it by 8 (in powers of two: weights reach 256 at
 // most, far inside both types), so most steps do not touch the accumulators or exchange lanes.
-// Weights are rounded to the values' 16 bits for the matrix cores (l sums them unrounded): relative
-// 2^-9 / 2^-12 a weight, the size of the output's own rounding. fp16's step is absolute below 2^-14, so
-// its weights are held 2^5 times as large (m is 5 below the maximum; they reach 2^13): at most 2^-30
-// of the row's largest weight a key, half an output's rounding over 2^17 keys.
+// Weights are rounded to the values' 16 bits for the matrix cores (l sums them unrounded):
+// relative 2^-9 / 2^-12 a weight, the size of the output's own rounding (against 64 bits the
+// outputs are off by 2.3e-3 / 2.9e-4 of their size, by 1.7e-3 / 2.1e-4 with weights of 32 bits).
+// fp16's step is absolute below 2^-14, so its weights are held 2^5 times as large (m is 5 below the
+// maximum; they reach 2^13): at most 2^-30 of the row's largest weight a key, half an output's
+// rounding over 2^17 keys.
 //
 // Memory: a wave keeps the next step's keys and values in flight (registers) while it works on
 // this one. Slots past the token's position are read but replaced: scores by -inf, values by 0.
 // Single tokens are bound by the cache's bytes: 64 sequences of lists of 64 blocks, 64 keys of 128
-// channels a block, 8 key/value heads take 162 us (6.5 TB/s). Prompts read most blocks from L2 and
+// channels a block, 8 key/value heads take 158 us (6.6 TB/s). Prompts read most blocks from L2 and
 // are bound by the steps' instructions (2053 tokens of 32 heads over 16 blocks: 136 us).
 #include <cmath>
 #include <type_traits>
@@ -892,10 +894,12 @@ inline AttendPlan attend_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int
   int64_t joined = 16 / (G < 16 ? G : 16);
   if (joined > kJoinTokens) joined = kJoinTokens;
   const int64_t entries = kJoinWaves * (count > 0 ? count : 1);
+  // workgroups of the small table on the GPU (four a CU, two of the wide heads); the larger table
+  // has one token a wave, or more workgroups than this
   const int64_t held = D <= 128 ? 1024 : 512;
   // Lists of which kJoinMost holds one token a wave: two of them by the larger table, where there
   // are more workgroups than the GPU holds and a block's work outweighs its entries' in the table
-  // (1000 tokens of 10 heads of 128, 96 blocks of 32 keys: 376 for 488; of 20 heads of 64: 573 for
+  // (1000 tokens of 10 heads of 128, 96 blocks of 32 keys: 382 for 488; of 20 heads of 64: 573 for
   // 519, but 551 for 650 with 70 blocks of 64). Lists of which it holds none: one, against a wave a
   // row (1000 tokens of 10 heads of 128, 200 blocks of 16: 747 for 1105; of 20 heads of 96: 1243
   // for 1103, but 1599 for 3035 with 160 blocks of 64).
@@ -946,9 +950,9 @@ extern "C" int rt_kv_attention(const void* q, int64_t q_token_stride, int64_t q_
                                const int32_t* seq_ids, const int32_t* page_table, int64_t B,
                                int64_t max_pages, float scale, void* out, float* lse,
                                void* workspace, size_t workspace_bytes, rt_stream_t stream) {
-  return rt_kv_attention_of(q, q_token_stride, q_head_stride, T, Hq, Hkv, D, dtype, k_cache, v_cache,
-                            P, page, blocks, count, positions, seq_ids, page_table, B, max_pages,
-                            scale, B, out, lse, workspace, workspace_bytes, stream);
+  return rt_kv_attention_of(q, q_token_stride, q_head_stride, T, Hq, Hkv, D, dtype, k_cache,
+                            v_cache, P, page, blocks, count, positions, seq_ids, page_table, B,
+                            max_pages, scale, B, out, lse, workspace, workspace_bytes, stream);
 }
 
 extern "C" int rt_kv_attention_of(const void* q, int64_t q_token_stride, int64_t q_head_stride,

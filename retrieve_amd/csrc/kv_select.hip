@@ -6,7 +6,7 @@
 // 2 * 256 * 127^2 < 2^23, so exact as fp32 too); the two products are rounded once each, in this
 // order, and rounding is monotone, so the largest over the heads is taken before the block's scale.
 //
-// Two launches.
+// One launch for single tokens over few blocks, else two: scores and cut.
 //
 // Scores: [blocks x columns] = bounds [c | |c|]^T on the int8 matrix cores, 16 blocks by 16 columns
 // an instruction; the columns stay in registers (quantised by the wave that needs them), the bounds
@@ -18,7 +18,7 @@
 // Bound: single tokens by the bounds' bytes, 2 D a (block, head) in scattered pieces (64 sequences
 // of 16K to 131K tokens in blocks of 64, 8 heads of 128 channels: 51 us, 3.0 TB/s, the longest
 // row's chain behind the others), one launch for up to 4096 blocks; a million tokens of one
-// sequence take 13 us of scores and 8 of keeping. Prompts by the vector instructions: a column's
+// sequence take 13 us of scores and 8 of the cut. Prompts by the vector instructions: a column's
 // codes (ten instructions a channel) and a block's key (about seven a head): 4099 tokens over 9K
 // to 30K take 76 us.
 //
@@ -55,8 +55,8 @@ struct SelectArgs {
 };
 
 // The key of a candidate's score, the group's times the block's scale (0: not a candidate). A score
-// that is not a number is the least. (The sum with 0 makes -0, of a block of scale 0, the other zero's
-// equal.)
+// that is not a number is the least. (The sum with 0 makes -0, of a block of scale 0, the other
+// zero's equal.)
 __device__ inline uint32_t score_key(float group, float scale) {
   return key_of_f32(fmaxf(fmaf(group, scale, 0.0f), -INFINITY));
 }
@@ -189,7 +189,8 @@ __device__ inline void score_blocks(const SelectArgs& a, int64_t t0, int head, i
         const float small = top > 0x1p100f ? 0x1p-64f : 1.0f;
         top *= small;
         const float r = 1.0f / top;
-        // (an infinite row: by 1 and r = 0 a finite channel is 0 and an infinite one NaN, as divided)
+        // (an infinite row: by 1 and r = 0 a finite channel is 0 and an infinite one NaN, as
+        // divided)
         if (r == 0.0f) top = 1.0f;
 #pragma unroll
         for (int s = 0; s < LOADS; ++s) {
@@ -333,9 +334,10 @@ __device__ inline void score_blocks(const SelectArgs& a, int64_t t0, int head, i
   }
 }
 
-// Four heads of 128 channels are worth three waves a SIMD with half the tiles in flight (prompts of
-// 4099 tokens: 78 us with the kept, 84 with two waves and four tiles); wider columns take two waves
-// or one.
+// Waves a SIMD, by the registers that the columns take. Four heads of 128 channels are worth three
+// with half the tiles in flight (prompts of 4099 tokens: 78 us scores and cut, 84 with two waves
+// and four tiles); fewer channels were not measured with three and keep two, wide ones with four
+// tiles fit once.
 template <int D, int NT, int GH>
 constexpr int kScoreOccupancy = D == 128 && GH == 4 ? 3 : D > 128 && NT == 4 ? 1 : 2;
 
@@ -720,7 +722,7 @@ __global__ void __launch_bounds__(WAVES* kWave) kv_keep_many_kernel(SelectArgs a
 // Both in one launch, a workgroup a (token, key/value head): decode over page tables of up to
 // kFusedMost blocks. The keys stay in LDS. Workgroups go to the eight XCDs in turn: each takes rows
 // side by side, as the heads of a token share lines of the page table and of the scales (64
-// sequences, 8 heads: 53 us, 57 with the heads spread).
+// sequences, 8 heads: 57 us with the heads spread, 53 with this step, 51 now).
 constexpr int kFusedWaves = 8;
 constexpr int kFusedMost = 4096;
 
@@ -748,15 +750,14 @@ __global__ void __launch_bounds__(kFusedWaves* kWave, D <= 128 && NT == 1 ? 4 : 
   }
 }
 
-
 // Whether tokens mostly share their sequences (`seqs` of them at most) and there are rows and keys
-// enough (their scores are then taken several tokens a wave), and whether a call is one launch: few enough places for 512
-// lanes to bound well, and two chunks a wave or rows enough to fill the GPU (one row of 1258
-// blocks: 13 us in two launches, 16 in one). Rows for little more than a workgroup a CU take less
-// as single tokens do (32 tokens of 8 heads of 128 over 470 blocks: 15 us for 21, 128 tokens 32 for
-// 22; 4 heads of 256: 64 tokens 19 for 41; 6 of 256 over 403: 93 tokens 36 for 26; over 2032
-// blocks, two launches where rows are few, 8 tokens of 4 heads of 256 18 for 36, 16 of 8 heads of
-// 128 27 for 19).
+// enough (their scores are then taken several tokens a wave), and whether a call is one launch: few
+// enough places for 512 lanes to bound well, and two chunks a wave or rows enough to fill the GPU
+// (one row of 1258 blocks: 13 us in two launches, 16 in one). Rows for little more than a workgroup
+// a CU take less as single tokens do (32 tokens of 8 heads of 128 over 470 blocks: 15 us for 21,
+// 128 tokens 32 for 22; 4 heads of 256: 64 tokens 19 for 41; 6 of 256 over 403: 93 tokens 36 for
+// 26; over 2032 blocks, two launches where rows are few, 8 tokens of 4 heads of 256 18 for 36, 16
+// of 8 heads of 128 27 for 19).
 inline bool select_prompt(int64_t T, int64_t Hkv, int64_t seqs, int64_t max_pages) {
   if (seqs <= 0 || T < 4 * seqs) return false;
   if (T > 320 / Hkv) return true;
@@ -802,12 +803,12 @@ inline SelectPlan select_plan(bool prompt, int64_t T, int64_t Hq, int64_t Hkv, i
   return p;
 }
 
-// In two launches a call's tokens are taken in slabs whose keys fit in kSlabBytes (of 64s of tokens,
-// whole waves of either form, where that many fit), one after the other over the same workspace, so
-// it grows neither with a prompt's length nor, but for a token's own rows, with the page table. A slab
-// has to fill the GPU: 4099 tokens of 8 heads behind 313 blocks of a table of 16384 columns take
-// 602 us in slabs of 128 MiB, 403 of 256, 269 of 512 and 168 in one of 2.1 GiB; 8192 tokens in a
-// table of 2048 columns 303, 232, and 202 in the one of 512.
+// In two launches a call's tokens are taken in slabs whose keys fit in kSlabBytes (of 64s of
+// tokens, whole waves of either form, where that many fit), one after the other over the same
+// workspace, so it grows neither with a prompt's length nor, but for a token's own rows, with the
+// page table. A slab has to fill the GPU: 4099 tokens of 8 heads behind 313 blocks of a table of
+// 16384 columns take 602 us in slabs of 128 MiB, 403 of 256, 269 of 512 and 168 in one of 2.1 GiB;
+// 8192 tokens in a table of 2048 columns 303, 232, and 202 in the one of 512.
 constexpr int64_t kSlabBytes = int64_t{512} << 20;
 inline int64_t select_slab(int64_t T, int64_t Hkv, int64_t max_pages) {
   const size_t row = align_up(static_cast<size_t>(max_pages > 0 ? max_pages : 1), kChunk);
@@ -852,9 +853,10 @@ inline int select_slab_blocks(SelectArgs a, const SelectPlan& plan, int dtype, i
   }
   // A wave a row while its keys fit in 16 registers a lane; then four waves, unless more places are
   // wanted than their lanes bound well; then sixteen. Of many rows each is cut by its own number of
-  // candidates, not by the table's width: the short ones a wave a row in a launch before (4099 tokens
-  // of 8 heads behind 313 blocks of a table of 16384 columns: 168 for 616 us). With fewer rows that
-  // launch costs what it saves (1024 rows behind 313 blocks of 2048 columns: 28 us for 23.5).
+  // candidates, not by the table's width: the short ones a wave a row in a launch before (4099
+  // tokens of 8 heads behind 313 blocks of a table of 16384 columns: 168 for 616 us). With fewer
+  // rows that launch costs what it saves (1024 rows behind 313 blocks of 2048 columns: 28 us for
+  // 23.5).
   const int64_t rows = a.T * a.Hkv;
   const dim3 one(static_cast<unsigned>(rows)), four(static_cast<unsigned>(cdiv(rows, 4)));
   const bool few = max_pages <= 64 * 16;

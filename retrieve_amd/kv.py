@@ -223,12 +223,12 @@ def append(q: Tensor, k: Tensor, v: Tensor, cos_sin: Tensor | None, positions: T
 
     ``cos_sin [length, rot]`` fp32 holds a position's ``rot / 2`` cosines, then its sines
     (:func:`rotary_table`); channels ``(i, i + rot / 2)`` turn together, ``(2 i, 2 i + 1)`` with
-    ``interleaved``; channels from ``rot`` on stay as they are; None rotates nothing. A token at the
-    last slot of its block fills the block's ``bounds``: ``[mid | half]`` of its stored keys' least
-    and largest values per channel, quantised as ``quantize_int8``'s rows. For that a sequence's
-    tokens come in order, side by side. Tokens that are padding (a position below 0, or past the
-    page table or ``cos_sin``; a sequence outside it; no page) write nothing and return a zero
-    row."""
+    ``interleaved``; channels from ``rot`` on stay as they are; None (or ``rot`` 0) rotates nothing.
+    A token at the last slot of its block fills the block's ``bounds``: ``[mid | half]`` of its
+    stored keys' least and largest values per channel, quantised as ``quantize_int8``'s rows. For
+    that a sequence's tokens come in order, side by side. Tokens that are padding (a position below
+    0, or past the page table or ``cos_sin``; a sequence outside it; no page) write nothing and
+    return a zero row."""
     args = (q, k, v, cos_sin, positions, seq_ids, page_table, k_cache, v_cache, bounds,
             bound_scales)
     call = _append if _eager(*args) else torch.ops.retrieve_kv.append

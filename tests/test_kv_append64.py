@@ -1,9 +1,10 @@
 """Appending against the formulas in 64 bits: what is stored, and the bounds of what is stored.
 
-Tolerances: a rotated value is two products and a sum rounded to fp32 and once to 16 bits: ``u |x| + 3
-2^-24 (|a| + |b|)`` (a cosine or sine is 1 at most; 2^-25 for fp16's least step). A bound's code is the
-quotient by the row's largest, times 127, rounded: half a code, and the fp32 roundings of the middle,
-the quotient, the product and the scale, each 2^-24 of at most 127 codes."""
+Tolerances: a rotated value is two products and a sum rounded to fp32 and once to 16 bits: ``u |x| +
+3 2^-24 (|a| + |b|)`` (a cosine or sine is 1 at most; 2^-25 for fp16's least step). A bound's code
+is the quotient by the row's largest, times 127, rounded: half a code, and the fp32 roundings of the
+middle, the quotient, the product and the scale, each 2^-24 of at most 127 codes.
+"""
 
 from __future__ import annotations
 
