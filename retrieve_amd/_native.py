@@ -161,6 +161,29 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [*[_c_p, _c_i64, _c_i64] * 3, *[_c_i64] * 4, _c_int, _c_p, _c_i64, _c_i64, _c_int, _c_p,
          _c_p, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_p],
     ),
+    "rt_kv_append_norm": (
+        _c_int,
+        [*[_c_p, _c_i64, _c_i64] * 3, *[_c_i64] * 4, _c_int, _c_p, _c_p, _c_int, ctypes.c_double,
+         _c_p, _c_i64, _c_i64, _c_int, _c_p, _c_p, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_i64,
+         _c_p, _c_p, _c_p, _c_p],
+    ),
+    "rt_kv_append_int8": (
+        _c_int,
+        [*[_c_p, _c_i64, _c_i64] * 3, *[_c_i64] * 4, _c_int, _c_p, _c_p, _c_int, ctypes.c_double,
+         _c_p, _c_i64, _c_i64, _c_int, _c_p, _c_p, _c_p, _c_i64, _c_i64, *[_c_p] * 6, _c_i64,
+         _c_i64, _c_p, _c_p, _c_p, _c_p],
+    ),
+    "rt_kv_read_int8": (
+        _c_int,
+        [*[_c_p] * 6, *[_c_i64] * 3, _c_int, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_i64, _c_i64, _c_p,
+         _c_p, _c_p],
+    ),
+    "rt_kv_attention_int8_workspace": (_c_sz, [_c_i64] * 6),
+    "rt_kv_attention_int8": (
+        _c_int,
+        [_c_p, *[_c_i64] * 6, _c_int, *[_c_p] * 6, _c_i64, _c_i64, _c_p, _c_i64, _c_p, _c_p, _c_p,
+         _c_i64, _c_i64, ctypes.c_float, _c_i64, _c_p, _c_p, _c_p, _c_sz, _c_p],
+    ),
     "rt_kv_select_workspace": (_c_sz, [_c_i64] * 7),
     "rt_kv_select": (
         _c_int,

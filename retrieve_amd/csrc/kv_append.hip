@@ -24,19 +24,17 @@
 #include <type_traits>
 
 #include "../../include/retrieve_amd.h"
-#include "kv_common.h"
+#include "kv_rotate.h"
 
 namespace rt {
 
 constexpr int kAppendThreads = 256;
 
-struct AppendArgs {
+struct AppendArgs : TurnArgs {
   const void *q, *k, *v;
   int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;  // token and head strides, elements
   int64_t T;
   int32_t Hq, Hkv;
-  const float* cos_sin;  // [table_len, rot], rot / 2 cosines then rot / 2 sines
-  int32_t table_len, rot;
   KvTokens tok;
   void *k_cache, *v_cache;
   int8_t* bounds;
@@ -47,94 +45,6 @@ struct AppendArgs {
   int32_t tile;           // tokens that one of them looks at
 };
 
-// How channel i meets its partner: halves of the rotated part with every half on whole chunks,
-// the same with other halves, or neighbouring channels.
-enum RotMode : int { kRotHalf = 0, kRotHalfOdd = 1, kRotPairs = 2 };
-
-__device__ inline float rot_first(float a, float b, float c, float s) {
-#pragma clang fp contract(off)
-  return a * c - b * s;
-}
-__device__ inline float rot_second(float b, float a, float c, float s) {
-#pragma clang fp contract(off)
-  return b * c + a * s;
-}
-
-// The cosines and sines of chunk `c`'s channels at a position (1, 0 past the rotated part).
-template <int MODE>
-struct Turn {
-  float c[8], s[8];
-  __device__ void load(const AppendArgs& a, int32_t pos, int chunk) {
-    const int half = a.rot >> 1;
-    const float* row = a.cos_sin + static_cast<int64_t>(pos) * a.rot;
-    if (MODE == kRotHalf && 8 * chunk < a.rot) {
-      const int j = 8 * chunk < half ? 8 * chunk : 8 * chunk - half;
-#pragma unroll
-      for (int e = 0; e < 8; e += 4) {
-        const v4f cv = *reinterpret_cast<const v4f*>(row + j + e);
-        const v4f sv = *reinterpret_cast<const v4f*>(row + half + j + e);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          c[e + i] = cv[i];
-          s[e + i] = sv[i];
-        }
-      }
-      return;
-    }
-    if (MODE == kRotPairs && a.rot % 8 == 0 && 8 * chunk < a.rot) {
-      const v4f cv = *reinterpret_cast<const v4f*>(row + 4 * chunk);
-      const v4f sv = *reinterpret_cast<const v4f*>(row + half + 4 * chunk);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        c[e] = cv[e >> 1];
-        s[e] = sv[e >> 1];
-      }
-      return;
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int i = 8 * chunk + e;
-      const int j = MODE == kRotPairs ? i >> 1 : i < half ? i : i - half;
-      c[e] = i < a.rot ? row[j] : 1.0f;
-      s[e] = i < a.rot ? row[half + j] : 0.0f;
-    }
-  }
-};
-
-// Chunk `chunk` of a row, read as x, after the rotation.
-template <class E, int MODE>
-__device__ inline typename Kv<E>::V8 rotated_chunk(const E* row, typename Kv<E>::V8 x, int chunk,
-                                                   const Turn<MODE>& t, int rot) {
-  using V8 = typename Kv<E>::V8;
-  if (8 * chunk >= rot) return x;
-  const int half = rot >> 1;
-  V8 y;
-  if (MODE == kRotPairs) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = x[e ^ 1];
-  } else if (MODE == kRotHalf) {
-    const int other = 8 * chunk < half ? 8 * chunk + half : 8 * chunk - half;
-    y = *reinterpret_cast<const V8*>(row + other);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int i = 8 * chunk + e;
-      y[e] = i < rot ? row[i < half ? i + half : i - half] : x[e];
-    }
-  }
-  V8 out;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int i = 8 * chunk + e;
-    const bool first = MODE == kRotPairs ? (i & 1) == 0 : i < half;
-    const float own = static_cast<float>(x[e]), other = static_cast<float>(y[e]);
-    const float z = first ? rot_first(own, other, t.c[e], t.s[e])
-                          : rot_second(own, other, t.c[e], t.s[e]);
-    out[e] = i < rot ? static_cast<E>(z) : x[e];
-  }
-  return out;
-}
-
 // Where a token's row goes: (page, head, slot), in elements.
 template <int D>
 __device__ inline int64_t cache_row(const AppendArgs& a, int32_t page, int head, int32_t pos) {
@@ -142,49 +52,7 @@ __device__ inline int64_t cache_row(const AppendArgs& a, int32_t page, int head,
   return ((block << a.tok.shift) + (pos & ((1 << a.tok.shift) - 1))) * D;
 }
 
-// A lane's two chunks of a row and what turns them. Split halves: partners in the rotated part,
-// neighbours' distance apart in the rest; otherwise the same place in either half of the row.
-template <class E, int D, int MODE>
-struct Pair {
-  using V8 = typename Kv<E>::V8;
-  static constexpr int C = D / 16;
-  int chunk[2];
-  Turn<MODE> turn[MODE == kRotHalf ? 1 : 2];
-  bool turned;  // split halves: in the rotated part
-
-  __device__ Pair(const AppendArgs& a, int lane) {
-    const int r = a.rot / 16;
-    turned = lane < r;
-    if (MODE == kRotHalf) {
-      chunk[0] = turned ? lane : lane + r;
-      chunk[1] = turned ? lane + r : lane + C;
-    } else {
-      chunk[0] = lane;
-      chunk[1] = lane + C;
-    }
-  }
-  __device__ void load(const AppendArgs& a, int32_t pos) {
-    turn[0].load(a, pos, chunk[0]);
-    if constexpr (MODE != kRotHalf) turn[1].load(a, pos, chunk[1]);
-  }
-  // x: the two chunks as read; `row` for partners elsewhere
-  __device__ void rotate(const E* row, int rot, V8 (&x)[2]) const {
-    if constexpr (MODE == kRotHalf) {
-      if (!turned) return;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float f = static_cast<float>(x[0][e]), s = static_cast<float>(x[1][e]);
-        x[0][e] = static_cast<E>(rot_first(f, s, turn[0].c[e], turn[0].s[e]));
-        x[1][e] = static_cast<E>(rot_second(s, f, turn[0].c[e], turn[0].s[e]));
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) x[i] = rotated_chunk<E, MODE>(row, x[i], chunk[i], turn[i], rot);
-    }
-  }
-};
-
-template <class E, int D, int MODE>
+template <class E, int D, int MODE, bool NORM>
 __device__ inline void move_rows(const AppendArgs& a, int64_t unit) {
   using V8 = typename Kv<E>::V8;
   constexpr int C = D / 16, SLOTS = kWave / C, FLIGHT = 2;
@@ -194,8 +62,8 @@ __device__ inline void move_rows(const AppendArgs& a, int64_t unit) {
   const KvPlace p = kv_place(a.tok, t);
   const int32_t page = p.last >= 0 ? kv_page(a.tok, p, p.last) : -1;
   const bool valid = page >= 0 && (a.rot == 0 || p.pos < a.table_len);
-  Pair<E, D, MODE> pair(a, lane);
-  if (valid && a.rot > 0) pair.load(a, p.pos);
+  Pair<E, D, MODE, NORM> pair(a, lane);
+  if (valid) pair.load(a, p.pos);
   const int rows = a.Hq + 2 * a.Hkv, step = a.row_parts * SLOTS;
   const E* q = static_cast<const E*>(a.q) + t * a.q_st;
   const E* k = static_cast<const E*>(a.k) + t * a.k_st;
@@ -224,7 +92,9 @@ __device__ inline void move_rows(const AppendArgs& a, int64_t unit) {
     for (int i = 0; i < FLIGHT; ++i) {
       const int r = r0 + i * step;
       if (r >= rows || (r >= a.Hq && !valid)) continue;
-      if (valid && r < a.Hq + a.Hkv && a.rot > 0) pair.rotate(from[i], a.rot, x[i]);
+      if (valid && r < a.Hq + a.Hkv && (NORM || a.rot > 0)) {
+        pair.apply(from[i], a, r < a.Hq ? 0 : 1, x[i]);
+      }
       E* to = r < a.Hq           ? to_q + r * D
               : r < a.Hq + a.Hkv ? static_cast<E*>(a.k_cache) + at + (r - a.Hq) * head
                                  : static_cast<E*>(a.v_cache) + at + (r - a.Hq - a.Hkv) * head;
@@ -234,17 +104,25 @@ __device__ inline void move_rows(const AppendArgs& a, int64_t unit) {
   }
 }
 
-template <class E, int D, int MODE>
+template <class E, int D, int MODE, bool NORM>
 __device__ inline void fill_bounds(const AppendArgs& a) {
   using V8 = typename Kv<E>::V8;
-  constexpr int C = D / 8, SLOTS = kAppendThreads / C;
+  // (a row's lanes are neighbours of one wave)
+  constexpr int C = D / 8, WAVE_SLOTS = kWave / C;
+  constexpr int SLOTS = kAppendThreads / kWave * WAVE_SLOTS;
   __shared__ float lows[SLOTS][D], highs[SLOTS][D];
   __shared__ float tops[kAppendThreads / kWave];
   const int head = static_cast<int>(blockIdx.x % a.Hkv);
   const int64_t t0 = static_cast<int64_t>(blockIdx.x / a.Hkv) * a.tile;
   const int size = 1 << a.tok.shift;
-  const int chunk = threadIdx.x % C, slot = threadIdx.x / C;
+  const int chunk = lane_id() % C;
+  const int slot = lane_id() / C < WAVE_SLOTS
+                       ? static_cast<int>(threadIdx.x / kWave) * WAVE_SLOTS + lane_id() / C
+                       : SLOTS;
   const E* k = static_cast<const E*>(a.k) + head * a.k_sh;
+  const HeadNorm& norm = a.norm[1];
+  Weights<E> w;
+  if (NORM) w.load(norm, chunk);
   // which of the tile's tokens complete a block: one a lane (the same in every wave)
   const int64_t mine = t0 + lane_id();
   bool full = false;
@@ -273,8 +151,10 @@ __device__ inline void fill_bounds(const AppendArgs& a) {
           Turn<MODE> turn;
           if (a.rot > 0) turn.load(a, pos, chunk);
           const E* row = k + from * a.k_st;
-          x = rotated_chunk<E, MODE>(row, reinterpret_cast<const V8*>(row)[chunk], chunk, turn,
-                                     a.rot);
+          const V8 own[1] = {reinterpret_cast<const V8*>(row)[chunk]};
+          float r = 1.0f;
+          if (NORM && norm.weight) r = row_scale<E, D, C>(own, chunk, a.eps);
+          x = turned_chunk<E, MODE, NORM>(row, own[0], chunk, turn, a, norm, r, w);
         } else {
           x = *reinterpret_cast<const V8*>(static_cast<const E*>(a.k_cache) +
                                            cache_row<D>(a, page, head, pos) + 8 * chunk);
@@ -319,13 +199,13 @@ __device__ inline void fill_bounds(const AppendArgs& a) {
   }
 }
 
-template <class E, int D, int MODE>
+template <class E, int D, int MODE, bool NORM>
 __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(AppendArgs a) {
   if (blockIdx.x < a.bound_groups) {
-    fill_bounds<E, D, MODE>(a);
+    fill_bounds<E, D, MODE, NORM>(a);
   } else {
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
-    move_rows<E, D, MODE>(
+    move_rows<E, D, MODE, NORM>(
         a, (blockIdx.x - a.bound_groups) * (kAppendThreads / kWave) + wave);
   }
 }
@@ -343,20 +223,33 @@ extern "C" int rt_kv_append(const void* q, int64_t q_token_stride, int64_t q_hea
                             const int32_t* page_table, int64_t B, int64_t max_pages, void* k_cache,
                             void* v_cache, int64_t P, int64_t page, int8_t* bounds,
                             float* bound_scales, void* q_out, rt_stream_t stream) {
+  return rt_kv_append_norm(q, q_token_stride, q_head_stride, k, k_token_stride, k_head_stride, v,
+                           v_token_stride, v_head_stride, T, Hq, Hkv, D, dtype, nullptr, nullptr, 0,
+                           0.0, cos_sin, table_len, rot, interleaved, positions, seq_ids, page_table,
+                           B, max_pages, k_cache, v_cache, P, page, bounds, bound_scales, q_out,
+                           stream);
+}
+
+extern "C" int rt_kv_append_norm(
+    const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+    int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
+    int64_t v_head_stride, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int dtype,
+    const void* q_weight, const void* k_weight, int wide_weights, double eps, const float* cos_sin,
+    int64_t table_len, int64_t rot, int interleaved, const int32_t* positions,
+    const int32_t* seq_ids, const int32_t* page_table, int64_t B, int64_t max_pages, void* k_cache,
+    void* v_cache, int64_t P, int64_t page, int8_t* bounds, float* bound_scales, void* q_out,
+    rt_stream_t stream) {
   if (const int st = kv_check(T, Hq, Hkv, D, dtype, B, max_pages, P, page)) return st;
-  RT_CHECK_ARG(rot >= 0 && rot % 2 == 0 && rot <= D, "the rotated part must be even, at most %lld",
-               static_cast<long long>(D));
-  RT_CHECK_ARG(table_len >= 0 && table_len <= INT32_MAX, "the rotary table has too many rows");
+  if (const int st = kv_check_turn(D, cos_sin, table_len, rot, q_weight, k_weight, eps)) return st;
   if (T == 0) return kOk;
-  RT_CHECK_ARG(q && k && v && positions && seq_ids && q_out && (rot == 0 || cos_sin),
-               "null pointer");
+  RT_CHECK_ARG(q && k && v && positions && seq_ids && q_out, "null pointer");
   RT_CHECK_ARG(B * max_pages == 0 || page_table, "null page table");
   RT_CHECK_ARG(P == 0 || (k_cache && v_cache && bounds && bound_scales), "null cache");
   RT_CHECK_ARG(kv_rows_aligned(q, q_token_stride, q_head_stride) &&
                    kv_rows_aligned(k, k_token_stride, k_head_stride) &&
                    kv_rows_aligned(v, v_token_stride, v_head_stride) &&
                    kv_rows_aligned(k_cache, 0, 0) && kv_rows_aligned(v_cache, 0, 0) &&
-                   kv_rows_aligned(q_out, 0, 0) && reinterpret_cast<uintptr_t>(cos_sin) % 16 == 0,
+                   kv_rows_aligned(q_out, 0, 0),
                "rows must start on 16 bytes");
   AppendArgs a{};
   a.q = q, a.k = k, a.v = v;
@@ -364,8 +257,8 @@ extern "C" int rt_kv_append(const void* q, int64_t q_token_stride, int64_t q_hea
   a.k_st = k_token_stride, a.k_sh = k_head_stride;
   a.v_st = v_token_stride, a.v_sh = v_head_stride;
   a.T = T, a.Hq = static_cast<int32_t>(Hq), a.Hkv = static_cast<int32_t>(Hkv);
-  a.cos_sin = cos_sin, a.table_len = static_cast<int32_t>(table_len);
-  a.rot = static_cast<int32_t>(rot);
+  static_cast<TurnArgs&>(a) = kv_turn_args(cos_sin, table_len, rot, q_weight, k_weight,
+                                           wide_weights, eps);
   a.tok = {positions, seq_ids, page_table, static_cast<int32_t>(B),
            static_cast<int32_t>(max_pages), static_cast<int32_t>(P), kv_shift(page)};
   a.k_cache = k_cache, a.v_cache = v_cache, a.bounds = bounds, a.scales = bound_scales;
@@ -384,20 +277,15 @@ extern "C" int rt_kv_append(const void* q, int64_t q_token_stride, int64_t q_hea
   const int64_t grid = bound_groups + cdiv(T * a.row_parts, kAppendThreads / kWave);
   RT_CHECK_ARG(grid <= INT32_MAX, "too many tokens");
   a.bound_groups = static_cast<uint32_t>(bound_groups);
-  const int mode = interleaved ? kRotPairs : rot % 16 == 0 ? kRotHalf : kRotHalfOdd;
   return kv_dispatch(dtype, D, [&](auto e, auto d) -> int {
     using E = decltype(e);
     constexpr int DD = decltype(d)::value;
-    const dim3 g(static_cast<unsigned>(grid)), b(kAppendThreads);
-    const hipStream_t s = static_cast<hipStream_t>(stream);
-    if (mode == kRotHalf) {
-      kv_append_kernel<E, DD, kRotHalf><<<g, b, 0, s>>>(a);
-    } else if (mode == kRotHalfOdd) {
-      kv_append_kernel<E, DD, kRotHalfOdd><<<g, b, 0, s>>>(a);
-    } else {
-      kv_append_kernel<E, DD, kRotPairs><<<g, b, 0, s>>>(a);
-    }
-    RT_CHECK_HIP(hipGetLastError());
-    return kOk;
+    return kv_turn_dispatch(rot, interleaved, q_weight || k_weight, [&](auto mode, auto norm) -> int {
+      kv_append_kernel<E, DD, decltype(mode)::value, decltype(norm)::value>
+          <<<dim3(static_cast<unsigned>(grid)), dim3(kAppendThreads), 0,
+             static_cast<hipStream_t>(stream)>>>(a);
+      RT_CHECK_HIP(hipGetLastError());
+      return kOk;
+    });
   });
 }

@@ -1,0 +1,483 @@
+// Appending to the 8-bit paged cache (kv_int8.h): norm and rotation on the way, a block's codes,
+// scales and bounds once it is full, its 16-bit rows until then.
+//
+// Norm and rotation are kv_rotate.h's. A token that takes its block's last slot completes it: the
+// block's rows that are part of this call are turned again from the input, earlier ones come from the
+// sequence's open block (or from the codes, where the block had been full and its sequence was cut
+// back into it), and the codes, scales and int8 bounds follow from the 16-bit rows. Bounds are those
+// of kv_append.hip.
+//
+// One launch, no workgroup waits for another. Workgroups at the grid's head look at a tile of tokens
+// for one head's keys or values and do the blocks completed there: rows to LDS once, their largest
+// magnitude, then codes (values transposed on the way out). In the others a wave moves a token's
+// queries, and its key and value rows to the open block. The open block is read (the first block
+// that a call completes) and written (the rows behind the last one) in the same call: a run of
+// tokens that begins in one block and ends in a later, open one has these rows written by the
+// workgroup that reads the open block first, after it has read.
+#include <type_traits>
+
+#include "../../include/retrieve_amd.h"
+#include "kv_int8.h"
+#include "kv_rotate.h"
+
+namespace rt {
+
+constexpr int kWriteThreads = 256, kWriteWaves = kWriteThreads / kWave;
+
+struct WriteArgs : TurnArgs {
+  const void *q, *k, *v;
+  int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;  // token and head strides, elements
+  int64_t T;
+  int32_t Hq, Hkv;
+  KvTokens tok;
+  KvInt8 cache;
+  int8_t* bounds;
+  float* bound_scales;
+  void* q_out;
+  int32_t row_parts;     // waves a token's rows are split over
+  uint32_t fill_groups;  // workgroups that look for full blocks
+  int32_t tile;          // tokens that one of them looks at
+};
+
+// A token's page where it is appended, -1 where it is padding.
+__device__ inline int32_t write_page(const WriteArgs& a, const KvPlace& p) {
+  if (p.last < 0 || (a.rot > 0 && p.pos >= a.table_len)) return -1;
+  return kv_page(a.tok, p, p.last);
+}
+// Whether token `at` of the call is position `pos` of sequence `seq` and not padding.
+__device__ inline bool is_token(const WriteArgs& a, int64_t at, int32_t seq, int64_t pos) {
+  if (at < 0 || at >= a.T || pos < 0 || a.tok.seq_ids[at] != seq || a.tok.positions[at] != pos) {
+    return false;
+  }
+  return write_page(a, kv_place(a.tok, at)) >= 0;
+}
+// Whether the block of token t (at p, not padding) stays open in this call.
+__device__ inline bool stays_open(const WriteArgs& a, int64_t t, const KvPlace& p, int32_t seq) {
+  const int32_t size = 1 << a.tok.shift, more = size - 1 - (p.pos & (size - 1));
+  return !is_token(a, t + more, seq, static_cast<int64_t>(p.pos) + more);
+}
+
+// Queries to q_out; key and value rows to the open block, where the call's run of their sequence's
+// tokens began in it.
+template <class E, int D, int MODE, bool NORM>
+__device__ inline void move_rows(const WriteArgs& a, int64_t unit) {
+  using V8 = typename Kv<E>::V8;
+  constexpr int C = D / 16, SLOTS = kWave / C, FLIGHT = 2;
+  const int lane = lane_id() % C, place = lane_id() / C;
+  const int64_t t = unit / a.row_parts;
+  if (t >= a.T || place >= SLOTS) return;
+  const KvPlace p = kv_place(a.tok, t);
+  const bool valid = write_page(a, p) >= 0;
+  const int size = 1 << a.tok.shift, slot = p.pos & (size - 1);
+  int rows = a.Hq;
+  int32_t seq = 0;
+  if (valid) {
+    seq = a.tok.seq_ids[t];
+    if (stays_open(a, t, p, seq) &&
+        !is_token(a, t - slot - 1, seq, static_cast<int64_t>(p.pos) - slot - 1)) {
+      rows += 2 * a.Hkv;
+    }
+  }
+  Pair<E, D, MODE, NORM> pair(a, lane);
+  if (valid) pair.load(a, p.pos);
+  const int step = a.row_parts * SLOTS;
+  const E* q = static_cast<const E*>(a.q) + t * a.q_st;
+  const E* k = static_cast<const E*>(a.k) + t * a.k_st;
+  const E* v = static_cast<const E*>(a.v) + t * a.v_st;
+  E* to_q = static_cast<E*>(a.q_out) + t * a.Hq * D;
+  const int64_t open = (static_cast<int64_t>(seq) * a.Hkv << a.tok.shift) * D;
+  for (int r0 = static_cast<int>(unit % a.row_parts) * SLOTS + place; r0 < rows;
+       r0 += FLIGHT * step) {
+    V8 x[FLIGHT][2];
+    const E* from[FLIGHT];
+#pragma unroll
+    for (int i = 0; i < FLIGHT; ++i) {
+      const int r = r0 + i * step;
+      from[i] = r < a.Hq           ? q + r * a.q_sh
+                : r < a.Hq + a.Hkv ? k + (r - a.Hq) * a.k_sh
+                                   : v + (r - a.Hq - a.Hkv) * a.v_sh;
+      x[i][0] = V8{};
+      x[i][1] = V8{};
+      if (valid && r < rows) {
+        x[i][0] = __builtin_nontemporal_load(reinterpret_cast<const V8*>(from[i]) + pair.chunk[0]);
+        x[i][1] = __builtin_nontemporal_load(reinterpret_cast<const V8*>(from[i]) + pair.chunk[1]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < FLIGHT; ++i) {
+      const int r = r0 + i * step;
+      if (r >= rows) continue;
+      if (valid && r < a.Hq + a.Hkv && (NORM || a.rot > 0)) {
+        pair.apply(from[i], a, r < a.Hq ? 0 : 1, x[i]);
+      }
+      const int64_t head = static_cast<int64_t>(D) << a.tok.shift;  // from head to head
+      if (r < a.Hq + a.Hkv) {
+        E* to = r < a.Hq ? to_q + r * D
+                         : static_cast<E*>(a.cache.k_tail) + open + (r - a.Hq) * head + slot * D;
+        __builtin_nontemporal_store(x[i][0], reinterpret_cast<V8*>(to) + pair.chunk[0]);
+        __builtin_nontemporal_store(x[i][1], reinterpret_cast<V8*>(to) + pair.chunk[1]);
+      } else {
+        E* to = static_cast<E*>(a.cache.v_tail) + open + (r - a.Hq - a.Hkv) * head + slot;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) to[(8 * pair.chunk[j] + e) << a.tok.shift] = x[i][j][e];
+        }
+      }
+    }
+  }
+}
+
+// The largest of x over the workgroup (`scratch`: a float a wave).
+__device__ inline float group_max(float x, float* scratch) {
+  for (int i = 1; i < kWave; i <<= 1) x = fmaxf(x, __shfl_xor(x, i));
+  __syncthreads();
+  if (lane_id() == 0) scratch[threadIdx.x / kWave] = x;
+  __syncthreads();
+  x = scratch[0];
+  for (int w = 1; w < kWriteWaves; ++w) x = fmaxf(x, scratch[w]);
+  return x;
+}
+
+// One head's keys (VALUES: values) of a tile of tokens.
+template <class E, int D, int MODE, bool NORM, bool VALUES>
+struct Fill {
+  using V8 = typename Kv<E>::V8;
+  // a row's chunks of 8 channels lie on neighbouring lanes of one wave
+  static constexpr int C = D / 8, WAVE_ROWS = kWave / C, ROWS = kWriteWaves * WAVE_ROWS;
+  const WriteArgs& a;
+  char* lds;       // the block's rows; then the channels' least and largest keys
+  float* scratch;  // a float a wave
+  int head, chunk, row;  // this thread's (row: ROWS where it has none)
+  Weights<E> w;
+
+  __device__ Fill(const WriteArgs& args, int h, char* shared, float* waves)
+      : a(args), lds(shared), scratch(waves), head(h) {
+    chunk = lane_id() % C;
+    row = lane_id() / C < WAVE_ROWS
+              ? static_cast<int>(threadIdx.x / kWave) * WAVE_ROWS + lane_id() / C
+              : ROWS;
+    if (NORM && !VALUES) w.load(a.norm[1], chunk);
+  }
+  // This thread's chunk of token `at`, whose position is `pos`.
+  __device__ V8 fresh(int64_t at, int32_t pos) const {
+    const E* from = VALUES ? static_cast<const E*>(a.v) + head * a.v_sh + at * a.v_st
+                           : static_cast<const E*>(a.k) + head * a.k_sh + at * a.k_st;
+    const V8 own[1] = {reinterpret_cast<const V8*>(from)[chunk]};
+    if constexpr (VALUES) {
+      return own[0];
+    } else {
+      Turn<MODE> turn;
+      if (a.rot > 0) turn.load(a, pos, chunk);
+      float r = 1.0f;
+      if (NORM && a.norm[1].weight) r = row_scale<E, D, C>(own, chunk, a.eps);
+      return turned_chunk<E, MODE, NORM>(from, own[0], chunk, turn, a, a.norm[1], r, w);
+    }
+  }
+  __device__ int64_t block(int64_t of) const { return (of * a.Hkv + head) << a.tok.shift; }
+  // The same of a slot that holds an earlier token, from the codes (scale above 0) or the open block.
+  __device__ V8 held(int32_t page, int32_t seq, int slot, float scale) const {
+    const int64_t full = block(page) * D, open = block(seq) * D;
+    V8 x;
+    if constexpr (VALUES) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int at = ((8 * chunk + e) << a.tok.shift) + slot;
+        x[e] = scale > 0.0f ? static_cast<E>(a.cache.v_codes[full + at] * scale)
+                            : static_cast<const E*>(a.cache.v_tail)[open + at];
+      }
+    } else {
+      const int at = slot * D + 8 * chunk;
+      if (scale > 0.0f) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = static_cast<E>(a.cache.k_codes[full + at + e] * scale);
+      } else {
+        x = *reinterpret_cast<const V8*>(static_cast<const E*>(a.cache.k_tail) + open + at);
+      }
+    }
+    return x;
+  }
+  __device__ void to_open(int32_t seq, int slot, V8 x) const {
+    const int64_t open = block(seq) * D;
+    if constexpr (VALUES) {
+      E* to = static_cast<E*>(a.cache.v_tail) + open + slot;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) to[(8 * chunk + e) << a.tok.shift] = x[e];
+    } else {
+      *reinterpret_cast<V8*>(static_cast<E*>(a.cache.k_tail) + open + slot * D + 8 * chunk) = x;
+    }
+  }
+  __device__ float* scale_of(int32_t page) const {
+    return (VALUES ? a.cache.v_scales : a.cache.k_scales) +
+           (static_cast<int64_t>(page) * a.Hkv + head);
+  }
+
+  // A block that had been full and is begun again behind slot `from`: its earlier rows in 16 bits.
+  __device__ void reopen(int32_t page, int32_t seq, int from) const {
+    const float scale = *scale_of(page);
+    if (row < ROWS) {
+      for (int o = row; o < from; o += ROWS) to_open(seq, o, held(page, seq, o, scale));
+    }
+    __syncthreads();  // (everyone has read the scale)
+    if (threadIdx.x == 0) *scale_of(page) = 0.0f;
+    __syncthreads();
+  }
+
+  // The block that token t completes.
+  __device__ void fill(int64_t t) const {
+    const KvPlace p = kv_place(a.tok, t);
+    const int32_t page = kv_page(a.tok, p, p.last), seq = a.tok.seq_ids[t];
+    const int size = 1 << a.tok.shift;
+    const float old = *scale_of(page);
+    float most = 0.0f, lo[8], hi[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      lo[e] = INFINITY;
+      hi[e] = -INFINITY;
+    }
+    if (row < ROWS) {
+      for (int o = row; o < size; o += ROWS) {
+        const int64_t from = t - (size - 1 - o);
+        const int32_t pos = p.pos - (size - 1 - o);
+        const bool here = from >= 0 && a.tok.positions[from] == pos && a.tok.seq_ids[from] == seq;
+        const V8 x = here ? fresh(from, pos) : held(page, seq, o, old);
+        *reinterpret_cast<V8*>(lds + (o * D + 8 * chunk) * 2) = x;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float f = static_cast<float>(x[e]);
+          most = fmaxf(most, finite_size(f));
+          if (!VALUES) {
+            lo[e] = fminf(lo[e], f);
+            hi[e] = fmaxf(hi[e], f);
+          }
+        }
+      }
+    }
+    most = fmaxf(group_max(most, scratch), kKvTopFloor);  // (its barriers: the rows are there)
+    const BlockCode code(most);
+    if (threadIdx.x == 0) *scale_of(page) = most / 127.0f;
+    if constexpr (VALUES) {
+      int8_t* to = a.cache.v_codes + block(page) * D;
+      // two channels and 16 slots a thread
+      for (int i = threadIdx.x; i < D / 2 * (size / 16); i += kWriteThreads) {
+        const int c = i % (D / 2), s = i / (D / 2) * 16;
+        v4i out[2];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t word[2] = {0u, 0u};
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            typedef E V2 __attribute__((ext_vector_type(2)));
+            const V2 x = *reinterpret_cast<const V2*>(lds + ((s + 4 * j + b) * D + 2 * c) * 2);
+            word[0] |= (static_cast<uint32_t>(code(static_cast<float>(x[0]))) & 255u) << (8 * b);
+            word[1] |= (static_cast<uint32_t>(code(static_cast<float>(x[1]))) & 255u) << (8 * b);
+          }
+          out[0][j] = static_cast<int>(word[0]);
+          out[1][j] = static_cast<int>(word[1]);
+        }
+        *reinterpret_cast<v4i*>(to + (2 * c << a.tok.shift) + s) = out[0];
+        *reinterpret_cast<v4i*>(to + ((2 * c + 1) << a.tok.shift) + s) = out[1];
+      }
+    } else {
+      typedef int V2i __attribute__((ext_vector_type(2)));
+      if (row < ROWS) {
+        for (int o = row; o < size; o += ROWS) {
+          const V8 x = *reinterpret_cast<const V8*>(lds + (o * D + 8 * chunk) * 2);
+          uint32_t word[2] = {0u, 0u};
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            word[e >> 2] |= (static_cast<uint32_t>(code(static_cast<float>(x[e]))) & 255u)
+                            << (8 * (e & 3));
+          }
+          *reinterpret_cast<V2i*>(a.cache.k_codes + (block(page) + o) * D + 8 * chunk) =
+              V2i{static_cast<int>(word[0]), static_cast<int>(word[1])};
+        }
+      }
+      __syncthreads();  // (the rows have been read)
+      bounds(page, lo, hi);
+    }
+    // The first block of a run that ends in an open one: that one's rows, which are not moved (the
+    // open block has been read now).
+    if (!is_token(a, t - size, seq, static_cast<int64_t>(p.pos) - size)) {
+      int64_t full = 0;  // blocks behind this one that are completed as well
+      for (;;) {
+        __syncthreads();
+        const int64_t n = size * (full + threadIdx.x + 1);
+        const uint64_t no = ~__ballot(is_token(a, t + n, seq, p.pos + n));
+        if (lane_id() == 0) scratch[threadIdx.x / kWave] = no ? __builtin_ctzll(no) : kWave;
+        __syncthreads();
+        int more = 0;
+        for (int i = 0; i < kWriteWaves && more == i * kWave; ++i) {
+          more += static_cast<int>(scratch[i]);
+        }
+        full += more;
+        if (more < kWriteThreads) break;
+      }
+      const int64_t first = t + size * full + 1;
+      const int32_t pos = static_cast<int32_t>(p.pos + size * full + 1);
+      if (row < ROWS) {
+        for (int o = row; o < size - 1; o += ROWS) {
+          if (!is_token(a, first + o, seq, static_cast<int64_t>(pos) + o)) break;
+          to_open(seq, o, fresh(first + o, pos + o));
+        }
+      }
+    }
+    __syncthreads();
+  }
+
+  // The bounds of a block from its channels' least and largest keys, a chunk a thread.
+  __device__ void bounds(int32_t page, const float (&lo)[8], const float (&hi)[8]) const {
+    float(*lows)[D] = reinterpret_cast<float(*)[D]>(lds);
+    float(*highs)[D] = lows + ROWS;
+    if (row < ROWS) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        lows[row][8 * chunk + e] = lo[e];
+        highs[row][8 * chunk + e] = hi[e];
+      }
+    }
+    __syncthreads();
+    const int d = threadIdx.x;
+    float mid = 0.0f, half = 0.0f;
+    if (d < D) {
+      float l = lows[0][d], h = highs[0][d];
+      for (int i = 1; i < ROWS; ++i) {
+        l = fminf(l, lows[i][d]);
+        h = fmaxf(h, highs[i][d]);
+      }
+      mid = (l + h) * 0.5f;
+      half = (h - l) * 0.5f;
+    }
+    const float top = fmaxf(group_max(fmaxf(fabsf(mid), half), scratch), kKvTopFloor);
+    const int64_t at = static_cast<int64_t>(page) * a.Hkv + head;
+    if (d < D) {
+      a.bounds[at * 2 * D + d] = static_cast<int8_t>(kv_code(mid, top));
+      a.bounds[at * 2 * D + D + d] = static_cast<int8_t>(kv_code(half, top));
+    }
+    if (d == 0) a.bound_scales[at] = top / 127.0f;
+  }
+
+  __device__ void run(int64_t t0, uint64_t* masks) {
+    const int size = 1 << a.tok.shift;
+    if (threadIdx.x < kWave) {  // one token a lane
+      const int64_t mine = t0 + lane_id();
+      bool full = false, again = false;
+      if (lane_id() < a.tile && mine < a.T) {
+        const KvPlace p = kv_place(a.tok, mine);
+        const int32_t page = write_page(a, p);
+        if (page >= 0) {
+          const int32_t seq = a.tok.seq_ids[mine];
+          const int slot = p.pos & (size - 1);
+          full = slot == size - 1;
+          // the first token of a block that stays open
+          if (!full &&
+              (slot == 0 || !is_token(a, mine - 1, seq, static_cast<int64_t>(p.pos) - 1)) &&
+              stays_open(a, mine, p, seq)) {
+            again = slot > 0 && *scale_of(page) > 0.0f;
+            if (!again) *scale_of(page) = 0.0f;
+          }
+        }
+      }
+      const uint64_t f = __ballot(full), r = __ballot(again);
+      if (lane_id() == 0) {
+        masks[0] = f;
+        masks[1] = r;
+      }
+    }
+    __syncthreads();
+    for (uint64_t left = masks[1]; left != 0; left &= left - 1) {
+      const int64_t t = t0 + __builtin_ctzll(left);
+      const KvPlace p = kv_place(a.tok, t);
+      reopen(kv_page(a.tok, p, p.last), a.tok.seq_ids[t], p.pos & (size - 1));
+    }
+    for (uint64_t left = masks[0]; left != 0; left &= left - 1) {
+      fill(t0 + __builtin_ctzll(left));
+    }
+  }
+};
+
+template <class E, int D, int MODE, bool NORM>
+__global__ void __launch_bounds__(kWriteThreads) kv_append_int8_kernel(WriteArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  __shared__ float scratch[kWriteWaves];
+  __shared__ uint64_t masks[2];
+  if (blockIdx.x < a.fill_groups) {
+    const int job = static_cast<int>(blockIdx.x % (2 * a.Hkv));
+    const int64_t t0 = static_cast<int64_t>(blockIdx.x / (2 * a.Hkv)) * a.tile;
+    if (job < a.Hkv) {
+      Fill<E, D, MODE, NORM, false>(a, job, lds, scratch).run(t0, masks);
+    } else {
+      Fill<E, D, MODE, NORM, true>(a, job - a.Hkv, lds, scratch).run(t0, masks);
+    }
+  } else {
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+    move_rows<E, D, MODE, NORM>(
+        a, static_cast<int64_t>(blockIdx.x - a.fill_groups) * kWriteWaves + wave);
+  }
+}
+
+}  // namespace rt
+
+using namespace rt;
+
+extern "C" int rt_kv_append_int8(
+    const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+    int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
+    int64_t v_head_stride, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int dtype,
+    const void* q_weight, const void* k_weight, int wide_weights, double eps, const float* cos_sin,
+    int64_t table_len, int64_t rot, int interleaved, const int32_t* positions,
+    const int32_t* seq_ids, const int32_t* page_table, int64_t B, int64_t max_pages,
+    int8_t* k_codes, int8_t* v_codes, float* k_scales, float* v_scales, void* k_tail, void* v_tail,
+    int64_t P, int64_t page, int8_t* bounds, float* bound_scales, void* q_out,
+    rt_stream_t stream) {
+  if (const int st = kv_check(T, Hq, Hkv, D, dtype, B, max_pages, P, page)) return st;
+  if (const int st = kv_check_turn(D, cos_sin, table_len, rot, q_weight, k_weight, eps)) return st;
+  if (T == 0) return kOk;
+  const KvInt8 cache{k_codes, v_codes, k_scales, v_scales, k_tail, v_tail};
+  if (const int st = kv_check_int8(cache, B, P)) return st;
+  RT_CHECK_ARG(q && k && v && positions && seq_ids && q_out, "null pointer");
+  RT_CHECK_ARG(B * max_pages == 0 || page_table, "null page table");
+  RT_CHECK_ARG(P == 0 || (bounds && bound_scales), "null bounds");
+  RT_CHECK_ARG(kv_rows_aligned(q, q_token_stride, q_head_stride) &&
+                   kv_rows_aligned(k, k_token_stride, k_head_stride) &&
+                   kv_rows_aligned(v, v_token_stride, v_head_stride) &&
+                   kv_rows_aligned(q_out, 0, 0),
+               "rows must start on 16 bytes");
+  WriteArgs a{};
+  static_cast<TurnArgs&>(a) = kv_turn_args(cos_sin, table_len, rot, q_weight, k_weight,
+                                           wide_weights, eps);
+  a.q = q, a.k = k, a.v = v;
+  a.q_st = q_token_stride, a.q_sh = q_head_stride;
+  a.k_st = k_token_stride, a.k_sh = k_head_stride;
+  a.v_st = v_token_stride, a.v_sh = v_head_stride;
+  a.T = T, a.Hq = static_cast<int32_t>(Hq), a.Hkv = static_cast<int32_t>(Hkv);
+  a.tok = {positions, seq_ids, page_table, static_cast<int32_t>(B),
+           static_cast<int32_t>(max_pages), static_cast<int32_t>(P), kv_shift(page)};
+  a.cache = cache, a.bounds = bounds, a.bound_scales = bound_scales;
+  a.q_out = q_out;
+  // Few tokens: a token's rows over as many waves as have one each. Many: one wave a token.
+  const int64_t all = cdiv(Hq + 2 * Hkv, kWave / (D / 16)), parts = cdiv(4096, T);
+  a.row_parts = static_cast<int32_t>(parts < all ? parts : all);
+  // Few tokens may all complete a block in one step: a workgroup for each, every head and keys and
+  // values, up to 1024 of them; in prompts 64 tokens a workgroup.
+  const int64_t tile = next_pow2(cdiv(T * Hkv, 512));
+  a.tile = static_cast<int32_t>(tile < 64 ? tile : 64);
+  const int64_t fill_groups = cdiv(T, a.tile) * Hkv * 2;
+  const int64_t grid = fill_groups + cdiv(T * a.row_parts, kWriteWaves);
+  RT_CHECK_ARG(grid <= INT32_MAX, "too many tokens");
+  a.fill_groups = static_cast<uint32_t>(fill_groups);
+  // a block's rows; the least and largest keys of a channel (two floats a thread's 8 channels)
+  const int64_t rows = page * D * 2, ends = kWriteThreads * 8 * 2 * 4;
+  const unsigned lds = static_cast<unsigned>(rows > ends ? rows : ends);
+  return kv_dispatch(dtype, D, [&](auto e, auto d) -> int {
+    using E = decltype(e);
+    constexpr int DD = decltype(d)::value;
+    return kv_turn_dispatch(rot, interleaved, q_weight || k_weight, [&](auto mode, auto norm) -> int {
+      kv_append_int8_kernel<E, DD, decltype(mode)::value, decltype(norm)::value>
+          <<<dim3(static_cast<unsigned>(grid)), dim3(kWriteThreads), lds,
+             static_cast<hipStream_t>(stream)>>>(a);
+      RT_CHECK_HIP(hipGetLastError());
+      return kOk;
+    });
+  });
+}

@@ -31,31 +31,13 @@
 #include <type_traits>
 
 #include "../../include/retrieve_amd.h"
-#include "kv_common.h"
+#include "kv_attend.h"
 #include "lds_load.h"
 
 namespace rt {
 
-constexpr int kAttendWaves = 4;
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-
-struct AttendArgs {
-  const void* q;
-  int64_t q_st, q_sh;
-  int64_t T;
-  int32_t Hq, Hkv, G, tiles;  // G query heads a key/value head, in tiles of 16
+struct AttendArgs : AttendBase {
   const void *k_cache, *v_cache;
-  const int32_t* blocks;  // [T, Hkv, count]
-  int32_t count;
-  KvTokens tok;
-  float scale;      // its magnitude (above 0) times log2 e; the queries carry its sign
-  bool minus;
-  int32_t parts;    // workgroups that share a row
-  int32_t joined;   // tokens a wave takes together
-  void* out;        // [T, Hq, D]
-  float* lse;       // [T, Hq]
-  float* part_out;  // [rows, parts, 16, D], sums of weights times values
-  float* part_ml;   // [rows, parts, 16, 2], maxima (powers of two) and sums
 };
 
 template <class E>
@@ -349,12 +331,6 @@ struct AttendWave {
     join_sums();
   }
 };
-
-// 1 / l; 0 for a row without a key; NaN stays.
-__device__ inline float inverse_sum(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
-__device__ inline float log_sum(float m, float l) {
-  return l == 0.0f ? -INFINITY : (m + __log2f(l)) * kLn2;
-}
 
 // This lane's column, query head `head` of token t, to the outputs.
 template <class E, int D>
@@ -800,79 +776,7 @@ __global__ void __launch_bounds__(kAttendWaves* kWave, D <= 128 ? 2 : 1)
   } else {
     w.template run<true>(a, t, head, tile, first, parts, lds[wave]);
   }
-  // the sums as fp32 rows of a head, 16-byte chunks permuted by the head (bank conflicts)
-  const int col = lane_id() & 15, grp = lane_id() >> 4;
-#pragma unroll
-  for (int i = 0; i < D / 16; ++i) {
-    *reinterpret_cast<v4f*>(lds[wave] + col * (D * 4) + (((4 * i + grp) ^ (col & 7)) << 4)) =
-        w.acc[i];
-  }
-  if (grp == 0) {
-    ml[wave][col][0] = w.m;
-    ml[wave][col][1] = w.l;
-  }
-  __syncthreads();
-  const int heads = a.G - tile * 16 < 16 ? a.G - tile * 16 : 16;
-  for (int i = threadIdx.x; i < heads * (D / 4); i += kAttendWaves * kWave) {
-    const int g = i / (D / 4), c = i % (D / 4);
-    float m = ml[0][g][0];
-#pragma unroll
-    for (int j = 1; j < kAttendWaves; ++j) m = fmaxf(m, ml[j][g][0]);
-    float l = 0.0f;
-    v4f sum{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int j = 0; j < kAttendWaves; ++j) {
-      const float f = __builtin_amdgcn_exp2f(ml[j][g][0] - m);
-      l += f * ml[j][g][1];
-      sum += f * *reinterpret_cast<const v4f*>(lds[j] + g * (D * 4) + ((c ^ (g & 7)) << 4));
-    }
-    if (a.parts == 1) {
-      typedef E V4 __attribute__((ext_vector_type(4)));
-      const int64_t r = t * a.Hq + head * a.G + tile * 16 + g;
-      const float inv = inverse_sum(l);
-      V4 x;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = static_cast<E>(sum[e] * inv);
-      *reinterpret_cast<V4*>(static_cast<E*>(a.out) + r * D + 4 * c) = x;
-      if (c == 0) a.lse[r] = log_sum(m, l);
-    } else {
-      const int64_t r = (row * a.parts + part) * 16 + g;
-      *reinterpret_cast<v4f*>(a.part_out + r * D + 4 * c) = sum;
-      if (c == 0) {
-        a.part_ml[2 * r] = m;
-        a.part_ml[2 * r + 1] = l;
-      }
-    }
-  }
-}
-
-// The parts of a row joined at their largest maximum, in order: a thread has 4 channels of a head.
-template <class E, int D>
-__global__ void __launch_bounds__(D / 4) kv_join_kernel(AttendArgs a) {
-  typedef E V4 __attribute__((ext_vector_type(4)));
-  const int64_t r = blockIdx.x;  // (token, query head)
-  const int64_t t = r / a.Hq;
-  const int hq = static_cast<int>(r % a.Hq), head = hq / a.G, g = hq % a.G;
-  const int64_t row = (t * a.Hkv + head) * a.tiles + g / 16;
-  const int64_t first = row * a.parts * 16 + g % 16;
-  float m = a.part_ml[2 * first];
-#pragma unroll 8
-  for (int p = 1; p < a.parts; ++p) m = fmaxf(m, a.part_ml[2 * (first + 16 * p)]);
-  float l = 0.0f;
-  v4f sum{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-  for (int p = 0; p < a.parts; ++p) {
-    const int64_t at = first + 16 * p;
-    const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * at] - m);
-    l += f * a.part_ml[2 * at + 1];
-    sum += f * *reinterpret_cast<const v4f*>(a.part_out + at * D + 4 * threadIdx.x);
-  }
-  const float inv = inverse_sum(l);
-  V4 x;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) x[e] = static_cast<E>(sum[e] * inv);
-  *reinterpret_cast<V4*>(static_cast<E*>(a.out) + r * D + 4 * threadIdx.x) = x;
-  if (threadIdx.x == 0) a.lse[r] = log_sum(m, l);
+  join_waves<E, D>(a, w.acc, w.m, w.l, t, head, tile, row, part, lds, ml);
 }
 
 // How a call of `seqs` sequences at most is spread: `parts` workgroups a row; 0: `joined` tokens a

@@ -1,0 +1,57 @@
+// The paged cache in 8 bits: its layout, and the code of a block's keys or values.
+//
+// A full block of one head holds its keys as int8 codes [page, D] and its values as codes [D, page],
+// each with one scale (a code stands for code * scale). A sequence's last block, not full yet, lies
+// in 16 bits in the sequence's open block, k_tail [page, D] and v_tail [D, page]; its page's scales
+// are 0 until it is full. So a code depends on its block's 16-bit numbers alone, never on how many
+// calls wrote them, and the latest keys are exact. Values lie transposed so that attention's second
+// product takes its operand (16 slots of a channel) straight from memory.
+#pragma once
+
+#include "kv_common.h"
+
+namespace rt {
+
+struct KvInt8 {
+  int8_t *k_codes, *v_codes;   // [P, Hkv, page, D], [P, Hkv, D, page]
+  float *k_scales, *v_scales;  // [P, Hkv]; 0: not full
+  void *k_tail, *v_tail;       // [B, Hkv, page, D], [B, Hkv, D, page]
+};
+
+// Codes of one block: code = 127 x / top to the nearest even, top its largest finite magnitude
+// (floored at kKvTopFloor). 127 x is exact (18 bits at most), and q + r (y - q top) with q = y r is
+// the quotient of y = 127 x rounded to nearest (kv_code_value's comment), so a tie between two codes
+// is seen as one. Infinities become +-127, NaN 0. A top above 2^100, whose reciprocal may lose bits,
+// comes in scaled by 2^-64 with its numbers.
+struct BlockCode {
+  float top, r, shrink;
+  __device__ explicit BlockCode(float most) {
+    shrink = most > 0x1p100f ? 0x1p-64f : 1.0f;
+    top = most * shrink;
+    r = 1.0f / top;
+  }
+  __device__ int operator()(float x) const {
+#pragma clang fp contract(off)
+    const float y = fminf(fmaxf(x * shrink, -top), top) * 127.0f;
+    const float q = y * r;
+    const float v = rintf(__builtin_fmaf(__builtin_fmaf(-q, top, y), r, q));
+    return x == x ? static_cast<int>(v) : 0;
+  }
+};
+// A number's part in `top`.
+__device__ inline float finite_size(float x) {
+  const float a = fabsf(x);
+  return a < INFINITY ? a : 0.0f;
+}
+
+// Host: the checks of an 8-bit cache's pointers.
+inline int kv_check_int8(const KvInt8& c, int64_t B, int64_t P) {
+  RT_CHECK_ARG(P == 0 || (c.k_codes && c.v_codes && c.k_scales && c.v_scales), "null cache");
+  RT_CHECK_ARG(B == 0 || (c.k_tail && c.v_tail), "null open blocks");
+  RT_CHECK_ARG(kv_rows_aligned(c.k_codes, 0, 0) && kv_rows_aligned(c.v_codes, 0, 0) &&
+                   kv_rows_aligned(c.k_tail, 0, 0) && kv_rows_aligned(c.v_tail, 0, 0),
+               "the cache must start on 16 bytes");
+  return kOk;
+}
+
+}  // namespace rt
