@@ -107,18 +107,21 @@ __device__ inline void move_rows(const AppendArgs& a, int64_t unit) {
 template <class E, int D, int MODE, bool NORM>
 __device__ inline void fill_bounds(const AppendArgs& a) {
   using V8 = typename Kv<E>::V8;
-  // (a row's lanes are neighbours of one wave)
+  // (a norm's lanes of a row are neighbours of one wave)
   constexpr int C = D / 8, WAVE_SLOTS = kWave / C;
-  constexpr int SLOTS = kAppendThreads / kWave * WAVE_SLOTS;
+  constexpr int SLOTS = NORM ? kAppendThreads / kWave * WAVE_SLOTS : kAppendThreads / C;
   __shared__ float lows[SLOTS][D], highs[SLOTS][D];
   __shared__ float tops[kAppendThreads / kWave];
   const int head = static_cast<int>(blockIdx.x % a.Hkv);
   const int64_t t0 = static_cast<int64_t>(blockIdx.x / a.Hkv) * a.tile;
   const int size = 1 << a.tok.shift;
-  const int chunk = lane_id() % C;
-  const int slot = lane_id() / C < WAVE_SLOTS
-                       ? static_cast<int>(threadIdx.x / kWave) * WAVE_SLOTS + lane_id() / C
-                       : SLOTS;
+  int chunk = threadIdx.x % C, slot = threadIdx.x / C;
+  if constexpr (NORM) {
+    chunk = lane_id() % C;
+    slot = lane_id() / C < WAVE_SLOTS
+               ? static_cast<int>(threadIdx.x / kWave) * WAVE_SLOTS + lane_id() / C
+               : SLOTS;
+  }
   const E* k = static_cast<const E*>(a.k) + head * a.k_sh;
   const HeadNorm& norm = a.norm[1];
   Weights<E> w;
@@ -199,8 +202,16 @@ __device__ inline void fill_bounds(const AppendArgs& a) {
   }
 }
 
+// Workgroups a CU that the registers have to leave room for (the rows in flight hide the memory:
+// fp16 rows of 256, neighbours turned, 245 us with 5, 234 with 6).
+constexpr int append_groups(int mode, bool norm) {
+  if (mode == kRotHalfOdd) return norm ? 3 : 4;
+  return norm ? 4 : mode == kRotPairs ? 6 : 5;
+}
+
 template <class E, int D, int MODE, bool NORM>
-__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads, append_groups(MODE, NORM))
+    kv_append_kernel(AppendArgs a) {
   if (blockIdx.x < a.bound_groups) {
     fill_bounds<E, D, MODE, NORM>(a);
   } else {

@@ -33,16 +33,14 @@ __device__ inline float log_sum(float m, float l) {
   return l == 0.0f ? -INFINITY : (m + __log2f(l)) * kLn2;
 }
 
-// A row's sums of the workgroup's waves joined at their largest maximum: to the outputs where one
-// workgroup has the whole row, else to the row's parts. acc: channel 16 i + 4 (lane / 16) + r of
-// column lane % 16.
-template <class E, int D>
-__device__ inline void join_waves(const AttendBase& a, const v4f (&acc)[D / 16], float m_wave,
-                                  float l_wave, int64_t t, int head, int tile, int64_t row,
-                                  int part, char (&lds)[kAttendWaves][64 * D],
-                                  float (&ml)[kAttendWaves][16][2]) {
-  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
-  // the sums as fp32 rows of a head, 16-byte chunks permuted by the head (bank conflicts)
+// The sums of the workgroup's waves over the same columns, joined at the largest maximum: f(column,
+// first of four channels, maximum, sum of weights, sums). acc: channel 16 i + 4 (lane / 16) + r of
+// column lane % 16; `columns` of them count.
+template <class E, int D, class F>
+__device__ inline void join_columns(const v4f (&acc)[D / 16], float m_wave, float l_wave, int wave,
+                                    char (&lds)[kAttendWaves][64 * D],
+                                    float (&ml)[kAttendWaves][16][2], int columns, F&& f) {
+  // the sums as fp32 rows of a column, 16-byte chunks permuted by the column (bank conflicts)
   const int col = lane_id() & 15, grp = lane_id() >> 4;
 #pragma unroll
   for (int i = 0; i < D / 16; ++i) {
@@ -54,8 +52,7 @@ __device__ inline void join_waves(const AttendBase& a, const v4f (&acc)[D / 16],
     ml[wave][col][1] = l_wave;
   }
   __syncthreads();
-  const int heads = a.G - tile * 16 < 16 ? a.G - tile * 16 : 16;
-  for (int i = threadIdx.x; i < heads * (D / 4); i += kAttendWaves * kWave) {
+  for (int i = threadIdx.x; i < columns * (D / 4); i += kAttendWaves * kWave) {
     const int g = i / (D / 4), c = i % (D / 4);
     float m = ml[0][g][0];
 #pragma unroll
@@ -64,10 +61,25 @@ __device__ inline void join_waves(const AttendBase& a, const v4f (&acc)[D / 16],
     v4f sum{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < kAttendWaves; ++j) {
-      const float f = __builtin_amdgcn_exp2f(ml[j][g][0] - m);
-      l += f * ml[j][g][1];
-      sum += f * *reinterpret_cast<const v4f*>(lds[j] + g * (D * 4) + ((c ^ (g & 7)) << 4));
+      const float x = __builtin_amdgcn_exp2f(ml[j][g][0] - m);
+      l += x * ml[j][g][1];
+      sum += x * *reinterpret_cast<const v4f*>(lds[j] + g * (D * 4) + ((c ^ (g & 7)) << 4));
     }
+    f(g, 4 * c, m, l, sum);
+  }
+}
+
+// A row's sums of the workgroup's waves: to the outputs where one workgroup has the whole row, else
+// to the row's parts.
+template <class E, int D>
+__device__ inline void join_waves(const AttendBase& a, const v4f (&acc)[D / 16], float m_wave,
+                                  float l_wave, int64_t t, int head, int tile, int64_t row,
+                                  int part, char (&lds)[kAttendWaves][64 * D],
+                                  float (&ml)[kAttendWaves][16][2]) {
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int heads = a.G - tile * 16 < 16 ? a.G - tile * 16 : 16;
+  join_columns<E, D>(acc, m_wave, l_wave, wave, lds, ml, heads,
+                     [&](int g, int ch, float m, float l, v4f sum) {
     if (a.parts == 1) {
       typedef E V4 __attribute__((ext_vector_type(4)));
       const int64_t r = t * a.Hq + head * a.G + tile * 16 + g;
@@ -75,17 +87,17 @@ __device__ inline void join_waves(const AttendBase& a, const v4f (&acc)[D / 16],
       V4 x;
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[e] = static_cast<E>(sum[e] * inv);
-      *reinterpret_cast<V4*>(static_cast<E*>(a.out) + r * D + 4 * c) = x;
-      if (c == 0) a.lse[r] = log_sum(m, l);
+      *reinterpret_cast<V4*>(static_cast<E*>(a.out) + r * D + ch) = x;
+      if (ch == 0) a.lse[r] = log_sum(m, l);
     } else {
       const int64_t r = (row * a.parts + part) * 16 + g;
-      *reinterpret_cast<v4f*>(a.part_out + r * D + 4 * c) = sum;
-      if (c == 0) {
+      *reinterpret_cast<v4f*>(a.part_out + r * D + ch) = sum;
+      if (ch == 0) {
         a.part_ml[2 * r] = m;
         a.part_ml[2 * r + 1] = l;
       }
     }
-  }
+  });
 }
 
 // The parts of a row joined at their largest maximum, in order: a thread has 4 channels of a head.

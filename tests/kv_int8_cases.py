@@ -79,14 +79,21 @@ def check_attention(got, c: o8.Cache, q, blocks, pos, seq, tab, scale=None):
     fp16 also has a least step, 2^-32 of the row's largest weight times value, at most). Scores are
     fp32 sums of D products, exact each: off by ``(D + 16) 2^-24 scale sum |q k|`` with the three
     products behind them; the exponent adds the logarithm of a block's scale (below 2^6 in size, its
-    rounding and the sum's 2^-18)."""
+    rounding and the sum's 2^-18).
+
+    The products are taken of ``code + 128``, and 128 times the sum of the other factor taken off
+    again: every addition to a sum (one for 32 products) rounds a number of up to 255 times that
+    factor's sum, by 2^-24. For a score that is ``2^-24 (D / 32 + 8) 255 s_k scale sum |q|``, for an
+    output ``2^-24 (keys / 32 + 16) 255 s_v``: 2^-15 to 2^-12 of a code's step."""
     d = q.shape[2]
     scale = 1 / np.sqrt(d) if scale is None else scale
     out, lse, spread, slack = c.attention(q, blocks, pos, seq, tab, scale)
     u, w = UNIT[c.kind], max(UNIT[c.kind], 2.0**-11)
     off = (d + 16) * 2.0**-24 * slack + 2.0**-17
+    off += 2.0**-24 * (d / 32 + 8) * 255 * c.ks.max() * abs(scale) * np.abs(q.astype(np.float64)).sum(-1)
     most = max(np.abs(c.v * c.vs[..., None, None]).max(initial=0), np.abs(np.nan_to_num(c.vt)).max())
-    least = 2.0**-32 * c.page * blocks.shape[2] * most
+    keys = c.page * blocks.shape[2]
+    least = 2.0**-32 * keys * most + 2.0**-24 * (keys / 32 + 16) * 255 * c.vs.max()
     tol = u * np.abs(out) + (w + 2 * off[..., None]) * spread * (1 + u) + least + 2.0**-25
     bad = ~(np.abs(got[0] - out) <= tol)
     assert not bad.any(), (np.argwhere(bad)[:5], got[0][bad][:5], out[bad][:5], tol[bad][:5])
