@@ -155,6 +155,20 @@ __device__ inline int value_offset(int channel, int sub) {
   }
 }
 
+// The largest of 16 numbers (NaN passed over) in 8 instructions; fmaxf would first quiet each, which
+// costs as many again. For results that have settled.
+__device__ inline float max3(float a, float b, float c) {
+  float x;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(x) : "v"(a), "v"(b), "v"(c));
+  return x;
+}
+__device__ inline float most_of(const v4f (&x)[4]) {
+  const float a = max3(x[0][0], x[0][1], x[0][2]), b = max3(x[0][3], x[1][0], x[1][1]);
+  const float c = max3(x[1][2], x[1][3], x[2][0]), d = max3(x[2][1], x[2][2], x[2][3]);
+  const float e = max3(x[3][0], x[3][1], x[3][2]);
+  return max3(max3(a, b, c), max3(d, e, x[3][3]), a);
+}
+
 // What a lane knows of its subtile (16 slots), 64 of them being looked up at a time.
 struct Subtile {
   int32_t page, at;  // physical page; first slot * 32 + keys (0: none)
@@ -207,7 +221,7 @@ struct Int8Wave {
   // and values.
   static constexpr bool kQueriesInLds = CT > 1;
   v8h qf[kQueriesInLds ? 1 : KS];
-  v8h* q_lds;  // [CT][KS][64]
+  const v8h* q_lds;  // [CT][KS][64]
   float factor[CT];  // what a score is multiplied by besides its block's scale
   float start[CT];   // -128 sum(q), in units of kCodeUnit
   bool odd[CT];      // the column's query is not finite
@@ -229,7 +243,8 @@ struct Int8Wave {
     return s < 2 * KL ? 64 * (s >> 1) + 16 * grp + 8 * (s & 1) : 64 * KL + 8 * grp;
   }
   // This lane's column of tile c is query head `head` of token t (zeros where it is not `real`).
-  __device__ void load_q(const AttendInt8Args& a, int c, int64_t t, int64_t head, bool real) {
+  __device__ void load_q(const AttendInt8Args& a, int c, int64_t t, int64_t head, bool real,
+                         v8h* lds = nullptr) {
     const int grp = lane_id() >> 4;
     const E* q = static_cast<const E*>(a.q) + (real ? t * a.q_st + head * a.q_sh : 0);
     V8 x[KS];
@@ -266,7 +281,7 @@ struct Int8Wave {
         sum += static_cast<float>(y[e]);
       }
       if constexpr (kQueriesInLds) {
-        q_lds[(c * KS + s) * kWave + lane_id()] = y;
+        lds[(c * KS + s) * kWave + lane_id()] = y;
       } else {
         qf[s] = y;
       }
@@ -380,12 +395,7 @@ struct Int8Wave {
     }
     f = fmaxf(f, 1.17549435e-38f);  // (a score of -inf stays that)
     if (!counts) lift = -INFINITY;
-    float top[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      top[j] = fmaxf(fmaxf(sc[j][0], sc[j][1]), fmaxf(sc[j][2], sc[j][3]));
-    }
-    const float high = fmaf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), f, lift);
+    const float high = fmaf(most_of(sc), f, lift);
     if (__any(high - m[c] > 8.0f + kLift)) {
       float next = fmaxf(high, __shfl_xor(high, 16));
       next = fmaxf(next, __shfl_xor(next, 32));
@@ -745,6 +755,7 @@ struct JoinInt8Lds {
   uint32_t list_who[kJoinEntries];
   int32_t counts[kAttendWaves];
   float ml[kAttendWaves][16][2];
+  float column[CT][16][3];  // factor, start, odd
 };
 
 // The pages of tokens t0 .. t0 + tokens - 1: how many.
@@ -843,9 +854,27 @@ __global__ void __launch_bounds__(kAttendWaves* kWave, D <= 128 ? 2 : 1)
     const KvPlace p = kv_place(a.tok, t0 + tok[c]);
     own[c] = real[c] && p.last >= 0 ? kv_page(a.tok, p, p.last) : -1;
     own_keys[c] = (p.pos & ((1 << SHIFT) - 1)) + 1;
-    w.load_q(a, c, t0 + tok[c], head * a.G + col % a.G, real[c]);  // (every wave writes the same)
+    if constexpr (CT == 1) w.load_q(a, c, t0 + tok[c], head * a.G + col % a.G, real[c]);
   }
-  __syncthreads();
+  if constexpr (CT > 1) {  // a wave a tile, for all
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+      if (wave != c) continue;
+      w.load_q(a, c, t0 + tok[c], head * a.G + col % a.G, real[c], lds.q);
+      if (grp == 0) {
+        lds.column[c][col][0] = w.factor[c];
+        lds.column[c][col][1] = w.start[c];
+        lds.column[c][col][2] = w.odd[c] ? 1.0f : 0.0f;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+      w.factor[c] = lds.column[c][col][0];
+      w.start[c] = lds.column[c][col][1];
+      w.odd[c] = lds.column[c][col][2] != 0.0f;
+    }
+  }
   constexpr int PER = 1 << (SHIFT - 4);  // subtiles of a page
   // Chunks of 16 steps, the waves in turn: lane l has subtile l % 4 of this wave's step l / 4.
   const int steps = (listed * PER + 3) / 4;
