@@ -143,68 +143,83 @@ __device__ inline float group_max(float x, float* scratch) {
 template <class E, int D, int MODE, bool NORM, bool VALUES>
 struct Fill {
   using V8 = typename Kv<E>::V8;
-  // a row's chunks of 8 channels lie on neighbouring lanes of one wave
-  static constexpr int C = D / 8, WAVE_ROWS = kWave / C, ROWS = kWriteWaves * WAVE_ROWS;
+  using Row = Pair<E, D, MODE, NORM && !VALUES>;
+  // a row's chunks of 8 channels, two a lane, lie on neighbouring lanes of one wave
+  static constexpr int C = D / 16, WAVE_ROWS = kWave / C, ROWS = kWriteWaves * WAVE_ROWS;
+  // rows in flight a lane (a key's cosines and sines take 16 to 64 registers)
+  static constexpr int FLIGHT = VALUES ? 4 : MODE == kRotHalf ? 2 : 1;
   const WriteArgs& a;
   char* lds;       // the block's rows; then the channels' least and largest keys
   float* scratch;  // a float a wave
-  int head, chunk, row;  // this thread's (row: ROWS where it has none)
-  Weights<E> w;
+  uint64_t* masks;
+  int head, row;   // this thread's (row: ROWS where it has none)
+  Row pair;
 
-  __device__ Fill(const WriteArgs& args, int h, char* shared, float* waves)
-      : a(args), lds(shared), scratch(waves), head(h) {
-    chunk = lane_id() % C;
+  __device__ Fill(const WriteArgs& args, int h, char* shared, float* waves, uint64_t* m)
+      : a(args), lds(shared), scratch(waves), masks(m), head(h), pair(args, lane_id() % C) {
     row = lane_id() / C < WAVE_ROWS
               ? static_cast<int>(threadIdx.x / kWave) * WAVE_ROWS + lane_id() / C
               : ROWS;
-    if (NORM && !VALUES) w.load(a.norm[1], chunk);
+    if (!VALUES) pair.load_weights(a, NORM ? 1 : 0);
   }
-  // This thread's chunk of token `at`, whose position is `pos`.
-  __device__ V8 fresh(int64_t at, int32_t pos) const {
-    const E* from = VALUES ? static_cast<const E*>(a.v) + head * a.v_sh + at * a.v_st
-                           : static_cast<const E*>(a.k) + head * a.k_sh + at * a.k_st;
-    const V8 own[1] = {reinterpret_cast<const V8*>(from)[chunk]};
-    if constexpr (VALUES) {
-      return own[0];
-    } else {
-      Turn<MODE> turn;
-      if (a.rot > 0) turn.load(a, pos, chunk);
-      float r = 1.0f;
-      if (NORM && a.norm[1].weight) r = row_scale<E, D, C>(own, chunk, a.eps);
-      return turned_chunk<E, MODE, NORM>(from, own[0], chunk, turn, a, a.norm[1], r, w);
+  __device__ const E* source(int64_t at) const {
+    return VALUES ? static_cast<const E*>(a.v) + head * a.v_sh + at * a.v_st
+                  : static_cast<const E*>(a.k) + head * a.k_sh + at * a.k_st;
+  }
+  // This thread's chunks of a token of this call: read, then turned.
+  __device__ void read(int64_t at, int32_t pos, Row& p, V8 (&x)[2]) const {
+    const E* from = source(at);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      x[i] = __builtin_nontemporal_load(reinterpret_cast<const V8*>(from) + pair.chunk[i]);
+    }
+    if constexpr (!VALUES) p.load_turn(a, pos);
+  }
+  __device__ void turn(int64_t at, const Row& p, V8 (&x)[2]) const {
+    if constexpr (!VALUES) {
+      if (NORM || a.rot > 0) p.apply(source(at), a, 1, x);
     }
   }
   __device__ int64_t block(int64_t of) const { return (of * a.Hkv + head) << a.tok.shift; }
-  // The same of a slot that holds an earlier token, from the codes (scale above 0) or the open block.
-  __device__ V8 held(int32_t page, int32_t seq, int slot, float scale) const {
+  // Earlier tokens, from the codes (scale above 0) or the open block: f(slot, channel, eight numbers)
+  // for eight channels of a slot of keys, eight slots of a channel of values; slots whose `skip(slot)`
+  // is all true are left out.
+  template <class S, class F>
+  __device__ void held(int32_t page, int32_t seq, float scale, S&& skip, F&& f) const {
     const int64_t full = block(page) * D, open = block(seq) * D;
-    V8 x;
-    if constexpr (VALUES) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int at = ((8 * chunk + e) << a.tok.shift) + slot;
-        x[e] = scale > 0.0f ? static_cast<E>(a.cache.v_codes[full + at] * scale)
-                            : static_cast<const E*>(a.cache.v_tail)[open + at];
-      }
-    } else {
-      const int at = slot * D + 8 * chunk;
+    const int size = 1 << a.tok.shift, line = VALUES ? size / 8 : D / 8;
+    const int8_t* codes = VALUES ? a.cache.v_codes : a.cache.k_codes;
+    const E* tail = static_cast<const E*>(VALUES ? a.cache.v_tail : a.cache.k_tail);
+#pragma unroll 1
+    for (int i = threadIdx.x; i < size * D / 8; i += kWriteThreads) {
+      const int slot = VALUES ? i % line * 8 : i / line, d = VALUES ? i / line : i % line * 8;
+      if (skip(slot)) continue;
+      V8 x;
       if (scale > 0.0f) {
+        typedef int V2i __attribute__((ext_vector_type(2)));
+        const V2i c = *reinterpret_cast<const V2i*>(codes + full + 8 * i);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = static_cast<E>(a.cache.k_codes[full + at + e] * scale);
+        for (int e = 0; e < 8; ++e) {
+          x[e] = static_cast<E>(static_cast<int8_t>(c[e >> 2] >> (8 * (e & 3))) * scale);
+        }
       } else {
-        x = *reinterpret_cast<const V8*>(static_cast<const E*>(a.cache.k_tail) + open + at);
+        x = *reinterpret_cast<const V8*>(tail + open + 8 * i);
       }
+      f(slot, d, x);
     }
-    return x;
   }
-  __device__ void to_open(int32_t seq, int slot, V8 x) const {
+  __device__ void to_open(int32_t seq, int slot, const V8 (&x)[2]) const {
     const int64_t open = block(seq) * D;
-    if constexpr (VALUES) {
-      E* to = static_cast<E*>(a.cache.v_tail) + open + slot;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) to[(8 * chunk + e) << a.tok.shift] = x[e];
-    } else {
-      *reinterpret_cast<V8*>(static_cast<E*>(a.cache.k_tail) + open + slot * D + 8 * chunk) = x;
+    for (int i = 0; i < 2; ++i) {
+      if constexpr (VALUES) {
+        E* to = static_cast<E*>(a.cache.v_tail) + open + slot;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) to[(8 * pair.chunk[i] + e) << a.tok.shift] = x[i][e];
+      } else {
+        E* to = static_cast<E*>(a.cache.k_tail) + open + slot * D;
+        reinterpret_cast<V8*>(to)[pair.chunk[i]] = x[i];
+      }
     }
   }
   __device__ float* scale_of(int32_t page) const {
@@ -214,48 +229,28 @@ struct Fill {
 
   // A block that had been full and is begun again behind slot `from`: its earlier rows in 16 bits.
   __device__ void reopen(int32_t page, int32_t seq, int from) const {
-    const float scale = *scale_of(page);
-    if (row < ROWS) {
-      for (int o = row; o < from; o += ROWS) to_open(seq, o, held(page, seq, o, scale));
-    }
+    E* to = static_cast<E*>(VALUES ? a.cache.v_tail : a.cache.k_tail) + block(seq) * D;
+    held(page, seq, *scale_of(page), [&](int slot) { return slot >= from; },
+         [&](int slot, int d, const V8& x) {
+      if constexpr (VALUES) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (slot + e < from) to[(d << a.tok.shift) + slot + e] = x[e];
+        }
+      } else {
+        *reinterpret_cast<V8*>(to + slot * D + d) = x;
+      }
+    });
     __syncthreads();  // (everyone has read the scale)
     if (threadIdx.x == 0) *scale_of(page) = 0.0f;
     __syncthreads();
   }
 
-  // The block that token t completes.
-  __device__ void fill(int64_t t) const {
-    const KvPlace p = kv_place(a.tok, t);
-    const int32_t page = kv_page(a.tok, p, p.last), seq = a.tok.seq_ids[t];
+  // The rows in LDS as codes.
+  template <bool ODD>
+  __device__ void encode(const BlockCode& code, int32_t page) const {
     const int size = 1 << a.tok.shift;
-    const float old = *scale_of(page);
-    float most = 0.0f, lo[8], hi[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      lo[e] = INFINITY;
-      hi[e] = -INFINITY;
-    }
-    if (row < ROWS) {
-      for (int o = row; o < size; o += ROWS) {
-        const int64_t from = t - (size - 1 - o);
-        const int32_t pos = p.pos - (size - 1 - o);
-        const bool here = from >= 0 && a.tok.positions[from] == pos && a.tok.seq_ids[from] == seq;
-        const V8 x = here ? fresh(from, pos) : held(page, seq, o, old);
-        *reinterpret_cast<V8*>(lds + (o * D + 8 * chunk) * 2) = x;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float f = static_cast<float>(x[e]);
-          most = fmaxf(most, finite_size(f));
-          if (!VALUES) {
-            lo[e] = fminf(lo[e], f);
-            hi[e] = fmaxf(hi[e], f);
-          }
-        }
-      }
-    }
-    most = fmaxf(group_max(most, scratch), kKvTopFloor);  // (its barriers: the rows are there)
-    const BlockCode code(most);
-    if (threadIdx.x == 0) *scale_of(page) = most / 127.0f;
+    typedef E V2 __attribute__((ext_vector_type(2)));
     if constexpr (VALUES) {
       int8_t* to = a.cache.v_codes + block(page) * D;
       // two channels and 16 slots a thread
@@ -264,39 +259,127 @@ struct Fill {
         v4i out[2];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          uint32_t word[2] = {0u, 0u};
+          V2 x[4];
 #pragma unroll
           for (int b = 0; b < 4; ++b) {
-            typedef E V2 __attribute__((ext_vector_type(2)));
-            const V2 x = *reinterpret_cast<const V2*>(lds + ((s + 4 * j + b) * D + 2 * c) * 2);
-            word[0] |= (static_cast<uint32_t>(code(static_cast<float>(x[0]))) & 255u) << (8 * b);
-            word[1] |= (static_cast<uint32_t>(code(static_cast<float>(x[1]))) & 255u) << (8 * b);
+            x[b] = *reinterpret_cast<const V2*>(lds + ((s + 4 * j + b) * D + 2 * c) * 2);
           }
-          out[0][j] = static_cast<int>(word[0]);
-          out[1][j] = static_cast<int>(word[1]);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            out[h][j] = code.template four<ODD>(
+                static_cast<float>(x[0][h]), static_cast<float>(x[1][h]),
+                static_cast<float>(x[2][h]), static_cast<float>(x[3][h]));
+          }
         }
         *reinterpret_cast<v4i*>(to + (2 * c << a.tok.shift) + s) = out[0];
         *reinterpret_cast<v4i*>(to + ((2 * c + 1) << a.tok.shift) + s) = out[1];
       }
     } else {
-      typedef int V2i __attribute__((ext_vector_type(2)));
-      if (row < ROWS) {
-        for (int o = row; o < size; o += ROWS) {
-          const V8 x = *reinterpret_cast<const V8*>(lds + (o * D + 8 * chunk) * 2);
-          uint32_t word[2] = {0u, 0u};
+      v4i* to = reinterpret_cast<v4i*>(a.cache.k_codes + block(page) * D);
+      for (int i = threadIdx.x; i < size * D / 16; i += kWriteThreads) {
+        v4i out;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            word[e >> 2] |= (static_cast<uint32_t>(code(static_cast<float>(x[e]))) & 255u)
-                            << (8 * (e & 3));
+        for (int h = 0; h < 2; ++h) {
+          const V8 x = *reinterpret_cast<const V8*>(lds + (2 * i + h) * 16);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            out[2 * h + j] = code.template four<ODD>(
+                static_cast<float>(x[4 * j]), static_cast<float>(x[4 * j + 1]),
+                static_cast<float>(x[4 * j + 2]), static_cast<float>(x[4 * j + 3]));
           }
-          *reinterpret_cast<V2i*>(a.cache.k_codes + (block(page) + o) * D + 8 * chunk) =
-              V2i{static_cast<int>(word[0]), static_cast<int>(word[1])};
+        }
+        to[i] = out;
+      }
+    }
+  }
+
+  // The block that token t completes.
+  __device__ void fill(int64_t t) const {
+    const KvPlace p = kv_place(a.tok, t);
+    const int32_t page = kv_page(a.tok, p, p.last), seq = a.tok.seq_ids[t];
+    const int size = 1 << a.tok.shift;
+    const float old = *scale_of(page);
+    // which slots hold tokens of this call: a thread a slot
+    {
+      const int o = threadIdx.x;
+      const int64_t from = t - (size - 1 - o);
+      const bool here = o < size && from >= 0 && a.tok.positions[from] == p.pos - (size - 1 - o) &&
+                        a.tok.seq_ids[from] == seq;
+      const uint64_t m = __ballot(here);
+      if (lane_id() == 0 && threadIdx.x < 2 * kWave) masks[2 + threadIdx.x / kWave] = m;
+    }
+    __syncthreads();
+    const uint64_t now[2] = {masks[2], masks[3]};
+    float most = 0.0f, none = 0.0f;
+    const auto see = [&](E x) {
+      const float f = static_cast<float>(x);
+      most = fmaxf(most, finite_size(f));
+      none = fmaf(f, 0.0f, none);  // (not a number beside one that is not finite)
+    };
+    const auto is_here = [&](int o) {
+      return ((o < kWave ? now[0] >> o : now[1] >> (o - kWave)) & 1) != 0;
+    };
+    if (row < ROWS) {
+      for (int o0 = row; o0 < size; o0 += FLIGHT * ROWS) {
+        V8 x[FLIGHT][2];
+        Row turned[FLIGHT];
+        bool here[FLIGHT];
+#pragma unroll
+        for (int i = 0; i < FLIGHT; ++i) {
+          const int o = o0 + i * ROWS;
+          here[i] = o < size && is_here(o);
+          turned[i] = pair;
+          if (here[i]) read(t - (size - 1 - o), p.pos - (size - 1 - o), turned[i], x[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < FLIGHT; ++i) {
+          const int o = o0 + i * ROWS;
+          if (!here[i]) continue;
+          turn(t - (size - 1 - o), turned[i], x[i]);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            *reinterpret_cast<V8*>(lds + (o * D + 8 * pair.chunk[j]) * 2) = x[i][j];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) see(x[i][j][e]);
+          }
         }
       }
-      __syncthreads();  // (the rows have been read)
-      bounds(page, lo, hi);
     }
-    // The first block of a run that ends in an open one: that one's rows, which are not moved (the
+    if (!is_here(0)) {  // (this call's are the last ones)
+      held(page, seq, old,
+           [&](int slot) {
+             bool all = is_here(slot);
+             if constexpr (VALUES) {
+               for (int e = 1; e < 8; ++e) all = all && is_here(slot + e);
+             }
+             return all;
+           },
+           [&](int slot, int d, const V8& x) {
+        if constexpr (VALUES) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            if (is_here(slot + e)) continue;
+            *reinterpret_cast<E*>(lds + ((slot + e) * D + d) * 2) = x[e];
+            see(x[e]);
+          }
+        } else {
+          *reinterpret_cast<V8*>(lds + (slot * D + d) * 2) = x;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) see(x[e]);
+        }
+      });
+    }
+    const bool odd = group_max(none == 0.0f ? 0.0f : 1.0f, scratch) > 0.0f;
+    most = fmaxf(group_max(most, scratch), kKvTopFloor);  // (its barriers: the rows are there)
+    const BlockCode code(most, odd);
+    if (threadIdx.x == 0) *scale_of(page) = most / 127.0f;
+    if (code.odd) {
+      encode<true>(code, page);
+    } else {
+      encode<false>(code, page);
+    }
+    if constexpr (!VALUES) bounds(page);
+  // The first block of a run that ends in an open one: that one's rows, which are not moved (the
     // open block has been read now).
     if (!is_token(a, t - size, seq, static_cast<int64_t>(p.pos) - size)) {
       int64_t full = 0;  // blocks behind this one that are completed as well
@@ -318,22 +401,42 @@ struct Fill {
       if (row < ROWS) {
         for (int o = row; o < size - 1; o += ROWS) {
           if (!is_token(a, first + o, seq, static_cast<int64_t>(pos) + o)) break;
-          to_open(seq, o, fresh(first + o, pos + o));
+          V8 x[2];
+          Row turned = pair;
+          read(first + o, pos + o, turned, x);
+          turn(first + o, turned, x);
+          to_open(seq, o, x);
         }
       }
     }
     __syncthreads();
   }
 
-  // The bounds of a block from its channels' least and largest keys, a chunk a thread.
-  __device__ void bounds(int32_t page, const float (&lo)[8], const float (&hi)[8]) const {
-    float(*lows)[D] = reinterpret_cast<float(*)[D]>(lds);
-    float(*highs)[D] = lows + ROWS;
-    if (row < ROWS) {
+  // The bounds of a block from its rows in LDS: two channels and a share of the slots a thread.
+  __device__ void bounds(int32_t page) const {
+    constexpr int PAIRS = D / 2, GROUPS = kWriteThreads / PAIRS;
+    typedef E V2 __attribute__((ext_vector_type(2)));
+    const int size = 1 << a.tok.shift, c = threadIdx.x % PAIRS, g = threadIdx.x / PAIRS;
+    float lo[2] = {INFINITY, INFINITY}, hi[2] = {-INFINITY, -INFINITY};
+    if (g < GROUPS) {
+#pragma unroll 4
+      for (int o = g; o < size; o += GROUPS) {
+        const V2 x = *reinterpret_cast<const V2*>(lds + (o * D + 2 * c) * 2);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        lows[row][8 * chunk + e] = lo[e];
-        highs[row][8 * chunk + e] = hi[e];
+        for (int h = 0; h < 2; ++h) {
+          lo[h] = fminf(lo[h], static_cast<float>(x[h]));
+          hi[h] = fmaxf(hi[h], static_cast<float>(x[h]));
+        }
+      }
+    }
+    __syncthreads();  // (the rows have been read)
+    float(*lows)[D] = reinterpret_cast<float(*)[D]>(lds);
+    float(*highs)[D] = lows + GROUPS;
+    if (g < GROUPS) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        lows[g][2 * c + h] = lo[h];
+        highs[g][2 * c + h] = hi[h];
       }
     }
     __syncthreads();
@@ -341,7 +444,7 @@ struct Fill {
     float mid = 0.0f, half = 0.0f;
     if (d < D) {
       float l = lows[0][d], h = highs[0][d];
-      for (int i = 1; i < ROWS; ++i) {
+      for (int i = 1; i < GROUPS; ++i) {
         l = fminf(l, lows[i][d]);
         h = fmaxf(h, highs[i][d]);
       }
@@ -357,7 +460,7 @@ struct Fill {
     if (d == 0) a.bound_scales[at] = top / 127.0f;
   }
 
-  __device__ void run(int64_t t0, uint64_t* masks) {
+  __device__ void run(int64_t t0) {
     const int size = 1 << a.tok.shift;
     if (threadIdx.x < kWave) {  // one token a lane
       const int64_t mine = t0 + lane_id();
@@ -396,18 +499,24 @@ struct Fill {
   }
 };
 
+// Workgroups a CU that the registers leave room for.
+constexpr int write_groups(int mode, bool norm) {
+  return mode == kRotHalfOdd ? 2 : norm ? 3 : 4;
+}
+
 template <class E, int D, int MODE, bool NORM>
-__global__ void __launch_bounds__(kWriteThreads) kv_append_int8_kernel(WriteArgs a) {
+__global__ void __launch_bounds__(kWriteThreads, write_groups(MODE, NORM))
+    kv_append_int8_kernel(WriteArgs a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   __shared__ float scratch[kWriteWaves];
-  __shared__ uint64_t masks[2];
+  __shared__ uint64_t masks[4];  // tokens that complete a block, that open one again; slots
   if (blockIdx.x < a.fill_groups) {
     const int job = static_cast<int>(blockIdx.x % (2 * a.Hkv));
     const int64_t t0 = static_cast<int64_t>(blockIdx.x / (2 * a.Hkv)) * a.tile;
     if (job < a.Hkv) {
-      Fill<E, D, MODE, NORM, false>(a, job, lds, scratch).run(t0, masks);
+      Fill<E, D, MODE, NORM, false>(a, job, lds, scratch, masks).run(t0);
     } else {
-      Fill<E, D, MODE, NORM, true>(a, job - a.Hkv, lds, scratch).run(t0, masks);
+      Fill<E, D, MODE, NORM, true>(a, job - a.Hkv, lds, scratch, masks).run(t0);
     }
   } else {
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
@@ -466,8 +575,8 @@ extern "C" int rt_kv_append_int8(
   const int64_t grid = fill_groups + cdiv(T * a.row_parts, kWriteWaves);
   RT_CHECK_ARG(grid <= INT32_MAX, "too many tokens");
   a.fill_groups = static_cast<uint32_t>(fill_groups);
-  // a block's rows; the least and largest keys of a channel (two floats a thread's 8 channels)
-  const int64_t rows = page * D * 2, ends = kWriteThreads * 8 * 2 * 4;
+  // a block's rows; the channels' least and largest keys (four floats a thread)
+  const int64_t rows = page * D * 2, ends = kWriteThreads * 4 * 4;
   const unsigned lds = static_cast<unsigned>(rows > ends ? rows : ends);
   return kv_dispatch(dtype, D, [&](auto e, auto d) -> int {
     using E = decltype(e);

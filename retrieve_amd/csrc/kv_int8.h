@@ -21,21 +21,35 @@ struct KvInt8 {
 // Codes of one block: code = 127 x / top to the nearest even, top its largest finite magnitude
 // (floored at kKvTopFloor). 127 x is exact (18 bits at most), and q + r (y - q top) with q = y r is
 // the quotient of y = 127 x rounded to nearest (kv_code_value's comment), so a tie between two codes
-// is seen as one. Infinities become +-127, NaN 0. A top above 2^100, whose reciprocal may lose bits,
+// is seen as one. Adding 1.5 2^23 rounds it to a whole number, whose byte is the last one of the sum.
+// `odd` blocks: infinities become +-127, NaN 0; a top above 2^100, whose reciprocal may lose bits,
 // comes in scaled by 2^-64 with its numbers.
 struct BlockCode {
   float top, r, shrink;
-  __device__ explicit BlockCode(float most) {
+  bool odd;
+  __device__ BlockCode(float most, bool not_finite) {
+    odd = not_finite || most > 0x1p100f;
     shrink = most > 0x1p100f ? 0x1p-64f : 1.0f;
     top = most * shrink;
     r = 1.0f / top;
   }
-  __device__ int operator()(float x) const {
+  template <bool ODD>
+  __device__ uint32_t word(float x) const {  // the code is its last byte
 #pragma clang fp contract(off)
-    const float y = fminf(fmaxf(x * shrink, -top), top) * 127.0f;
+    float y = x * 127.0f;
+    if constexpr (ODD) {
+      y = fminf(fmaxf(x * shrink, -top), top) * 127.0f;
+      y = x == x ? y : 0.0f;
+    }
     const float q = y * r;
-    const float v = rintf(__builtin_fmaf(__builtin_fmaf(-q, top, y), r, q));
-    return x == x ? static_cast<int>(v) : 0;
+    return __builtin_bit_cast(uint32_t,
+                              __builtin_fmaf(__builtin_fmaf(-q, top, y), r, q) + 12582912.0f);
+  }
+  template <bool ODD>
+  __device__ int four(float a, float b, float c, float d) const {
+    const uint32_t ab = __builtin_amdgcn_perm(word<ODD>(b), word<ODD>(a), 0x0c0c0400u);
+    const uint32_t cd = __builtin_amdgcn_perm(word<ODD>(d), word<ODD>(c), 0x0c0c0400u);
+    return static_cast<int>(ab | cd << 16);
   }
 };
 // A number's part in `top`.

@@ -44,17 +44,21 @@ __device__ inline float rot_second(float b, float a, float c, float s) {
   return b * c + a * s;
 }
 
-// The cosines and sines of chunk `c`'s channels at a position (1, 0 past the rotated part).
+// The cosines and sines of a chunk's channels at a position (1, 0 past the rotated part); neighbours
+// that turn together share theirs.
 template <int MODE>
 struct Turn {
-  float c[8], s[8];
+  static constexpr int N = MODE == kRotPairs ? 4 : 8;
+  float c[N], s[N];
+  __device__ float cos(int e) const { return c[MODE == kRotPairs ? e >> 1 : e]; }
+  __device__ float sin(int e) const { return s[MODE == kRotPairs ? e >> 1 : e]; }
   __device__ void load(const TurnArgs& a, int32_t pos, int chunk) {
     const int half = a.rot >> 1;
     const float* row = a.cos_sin + static_cast<int64_t>(pos) * a.rot;
-    if (MODE == kRotHalf && 8 * chunk < a.rot) {
-      const int j = 8 * chunk < half ? 8 * chunk : 8 * chunk - half;
+    if ((MODE == kRotHalf || (MODE == kRotPairs && a.rot % 8 == 0)) && 8 * chunk < a.rot) {
+      const int j = MODE == kRotPairs ? 4 * chunk : 8 * chunk < half ? 8 * chunk : 8 * chunk - half;
 #pragma unroll
-      for (int e = 0; e < 8; e += 4) {
+      for (int e = 0; e < N; e += 4) {
         const v4f cv = *reinterpret_cast<const v4f*>(row + j + e);
         const v4f sv = *reinterpret_cast<const v4f*>(row + half + j + e);
 #pragma unroll
@@ -65,19 +69,9 @@ struct Turn {
       }
       return;
     }
-    if (MODE == kRotPairs && a.rot % 8 == 0 && 8 * chunk < a.rot) {
-      const v4f cv = *reinterpret_cast<const v4f*>(row + 4 * chunk);
-      const v4f sv = *reinterpret_cast<const v4f*>(row + half + 4 * chunk);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        c[e] = cv[e >> 1];
-        s[e] = sv[e >> 1];
-      }
-      return;
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int i = 8 * chunk + e;
+    for (int e = 0; e < N; ++e) {
+      const int i = MODE == kRotPairs ? 8 * chunk + 2 * e : 8 * chunk + e;
       const int j = MODE == kRotPairs ? i >> 1 : i < half ? i : i - half;
       c[e] = i < a.rot ? row[j] : 1.0f;
       s[e] = i < a.rot ? row[half + j] : 0.0f;
@@ -181,8 +175,8 @@ __device__ inline typename Kv<E>::V8 turned_chunk(const E* row, typename Kv<E>::
   for (int e = 0; e < 8; ++e) {
     const int i = 8 * chunk + e;
     const bool first = MODE == kRotPairs ? (i & 1) == 0 : i < half;
-    const float z = first ? rot_first(own[e], other[e], t.c[e], t.s[e])
-                          : rot_second(own[e], other[e], t.c[e], t.s[e]);
+    const float z = first ? rot_first(own[e], other[e], t.cos(e), t.sin(e))
+                          : rot_second(own[e], other[e], t.cos(e), t.sin(e));
     out[e] = i < a.rot ? static_cast<E>(z) : NORM ? static_cast<E>(own[e]) : x[e];
   }
   return out;
@@ -200,6 +194,7 @@ struct Pair {
   bool turned;  // split halves: in the rotated part
   Weights<E> weights[NORM ? 2 : 1][2];  // of queries, of keys
 
+  Pair() = default;
   __device__ Pair(const TurnArgs& a, int lane) {
     const int r = a.rot / 16;
     part = lane;
@@ -213,16 +208,20 @@ struct Pair {
     }
   }
   __device__ void load(const TurnArgs& a, int32_t pos) {
+    load_turn(a, pos);
+    load_weights(a, 0);
+    load_weights(a, 1);
+  }
+  __device__ void load_turn(const TurnArgs& a, int32_t pos) {
     if (a.rot > 0) {
       turn[0].load(a, pos, chunk[0]);
       if constexpr (MODE != kRotHalf) turn[1].load(a, pos, chunk[1]);
     }
+  }
+  __device__ void load_weights(const TurnArgs& a, int kind) {
     if constexpr (NORM) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) weights[i][j].load(a.norm[i], chunk[j]);
-      }
+      for (int j = 0; j < 2; ++j) weights[kind][j].load(a.norm[kind], chunk[j]);
     }
   }
   // x: the two chunks as read, of a query (kind 0) or a key (1); `row` for partners elsewhere
