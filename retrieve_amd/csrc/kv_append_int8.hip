@@ -8,8 +8,8 @@
 // of kv_append.hip.
 //
 // One launch, no workgroup waits for another. Workgroups at the grid's head look at a tile of tokens
-// for one head's keys or values and do the blocks completed there: rows to LDS once, their largest
-// magnitude, then codes (values transposed on the way out). In the others a wave moves a token's
+// for one head's keys or values and do the blocks completed there: rows in registers, their largest
+// magnitude, then codes (values transposed through LDS). In the others a wave moves a token's
 // queries, and its key and value rows to the open block. The open block is read (the first block
 // that a call completes) and written (the rows behind the last one) in the same call: a run of
 // tokens that begins in one block and ends in a later, open one has these rows written by the
@@ -139,6 +139,11 @@ __device__ inline float group_max(float x, float* scratch) {
   return x;
 }
 
+// The same of a whole number up to 2^16.
+__device__ inline int group_max(int x, float* scratch) {
+  return static_cast<int>(group_max(static_cast<float>(x), scratch));
+}
+
 // One head's keys (VALUES: values) of a tile of tokens.
 template <class E, int D, int MODE, bool NORM, bool VALUES>
 struct Fill {
@@ -146,10 +151,9 @@ struct Fill {
   using Row = Pair<E, D, MODE, NORM && !VALUES>;
   // a row's chunks of 8 channels, two a lane, lie on neighbouring lanes of one wave
   static constexpr int C = D / 16, WAVE_ROWS = kWave / C, ROWS = kWriteWaves * WAVE_ROWS;
-  // rows in flight a lane (a key's cosines and sines take 16 to 64 registers)
-  static constexpr int FLIGHT = VALUES ? 4 : MODE == kRotHalf ? 2 : 1;
+  static constexpr int ALL = (128 + ROWS - 1) / ROWS;  // rows a lane of the largest block
   const WriteArgs& a;
-  char* lds;       // the block's rows; then the channels' least and largest keys
+  char* lds;       // the lanes' least and largest keys; the values' codes
   float* scratch;  // a float a wave
   uint64_t* masks;
   int head, row;   // this thread's (row: ROWS where it has none)
@@ -166,48 +170,24 @@ struct Fill {
     return VALUES ? static_cast<const E*>(a.v) + head * a.v_sh + at * a.v_st
                   : static_cast<const E*>(a.k) + head * a.k_sh + at * a.k_st;
   }
-  // This thread's chunks of a token of this call: read, then turned.
-  __device__ void read(int64_t at, int32_t pos, Row& p, V8 (&x)[2]) const {
-    const E* from = source(at);
+  // This thread's chunks of a row.
+  __device__ void read(const E* from, V8 (&x)[2]) const {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       x[i] = __builtin_nontemporal_load(reinterpret_cast<const V8*>(from) + pair.chunk[i]);
     }
-    if constexpr (!VALUES) p.load_turn(a, pos);
   }
-  __device__ void turn(int64_t at, const Row& p, V8 (&x)[2]) const {
+  // The chunks of a token of this call turned.
+  __device__ void turn(int64_t at, int32_t pos, V8 (&x)[2]) const {
     if constexpr (!VALUES) {
-      if (NORM || a.rot > 0) p.apply(source(at), a, 1, x);
+      if (NORM || a.rot > 0) {
+        Row p = pair;
+        p.load_turn(a, pos);
+        p.apply(source(at), a, 1, x);
+      }
     }
   }
   __device__ int64_t block(int64_t of) const { return (of * a.Hkv + head) << a.tok.shift; }
-  // Earlier tokens, from the codes (scale above 0) or the open block: f(slot, channel, eight numbers)
-  // for eight channels of a slot of keys, eight slots of a channel of values; slots whose `skip(slot)`
-  // is all true are left out.
-  template <class S, class F>
-  __device__ void held(int32_t page, int32_t seq, float scale, S&& skip, F&& f) const {
-    const int64_t full = block(page) * D, open = block(seq) * D;
-    const int size = 1 << a.tok.shift, line = VALUES ? size / 8 : D / 8;
-    const int8_t* codes = VALUES ? a.cache.v_codes : a.cache.k_codes;
-    const E* tail = static_cast<const E*>(VALUES ? a.cache.v_tail : a.cache.k_tail);
-#pragma unroll 1
-    for (int i = threadIdx.x; i < size * D / 8; i += kWriteThreads) {
-      const int slot = VALUES ? i % line * 8 : i / line, d = VALUES ? i / line : i % line * 8;
-      if (skip(slot)) continue;
-      V8 x;
-      if (scale > 0.0f) {
-        typedef int V2i __attribute__((ext_vector_type(2)));
-        const V2i c = *reinterpret_cast<const V2i*>(codes + full + 8 * i);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          x[e] = static_cast<E>(static_cast<int8_t>(c[e >> 2] >> (8 * (e & 3))) * scale);
-        }
-      } else {
-        x = *reinterpret_cast<const V8*>(tail + open + 8 * i);
-      }
-      f(slot, d, x);
-    }
-  }
   __device__ void to_open(int32_t seq, int slot, const V8 (&x)[2]) const {
     const int64_t open = block(seq) * D;
 #pragma unroll
@@ -227,79 +207,126 @@ struct Fill {
            (static_cast<int64_t>(page) * a.Hkv + head);
   }
 
-  // A block that had been full and is begun again behind slot `from`: its earlier rows in 16 bits.
+  // A block that had been full and is gone on with behind slot `from`: its earlier rows in the open
+  // block, eight channels of a slot (values: eight slots of a channel) a thread.
   __device__ void reopen(int32_t page, int32_t seq, int from) const {
+    const float scale = *scale_of(page);
+    const int size = 1 << a.tok.shift, line = VALUES ? size / 8 : D / 8;
+    const int8_t* codes = (VALUES ? a.cache.v_codes : a.cache.k_codes) + block(page) * D;
     E* to = static_cast<E*>(VALUES ? a.cache.v_tail : a.cache.k_tail) + block(seq) * D;
-    held(page, seq, *scale_of(page), [&](int slot) { return slot >= from; },
-         [&](int slot, int d, const V8& x) {
-      if constexpr (VALUES) {
+    for (int i = threadIdx.x; i < size * D / 8; i += kWriteThreads) {
+      const int slot = VALUES ? i % line * 8 : i / line;
+      if (slot >= from) continue;
+      typedef int V2i __attribute__((ext_vector_type(2)));
+      const V2i c = *reinterpret_cast<const V2i*>(codes + 8 * i);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if (slot + e < from) to[(d << a.tok.shift) + slot + e] = x[e];
-        }
-      } else {
-        *reinterpret_cast<V8*>(to + slot * D + d) = x;
+      for (int e = 0; e < 8; ++e) {
+        if (VALUES && slot + e >= from) break;
+        to[8 * i + e] = static_cast<E>(static_cast<int8_t>(c[e >> 2] >> (8 * (e & 3))) * scale);
       }
-    });
+    }
     __syncthreads();  // (everyone has read the scale)
     if (threadIdx.x == 0) *scale_of(page) = 0.0f;
     __syncthreads();
   }
 
-  // The rows in LDS as codes.
+  // Rows as codes: keys to the cache, values to LDS, whence they go to the cache transposed.
   template <bool ODD>
-  __device__ void encode(const BlockCode& code, int32_t page) const {
-    const int size = 1 << a.tok.shift;
-    typedef E V2 __attribute__((ext_vector_type(2)));
-    if constexpr (VALUES) {
-      int8_t* to = a.cache.v_codes + block(page) * D;
-      // two channels and 16 slots a thread
-      for (int i = threadIdx.x; i < D / 2 * (size / 16); i += kWriteThreads) {
-        const int c = i % (D / 2), s = i / (D / 2) * 16;
-        v4i out[2];
+  __device__ void encode(const BlockCode& code, int32_t page, const V8 (&x)[ALL][2],
+                         const bool (&mine)[ALL]) const {
+    typedef int V2i __attribute__((ext_vector_type(2)));
+    char* to = VALUES ? lds : reinterpret_cast<char*>(a.cache.k_codes) + block(page) * D;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          V2 x[4];
+    for (int i = 0; i < ALL; ++i) {
+      if (!mine[i]) continue;
 #pragma unroll
-          for (int b = 0; b < 4; ++b) {
-            x[b] = *reinterpret_cast<const V2*>(lds + ((s + 4 * j + b) * D + 2 * c) * 2);
-          }
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            out[h][j] = code.template four<ODD>(
-                static_cast<float>(x[0][h]), static_cast<float>(x[1][h]),
-                static_cast<float>(x[2][h]), static_cast<float>(x[3][h]));
-          }
-        }
-        *reinterpret_cast<v4i*>(to + (2 * c << a.tok.shift) + s) = out[0];
-        *reinterpret_cast<v4i*>(to + ((2 * c + 1) << a.tok.shift) + s) = out[1];
-      }
-    } else {
-      v4i* to = reinterpret_cast<v4i*>(a.cache.k_codes + block(page) * D);
-      for (int i = threadIdx.x; i < size * D / 16; i += kWriteThreads) {
-        v4i out;
+      for (int j = 0; j < 2; ++j) {
+        V2i out;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const V8 x = *reinterpret_cast<const V8*>(lds + (2 * i + h) * 16);
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            out[2 * h + j] = code.template four<ODD>(
-                static_cast<float>(x[4 * j]), static_cast<float>(x[4 * j + 1]),
-                static_cast<float>(x[4 * j + 2]), static_cast<float>(x[4 * j + 3]));
-          }
+          out[h] = code.template four<ODD>(
+              static_cast<float>(x[i][j][4 * h]), static_cast<float>(x[i][j][4 * h + 1]),
+              static_cast<float>(x[i][j][4 * h + 2]), static_cast<float>(x[i][j][4 * h + 3]));
         }
-        to[i] = out;
+        *reinterpret_cast<V2i*>(to + (row + i * ROWS) * D + 8 * pair.chunk[j]) = out;
+      }
+    }
+  }
+  // Earlier values, eight slots of a channel a thread (they lie transposed): f(slot, channel, eight
+  // numbers).
+  template <class F>
+  __device__ void earlier_values(int32_t seq, int count, F&& f) const {
+    const int line = 1 << (a.tok.shift - 3);
+    const V8* from = reinterpret_cast<const V8*>(static_cast<const E*>(a.cache.v_tail) +
+                                                 block(seq) * D);
+    for (int i = threadIdx.x; i < line * D; i += kWriteThreads) {
+      if (i % line * 8 < count) f(i % line * 8, i / line, from[i]);
+    }
+  }
+  // The staged codes [slot][channel] to the cache: four channels of 16 slots a thread.
+  __device__ void transpose(int32_t page) const {
+    const int size = 1 << a.tok.shift;
+    int8_t* to = a.cache.v_codes + block(page) * D;
+    for (int i = threadIdx.x; i < D / 4 * (size / 16); i += kWriteThreads) {
+      const int c = i % (D / 4) * 4, s = i / (D / 4) * 16;
+      v4i out[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t x[4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          x[b] = *reinterpret_cast<const uint32_t*>(lds + (s + 4 * j + b) * D + c);
+        }
+        // bytes (slot, channel) 4 x 4 the other way round
+        const uint32_t p = __builtin_amdgcn_perm(x[1], x[0], 0x05010400u);
+        const uint32_t q = __builtin_amdgcn_perm(x[3], x[2], 0x05010400u);
+        const uint32_t r = __builtin_amdgcn_perm(x[1], x[0], 0x07030602u);
+        const uint32_t t = __builtin_amdgcn_perm(x[3], x[2], 0x07030602u);
+        out[0][j] = static_cast<int>(__builtin_amdgcn_perm(q, p, 0x05040100u));
+        out[1][j] = static_cast<int>(__builtin_amdgcn_perm(q, p, 0x07060302u));
+        out[2][j] = static_cast<int>(__builtin_amdgcn_perm(t, r, 0x05040100u));
+        out[3][j] = static_cast<int>(__builtin_amdgcn_perm(t, r, 0x07060302u));
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        *reinterpret_cast<v4i*>(to + ((c + k) << a.tok.shift) + s) = out[k];
       }
     }
   }
 
-  // The block that token t completes.
+  // The largest finite magnitude of a block that has others.
+  __device__ float finite_most(int32_t seq, int earlier, const V8 (&x)[ALL][2],
+                               const bool (&mine)[ALL]) const {
+    float most = 0.0f;
+#pragma unroll
+    for (int i = 0; i < ALL; ++i) {
+      if (!mine[i]) continue;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          most = fmaxf(most, finite_size(static_cast<float>(x[i][j][e])));
+        }
+      }
+    }
+    if constexpr (VALUES) {
+      earlier_values(seq, earlier, [&](int slot, int, V8 v) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (slot + e < earlier) most = fmaxf(most, finite_size(static_cast<float>(v[e])));
+        }
+      });
+    }
+    return most;
+  }
+
+  // The block that token t completes. Its rows stay in registers: their largest magnitude first, then
+  // the codes.
   __device__ void fill(int64_t t) const {
     const KvPlace p = kv_place(a.tok, t);
     const int32_t page = kv_page(a.tok, p, p.last), seq = a.tok.seq_ids[t];
     const int size = 1 << a.tok.shift;
-    const float old = *scale_of(page);
-    // which slots hold tokens of this call: a thread a slot
+    // the slots before this call's tokens: a thread a slot
     {
       const int o = threadIdx.x;
       const int64_t from = t - (size - 1 - o);
@@ -309,77 +336,76 @@ struct Fill {
       if (lane_id() == 0 && threadIdx.x < 2 * kWave) masks[2 + threadIdx.x / kWave] = m;
     }
     __syncthreads();
-    const uint64_t now[2] = {masks[2], masks[3]};
-    float most = 0.0f, none = 0.0f;
-    const auto see = [&](E x) {
-      const float f = static_cast<float>(x);
-      most = fmaxf(most, finite_size(f));
-      none = fmaf(f, 0.0f, none);  // (not a number beside one that is not finite)
-    };
-    const auto is_here = [&](int o) {
-      return ((o < kWave ? now[0] >> o : now[1] >> (o - kWave)) & 1) != 0;
-    };
-    if (row < ROWS) {
-      for (int o0 = row; o0 < size; o0 += FLIGHT * ROWS) {
-        V8 x[FLIGHT][2];
-        Row turned[FLIGHT];
-        bool here[FLIGHT];
+    const uint64_t lo = masks[2], hi = masks[3];
+    const int earlier = lo ? __builtin_ctzll(lo) : kWave + __builtin_ctzll(hi);  // (t is among them)
+    if (earlier > 0 && *scale_of(page) > 0.0f) reopen(page, seq, earlier);
+    V8 x[ALL][2];
+    bool mine[ALL];
 #pragma unroll
-        for (int i = 0; i < FLIGHT; ++i) {
-          const int o = o0 + i * ROWS;
-          here[i] = o < size && is_here(o);
-          turned[i] = pair;
-          if (here[i]) read(t - (size - 1 - o), p.pos - (size - 1 - o), turned[i], x[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < FLIGHT; ++i) {
-          const int o = o0 + i * ROWS;
-          if (!here[i]) continue;
-          turn(t - (size - 1 - o), turned[i], x[i]);
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            *reinterpret_cast<V8*>(lds + (o * D + 8 * pair.chunk[j]) * 2) = x[i][j];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) see(x[i][j][e]);
-          }
-        }
+    for (int i = 0; i < ALL; ++i) {
+      const int o = row + i * ROWS;
+      mine[i] = row < ROWS && o < size && (!VALUES || o >= earlier);
+      if (mine[i]) {
+        read(o < earlier ? static_cast<const E*>(a.cache.k_tail) + (block(seq) + o) * D
+                         : source(t - (size - 1 - o)),
+             x[i]);
       }
     }
-    if (!is_here(0)) {  // (this call's are the last ones)
-      held(page, seq, old,
-           [&](int slot) {
-             bool all = is_here(slot);
-             if constexpr (VALUES) {
-               for (int e = 1; e < 8; ++e) all = all && is_here(slot + e);
-             }
-             return all;
-           },
-           [&](int slot, int d, const V8& x) {
-        if constexpr (VALUES) {
+    // the largest magnitude, as the 15 bits below the sign
+    v2u16 bits{0, 0};
+    const auto see = [&](const V8& v) {
+      const v4i w = __builtin_bit_cast(v4i, v);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            if (is_here(slot + e)) continue;
-            *reinterpret_cast<E*>(lds + ((slot + e) * D + d) * 2) = x[e];
-            see(x[e]);
-          }
-        } else {
-          *reinterpret_cast<V8*>(lds + (slot * D + d) * 2) = x;
+      for (int i = 0; i < 4; ++i) bits = max_magnitude(bits, static_cast<uint32_t>(w[i]));
+    };
 #pragma unroll
-          for (int e = 0; e < 8; ++e) see(x[e]);
+    for (int i = 0; i < ALL; ++i) {
+      const int o = row + i * ROWS;
+      if (!mine[i]) continue;
+      if (o >= earlier) turn(t - (size - 1 - o), p.pos - (size - 1 - o), x[i]);
+      see(x[i][0]);
+      see(x[i][1]);
+    }
+    if constexpr (VALUES) {
+      earlier_values(seq, earlier, [&](int slot, int, V8 v) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (slot + e >= earlier) v[e] = static_cast<E>(0.0f);
         }
+        see(v);
       });
     }
-    const bool odd = group_max(none == 0.0f ? 0.0f : 1.0f, scratch) > 0.0f;
-    most = fmaxf(group_max(most, scratch), kKvTopFloor);  // (its barriers: the rows are there)
+    const int top = group_max(bits[0] > bits[1] ? bits[0] : bits[1], scratch);
+    const bool odd = top >= kInfinityBits<E>;
+    float most = from_bits<E>(top);
+    if (odd) most = group_max(finite_most(seq, earlier, x, mine), scratch);
+    most = fmaxf(most, kKvTopFloor);
     const BlockCode code(most, odd);
     if (threadIdx.x == 0) *scale_of(page) = most / 127.0f;
     if (code.odd) {
-      encode<true>(code, page);
+      encode<true>(code, page, x, mine);
     } else {
-      encode<false>(code, page);
+      encode<false>(code, page, x, mine);
     }
-    if constexpr (!VALUES) bounds(page);
-  // The first block of a run that ends in an open one: that one's rows, which are not moved (the
+    if constexpr (VALUES) {
+      earlier_values(seq, earlier, [&](int slot, int d, V8 v) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (slot + e >= earlier) break;
+          const uint32_t w = code.template word<true>(static_cast<float>(v[e]));
+          lds[(slot + e) * D + d] = static_cast<char>(w);
+        }
+      });
+      __syncthreads();
+      transpose(page);
+    } else {
+      if (odd) {
+        bounds<true>(page, x, mine);
+      } else {
+        bounds<false>(page, x, mine);
+      }
+    }
+    // The first block of a run that ends in an open one: that one's rows, which are not moved (the
     // open block has been read now).
     if (!is_token(a, t - size, seq, static_cast<int64_t>(p.pos) - size)) {
       int64_t full = 0;  // blocks behind this one that are completed as well
@@ -402,9 +428,8 @@ struct Fill {
         for (int o = row; o < size - 1; o += ROWS) {
           if (!is_token(a, first + o, seq, static_cast<int64_t>(pos) + o)) break;
           V8 x[2];
-          Row turned = pair;
-          read(first + o, pos + o, turned, x);
-          turn(first + o, turned, x);
+          read(source(first + o), x);
+          turn(first + o, pos + o, x);
           to_open(seq, o, x);
         }
       }
@@ -412,41 +437,67 @@ struct Fill {
     __syncthreads();
   }
 
-  // The bounds of a block from its rows in LDS: two channels and a share of the slots a thread.
-  __device__ void bounds(int32_t page) const {
-    constexpr int PAIRS = D / 2, GROUPS = kWriteThreads / PAIRS;
-    typedef E V2 __attribute__((ext_vector_type(2)));
-    const int size = 1 << a.tok.shift, c = threadIdx.x % PAIRS, g = threadIdx.x / PAIRS;
-    float lo[2] = {INFINITY, INFINITY}, hi[2] = {-INFINITY, -INFINITY};
-    if (g < GROUPS) {
-#pragma unroll 4
-      for (int o = g; o < size; o += GROUPS) {
-        const V2 x = *reinterpret_cast<const V2*>(lds + (o * D + 2 * c) * 2);
+  // The bounds of a block: a lane's least and largest keys (16-bit numbers all) through LDS. ODD: NaN
+  // is passed over.
+  template <bool ODD>
+  __device__ void bounds(int32_t page, const V8 (&x)[ALL][2], const bool (&mine)[ALL]) const {
+    E(*lows)[D] = reinterpret_cast<E(*)[D]>(lds);
+    E(*highs)[D] = lows + ROWS;
+    if (row < ROWS) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          lo[h] = fminf(lo[h], static_cast<float>(x[h]));
-          hi[h] = fmaxf(hi[h], static_cast<float>(x[h]));
+      for (int j = 0; j < 2; ++j) {
+        V8 low, high;
+        if constexpr (ODD) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            float l = INFINITY, h = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < ALL; ++i) {
+              const float f = static_cast<float>(x[i][j][e]);
+              l = mine[i] ? fminf(l, f) : l;
+              h = mine[i] ? fmaxf(h, f) : h;
+            }
+            low[e] = static_cast<E>(l);
+            high[e] = static_cast<E>(h);
+          }
+        } else {
+          v4i ends[2];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            v2i16 l, h;
+#pragma unroll
+            for (int i = 0; i < ALL; ++i) {
+              const v4i w = __builtin_bit_cast(v4i, x[i][j]);
+              const v2i16 v = ordered(static_cast<uint32_t>(w[k]));
+              if (i == 0) {  // (a lane has its first row, or none)
+                l = h = v;
+              } else if (mine[i]) {
+                l = __builtin_elementwise_min(l, v);
+                h = __builtin_elementwise_max(h, v);
+              }
+            }
+            ends[0][k] = __builtin_bit_cast(
+                int, ordered(__builtin_bit_cast(uint32_t, l)));
+            ends[1][k] = __builtin_bit_cast(
+                int, ordered(__builtin_bit_cast(uint32_t, h)));
+          }
+          low = __builtin_bit_cast(V8, ends[0]);
+          high = __builtin_bit_cast(V8, ends[1]);
         }
-      }
-    }
-    __syncthreads();  // (the rows have been read)
-    float(*lows)[D] = reinterpret_cast<float(*)[D]>(lds);
-    float(*highs)[D] = lows + GROUPS;
-    if (g < GROUPS) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        lows[g][2 * c + h] = lo[h];
-        highs[g][2 * c + h] = hi[h];
+        *reinterpret_cast<V8*>(&lows[row][8 * pair.chunk[j]]) = low;
+        *reinterpret_cast<V8*>(&highs[row][8 * pair.chunk[j]]) = high;
       }
     }
     __syncthreads();
     const int d = threadIdx.x;
     float mid = 0.0f, half = 0.0f;
     if (d < D) {
-      float l = lows[0][d], h = highs[0][d];
-      for (int i = 1; i < GROUPS; ++i) {
-        l = fminf(l, lows[i][d]);
-        h = fmaxf(h, highs[i][d]);
+      const int rows = ROWS < (1 << a.tok.shift) ? ROWS : 1 << a.tok.shift;
+      float l = static_cast<float>(lows[0][d]), h = static_cast<float>(highs[0][d]);
+#pragma unroll 4
+      for (int i = 1; i < rows; ++i) {
+        l = fminf(l, static_cast<float>(lows[i][d]));
+        h = fmaxf(h, static_cast<float>(highs[i][d]));
       }
       mid = (l + h) * 0.5f;
       half = (h - l) * 0.5f;
@@ -500,12 +551,13 @@ struct Fill {
 };
 
 // Workgroups a CU that the registers leave room for.
-constexpr int write_groups(int mode, bool norm) {
-  return mode == kRotHalfOdd ? 2 : norm ? 3 : 4;
+constexpr int write_groups(int D, int mode, bool norm) {
+  if (D > 128 || mode == kRotHalfOdd) return 2;
+  return norm ? 3 : 4;
 }
 
 template <class E, int D, int MODE, bool NORM>
-__global__ void __launch_bounds__(kWriteThreads, write_groups(MODE, NORM))
+__global__ void __launch_bounds__(kWriteThreads, write_groups(D, MODE, NORM))
     kv_append_int8_kernel(WriteArgs a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   __shared__ float scratch[kWriteWaves];
@@ -575,9 +627,9 @@ extern "C" int rt_kv_append_int8(
   const int64_t grid = fill_groups + cdiv(T * a.row_parts, kWriteWaves);
   RT_CHECK_ARG(grid <= INT32_MAX, "too many tokens");
   a.fill_groups = static_cast<uint32_t>(fill_groups);
-  // a block's rows; the channels' least and largest keys (four floats a thread)
-  const int64_t rows = page * D * 2, ends = kWriteThreads * 4 * 4;
-  const unsigned lds = static_cast<unsigned>(rows > ends ? rows : ends);
+  // a block's codes of values; least and largest keys (32 numbers of 16 bits a thread)
+  const int64_t codes = page * D, ends = kWriteThreads * 32 * 2;
+  const unsigned lds = static_cast<unsigned>(codes > ends ? codes : ends);
   return kv_dispatch(dtype, D, [&](auto e, auto d) -> int {
     using E = decltype(e);
     constexpr int DD = decltype(d)::value;

@@ -58,6 +58,28 @@ __device__ inline float finite_size(float x) {
   return a < INFINITY ? a : 0.0f;
 }
 
+// Numbers of 16 bits two at a time, as whole numbers: their magnitudes order like the bits below the
+// sign, and they themselves like two's complement once negative ones have these bits flipped.
+typedef unsigned short v2u16 __attribute__((ext_vector_type(2)));
+typedef short v2i16 __attribute__((ext_vector_type(2)));
+__device__ inline v2u16 max_magnitude(v2u16 most, uint32_t x) {
+  return __builtin_elementwise_max(most, __builtin_bit_cast(v2u16, x & 0x7fff7fffu));
+}
+__device__ inline v2i16 ordered(uint32_t x) {  // (its own inverse)
+  const v2i16 v = __builtin_bit_cast(v2i16, x);
+  const uint32_t flip = __builtin_bit_cast(uint32_t, v >> 15) & 0x7fff7fffu;
+  return __builtin_bit_cast(v2i16, x ^ flip);
+}
+template <class E>
+inline constexpr int kInfinityBits = 0x7f80;  // from here on: not finite
+template <>
+inline constexpr int kInfinityBits<_Float16> = 0x7c00;
+template <class E>
+__device__ inline float from_bits(int bits) {
+  const unsigned short b = static_cast<unsigned short>(bits);
+  return static_cast<float>(__builtin_bit_cast(E, b));
+}
+
 // Host: the checks of an 8-bit cache's pointers.
 inline int kv_check_int8(const KvInt8& c, int64_t B, int64_t P) {
   RT_CHECK_ARG(P == 0 || (c.k_codes && c.v_codes && c.k_scales && c.v_scales), "null cache");

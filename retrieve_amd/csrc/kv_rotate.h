@@ -125,7 +125,15 @@ __device__ inline float row_scale(const typename Kv<E>::V8 (&x)[N], int part, do
     const int base = lane_id() - part;
     sum = (__shfl(sum, base) + __shfl(sum, base + P)) + __shfl(sum, base + 2 * P);
   }
-  return static_cast<float>(1.0 / __builtin_sqrt(sum / D + eps));
+  // 1 / sqrt by two Newton steps on the instruction's 23 bits (a division and a root in 64 bits take
+  // 45 instructions); infinite and 0 (of 0 and of an infinity) as it gives them.
+  const double mean = sum * (1.0 / D) + eps;
+  double y = __builtin_amdgcn_rsq(mean);
+  if (y > 0.0 && y < INFINITY) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) y = __builtin_fma(0.5 * y, __builtin_fma(-mean * y, y, 1.0), y);
+  }
+  return static_cast<float>(y);
 }
 
 // Chunk `chunk` of a row, read as x, after the norm (r and the chunk's weights; NORM only) and the
@@ -171,10 +179,18 @@ __device__ inline typename Kv<E>::V8 turned_chunk(const E* row, typename Kv<E>::
       if (NORM && i < a.rot) other[e] = other[e] * r * Weights<E>::at(norm, at);
     }
   }
+  if (MODE == kRotPairs && 8 * chunk + 8 <= a.rot) {  // (the whole chunk turns)
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      out[e] = static_cast<E>(rot_first(own[e], own[e + 1], t.cos(e), t.sin(e)));
+      out[e + 1] = static_cast<E>(rot_second(own[e + 1], own[e], t.cos(e), t.sin(e)));
+    }
+    return out;
+  }
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const int i = 8 * chunk + e;
-    const bool first = MODE == kRotPairs ? (i & 1) == 0 : i < half;
+    const bool first = MODE == kRotPairs ? (e & 1) == 0 : i < half;
     const float z = first ? rot_first(own[e], other[e], t.cos(e), t.sin(e))
                           : rot_second(own[e], other[e], t.cos(e), t.sin(e));
     out[e] = i < a.rot ? static_cast<E>(z) : NORM ? static_cast<E>(own[e]) : x[e];
@@ -233,15 +249,28 @@ struct Pair {
     }
     if constexpr (MODE == kRotHalf) {
       if (!NORM && !turned) return;
+      float f[8], s[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        float f = static_cast<float>(x[0][e]), s = static_cast<float>(x[1][e]);
+        f[e] = static_cast<float>(x[0][e]);
+        s[e] = static_cast<float>(x[1][e]);
         if constexpr (NORM) {
-          f = f * r * (kind ? weights[1][0].w[e] : weights[0][0].w[e]);
-          s = s * r * (kind ? weights[1][1].w[e] : weights[0][1].w[e]);
+          f[e] = f[e] * r * (kind ? weights[1][0].w[e] : weights[0][0].w[e]);
+          s[e] = s[e] * r * (kind ? weights[1][1].w[e] : weights[0][1].w[e]);
         }
-        x[0][e] = static_cast<E>(turned ? rot_first(f, s, turn[0].c[e], turn[0].s[e]) : f);
-        x[1][e] = static_cast<E>(turned ? rot_second(s, f, turn[0].c[e], turn[0].s[e]) : s);
+      }
+      if (turned) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          x[0][e] = static_cast<E>(rot_first(f[e], s[e], turn[0].c[e], turn[0].s[e]));
+          x[1][e] = static_cast<E>(rot_second(s[e], f[e], turn[0].c[e], turn[0].s[e]));
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          x[0][e] = static_cast<E>(f[e]);
+          x[1][e] = static_cast<E>(s[e]);
+        }
       }
     } else {
 #pragma unroll
