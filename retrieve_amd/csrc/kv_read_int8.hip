@@ -20,20 +20,23 @@ struct ReadArgs {
   void *k_out, *v_out;  // [T, Hkv, D]
 };
 
-// Sixteen codes as 16-bit numbers.
+// Eight codes as 16-bit numbers.
 template <class E>
-__device__ inline void widen(v4i codes, float scale, typename Kv<E>::V8 (&x)[2]) {
+__device__ inline typename Kv<E>::V8 widen(int lo, int hi, float scale) {
+  typename Kv<E>::V8 x;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int code = static_cast<int8_t>(codes[i >> 2] >> (8 * (i & 3)));
-    x[i >> 3][i & 7] = static_cast<E>(static_cast<float>(code) * scale);
+  for (int i = 0; i < 8; ++i) {
+    const int code = static_cast<int8_t>((i < 4 ? lo : hi) >> (8 * (i & 3)));
+    x[i] = static_cast<E>(static_cast<float>(code) * scale);
   }
+  return x;
 }
 
 template <class E, int D>
 __global__ void __launch_bounds__(kReadWaves* kWave) kv_read_int8_kernel(ReadArgs a) {
   using V8 = typename Kv<E>::V8;
   constexpr int C = D / 16, ROWS = kWave / C;  // a row's lanes; rows at once
+  constexpr int KP = (16 + ROWS - 1) / ROWS, VP = (D + kWave - 1) / kWave;  // loads a lane
   __shared__ __attribute__((aligned(16))) E turned[kReadWaves][16][D];
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   const int lane = lane_id();
@@ -73,42 +76,83 @@ __global__ void __launch_bounds__(kReadWaves* kWave) kv_read_int8_kernel(ReadArg
     const float vs = pg >= 0 ? a.cache.v_scales[row] : 0.0f;
     const int64_t full = (row << a.tok.shift) * D;
     const int64_t open = ((static_cast<int64_t>(sq) * a.Hkv + head) << a.tok.shift) * D;
-    const int c = lane % C;
-    for (int r = lane / C < ROWS ? lane / C : n; r < n; r += ROWS) {
-      V8 x[2] = {V8{}, V8{}};
+    const int c = lane % C, r0 = lane / C < ROWS ? lane / C : 16;
+    // everything of the run under way at once: keys row by row, values 16 slots of a channel
+    typedef int V2i __attribute__((ext_vector_type(2)));
+    V2i kc[KP][2];  // (chunks c and c + C of 8 channels: neighbours store side by side)
+    v4i vc[VP];
+    V8 kt[KP][2], vt[VP][2];
+#pragma unroll
+    for (int i = 0; i < KP; ++i) {
+      const int r = r0 + i * ROWS;
+      if (r >= n || pg < 0) continue;
       if (ks > 0.0f) {
-        widen<E>(*reinterpret_cast<const v4i*>(a.cache.k_codes + full + (slot + r) * D + 16 * c),
-                 ks, x);
-      } else if (pg >= 0) {
+        const V2i* from =
+            reinterpret_cast<const V2i*>(a.cache.k_codes + full + (slot + r) * D);
+        kc[i][0] = __builtin_nontemporal_load(from + c);
+        kc[i][1] = __builtin_nontemporal_load(from + c + C);
+      } else {
         const V8* from = reinterpret_cast<const V8*>(static_cast<const E*>(a.cache.k_tail) + open +
-                                                     (slot + r) * D + 16 * c);
-        x[0] = from[0];
-        x[1] = from[1];
+                                                     (slot + r) * D);
+        kt[i][0] = from[c];
+        kt[i][1] = from[c + C];
       }
-      V8* out = reinterpret_cast<V8*>(k_out + r * step + 16 * c);
-      out[0] = x[0];
-      out[1] = x[1];
     }
-    for (int d = lane; d < D; d += kWave) {
-      V8 x[2] = {V8{}, V8{}};
-      const int64_t from = (d << a.tok.shift) + (slot & ~15);
+#pragma unroll
+    for (int i = 0; i < VP; ++i) {
+      const int d = lane + i * kWave;
+      const int64_t from = (static_cast<int64_t>(d) << a.tok.shift) + (slot & ~15);
+      if (d >= D || pg < 0) continue;
       if (vs > 0.0f) {
-        widen<E>(*reinterpret_cast<const v4i*>(a.cache.v_codes + full + from), vs, x);
-      } else if (pg >= 0) {
+        // (the other runs of the block take the rest of the line: not streamed)
+        vc[i] = *reinterpret_cast<const v4i*>(a.cache.v_codes + full + from);
+      } else {
         const V8* tail = reinterpret_cast<const V8*>(static_cast<const E*>(a.cache.v_tail) + open +
                                                      from);
-        x[0] = tail[0];
-        x[1] = tail[1];
+        vt[i][0] = tail[0];
+        vt[i][1] = tail[1];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < KP; ++i) {
+      const int r = r0 + i * ROWS;
+      if (r >= n) continue;
+      V8 x[2] = {V8{}, V8{}};
+      if (ks > 0.0f) {
+        x[0] = widen<E>(kc[i][0][0], kc[i][0][1], ks);
+        x[1] = widen<E>(kc[i][1][0], kc[i][1][1], ks);
+      } else if (pg >= 0) {
+        x[0] = kt[i][0];
+        x[1] = kt[i][1];
+      }
+      V8* out = reinterpret_cast<V8*>(k_out + r * step);
+      out[c] = x[0];
+      out[c + C] = x[1];
+    }
+#pragma unroll
+    for (int i = 0; i < VP; ++i) {
+      const int d = lane + i * kWave;
+      if (d >= D) continue;
+      V8 x[2] = {V8{}, V8{}};
+      if (vs > 0.0f) {
+        x[0] = widen<E>(vc[i][0], vc[i][1], vs);
+        x[1] = widen<E>(vc[i][2], vc[i][3], vs);
+      } else if (pg >= 0) {
+        x[0] = vt[i][0];
+        x[1] = vt[i][1];
       }
 #pragma unroll
-      for (int i = 0; i < 16; ++i) turned[wave][i][d] = x[i >> 3][i & 7];
+      for (int e = 0; e < 16; ++e) turned[wave][e][d] = x[e >> 3][e & 7];
     }
     wave_sync_memory();
-    for (int r = lane / C < ROWS ? lane / C : n; r < n; r += ROWS) {
-      const V8* from = reinterpret_cast<const V8*>(&turned[wave][(slot & 15) + r][16 * c]);
-      V8* out = reinterpret_cast<V8*>(v_out + r * step + 16 * c);
-      out[0] = from[0];
-      out[1] = from[1];
+#pragma unroll
+    for (int i = 0; i < KP; ++i) {
+      const int r = r0 + i * ROWS;
+      if (r >= n) continue;
+      const V8* from = reinterpret_cast<const V8*>(turned[wave][(slot & 15) + r]);
+      V8* out = reinterpret_cast<V8*>(v_out + r * step);
+      out[c] = from[c];
+      out[c + C] = from[c + C];
     }
     wave_sync_memory();
   }
