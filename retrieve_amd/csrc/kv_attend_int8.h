@@ -181,15 +181,18 @@ struct Subtile {
     ks = inv = 1.0f;
     lift = 0.0f;
   }
-  // Its page's scales; whether it is open.
-  __device__ bool scales(const AttendInt8Args& a, int32_t p, int head) {
-    const int64_t row = static_cast<int64_t>(p) * a.Hkv + head;
-    const float k = a.cache.k_scales[row], v = a.cache.v_scales[row];
-    if (!(k > 0.0f)) return true;
-    ks = k;
-    lift = __builtin_amdgcn_logf(v);
-    inv = 1.0f / v;
-    return false;
+  // Its page's scales, and what is kept of them; false: the page has no codes.
+  __device__ void scales(const AttendInt8Args& a, int head, float (&scale)[2]) const {
+    const int64_t row = static_cast<int64_t>(page) * a.Hkv + head;
+    scale[0] = a.cache.k_scales[row];
+    scale[1] = a.cache.v_scales[row];
+  }
+  __device__ bool take(const float (&scale)[2]) {
+    if (!(scale[0] > 0.0f)) return false;
+    ks = scale[0];
+    lift = __builtin_amdgcn_logf(scale[1]);
+    inv = 1.0f / scale[1];
+    return true;
   }
 };
 // A step's four subtiles (subtiles 4 i to 4 i + 3), of which this lane has the scores of one.
@@ -242,16 +245,21 @@ struct Int8Wave {
   __device__ static int channel(int s, int grp) {
     return s < 2 * KL ? 64 * (s >> 1) + 16 * grp + 8 * (s & 1) : 64 * KL + 8 * grp;
   }
-  // This lane's column of tile c is query head `head` of token t (zeros where it is not `real`).
-  __device__ void load_q(const AttendInt8Args& a, int c, int64_t t, int64_t head, bool real,
-                         v8h* lds = nullptr) {
-    const int grp = lane_id() >> 4;
+  // This lane's column of a tile is query head `head` of token t (its first row where it is not `real`).
+  __device__ static void fetch_q(const AttendInt8Args& a, int64_t t, int64_t head, bool real,
+                                 V8 (&x)[KS]) {
     const E* q = static_cast<const E*>(a.q) + (real ? t * a.q_st + head * a.q_sh : 0);
-    V8 x[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      x[s] = *reinterpret_cast<const V8*>(q + channel(s, lane_id() >> 4));
+    }
+  }
+  // The fetched queries as tile c's (zeros where they are not `real`).
+  __device__ void take_q(const AttendInt8Args& a, int c, const V8 (&x)[KS], bool real,
+                         v8h* lds = nullptr) {
     float most = 0.0f, none = 0.0f;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      x[s] = *reinterpret_cast<const V8*>(q + channel(s, grp));
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float f = static_cast<float>(x[s][e]);
@@ -313,7 +321,7 @@ struct Int8Wave {
     }
     return x;
   }
-  // A step's keys to LDS: 64 rows, chunks permuted (key_chunk).
+  // A step's keys to LDS: 64 rows, chunks permuted (key_chunk). STREAM: rows that are read once.
   template <bool STREAM>
   __device__ static void load_k(const AttendInt8Args& a, const Subtile& s, int head, int quad,
                                 char* lds) {
@@ -329,17 +337,17 @@ struct Int8Wave {
 #pragma unroll
     for (int x = 0; x < LOADS; ++x) {
       const int at = x * kWave + lane_id(), row = at / (D / 16), c = at % (D / 16);
-      const uint32_t in = static_cast<uint32_t>(row * D + 16 * key_chunk<D>(row, c));
+      const int in = row * D + 16 * key_chunk<D>(row, c);
       if constexpr (SHIFT >= 6) {
-        load_to_lds<STREAM>(first + in, lds + x * 1024);
+        buffer_load_lds<16, STREAM>(first, 64 * D, in, lds + x * 1024);
       } else if constexpr (D % 64 == 0) {
         constexpr int EACH = D / 64;  // loads of a subtile
         if (x > 0 && x % EACH == 0) first = of(x / EACH);
-        load_to_lds<STREAM>(first + (in - x / EACH * (16 * D)), lds + x * 1024);
+        buffer_load_lds<16, STREAM>(first, 16 * D, in - x / EACH * (16 * D), lds + x * 1024);
       } else {
         const int from = 4 * quad + (row >> 4);
-        const int8_t* mine = rows(__shfl(s.page, from), __shfl(s.at, from));
-        load_to_lds<STREAM>(mine + (in - (row >> 4) * (16 * D)), lds + x * 1024);
+        load_to_lds<STREAM>(rows(__shfl(s.page, from), __shfl(s.at, from)) + (in - (row >> 4) * (16 * D)),
+                            lds + x * 1024);
       }
     }
   }
@@ -360,17 +368,19 @@ struct Int8Wave {
       const int at = x * kWave + lane_id();
       if constexpr (SHIFT >= 6) {
         const int channel = at >> 2, in = value_offset<D, SHIFT>(channel, at & 3) - 64 * channel;
-        load_to_lds<STREAM>(first + static_cast<uint32_t>((channel << SHIFT) + in), lds + x * 1024);
+        // (of a channel of 128 slots another step takes the rest of the line)
+        buffer_load_lds<16, STREAM && SHIFT == 6>(first, D << SHIFT, (channel << SHIFT) + in,
+                                                  lds + x * 1024);
       } else if constexpr (SHIFT == 5) {
         constexpr int EACH = LOADS / 2;  // loads of a page
         if (x == EACH) first = of(2);
         const int in = at - x / EACH * (2 * D), channel = in >> 1;
-        load_to_lds<STREAM>(first + static_cast<uint32_t>(value_offset<D, SHIFT>(channel, in & 1)),
-                            lds + x * 1024);
+        buffer_load_lds<16, STREAM>(first, D << SHIFT, value_offset<D, SHIFT>(channel, in & 1),
+                                    lds + x * 1024);
       } else if constexpr (D % 64 == 0) {
         constexpr int EACH = D / 64;
         if (x > 0 && x % EACH == 0) first = of(x / EACH);
-        load_to_lds<STREAM>(first + static_cast<uint32_t>(16 * (at - x / EACH * D)), lds + x * 1024);
+        buffer_load_lds<16, STREAM>(first, D << SHIFT, 16 * (at - x / EACH * D), lds + x * 1024);
       } else {
         const int sub = at / D;
         load_to_lds<STREAM>(page(__shfl(s.page, 4 * quad + sub)) + 16 * (at - sub * D),
@@ -612,6 +622,10 @@ struct Int8Wave {
   }
 };
 
+// Waves a SIMD that the registers leave room for: as many as the workgroups' LDS does (512 D bytes
+// and up to 20 KiB each of a CU's 160 KiB).
+constexpr int attend_int8_waves(int D) { return D > 128 ? 1 : 2; }
+
 // Single tokens, and few rows: the workgroup's waves (and `parts` workgroups) share a row's list in
 // units of 64 keys.
 template <class E, int D, int SHIFT>
@@ -636,10 +650,12 @@ struct SplitWave : Int8Wave<E, D, SHIFT, 1> {
         const int32_t slot = static_cast<int32_t>(key) & ((1 << SHIFT) - 1);
         const int32_t n = place.pos - (block << SHIFT) - slot + 1;
         if (p >= 0 && n > 0) {
-          is_open = s.scales(a, p, head);
+          s.page = p;
+          float scale[2];
+          s.scales(a, head, scale);
+          is_open = !s.take(scale);
           // (a block before the token's own that has no codes was never filled)
           if (!is_open || block == place.last) {
-            s.page = p;
             s.at = slot * 32 + (n < 16 ? n : 16);
           }
         }
@@ -649,9 +665,9 @@ struct SplitWave : Int8Wave<E, D, SHIFT, 1> {
     open = __ballot(s.at != 0 && is_open);
     return true;
   }
-  template <bool STREAM>
+  // `stream`: others do not read these blocks.
   __device__ void run(const AttendInt8Args& a, int64_t t, int head, int tile, int part, int parts,
-                      char* keys, char* values) {
+                      bool stream, char* keys, char* values) {
     this->clear();
     const int g = tile * 16 + (lane_id() & 15), grp = lane_id() >> 4;
     const int64_t hq = head * a.G + g;
@@ -659,7 +675,11 @@ struct SplitWave : Int8Wave<E, D, SHIFT, 1> {
     this->odd[0] = false;
     if (place.last < 0) return;
     const int32_t* list = a.blocks + (t * a.Hkv + head) * a.count;
-    this->load_q(a, 0, t, hq, g < a.G);
+    {
+      typename Kv<E>::V8 q[D / 32];
+      Base::fetch_q(a, t, hq, g < a.G, q);
+      this->take_q(a, 0, q, g < a.G);
+    }
     Subtile s;
     uint64_t full, open;
     for (int chunk = 0; fetch(a, list, place, head, part, parts, chunk, s, full, open); ++chunk) {
@@ -672,10 +692,24 @@ struct SplitWave : Int8Wave<E, D, SHIFT, 1> {
         then = this->step_of(s, i);
         late_counts = (all >> (4 * i + grp)) & 1;
       };
+      auto load_k = [&] {
+        if (stream) {
+          this->template load_k<true>(a, s, head, then.i, keys);
+        } else {
+          this->template load_k<false>(a, s, head, then.i, keys);
+        }
+      };
+      auto load_v = [&] {
+        if (stream) {
+          this->template load_v<true>(a, s, head, then.i, values);
+        } else {
+          this->template load_v<false>(a, s, head, then.i, values);
+        }
+      };
       if (more) {
         next();
-        this->template load_k<STREAM>(a, s, head, then.i, keys);
-        this->template load_v<STREAM>(a, s, head, then.i, values);
+        load_k();
+        load_v();
       }
       while (more) {
         const Step now = then;
@@ -684,9 +718,7 @@ struct SplitWave : Int8Wave<E, D, SHIFT, 1> {
         if (more) next();
         const int n[1] = {now.at & 31};
         const bool c[1] = {counts};
-        this->step(keys, values, now, c, n, __any(n[0] != 16), more,
-                   [&] { this->template load_k<STREAM>(a, s, head, then.i, keys); },
-                   [&] { this->template load_v<STREAM>(a, s, head, then.i, values); });
+        this->step(keys, values, now, c, n, __any(n[0] != 16), more, load_k, load_v);
       }
       while (open != 0) {
         const int i = __builtin_ctzll(open) >> 2, own = 4 * i + grp;
@@ -702,7 +734,7 @@ struct SplitWave : Int8Wave<E, D, SHIFT, 1> {
 };
 
 template <class E, int D, int SHIFT>
-__global__ void __launch_bounds__(kAttendWaves* kWave, D <= 128 ? 2 : 1)
+__global__ void __launch_bounds__(kAttendWaves* kWave, attend_int8_waves(D))
     kv_attend_int8_split_kernel(AttendInt8Args a) {
   __shared__ __attribute__((aligned(16))) char lds[kAttendWaves][64 * D];  // keys, then sums
   __shared__ __attribute__((aligned(16))) char values[kAttendWaves][64 * D];
@@ -719,11 +751,7 @@ __global__ void __launch_bounds__(kAttendWaves* kWave, D <= 128 ? 2 : 1)
   const bool beside = (t > 0 && a.tok.seq_ids[t - 1] == seq) ||
                       (t + 1 < a.T && a.tok.seq_ids[t + 1] == seq);
   const int first = part * kAttendWaves + wave, parts = a.parts * kAttendWaves;
-  if (beside) {
-    w.template run<false>(a, t, head, tile, first, parts, lds[wave], values[wave]);
-  } else {
-    w.template run<true>(a, t, head, tile, first, parts, lds[wave], values[wave]);
-  }
+  w.run(a, t, head, tile, first, parts, !beside, lds[wave], values[wave]);
   w.finish();
   join_waves<E, D>(a, w.acc[0], w.m[0], w.l[0], t, head, tile, row, part, lds, ml);
 }
@@ -830,7 +858,7 @@ __device__ inline int join_lists(const AttendInt8Args& a, int64_t t0, int tokens
 }
 
 template <class E, int D, int SHIFT, int CT>
-__global__ void __launch_bounds__(kAttendWaves* kWave, D <= 128 ? 2 : 1)
+__global__ void __launch_bounds__(kAttendWaves* kWave, attend_int8_waves(D))
     kv_attend_int8_joined_kernel(AttendInt8Args a) {
   __shared__ __attribute__((aligned(16))) JoinInt8Lds<D, CT> lds;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
@@ -841,6 +869,7 @@ __global__ void __launch_bounds__(kAttendWaves* kWave, D <= 128 ? 2 : 1)
   const int listed = join_lists(a, t0, tokens, head, lds);
   const int each = 16 / a.G;  // tokens of a tile
   Int8Wave<E, D, SHIFT, CT> w;
+  using V8 = typename Kv<E>::V8;
   w.clear();
   w.q_lds = lds.q;
   bool real[CT];
@@ -854,13 +883,19 @@ __global__ void __launch_bounds__(kAttendWaves* kWave, D <= 128 ? 2 : 1)
     const KvPlace p = kv_place(a.tok, t0 + tok[c]);
     own[c] = real[c] && p.last >= 0 ? kv_page(a.tok, p, p.last) : -1;
     own_keys[c] = (p.pos & ((1 << SHIFT) - 1)) + 1;
-    if constexpr (CT == 1) w.load_q(a, c, t0 + tok[c], head * a.G + col % a.G, real[c]);
+    if constexpr (CT == 1) {
+      V8 x[D / 32];
+      w.fetch_q(a, t0 + tok[c], head * a.G + col % a.G, real[c], x);
+      w.take_q(a, c, x, real[c]);
+    }
   }
   if constexpr (CT > 1) {  // a wave a tile, for all
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
       if (wave != c) continue;
-      w.load_q(a, c, t0 + tok[c], head * a.G + col % a.G, real[c], lds.q);
+      V8 x[D / 32];
+      w.fetch_q(a, t0 + tok[c], head * a.G + col % a.G, real[c], x);
+      w.take_q(a, c, x, real[c], lds.q);
       if (grp == 0) {
         lds.column[c][col][0] = w.factor[c];
         lds.column[c][col][1] = w.start[c];
@@ -887,7 +922,9 @@ __global__ void __launch_bounds__(kAttendWaves* kWave, D <= 128 ? 2 : 1)
       s.page = lds.list[i / PER];
       s.who = lds.list_who[i / PER];
       s.at = i % PER * 16 * 32 + 16;
-      is_open = s.scales(a, s.page, head);
+      float scale[2];
+      s.scales(a, head, scale);
+      is_open = !s.take(scale);
     }
     // (open pages are their tokens' own or were never filled)
     uint64_t full = __ballot(s.at != 0 && !is_open), open = __ballot(s.at != 0 && is_open);
