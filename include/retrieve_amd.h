@@ -592,9 +592,10 @@ int rt_kv_append(const void* q, int64_t q_token_stride, int64_t q_head_stride, c
                  void* q_out, rt_stream_t stream);
 
 /* rt_kv_append whose query and key heads are normed before the rotation: y = x r w with r = 1 /
- * sqrt(mean(x^2) + eps) over the head's D channels (the sum in double, r, x r and the product with w
- * each rounded to float once; nothing is rounded to 16 bits before the rotation). q_weight, k_weight
- * [D], float where `wide_weights`, else of the rows' type; null: those heads are not normed. eps >= 0. */
+ * sqrt(mean(x^2) + eps) over the head's D channels (the sum in double, r, x r and the product with
+ * w each rounded to float once; nothing is rounded to 16 bits before the rotation). q_weight,
+ * k_weight [D], float where `wide_weights`, else of the rows' type; null: those heads are not
+ * normed. eps >= 0. */
 int rt_kv_append_norm(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
                       int64_t k_token_stride, int64_t k_head_stride, const void* v,
                       int64_t v_token_stride, int64_t v_head_stride, int64_t T, int64_t Hq,
@@ -608,15 +609,16 @@ int rt_kv_append_norm(const void* q, int64_t q_token_stride, int64_t q_head_stri
 /* The cache in 8 bits: k_codes int8 [P, Hkv, page, D], v_codes int8 [P, Hkv, D, page] (values
  * transposed), k_scales, v_scales float [P, Hkv] (a code stands for code * scale), and each
  * sequence's open block, its last one while it is not full, in 16 bits: k_tail [B, Hkv, page, D],
- * v_tail [B, Hkv, D, page]. All start on 16 bytes. A page whose scales are 0 is not full: its tokens are
- * in its sequence's open block. Bounds as in the 16-bit cache, from the 16-bit keys.
+ * v_tail [B, Hkv, D, page]. All start on 16 bytes. A page whose scales are 0 is not full: its
+ * tokens are in its sequence's open block. Bounds as in the 16-bit cache, from the 16-bit keys.
  *
- * rt_kv_append_norm into it. A token at the last slot of its block completes it: its keys become codes
- * rint(127 x / a) with a = max(max |x| over the block's finite keys of the head, 1e-8) and scale a /
- * 127 (infinities +-127, NaN 0), its values the same. The other tokens' rows go to the open block and
- * their page's scales become 0. A call's tokens of a sequence lie side by side, in order, and are its
- * end from then on: positions behind them are no longer held. A sequence that goes on inside a block
- * that was full (it has been cut back) has the block's earlier tokens from their codes. */
+ * rt_kv_append_norm into it. A token at the last slot of its block completes it: its keys become
+ * codes rint(127 x / a) with a = max(max |x| over the block's finite keys of the head, 1e-8) and
+ * scale a / 127 (infinities +-127, NaN 0), its values the same. The other tokens' rows go to the
+ * open block and their page's scales become 0. A call's tokens of a sequence lie side by side, in
+ * order, and are its end from then on: positions behind them are no longer held. A sequence that
+ * goes on inside a block that was full (it has been cut back) has the block's earlier tokens from
+ * their codes. */
 int rt_kv_append_int8(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
                       int64_t k_token_stride, int64_t k_head_stride, const void* v,
                       int64_t v_token_stride, int64_t v_head_stride, int64_t T, int64_t Hq,
@@ -628,8 +630,8 @@ int rt_kv_append_int8(const void* q, int64_t q_token_stride, int64_t q_head_stri
                       float* v_scales, void* k_tail, void* v_tail, int64_t P, int64_t page,
                       int8_t* bounds, float* bound_scales, void* q_out, rt_stream_t stream);
 
-/* Tokens of the 8-bit cache in 16 bits -> k_out, v_out [T, Hkv, D]: code * scale rounded once, the open
- * block's rows as they are. Padding tokens (and tokens without a page) give zeros. */
+/* Tokens of the 8-bit cache in 16 bits -> k_out, v_out [T, Hkv, D]: code * scale rounded once, the
+ * open block's rows as they are. Padding tokens (and tokens without a page) give zeros. */
 int rt_kv_read_int8(const int8_t* k_codes, const int8_t* v_codes, const float* k_scales,
                     const float* v_scales, const void* k_tail, const void* v_tail, int64_t T,
                     int64_t Hkv, int64_t D, int dtype, int64_t P, int64_t page,
@@ -690,8 +692,9 @@ int rt_kv_attention_of(const void* q, int64_t q_token_stride, int64_t q_head_str
                        int64_t sequences, void* out, float* lse, void* workspace,
                        size_t workspace_bytes, rt_stream_t stream);
 
-/* rt_kv_attention_of over the 8-bit cache. Listed blocks before the token's own that were never filled
- * (scales of 0) are skipped. The row of a query that holds an infinity or a NaN is not a number. */
+/* rt_kv_attention_of over the 8-bit cache. Listed blocks before the token's own that were never
+ * filled (scales of 0) are skipped. The row of a query that holds an infinity or a NaN is not a
+ * number. */
 size_t rt_kv_attention_int8_workspace(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t page,
                                       int64_t count);
 int rt_kv_attention_int8(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t T,

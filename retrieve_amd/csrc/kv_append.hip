@@ -291,7 +291,8 @@ extern "C" int rt_kv_append_norm(
   return kv_dispatch(dtype, D, [&](auto e, auto d) -> int {
     using E = decltype(e);
     constexpr int DD = decltype(d)::value;
-    return kv_turn_dispatch(rot, interleaved, q_weight || k_weight, [&](auto mode, auto norm) -> int {
+    const bool normed = q_weight || k_weight;
+    return kv_turn_dispatch(rot, interleaved, normed, [&](auto mode, auto norm) -> int {
       kv_append_kernel<E, DD, decltype(mode)::value, decltype(norm)::value>
           <<<dim3(static_cast<unsigned>(grid)), dim3(kAppendThreads), 0,
              static_cast<hipStream_t>(stream)>>>(a);

@@ -2,17 +2,17 @@
 // scales and bounds once it is full, its 16-bit rows until then.
 //
 // Norm and rotation are kv_rotate.h's. A token that takes its block's last slot completes it: the
-// block's rows that are part of this call are turned again from the input, earlier ones come from the
-// sequence's open block (or from the codes, where the block had been full and its sequence was cut
-// back into it), and the codes, scales and int8 bounds follow from the 16-bit rows. Bounds are those
-// of kv_append.hip.
+// block's rows that are part of this call are turned again from the input, earlier ones come from
+// the sequence's open block (or from the codes, where the block had been full and its sequence was
+// cut back into it), and the codes, scales and int8 bounds follow from the 16-bit rows. Bounds are
+// those of kv_append.hip.
 //
-// One launch, no workgroup waits for another. Workgroups at the grid's head look at a tile of tokens
-// for one head's keys or values and do the blocks completed there: rows in registers, their largest
-// magnitude, then codes (values transposed through LDS). In the others a wave moves a token's
-// queries, and its key and value rows to the open block. The open block is read (the first block
-// that a call completes) and written (the rows behind the last one) in the same call: a run of
-// tokens that begins in one block and ends in a later, open one has these rows written by the
+// One launch, no workgroup waits for another. Workgroups at the grid's head look at a tile of
+// tokens for one head's keys or values and do the blocks completed there: rows in registers, their
+// largest magnitude, then codes (values transposed through LDS). In the others a wave moves a
+// token's queries, and its key and value rows to the open block. The open block is read (the first
+// block that a call completes) and written (the rows behind the last one) in the same call: a run
+// of tokens that begins in one block and ends in a later, open one has these rows written by the
 // workgroup that reads the open block first, after it has read.
 #pragma once
 
@@ -23,7 +23,8 @@
 
 namespace rt {
 
-// A workgroup's threads: a lane holds up to four rows' chunks of a block of 128 slots, 32 registers.
+// A workgroup's threads: a lane holds up to four rows' chunks of a block of 128 slots, 32
+// registers.
 constexpr int write_threads(int64_t D) { return D > 128 ? 512 : 256; }
 
 struct WriteArgs : TurnArgs {
@@ -325,8 +326,8 @@ struct Fill {
     return most;
   }
 
-  // The block that token t completes. Its rows stay in registers: their largest magnitude first, then
-  // the codes.
+  // The block that token t completes. Its rows stay in registers: their largest magnitude first,
+  // then the codes.
   __device__ void fill(int64_t t) const {
     const KvPlace p = kv_place(a.tok, t);
     const int32_t page = kv_page(a.tok, p, p.last), seq = a.tok.seq_ids[t];
@@ -342,7 +343,8 @@ struct Fill {
     }
     __syncthreads();
     const uint64_t lo = masks[2], hi = masks[3];
-    const int earlier = lo ? __builtin_ctzll(lo) : kWave + __builtin_ctzll(hi);  // (t is among them)
+    // (t is among them)
+    const int earlier = lo ? __builtin_ctzll(lo) : kWave + __builtin_ctzll(hi);
     if (earlier > 0 && *scale_of(page) > 0.0f) reopen(page, seq, earlier);
     V8 x[ALL][2];
     bool mine[ALL];
@@ -442,8 +444,8 @@ struct Fill {
     __syncthreads();
   }
 
-  // The bounds of a block: a lane's least and largest keys (16-bit numbers all) through LDS. ODD: NaN
-  // is passed over.
+  // The bounds of a block: a lane's least and largest keys (16-bit numbers all) through LDS. ODD:
+  // NaN is passed over.
   template <bool ODD>
   __device__ void bounds(int32_t page, const V8 (&x)[ALL][2], const bool (&mine)[ALL]) const {
     E(*lows)[D] = reinterpret_cast<E(*)[D]>(lds);

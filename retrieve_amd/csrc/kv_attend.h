@@ -1,5 +1,5 @@
-// What attention over a paged cache in 16 and in 8 bits shares: the arguments of a call, and the join
-// of a row's parts.
+// What attention over a paged cache in 16 and in 8 bits shares: the arguments of a call, and the
+// join of a row's parts.
 #pragma once
 
 #include "kv_common.h"

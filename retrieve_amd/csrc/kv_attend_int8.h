@@ -8,33 +8,34 @@
 // subnormal u 2^-24, which they take exactly, so 4 codes cost 3 instructions (1024 + u, less 1152,
 // would be 5). The 128 too many are taken off as 128 sum(q) where the first product starts and as
 // 128 sum(p), an operand of constant codes, behind the second. bf16 queries become fp16 as well: a
-// row is scaled by a power of two so that its largest magnitude is in [2^14, 2^15), where fp16 holds
-// every 8-bit significand down to 2^-17; what is lost is below 2^-39 of the row's largest.
+// row is scaled by a power of two so that its largest magnitude is in [2^14, 2^15), where fp16
+// holds every 8-bit significand down to 2^-17; what is lost is below 2^-39 of the row's largest.
 //
 // The scale of a block's keys multiplies the scores; that of its values, s_v, goes into the
-// exponent: with t = x log2 e + log2 s_v and m the running maximum of t, p = 2^(t - m) is the weight
-// that the second product wants (codes stand for s_v each), and p / s_v what the sum of weights
-// wants. So neither product is rescaled from block to block. p is rounded to fp16 (2^-11, and held
-// 2^7 times as large as the maximum says: it reaches 2^15, its step below 2^-14 is 2^-31 of the
-// largest weight) whatever the queries' type; the sum takes it unrounded. The maximum is raised only
-// where a score passes it by 8 (in powers of two), so most steps exchange nothing between lanes.
+// exponent: with t = x log2 e + log2 s_v and m the running maximum of t, p = 2^(t - m) is the
+// weight that the second product wants (codes stand for s_v each), and p / s_v what the sum of
+// weights wants. So neither product is rescaled from block to block. p is rounded to fp16 (2^-11,
+// and held 2^7 times as large as the maximum says: it reaches 2^15, its step below 2^-14 is 2^-31
+// of the largest weight) whatever the queries' type; the sum takes it unrounded. The maximum is
+// raised only where a score passes it by 8 (in powers of two), so most steps exchange nothing
+// between lanes.
 //
 // A wave holds columns, 16 query heads a tile: heads of one token, or heads of several tokens that
-// share a key/value head. It takes 64 keys a step, four subtiles of 16 slots, lane group g (lanes 16 g
-// to 16 g + 15) having subtile g:
-//   S^T [keys x columns] = K Q^T     four products of 16 keys: row m of product j is slot 4 j + m % 4
-//                                  of subtile m / 4, so that lane group g gets slots 4 j .. 4 j + 3
-//                                  of its own subtile: 16 neighbouring slots over the four products;
-//   O^T [channels x columns] += V^T P^T   the weights are where the first product left them, and the
-//                                  operand V^T is 16 bytes of a channel (values lie transposed).
+// share a key/value head. It takes 64 keys a step, four subtiles of 16 slots, lane group g (lanes
+// 16 g to 16 g + 15) having subtile g:
+//   S^T [keys x columns] = K Q^T: four products of 16 keys, row m of product j being slot 4 j + m % 4
+//     of subtile m / 4, so that lane group g gets slots 4 j .. 4 j + 3 of its own subtile: 16
+//     neighbouring slots over the four products;
+//   O^T [channels x columns] += V^T P^T: the weights are where the first product left them, and the
+//     operand V^T is 16 bytes of a channel (values lie transposed).
 // A lane's column is one head in both products: maxima, sums and rescaling stay in the lane.
 //
 // An operand's neighbouring lanes hold different rows (keys, channels). Loaded like that, every
 // lane's 16 bytes are an access of their own (56 of 64 lanes' counted; prompts of 2053 tokens were
 // bound by that, 210 us). So memory is read in its own order, 1 KiB a load, straight to the wave's
 // own LDS, and the operands from there: the next step's keys as soon as this one's are read, its
-// values likewise. 16-byte chunks are permuted by the row where they are loaded, so that those of one
-// read lie in different banks.
+// values likewise. 16-byte chunks are permuted by the row where they are loaded, so that those of
+// one read lie in different banks.
 #pragma once
 
 #include <type_traits>
@@ -82,8 +83,8 @@ __device__ inline v8h codes_of_128() {
   return x.v;
 }
 
-// A lane's 16 bytes at `from` straight to lds + 16 lane. STREAM: of rows that are read once (not kept
-// in L2 before others).
+// A lane's 16 bytes at `from` straight to lds + 16 lane. STREAM: of rows that are read once (not
+// kept in L2 before others).
 template <bool STREAM>
 __device__ inline void load_to_lds(const int8_t* from, char* lds) {
   auto* g = (const __attribute__((address_space(1))) void*)(from);
@@ -95,9 +96,9 @@ __device__ inline void load_to_lds(const int8_t* from, char* lds) {
   }
 }
 
-// N reads of 16 bytes from LDS, STEP bytes apart, waited for. As instructions of the compiler's they
-// would wait for every load to LDS under way (it cannot tell the places apart); here the caller has
-// waited for the ones that count.
+// N reads of 16 bytes from LDS, STEP bytes apart, waited for. As instructions of the compiler's
+// they would wait for every load to LDS under way (it cannot tell the places apart); here the
+// caller has waited for the ones that count.
 __device__ inline uint32_t lds_address(const void* p) {
   return static_cast<uint32_t>(
       reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) char*)(p)));
@@ -141,8 +142,8 @@ __device__ inline int key_chunk(int row, int c) {
   if constexpr (D == 128) return c ^ (b1 | s0 << 1 | (s1 ^ b0) << 2);
   return c < D / 64 * 4 ? c ^ (s0 | (s1 ^ b1) << 1) : c;
 }
-// Staged values: pages of 64 slots and more: channels of four chunks, one a subtile; pages of 32: page
-// by page, channels of two; pages of 16: subtile by subtile, channels of one.
+// Staged values: pages of 64 slots and more: channels of four chunks, one a subtile; pages of 32:
+// page by page, channels of two; pages of 16: subtile by subtile, channels of one.
 template <int D, int SHIFT>
 __device__ inline int value_offset(int channel, int sub) {
   if constexpr (SHIFT >= 6) {
@@ -155,8 +156,8 @@ __device__ inline int value_offset(int channel, int sub) {
   }
 }
 
-// The largest of 16 numbers (NaN passed over) in 8 instructions; fmaxf would first quiet each, which
-// costs as many again. For results that have settled.
+// The largest of 16 numbers (NaN passed over) in 8 instructions; fmaxf would first quiet each,
+// which costs as many again. For results that have settled.
 __device__ inline float max3(float a, float b, float c) {
   float x;
   asm("v_max3_f32 %0, %1, %2, %3" : "=v"(x) : "v"(a), "v"(b), "v"(c));
@@ -209,8 +210,8 @@ __device__ inline float lane_value(float x, int lane) {
 }
 
 // A wave's queries, accumulators and sums: CT tiles of 16 columns, lane % 16 of each tile this
-// lane's. acc: channel 16 i + 4 (lane / 16) + r, in units of kCodeUnit and with 128 sum(p) too much,
-// which is in `over`; m: the maximum of t less kLift, l: this lane's share of the sum.
+// lane's. acc: channel 16 i + 4 (lane / 16) + r, in units of kCodeUnit and with 128 sum(p) too
+// much, which is in `over`; m: the maximum of t less kLift, l: this lane's share of the sum.
 template <class E, int D, int SHIFT, int CT>
 struct Int8Wave {
   using V8 = typename Kv<E>::V8;
@@ -220,8 +221,8 @@ struct Int8Wave {
   static constexpr float kLift = 7.0f;            // maximum - m
   v4f acc[CT][DT], over[CT];
   float m[CT], l[CT];
-  // Two tiles' queries stay in LDS: in registers they would spill others beside the next step's keys
-  // and values.
+  // Two tiles' queries stay in LDS: in registers they would spill others beside the next step's
+  // keys and values.
   static constexpr bool kQueriesInLds = CT > 1;
   v8h qf[kQueriesInLds ? 1 : KS];
   const v8h* q_lds;  // [CT][KS][64]
@@ -229,7 +230,7 @@ struct Int8Wave {
   float start[CT];   // -128 sum(q), in units of kCodeUnit
   bool odd[CT];      // the column's query is not finite
   static constexpr int LOADS = D / 16;  // of 64 keys' codes, of their values': 1 KiB each
-  static constexpr int STAGE = 64 * D;  // bytes of a step's keys in the wave's LDS, and of its values
+  static constexpr int STAGE = 64 * D;  // bytes of a step's keys in the wave's LDS; its values too
 
   __device__ void clear() {
 #pragma unroll
@@ -245,7 +246,8 @@ struct Int8Wave {
   __device__ static int channel(int s, int grp) {
     return s < 2 * KL ? 64 * (s >> 1) + 16 * grp + 8 * (s & 1) : 64 * KL + 8 * grp;
   }
-  // This lane's column of a tile is query head `head` of token t (its first row where it is not `real`).
+  // This lane's column of a tile is query head `head` of token t (its first row where it is not
+  // `real`).
   __device__ static void fetch_q(const AttendInt8Args& a, int64_t t, int64_t head, bool real,
                                  V8 (&x)[KS]) {
     const E* q = static_cast<const E*>(a.q) + (real ? t * a.q_st + head * a.q_sh : 0);
@@ -346,7 +348,8 @@ struct Int8Wave {
         buffer_load_lds<16, STREAM>(first, 16 * D, in - x / EACH * (16 * D), lds + x * 1024);
       } else {
         const int from = 4 * quad + (row >> 4);
-        load_to_lds<STREAM>(rows(__shfl(s.page, from), __shfl(s.at, from)) + (in - (row >> 4) * (16 * D)),
+        const int8_t* const mine = rows(__shfl(s.page, from), __shfl(s.at, from));
+        load_to_lds<STREAM>(mine + (in - (row >> 4) * (16 * D)),
                             lds + x * 1024);
       }
     }
@@ -432,9 +435,9 @@ struct Int8Wave {
     }
     l[c] = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), inv, l[c]);
   }
-  // One step on what load_k and load_v have under way to `keys` and `values`; `fetch_k` and `fetch_v`
-  // start the next one's loads there (`more`) as soon as this one's operands are read. counts, n: of
-  // each tile's column in this lane's subtile; `some`: a lane's n is not 16.
+  // One step on what load_k and load_v have under way to `keys` and `values`; `fetch_k` and
+  // `fetch_v` start the next one's loads there (`more`) as soon as this one's operands are read.
+  // counts, n: of each tile's column in this lane's subtile; `some`: a lane's n is not 16.
   template <class FK, class FV>
   __device__ void step(const char* keys, const char* values, const Step& s,
                        const bool (&counts)[CT], const int (&n)[CT], bool some, bool more,
@@ -541,8 +544,8 @@ struct Int8Wave {
   // One step of tile c over a sequence's open block: 16-bit rows, in their own type. This lane's
   // subtile begins at slot `first`, its column (head hq of token t) has n keys of it; n_most, the
   // most of any column. Once a list at most, so the queries are read again. Values that are not
-  // finite would reach the columns that do not have them (0 times infinity): where there are any, each
-  // token's sums are taken alone.
+  // finite would reach the columns that do not have them (0 times infinity): where there are any,
+  // each token's sums are taken alone.
   __device__ void open_step(const AttendInt8Args& a, int c, int64_t seq, int head, int64_t t,
                             int64_t hq, bool real, int first, int n, int n_most, int tokens,
                             int tok) {
@@ -631,8 +634,8 @@ constexpr int attend_int8_waves(int D) { return D > 128 ? 1 : 2; }
 template <class E, int D, int SHIFT>
 struct SplitWave : Int8Wave<E, D, SHIFT, 1> {
   using Base = Int8Wave<E, D, SHIFT, 1>;
-  // Chunk `chunk` of this wave's units of 64 keys (units part, part + parts, ...): a subtile a lane,
-  // those with keys in codes (`full`) and in the open block. False: past the list's end.
+  // Chunk `chunk` of this wave's units of 64 keys (units part, part + parts, ...): a subtile a
+  // lane, those with keys in codes (`full`) and in the open block. False: past the list's end.
   __device__ static bool fetch(const AttendInt8Args& a, const int32_t* list, const KvPlace& place,
                                int head, int part, int parts, int chunk, Subtile& s,
                                uint64_t& full, uint64_t& open) {
@@ -757,9 +760,10 @@ __global__ void __launch_bounds__(kAttendWaves* kWave, attend_int8_waves(D))
 }
 
 // Prompts: a workgroup holds the heads of several neighbouring tokens (CT tiles of 16 columns,
-// floor(16 / G) tokens each) and passes once over all the blocks that any of them lists, each column
-// counting its own: neighbours mostly choose alike, so a block's codes are loaded and widened once
-// for them. Its waves take the steps in turn, each with all the columns, and join their sums.
+// floor(16 / G) tokens each) and passes once over all the blocks that any of them lists, each
+// column counting its own: neighbours mostly choose alike, so a block's codes are loaded and
+// widened once for them. Its waves take the steps in turn, each with all the columns, and join
+// their sums.
 //
 // The lists are joined by physical page in a hash table in LDS: of a page's entries the first (by
 // token, then place) stands for all and holds the tokens' bits; the pages are taken in the order of

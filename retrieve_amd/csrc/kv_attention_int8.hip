@@ -53,6 +53,10 @@ extern "C" int rt_kv_attention_int8(
   if (const int st = kv_check(T, Hq, Hkv, D, dtype, B, max_pages, P, page)) return st;
   RT_CHECK_ARG(count >= 0 && count <= (1 << 20), "count must be in [0, 2^20], got %lld",
                static_cast<long long>(count));
+  RT_CHECK_ARG(std::isfinite(scale * kLog2e), "the scale must be finite, got %g",
+               static_cast<double>(scale));
+  RT_CHECK_ARG(sequences >= 0, "sequences must not be negative, got %lld",
+               static_cast<long long>(sequences));
   if (T == 0) return kOk;
   RT_CHECK_ARG(q && positions && seq_ids && out && lse && (count == 0 || blocks), "null pointer");
   RT_CHECK_ARG(B * max_pages == 0 || page_table, "null page table");
@@ -63,10 +67,6 @@ extern "C" int rt_kv_attention_int8(
   RT_CHECK_ARG(kv_rows_aligned(q, q_token_stride, q_head_stride) && kv_rows_aligned(out, 0, 0),
                "rows must start on 16 bytes");
   RT_CHECK_ARG(T * Hq <= INT32_MAX, "too many tokens");
-  RT_CHECK_ARG(std::isfinite(scale * kLog2e), "the scale must be finite, got %g",
-               static_cast<double>(scale));
-  RT_CHECK_ARG(sequences >= 0, "sequences must not be negative, got %lld",
-               static_cast<long long>(sequences));
   const size_t need = rt_kv_attention_int8_workspace(T, Hq, Hkv, D, page, count);
   if (workspace_bytes < need || (need > 0 && workspace == nullptr)) {
     set_error("workspace too small: %zu < %zu", workspace_bytes, need);

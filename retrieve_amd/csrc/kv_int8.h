@@ -1,11 +1,11 @@
 // The paged cache in 8 bits: its layout, and the code of a block's keys or values.
 //
-// A full block of one head holds its keys as int8 codes [page, D] and its values as codes [D, page],
-// each with one scale (a code stands for code * scale). A sequence's last block, not full yet, lies
-// in 16 bits in the sequence's open block, k_tail [page, D] and v_tail [D, page]; its page's scales
-// are 0 until it is full. So a code depends on its block's 16-bit numbers alone, never on how many
-// calls wrote them, and the latest keys are exact. Values lie transposed so that attention's second
-// product takes its operand (16 slots of a channel) straight from memory.
+// A full block of one head holds its keys as int8 codes [page, D] and its values transposed, codes
+// [D, page], each with one scale (a code stands for code * scale). A sequence's last block, not full
+// yet, lies in 16 bits in the sequence's open block, k_tail [page, D] and v_tail [D, page]; its
+// page's scales are 0 until it is full. So a code depends on its block's 16-bit numbers alone,
+// never on how many calls wrote them, and the latest keys are exact. Transposed values give
+// attention's second product its operand (16 slots of a channel) as it lies in memory.
 #pragma once
 
 #include "kv_common.h"
@@ -20,10 +20,10 @@ struct KvInt8 {
 
 // Codes of one block: code = 127 x / top to the nearest even, top its largest finite magnitude
 // (floored at kKvTopFloor). 127 x is exact (18 bits at most), and q + r (y - q top) with q = y r is
-// the quotient of y = 127 x rounded to nearest (kv_code_value's comment), so a tie between two codes
-// is seen as one. Adding 1.5 2^23 rounds it to a whole number, whose byte is the last one of the sum.
-// `odd` blocks: infinities become +-127, NaN 0; a top above 2^100, whose reciprocal may lose bits,
-// comes in scaled by 2^-64 with its numbers.
+// the quotient of y = 127 x rounded to nearest (kv_code_value's comment), so a tie between two
+// codes is seen as one. Adding 1.5 2^23 rounds it to a whole number, whose byte is the last one of
+// the sum. `odd` blocks: infinities become +-127, NaN 0; a top above 2^100, whose reciprocal may
+// lose bits, comes in scaled by 2^-64 with its numbers.
 struct BlockCode {
   float top, r, shrink;
   bool odd;
@@ -58,8 +58,8 @@ __device__ inline float finite_size(float x) {
   return a < INFINITY ? a : 0.0f;
 }
 
-// Numbers of 16 bits two at a time, as whole numbers: their magnitudes order like the bits below the
-// sign, and they themselves like two's complement once negative ones have these bits flipped.
+// Numbers of 16 bits two at a time, as whole numbers: their magnitudes order like the bits below
+// the sign, and they themselves like two's complement once negative ones have these bits flipped.
 typedef unsigned short v2u16 __attribute__((ext_vector_type(2)));
 typedef short v2i16 __attribute__((ext_vector_type(2)));
 __device__ inline v2u16 max_magnitude(v2u16 most, uint32_t x) {

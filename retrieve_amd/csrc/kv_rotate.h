@@ -1,10 +1,10 @@
 // The rotary position, and the norm before it, of one row's chunks of 8 channels: what the paged
 // cache's appending kernels apply to queries and keys on their way.
 //
-// Norm: y = x r w with r = 1 / sqrt(mean(x^2) + eps). The sum runs in 64 bits (the squares of 16-bit
-// numbers are exact there, so r does not depend on the order in which lanes add), r is rounded once
-// to fp32 and each of the two products once more: the same bits in whichever lane layout, so a
-// block's codes do not depend on how its tokens were split over calls.
+// Norm: y = x r w with r = 1 / sqrt(mean(x^2) + eps). The sum runs in 64 bits (the squares of
+// 16-bit numbers are exact there, so r does not depend on the order in which lanes add), r is
+// rounded once to fp32 and each of the two products once more: the same bits in whichever lane
+// layout, so a block's codes do not depend on how its tokens were split over calls.
 //
 // Rotation: with (c, s) the table's cosine and sine of the token's position, a pair of channels
 // (a, b) becomes (a c - b s, b c + a s), every product and sum rounded once to fp32 (no fused
@@ -44,8 +44,8 @@ __device__ inline float rot_second(float b, float a, float c, float s) {
   return b * c + a * s;
 }
 
-// The cosines and sines of a chunk's channels at a position (1, 0 past the rotated part); neighbours
-// that turn together share theirs.
+// The cosines and sines of a chunk's channels at a position (1, 0 past the rotated part);
+// neighbours that turn together share theirs.
 template <int MODE>
 struct Turn {
   static constexpr int N = MODE == kRotPairs ? 4 : 8;
@@ -125,8 +125,8 @@ __device__ inline float row_scale(const typename Kv<E>::V8 (&x)[N], int part, do
     const int base = lane_id() - part;
     sum = (__shfl(sum, base) + __shfl(sum, base + P)) + __shfl(sum, base + 2 * P);
   }
-  // 1 / sqrt by two Newton steps on the instruction's 23 bits (a division and a root in 64 bits take
-  // 45 instructions); infinite and 0 (of 0 and of an infinity) as it gives them.
+  // 1 / sqrt by two Newton steps on the instruction's 23 bits (a division and a root in 64 bits
+  // take 45 instructions); infinite and 0 (of 0 and of an infinity) as it gives them.
   const double mean = sum * (1.0 / D) + eps;
   double y = __builtin_amdgcn_rsq(mean);
   if (y > 0.0 && y < INFINITY) {
@@ -198,9 +198,9 @@ __device__ inline typename Kv<E>::V8 turned_chunk(const E* row, typename Kv<E>::
   return out;
 }
 
-// A lane's two chunks of a row, what turns them and the norms' weights. Split halves: partners in the
-// rotated part, neighbours' distance apart in the rest; otherwise the same place in either half of
-// the row.
+// A lane's two chunks of a row, what turns them and the norms' weights. Split halves: partners in
+// the rotated part, neighbours' distance apart in the rest; otherwise the same place in either half
+// of the row.
 template <class E, int D, int MODE, bool NORM>
 struct Pair {
   using V8 = typename Kv<E>::V8;
