@@ -509,6 +509,9 @@ struct Int8Wave {
     v8h p[CT][2];
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
+      // (a tile none of whose columns counts the step: weights of 0, without their exponentials)
+      p[c][0] = p[c][1] = v8h{};
+      if (CT > 1 && !__any(counts[c])) continue;
       weigh(c, sc[c], s.ks * factor[c], s.lift, s.inv, counts[c], n[c], some, p[c]);
     }
     constexpr int ROW = SHIFT >= 6 ? 64 : SHIFT == 5 ? 32 : 16;  // bytes of a staged channel
