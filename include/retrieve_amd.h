@@ -616,9 +616,9 @@ int rt_kv_append_norm(const void* q, int64_t q_token_stride, int64_t q_head_stri
  * codes rint(127 x / a) with a = max(max |x| over the block's finite keys of the head, 1e-8) and
  * scale a / 127 (infinities +-127, NaN 0), its values the same. The other tokens' rows go to the
  * open block and their page's scales become 0. A call's tokens of a sequence lie side by side, in
- * order, and are its end from then on: positions behind them are no longer held. A sequence that
- * goes on inside a block that was full (it has been cut back) has the block's earlier tokens from
- * their codes. */
+ * order, at consecutive positions whose blocks have pages (or none from some block on), and are its
+ * end from then on: positions behind them are no longer held. A sequence that goes on inside a
+ * block that was full (it has been cut back) has the block's earlier tokens from their codes. */
 int rt_kv_append_int8(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
                       int64_t k_token_stride, int64_t k_head_stride, const void* v,
                       int64_t v_token_stride, int64_t v_head_stride, int64_t T, int64_t Hq,

@@ -20,7 +20,8 @@
 // Bound by memory: every row is read and written once. 32768 tokens of 32 rows of 256 channels take
 // 229 to 234 us (4.8 TB/s, what a large copy reaches) with nontemporal loads and stores (when they
 // were taken 238, 283 with ordinary stores; four rows in flight instead of two 250). A decode step
-// is bound by its launch (3 us).
+// is bound by its launch (3 us). With norms 9001 tokens of 48 rows of 128 channels take 54 us (47 at
+// that rate), a decode step 4.
 #include <type_traits>
 
 #include "../../include/retrieve_amd.h"

@@ -54,9 +54,9 @@ extern "C" int rt_kv_append_int8(
   // a block's codes of values; least and largest keys (32 numbers of 16 bits a thread)
   const int64_t codes = page * D, ends = write_threads(D) * 32 * 2;
   const unsigned lds = static_cast<unsigned>(codes > ends ? codes : ends);
-  AppendInt8* const launch = dtype == kKvBf16 ? D > 128 ? append_int8_bf16_256 : append_int8_bf16_128
-                             : D > 128        ? append_int8_f16_256
-                                              : append_int8_f16_128;
+  AppendInt8* const launch =
+      dtype == kKvBf16 ? (D > 128 ? append_int8_bf16_256 : append_int8_bf16_128)
+                       : (D > 128 ? append_int8_f16_256 : append_int8_f16_128);
   return launch(D, a, static_cast<unsigned>(grid), lds, interleaved != 0,
                 static_cast<hipStream_t>(stream));
 }

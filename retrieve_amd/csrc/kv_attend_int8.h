@@ -23,8 +23,8 @@
 // A wave holds columns, 16 query heads a tile: heads of one token, or heads of several tokens that
 // share a key/value head. It takes 64 keys a step, four subtiles of 16 slots, lane group g (lanes
 // 16 g to 16 g + 15) having subtile g:
-//   S^T [keys x columns] = K Q^T: four products of 16 keys, row m of product j being slot 4 j + m % 4
-//     of subtile m / 4, so that lane group g gets slots 4 j .. 4 j + 3 of its own subtile: 16
+//   S^T [keys x columns] = K Q^T: four products of 16 keys, row m of product j being slot 4 j +
+//     m % 4 of subtile m / 4, so that lane group g gets slots 4 j .. 4 j + 3 of its own subtile: 16
 //     neighbouring slots over the four products;
 //   O^T [channels x columns] += V^T P^T: the weights are where the first product left them, and the
 //     operand V^T is 16 bytes of a channel (values lie transposed).
@@ -36,6 +36,13 @@
 // own LDS, and the operands from there: the next step's keys as soon as this one's are read, its
 // values likewise. 16-byte chunks are permuted by the row where they are loaded, so that those of
 // one read lie in different banks.
+//
+// Single tokens are bound by memory: 64 of them over 64 blocks of 64 keys (8 heads of 128 channels,
+// 526 MB of codes) take 93 us, 5.6 TB/s; about 15 us of that are the start (lists, pages and scales
+// are looked up one after the other before the first codes) and the end, the rest runs at 6.7 TB/s.
+// Prompts are bound by the vector instructions: 2053 tokens over 16 blocks each take 154 us, of
+// which a third makes codes into fp16 and a third is the softmax. 8 tokens share a pass there; 4,
+// whose codes are widened for one tile of columns, take 169.
 #pragma once
 
 #include <type_traits>

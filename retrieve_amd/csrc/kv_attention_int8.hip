@@ -15,12 +15,12 @@ inline AttendInt8Plan attend_int8_plan(int64_t T, int64_t Hq, int64_t Hkv, int64
   p.rows = T * Hkv * p.tiles;
   p.parts = 0;
   // Prompts: as many neighbouring tokens a workgroup as two tiles of columns hold, the table of
-  // their lists takes and leave two workgroups a CU. Two or more join their lists: over 1024 keys of
-  // 8 heads of 128 channels 128 tokens take 25 us and 37 split, 256 30 and 59, 1024 97 and 209 (of
-  // 64 channels 128 tokens 17 and 21, of 256 73 and 120). One token a workgroup would take what it
-  // takes split where the lists are short (64 tokens: 20 and 21), and longer where they are not.
-  // Where most sequences have one token there is less to share: 256 tokens of 250 take 135 joined and
-  // 125 split, of 128 sequences (64 blocks each) 280 and 253, of 64 (16 blocks) 63 and 89.
+  // their lists takes and leave two workgroups a CU. Two or more join their lists: over 1024 keys
+  // of 8 heads of 128 channels 128 tokens take 25 us and 37 split, 256 30 and 59, 1024 97 and 209
+  // (of 64 channels 128 tokens 17 and 21, of 256 73 and 120). One token a workgroup would take what
+  // it takes split where the lists are short (64 tokens: 20 and 21), and longer where they are not.
+  // Where most sequences have one token there is less to share: 256 tokens of 250 take 135 joined
+  // and 125 split, of 128 sequences (64 blocks each) 280 and 253, of 64 (16 blocks) 63 and 89.
   int64_t joined = T > 2 * seqs && G <= 16 ? 2 * (16 / G) : 0;
   while (joined > 1 && (joined * count > kJoinEntries || cdiv(T, joined) * Hkv < 512)) joined /= 2;
   p.joined = static_cast<int32_t>(joined);

@@ -1,9 +1,9 @@
 // The paged cache in 8 bits: its layout, and the code of a block's keys or values.
 //
 // A full block of one head holds its keys as int8 codes [page, D] and its values transposed, codes
-// [D, page], each with one scale (a code stands for code * scale). A sequence's last block, not full
-// yet, lies in 16 bits in the sequence's open block, k_tail [page, D] and v_tail [D, page]; its
-// page's scales are 0 until it is full. So a code depends on its block's 16-bit numbers alone,
+// [D, page], each with one scale (a code stands for code * scale). A sequence's last block, not
+// full yet, lies in 16 bits in the sequence's open block, k_tail [page, D] and v_tail [D, page];
+// its page's scales are 0 until it is full. So a code depends on its block's 16-bit numbers alone,
 // never on how many calls wrote them, and the latest keys are exact. Transposed values give
 // attention's second product its operand (16 slots of a channel) as it lies in memory.
 #pragma once

@@ -19,8 +19,9 @@ Tokens are packed: token ``t`` is at ``positions[t]`` of sequence ``seq_ids[t]``
 int32. One token a sequence is a decode step, many a prompt; a call may mix them. Caches are ``[P,
 Hkv, page, D]`` (a block of one head is contiguous), bounds int8 ``[P, Hkv, 2 D]`` with scales fp32
 ``[P, Hkv]``. :class:`PagedCache` (:class:`Int8PagedCache`) holds them and makes the calls;
-:func:`rotary_table` builds the table of cosines and sines. No counterpart in the reference; serving only: the ops have no
-gradients (a backward pass through one warns and stops there, a forward-mode tangent is refused).
+:func:`rotary_table` builds the table of cosines and sines. No counterpart in the reference; serving
+only: the ops have no gradients (a backward pass through one warns and stops there, a forward-mode
+tangent is refused).
 
 The ops check their arguments here (``ValueError`` on shapes, ``TypeError`` on dtypes), allocate
 from torch's caching allocator and enqueue on torch's current stream, without a host
@@ -61,8 +62,8 @@ _lib8.define("append(Tensor q, Tensor k, Tensor v, Tensor? cos_sin, Tensor posit
              "Tensor(g!) bounds, Tensor(h!) bound_scales, bool interleaved=False, "
              "Tensor? q_weight=None, Tensor? k_weight=None, float eps=1e-6) -> Tensor")
 _lib8.define("read(Tensor k_codes, Tensor v_codes, Tensor k_scales, Tensor v_scales, "
-             "Tensor k_tail, Tensor v_tail, Tensor positions, Tensor seq_ids, Tensor page_table) -> "
-             "(Tensor, Tensor)")
+             "Tensor k_tail, Tensor v_tail, Tensor positions, Tensor seq_ids, Tensor page_table) "
+             "-> (Tensor, Tensor)")
 _lib8.define("block_attention(Tensor q, Tensor k_codes, Tensor v_codes, Tensor k_scales, "
              "Tensor v_scales, Tensor k_tail, Tensor v_tail, Tensor blocks, Tensor positions, "
              "Tensor seq_ids, Tensor page_table, float? scale=None, int? sequences=None) -> "
@@ -283,9 +284,9 @@ def append(q: Tensor, k: Tensor, v: Tensor, cos_sin: Tensor | None, positions: T
     0, or past the page table or ``cos_sin``; a sequence outside it; no page) write nothing and
     return a zero row.
 
-    ``q_weight``, ``k_weight`` ``[D]`` (of ``q``'s dtype, or float32): each head of the queries, of the
-    keys is normed before the rotation, ``x / sqrt(mean(x ** 2) + eps) * weight``: the sum in 64 bits,
-    then fp32 up to the one rounding behind the rotation."""
+    ``q_weight``, ``k_weight`` ``[D]`` (of ``q``'s dtype, or float32): each head of the queries, of
+    the keys is normed before the rotation, ``x / sqrt(mean(x ** 2) + eps) * weight``: the sum in 64
+    bits, then fp32 up to the one rounding behind the rotation."""
     args = (q, k, v, cos_sin, positions, seq_ids, page_table, k_cache, v_cache, bounds,
             bound_scales)
     call = _append if _eager(*args, q_weight, k_weight) else torch.ops.retrieve_kv.append
@@ -470,18 +471,20 @@ def append_int8(q: Tensor, k: Tensor, v: Tensor, cos_sin: Tensor | None, positio
                 k_scales: Tensor, v_scales: Tensor, k_tail: Tensor, v_tail: Tensor, bounds: Tensor,
                 bound_scales: Tensor, interleaved: bool = False, q_weight: Tensor | None = None,
                 k_weight: Tensor | None = None, eps: float = 1e-6) -> Tensor:
-    """:func:`append` into a cache in 8 bits: ``k_codes`` int8 ``[P, Hkv, page, D]``, ``v_codes`` int8
-    ``[P, Hkv, D, page]`` (values transposed), ``k_scales``, ``v_scales`` fp32 ``[P, Hkv]`` (zeros to
-    begin with) and the sequences' open blocks in 16 bits, ``k_tail [B, Hkv, page, D]`` and ``v_tail
-    [B, Hkv, D, page]``, one for each row of the page table. Returns the rotated queries.
+    """:func:`append` into a cache in 8 bits: ``k_codes`` int8 ``[P, Hkv, page, D]``, ``v_codes``
+    int8 ``[P, Hkv, D, page]`` (values transposed), ``k_scales``, ``v_scales`` fp32 ``[P, Hkv]``
+    (zeros to begin with) and the sequences' open blocks in 16 bits, ``k_tail [B, Hkv, page, D]``
+    and ``v_tail [B, Hkv, D, page]``, one for each row of the page table. Returns the rotated
+    queries.
 
     A token at the last slot of its block completes it: its keys of a head (rotated, in 16 bits)
     become codes ``round(127 x / a)`` of one scale ``a / 127``, ``a`` the largest finite magnitude
     (1e-8 at least); infinities become ``+-127``, NaN 0; its values the same. The bounds are
     :func:`append`'s. Until then its tokens lie in the open block and its page's scales are 0.
 
-    A call's tokens of a sequence lie side by side, in order, and are its end from then on: what it
-    held at later positions is dropped. A sequence may be cut back so, also into a block that was
+    A call's tokens of a sequence lie side by side, in order, at consecutive positions whose blocks
+    have pages (or none from some block on), and are its end from then on: what it held at later
+    positions is dropped. A sequence may be cut back so, also into a block that was
     full (whose earlier tokens then come from their codes). Sequences may share full pages, not an
     open block."""
     args = (q, k, v, cos_sin, positions, seq_ids, page_table, k_codes, v_codes, k_scales, v_scales,
@@ -512,10 +515,10 @@ def _read_int8(k_codes, v_codes, k_scales, v_scales, k_tail, v_tail, positions, 
 def read_int8(k_codes: Tensor, v_codes: Tensor, k_scales: Tensor, v_scales: Tensor, k_tail: Tensor,
               v_tail: Tensor, positions: Tensor, seq_ids: Tensor, page_table: Tensor
               ) -> tuple[Tensor, Tensor]:
-    """Tokens of a cache in 8 bits (:func:`append_int8`'s tensors) in 16 bits again: ``(k, v)``, each
-    ``[T, Hkv, D]``, the keys rotated as they are held. Codes times their scale, rounded once; tokens
-    of the open block as they were appended; zeros for padding and for blocks without a page. Tokens
-    may come in any order, runs of one sequence are read fastest."""
+    """Tokens of a cache in 8 bits (:func:`append_int8`'s tensors) in 16 bits again: ``(k, v)``,
+    each ``[T, Hkv, D]``, the keys rotated as they are held. Codes times their scale, rounded once;
+    tokens of the open block as they were appended; zeros for padding and for blocks without a page.
+    Tokens may come in any order, runs of one sequence are read fastest."""
     args = (k_codes, v_codes, k_scales, v_scales, k_tail, v_tail, positions, seq_ids, page_table)
     call = _read_int8 if _eager(*args) else torch.ops.retrieve_kv_int8.read
     return call(*args)
@@ -553,10 +556,10 @@ def block_attention_int8(q: Tensor, k_codes: Tensor, v_codes: Tensor, k_scales: 
                          positions: Tensor, seq_ids: Tensor, page_table: Tensor,
                          scale: float | None = None, sequences: int | None = None
                          ) -> tuple[Tensor, Tensor]:
-    """:func:`block_attention` over a cache in 8 bits (:func:`append_int8`'s tensors): a full block's
-    keys and values are what their codes stand for (never rounded to 16 bits), the token's own block
-    is read from its sequence's open block while it is not full. Listed blocks before it that were
-    never filled are skipped. The row of a query that is not finite is not a number."""
+    """:func:`block_attention` over a cache in 8 bits (:func:`append_int8`'s tensors): a full
+    block's keys and values are what their codes stand for (never rounded to 16 bits), the token's
+    own block is read from its sequence's open block while it is not full. Listed blocks before it
+    that were never filled are skipped. The row of a query that is not finite is not a number."""
     args = (q, k_codes, v_codes, k_scales, v_scales, k_tail, v_tail, blocks, positions, seq_ids,
             page_table)
     call = _attention_int8 if _eager(*args) else torch.ops.retrieve_kv_int8.block_attention
