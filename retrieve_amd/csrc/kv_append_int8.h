@@ -223,7 +223,7 @@ struct Fill {
            (static_cast<int64_t>(page) * a.Hkv + head);
   }
 
-  // A block that had been full and is gone on with behind slot `from`: its earlier rows in the open
+  // A block that had been full and stays open behind slot `from`: its earlier rows to the open
   // block, eight channels of a slot (values: eight slots of a channel) a thread.
   __device__ void reopen(int32_t page, int32_t seq, int from) const {
     const float scale = *scale_of(page);
@@ -233,12 +233,11 @@ struct Fill {
     for (int i = threadIdx.x; i < size * D / 8; i += THREADS) {
       const int slot = VALUES ? i % line * 8 : i / line;
       if (slot >= from) continue;
-      typedef int V2i __attribute__((ext_vector_type(2)));
-      const V2i c = *reinterpret_cast<const V2i*>(codes + 8 * i);
+      const V8 x = numbers(codes + 8 * i, scale);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         if (VALUES && slot + e >= from) break;
-        to[8 * i + e] = static_cast<E>(static_cast<int8_t>(c[e >> 2] >> (8 * (e & 3))) * scale);
+        to[8 * i + e] = x[e];
       }
     }
     __syncthreads();  // (everyone has read the scale)
@@ -268,15 +267,35 @@ struct Fill {
       }
     }
   }
+  // Eight codes as the 16-bit numbers that they stand for.
+  __device__ static V8 numbers(const int8_t* codes, float scale) {
+    typedef int V2i __attribute__((ext_vector_type(2)));
+    const V2i c = *reinterpret_cast<const V2i*>(codes);
+    V8 x;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      x[e] = static_cast<E>(static_cast<int8_t>(c[e >> 2] >> (8 * (e & 3))) * scale);
+    }
+    return x;
+  }
+  // Where the rows before this call's tokens are: the sequence's open block, or the codes of `page`
+  // where it had been full (`scale` > 0; the open block then stays as it is).
+  struct Earlier {
+    int32_t seq, page;
+    int count;  // of them
+    float scale;
+  };
   // Earlier values, eight slots of a channel a thread (they lie transposed): f(slot, channel, eight
   // numbers).
   template <class F>
-  __device__ void earlier_values(int32_t seq, int count, F&& f) const {
+  __device__ void earlier_values(const Earlier& had, F&& f) const {
     const int line = 1 << (a.tok.shift - 3);
     const V8* from = reinterpret_cast<const V8*>(static_cast<const E*>(a.cache.v_tail) +
-                                                 block(seq) * D);
+                                                 block(had.seq) * D);
+    const int8_t* codes = a.cache.v_codes + block(had.page) * D;
     for (int i = threadIdx.x; i < line * D; i += THREADS) {
-      if (i % line * 8 < count) f(i % line * 8, i / line, from[i]);
+      if (i % line * 8 >= had.count) continue;
+      f(i % line * 8, i / line, had.scale > 0.0f ? numbers(codes + 8 * i, had.scale) : from[i]);
     }
   }
   // The staged codes [slot][channel] to the cache: four channels of 16 slots a thread.
@@ -311,7 +330,7 @@ struct Fill {
   }
 
   // The largest finite magnitude of a block that has others.
-  __device__ float finite_most(int32_t seq, int earlier, const V8 (&x)[ALL][2],
+  __device__ float finite_most(const Earlier& had, const V8 (&x)[ALL][2],
                                const bool (&mine)[ALL]) const {
     float most = 0.0f;
 #pragma unroll
@@ -326,10 +345,10 @@ struct Fill {
       }
     }
     if constexpr (VALUES) {
-      earlier_values(seq, earlier, [&](int slot, int, V8 v) {
+      earlier_values(had, [&](int slot, int, V8 v) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          if (slot + e < earlier) most = fmaxf(most, finite_size(static_cast<float>(v[e])));
+          if (slot + e < had.count) most = fmaxf(most, finite_size(static_cast<float>(v[e])));
         }
       });
     }
@@ -355,7 +374,7 @@ struct Fill {
     const uint64_t lo = masks[2], hi = masks[3];
     // (t is among them)
     const int earlier = lo ? __builtin_ctzll(lo) : kWave + __builtin_ctzll(hi);
-    if (earlier > 0 && *scale_of(page) > 0.0f) reopen(page, seq, earlier);
+    const Earlier had{seq, page, earlier, earlier > 0 ? *scale_of(page) : 0.0f};
     V8 x[ALL][2];
     bool mine[ALL];
 #pragma unroll
@@ -366,6 +385,16 @@ struct Fill {
         read(o < earlier ? static_cast<const E*>(a.cache.k_tail) + (block(seq) + o) * D
                          : source(t - (size - 1 - o)),
              x[i]);
+      }
+    }
+    if (!VALUES && had.scale > 0.0f) {  // (the rows of the open block are not this block's)
+#pragma unroll
+      for (int i = 0; i < ALL; ++i) {
+        const int o = row + i * ROWS;
+        if (!mine[i] || o >= earlier) continue;
+        const int8_t* codes = a.cache.k_codes + (block(page) + o) * D;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) x[i][j] = numbers(codes + 8 * pair.chunk[j], had.scale);
       }
     }
     // the largest magnitude, as the 15 bits below the sign
@@ -384,7 +413,7 @@ struct Fill {
       see(x[i][1]);
     }
     if constexpr (VALUES) {
-      earlier_values(seq, earlier, [&](int slot, int, V8 v) {
+      earlier_values(had, [&](int slot, int, V8 v) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           if (slot + e >= earlier) v[e] = static_cast<E>(0.0f);
@@ -395,7 +424,7 @@ struct Fill {
     const int top = group_max<WAVES>(bits[0] > bits[1] ? bits[0] : bits[1], scratch);
     const bool odd = top >= kInfinityBits<E>;
     float most = from_bits<E>(top);
-    if (odd) most = group_max<WAVES>(finite_most(seq, earlier, x, mine), scratch);
+    if (odd) most = group_max<WAVES>(finite_most(had, x, mine), scratch);
     most = fmaxf(most, kKvTopFloor);
     const BlockCode code(most, odd);
     if (threadIdx.x == 0) *scale_of(page) = most / 127.0f;
@@ -405,7 +434,7 @@ struct Fill {
       encode<false>(code, page, x, mine);
     }
     if constexpr (VALUES) {
-      earlier_values(seq, earlier, [&](int slot, int d, V8 v) {
+      earlier_values(had, [&](int slot, int d, V8 v) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           if (slot + e >= earlier) break;

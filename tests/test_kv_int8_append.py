@@ -233,3 +233,27 @@ def test_offsets_past_32_bits(dev):
         assert np.array_equal(back(got[where[:2]]), expected[order[:2]])
     assert np.array_equal(back(kt)[0, :, :5], c.kt[0, :, :5])
     assert int((ks > 0).sum()) == 16
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,d,page", [("bf16", 64, 16), ("fp16", 256, 128)])
+def test_open_rows_behind_the_end_stay(dev, kind, d, page):
+    """A run that completes a block its sequence was cut back into (the earlier rows come from the
+    codes) and ends in the next one, and a run that completes an open block: the open block's rows
+    from the end on are as they were."""
+    had_new = [(page - 3, 5), (2 * page + 9, page - 5), (page // 2, page // 2 + 2)]
+    c, qkv, pos, seq, tab = start(d, page, had_new, 4, 2, d, kind)
+    for i in (tab[0, 0], tab[1, 2]):  # full so far
+        c.ks[i] = c.vs[i] = 0.03
+        c.open_of[0] = c.open_of[1] = None
+    print(f"append int8 {kind} d={d} page={page}: rows behind the end", flush=True)
+    state, before = on_gpu(dev, c), c.copy()
+    got = append(dev, c, state, qkv, 4, 2, None, pos, seq, tab)
+    assert np.array_equal(got, want(c, qkv, 4, 2, None, pos, seq, tab))
+    same(state, c)
+    kt, vt = back(state[0][4]), back(state[0][5])
+    for s, (had, new) in enumerate(had_new):
+        end = (had + new) % page
+        assert 0 < end < had % page
+        assert np.array_equal(kt[s, :, end:], before.kt[s, :, end:]), s
+        assert np.array_equal(vt[s, :, :, end:], before.vt[s, :, :, end:]), s
