@@ -23,8 +23,8 @@
 // instruction (230 to 212), and eight waves a workgroup where a block has more than 128 channels
 // (212 to 189: more rows under way a CU); earlier rows that come from codes are taken there, not by
 // way of the open block (189 to 172 where a call's first blocks have such rows). Workgroups of both
-// kinds alternating in the grid instead of the blocks' first were slower. A decode step is bound by its launch (5 us; 203 tokens of 14
-// heads of 64 11 us).
+// kinds alternating in the grid instead of the blocks' first were slower. A decode step is bound by
+// its launch (5 us; 203 tokens of 14 heads of 64 11 us).
 #pragma once
 
 #include <type_traits>
