@@ -377,3 +377,21 @@ def test_calls_without_tokens(dev, name):
     for x in got if isinstance(got, tuple) else (got,):
         assert x.shape[0] == 0
     assert all(np.array_equal(back(a), back(b)) for a, b in zip(args, before))
+
+
+@pytest.mark.parametrize("d", [64, 256])
+@pytest.mark.parametrize("heads,heads_kv", [(1, 1), (32, 8), (20, 20), (40, 1)])
+def test_the_workspace_holds_every_form(heads, heads_kv, d):
+    """Rows that are split have their parts in the workspace, and the calls of one size have one
+    workspace, however many sequences they name: 16 columns of ``d`` sums, a maximum and a sum for
+    each part, of enough parts for 512 workgroups or as many as the lists have units for."""
+    from retrieve_amd import _native as nat
+
+    need = nat.lib().rt_kv_attention_int8_workspace
+    tiles = -(-(heads // heads_kv) // 16)
+    for tokens in (1, 2, 15, 16, 63, 64, 65, 200, 511, 512, 2000):
+        for count, page in ((1, 16), (16, 64), (96, 16), (600, 128)):
+            rows = tokens * heads_kv * tiles
+            parts = max(1, min(-(-512 // rows), -(-count * page // 256)))
+            want = 4 * rows * parts * 16 * (d + 2) if parts > 1 else 0
+            assert need(tokens, heads, heads_kv, d, page, count) == want, (tokens, count, page)
