@@ -18,7 +18,8 @@
 // and held 2^7 times as large as the maximum says: it reaches 2^15, its step below 2^-14 is 2^-31
 // of the largest weight) whatever the queries' type; the sum takes it unrounded. The maximum is
 // raised only where a score passes it by 8 (in powers of two), so most steps exchange nothing
-// between lanes.
+// between lanes. A score and its maximum meet in one fused multiply-add; of scores past 2^23, where
+// that would differ from the rounded maximum by whole powers of two, each is rounded first (`far`).
 //
 // A wave holds columns, 16 query heads a tile: heads of one token, or heads of several tokens that
 // share a key/value head. It takes 64 keys a step, four subtiles of 16 slots, lane group g (lanes
@@ -226,8 +227,10 @@ struct Int8Wave {
   static constexpr int KL = D / 64;               // 16-byte loads of a key a lane
   static constexpr bool HALF = D % 64 != 0;       // and one of 8 bytes
   static constexpr float kLift = 7.0f;            // maximum - m
+  static constexpr float kFar = 0x1p23f;
   v4f acc[CT][DT], over[CT];
   float m[CT], l[CT];
+  bool far[CT];  // a maximum has been past kFar, in some column of the tile
   // Two tiles' queries stay in LDS: in registers they would spill others beside the next step's
   // keys and values.
   static constexpr bool kQueriesInLds = CT > 1;
@@ -247,6 +250,7 @@ struct Int8Wave {
       over[c] = v4f{0.f, 0.f, 0.f, 0.f};
       m[c] = -3.402823466e38f;
       l[c] = 0.0f;
+      far[c] = false;
     }
   }
   // The first of a lane group's eight channels in step s of the first product.
@@ -398,6 +402,18 @@ struct Int8Wave {
       }
     }
   }
+  // Scores as exponents t, the product and the sum rounded once each: the largest is then its column's
+  // maximum exactly.
+  __device__ static void exponents(v4f (&sc)[4], float f, float lift) {
+#pragma clang fp contract(off)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        sc[j][r] = lift == -INFINITY ? -INFINITY : sc[j][r] * f + lift;
+      }
+    }
+  }
   // The weights of tile c's scores (slot 4 j + r of this lane's subtile): the maximum raised, the
   // sum extended. f multiplies the scores, lift is the logarithm of what the values stand for, inv
   // its inverse. A column has the subtile's first n keys (`some` lane's n is not 16, or its scores
@@ -415,8 +431,17 @@ struct Int8Wave {
     }
     f = fmaxf(f, 1.17549435e-38f);  // (a score of -inf stays that)
     if (!counts) lift = -INFINITY;
-    const float high = fmaf(most_of(sc), f, lift);
-    if (__any(high - m[c] > 8.0f + kLift)) {
+    float high = fmaf(most_of(sc), f, lift);
+    bool raise = __any(high - m[c] > 8.0f + kLift);
+    if (far[c] || (raise && __any(fabsf(high) > kFar && high != -INFINITY))) {
+      far[c] = true;
+      exponents(sc, f, lift);
+      f = 1.0f;
+      lift = 0.0f;
+      high = most_of(sc);
+      raise = __any(high - m[c] > 8.0f + kLift);
+    }
+    if (raise) {
       float next = fmaxf(high, __shfl_xor(high, 16));
       next = fmaxf(next, __shfl_xor(next, 32));
       next = fmaxf(next - kLift, m[c]);
