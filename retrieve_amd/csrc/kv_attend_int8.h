@@ -10,6 +10,8 @@
 // 128 sum(p), an operand of constant codes, behind the second. bf16 queries become fp16 as well: a
 // row is scaled by a power of two so that its largest magnitude is in [2^14, 2^15), where fp16
 // holds every 8-bit significand down to 2^-17; what is lost is below 2^-39 of the row's largest.
+// The row's power of two and the scale's come back as one whole exponent, applied to the block's
+// scale times the scale's significand (kShift).
 //
 // The scale of a block's keys multiplies the scores; that of its values, s_v, goes into the
 // exponent: with t = x log2 e + log2 s_v and m the running maximum of t, p = 2^(t - m) is the
@@ -56,6 +58,8 @@ namespace rt {
 
 struct AttendInt8Args : AttendBase {
   KvInt8 cache;
+  float size;  // scale = size * 2^power, size in [0.5, 1)
+  int32_t power;
 };
 
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
@@ -69,6 +73,7 @@ __device__ inline v4f mma16(Kv<__bf16>::V8 a, Kv<__bf16>::V8 b, v4f c) {
 }
 
 // Eight codes (two words), plus 128, as fp16 in units of 2^-24.
+constexpr int kCodeBits = 24;
 constexpr float kCodeUnit = 0x1p-24f;
 __device__ inline v8h codes_to_half(int lo, int hi) {
   const uint32_t a = static_cast<uint32_t>(lo) ^ 0x80808080u;
@@ -182,7 +187,7 @@ __device__ inline float most_of(const v4f (&x)[4]) {
 struct Subtile {
   int32_t page, at;  // physical page; first slot * 32 + keys (0: none)
   uint32_t who;      // the tokens whose lists hold it
-  float ks, lift, inv;  // the keys' scale; the values' one's logarithm and inverse
+  float ks, lift, inv;  // the keys' scale times a.size; the values' one's logarithm and inverse
   __device__ void clear() {
     page = 0;
     at = 0;
@@ -196,9 +201,9 @@ struct Subtile {
     scale[0] = a.cache.k_scales[row];
     scale[1] = a.cache.v_scales[row];
   }
-  __device__ bool take(const float (&scale)[2]) {
+  __device__ bool take(const AttendInt8Args& a, const float (&scale)[2]) {
     if (!(scale[0] > 0.0f)) return false;
-    ks = scale[0];
+    ks = scale[0] * a.size;
     lift = __builtin_amdgcn_logf(scale[1]);
     inv = 1.0f / scale[1];
     return true;
@@ -228,6 +233,12 @@ struct Int8Wave {
   static constexpr bool HALF = D % 64 != 0;       // and one of 8 bytes
   static constexpr float kLift = 7.0f;            // maximum - m
   static constexpr float kFar = 0x1p23f;
+  static constexpr float kLeast = 1.17549435e-38f, kMost = 3.402823466e38f;  // (normal, finite)
+  // Products with codes are whole multiples of 2^-48 (query and code steps are 2^-24): with 2^48
+  // any but 0 is 1 at least, so their factor, held 2^48 times too small, is finite beside every
+  // score that is. (Below 2^-78 it loses bits then, of scores below 2^-70.)
+  static constexpr int kShift = 48;
+  static constexpr float kUnits = 0x1p48f;  // 2^kShift
   v4f acc[CT][DT], over[CT];
   float m[CT], l[CT];
   bool far[CT];  // a maximum has been past kFar, in some column of the tile
@@ -236,9 +247,9 @@ struct Int8Wave {
   static constexpr bool kQueriesInLds = CT > 1;
   v8h qf[kQueriesInLds ? 1 : KS];
   const v8h* q_lds;  // [CT][KS][64]
-  float factor[CT];  // what a score is multiplied by besides its block's scale
-  float start[CT];   // -128 sum(q), in units of kCodeUnit
-  bool odd[CT];      // the column's query is not finite
+  int power[CT];    // a score is multiplied by its block's ks * 2^(power + kShift)
+  float start[CT];  // -128 sum(q), in units of kCodeUnit
+  bool odd[CT];     // the column's query is not finite
   static constexpr int LOADS = D / 16;  // of 64 keys' codes, of their values': 1 KiB each
   static constexpr int STAGE = 64 * D;  // bytes of a step's keys in the wave's LDS; its values too
 
@@ -310,7 +321,7 @@ struct Int8Wave {
 #pragma unroll
     for (int i = 16; i < kWave; i <<= 1) sum += __shfl_xor(sum, i);
     start[c] = sum * (-128.0f * kCodeUnit);
-    factor[c] = ldexpf(a.scale, -up) * (1.0f / kCodeUnit);
+    power[c] = a.power - up + kCodeBits - kShift;
   }
 
   // The step of quad i. Its page is one where pages hold 64 slots or more.
@@ -402,23 +413,23 @@ struct Int8Wave {
       }
     }
   }
-  // Scores as exponents t, the product and the sum rounded once each: the largest is then its column's
-  // maximum exactly.
-  __device__ static void exponents(v4f (&sc)[4], float f, float lift) {
+  // Scores as exponents t, the product (of `unit` sc) and the sum rounded once each: the largest is
+  // then its column's maximum exactly.
+  __device__ static void exponents(v4f (&sc)[4], float unit, float f, float lift) {
 #pragma clang fp contract(off)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        sc[j][r] = lift == -INFINITY ? -INFINITY : sc[j][r] * f + lift;
+        sc[j][r] = lift == -INFINITY ? -INFINITY : sc[j][r] * unit * f + lift;
       }
     }
   }
   // The weights of tile c's scores (slot 4 j + r of this lane's subtile): the maximum raised, the
-  // sum extended. f multiplies the scores, lift is the logarithm of what the values stand for, inv
-  // its inverse. A column has the subtile's first n keys (`some` lane's n is not 16, or its scores
-  // may not be numbers), or none of them where it does not count.
-  template <class P>
+  // sum extended. f multiplies the scores (CODES: f * 2^kShift), lift is the logarithm of what the
+  // values stand for, inv its inverse. A column has the subtile's first n keys (`some` lane's n is
+  // not 16, or its scores may not be numbers), or none of them where it does not count.
+  template <bool CODES, class P>
   __device__ void weigh(int c, v4f (&sc)[4], float f, float lift, float inv, bool counts, int n,
                         bool some, P (&p)[2]) {
     settle(sc);
@@ -429,28 +440,33 @@ struct Int8Wave {
         for (int r = 0; r < 4; ++r) sc[j][r] = counts && 4 * j + r < n ? sc[j][r] : -INFINITY;
       }
     }
-    f = fmaxf(f, 1.17549435e-38f);  // (a score of -inf stays that)
+    // (a score of -inf stays that, and one of 0)
+    const float held = f;
+    f = __builtin_amdgcn_fmed3f(CODES ? f * kUnits : f, kLeast, kMost);
     if (!counts) lift = -INFINITY;
     float high = fmaf(most_of(sc), f, lift);
     bool raise = __any(high - m[c] > 8.0f + kLift);
-    if (far[c] || (raise && __any(fabsf(high) > kFar && high != -INFINITY))) {
-      far[c] = true;
-      exponents(sc, f, lift);
-      f = 1.0f;
-      lift = 0.0f;
-      high = most_of(sc);
-      raise = __any(high - m[c] > 8.0f + kLift);
-    }
-    if (raise) {
-      float next = fmaxf(high, __shfl_xor(high, 16));
-      next = fmaxf(next, __shfl_xor(next, 32));
-      next = fmaxf(next - kLift, m[c]);
-      const float keep = __builtin_amdgcn_exp2f(m[c] - next);
-      m[c] = next;
-      l[c] *= keep;
-      over[c] *= keep;
+    if (raise || far[c]) {
+      if (far[c] || __any(fabsf(high) > kFar && high != -INFINITY)) {
+        far[c] = true;
+        if (CODES) f = fminf(fmaxf(held, 0x1p-149f), kMost);
+        exponents(sc, CODES ? kUnits : 1.0f, f, lift);
+        f = 1.0f;
+        lift = 0.0f;
+        high = most_of(sc);
+        raise = __any(high - m[c] > 8.0f + kLift);
+      }
+      if (raise) {
+        float next = fmaxf(high, __shfl_xor(high, 16));
+        next = fmaxf(next, __shfl_xor(next, 32));
+        next = fmaxf(next - kLift, m[c]);
+        const float keep = __builtin_amdgcn_exp2f(m[c] - next);
+        m[c] = next;
+        l[c] *= keep;
+        over[c] *= keep;
 #pragma unroll
-      for (int i = 0; i < DT; ++i) acc[c][i] *= keep;
+        for (int i = 0; i < DT; ++i) acc[c][i] *= keep;
+      }
     }
     const float less = lift - m[c];
     float sum[4];
@@ -544,7 +560,7 @@ struct Int8Wave {
       // (a tile none of whose columns counts the step: weights of 0, without their exponentials)
       p[c][0] = p[c][1] = v8h{};
       if (CT > 1 && !__any(counts[c])) continue;
-      weigh(c, sc[c], s.ks * factor[c], s.lift, s.inv, counts[c], n[c], some, p[c]);
+      weigh<true>(c, sc[c], ldexpf(s.ks, power[c]), s.lift, s.inv, counts[c], n[c], some, p[c]);
     }
     constexpr int ROW = SHIFT >= 6 ? 64 : SHIFT == 5 ? 32 : 16;  // bytes of a staged channel
     const uint32_t v_at = lds_address(values) + value_offset<D, SHIFT>(col, grp);
@@ -604,7 +620,7 @@ struct Int8Wave {
       }
     }
     V8 p[2];
-    weigh(c, sc, a.scale, 0.0f, 1.0f, n > 0, n, true, p);
+    weigh<false>(c, sc, a.scale, 0.0f, 1.0f, n > 0, n, true, p);
     const E* v = static_cast<const E*>(a.cache.v_tail) + open + (col << SHIFT) + first;
     float none = 0.0f;
 #pragma unroll
@@ -661,8 +677,11 @@ struct Int8Wave {
 };
 
 // Waves a SIMD that the registers leave room for: as many as the workgroups' LDS does (512 D bytes
-// and up to 20 KiB each of a CU's 160 KiB).
-constexpr int attend_int8_waves(int D) { return D > 128 ? 1 : 2; }
+// and up to 20 KiB each of a CU's 160 KiB); heads of 64 channels over pages of 16 and 32 hold more
+// of a step's addresses, and would spill.
+constexpr int attend_int8_waves(int D, int shift) {
+  return D > 128 ? 1 : D > 64 || shift < 6 ? 2 : 3;
+}
 
 // Single tokens, and few rows: the workgroup's waves (and `parts` workgroups) share a row's list in
 // units of 64 keys.
@@ -691,7 +710,7 @@ struct SplitWave : Int8Wave<E, D, SHIFT, 1> {
           s.page = p;
           float scale[2];
           s.scales(a, head, scale);
-          is_open = !s.take(scale);
+          is_open = !s.take(a, scale);
           // (a block before the token's own that has no codes was never filled)
           if (!is_open || block == place.last) {
             s.at = slot * 32 + (n < 16 ? n : 16);
@@ -772,7 +791,7 @@ struct SplitWave : Int8Wave<E, D, SHIFT, 1> {
 };
 
 template <class E, int D, int SHIFT>
-__global__ void __launch_bounds__(kAttendWaves* kWave, attend_int8_waves(D))
+__global__ void __launch_bounds__(kAttendWaves* kWave, attend_int8_waves(D, SHIFT))
     kv_attend_int8_split_kernel(AttendInt8Args a) {
   __shared__ __attribute__((aligned(16))) char lds[kAttendWaves][64 * D];  // keys, then sums
   __shared__ __attribute__((aligned(16))) char values[kAttendWaves][64 * D];
@@ -822,7 +841,7 @@ struct JoinInt8Lds {
   uint32_t list_who[kJoinEntries];
   int32_t counts[kAttendWaves];
   float ml[kAttendWaves][16][2];
-  float column[CT][16][3];  // factor, start, odd
+  float column[CT][16][3];  // power, start, odd
 };
 
 // The pages of tokens t0 .. t0 + tokens - 1: how many.
@@ -897,7 +916,7 @@ __device__ inline int join_lists(const AttendInt8Args& a, int64_t t0, int tokens
 }
 
 template <class E, int D, int SHIFT, int CT>
-__global__ void __launch_bounds__(kAttendWaves* kWave, attend_int8_waves(D))
+__global__ void __launch_bounds__(kAttendWaves* kWave, attend_int8_waves(D, SHIFT))
     kv_attend_int8_joined_kernel(AttendInt8Args a) {
   __shared__ __attribute__((aligned(16))) JoinInt8Lds<D, CT> lds;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
@@ -936,7 +955,7 @@ __global__ void __launch_bounds__(kAttendWaves* kWave, attend_int8_waves(D))
       w.fetch_q(a, t0 + tok[c], head * a.G + col % a.G, real[c], x);
       w.take_q(a, c, x, real[c], lds.q);
       if (grp == 0) {
-        lds.column[c][col][0] = w.factor[c];
+        lds.column[c][col][0] = static_cast<float>(w.power[c]);
         lds.column[c][col][1] = w.start[c];
         lds.column[c][col][2] = w.odd[c] ? 1.0f : 0.0f;
       }
@@ -944,7 +963,7 @@ __global__ void __launch_bounds__(kAttendWaves* kWave, attend_int8_waves(D))
     __syncthreads();
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
-      w.factor[c] = lds.column[c][col][0];
+      w.power[c] = static_cast<int>(lds.column[c][col][0]);
       w.start[c] = lds.column[c][col][1];
       w.odd[c] = lds.column[c][col][2] != 0.0f;
     }
@@ -963,7 +982,7 @@ __global__ void __launch_bounds__(kAttendWaves* kWave, attend_int8_waves(D))
       s.at = i % PER * 16 * 32 + 16;
       float scale[2];
       s.scales(a, head, scale);
-      is_open = !s.take(scale);
+      is_open = !s.take(a, scale);
     }
     // (open pages are their tokens' own or were never filled)
     uint64_t full = __ballot(s.at != 0 && !is_open), open = __ballot(s.at != 0 && is_open);

@@ -89,6 +89,7 @@ extern "C" int rt_kv_attention_int8(
            static_cast<int32_t>(max_pages), static_cast<int32_t>(P), kv_shift(page)};
   // (a scale of 0 becomes the least number: the scores are 0 all the same, and -inf stays -inf)
   a.scale = fmaxf(fabsf(scale * kLog2e), 1.17549435e-38f), a.minus = scale < 0.0f;
+  a.size = std::frexp(a.scale, &a.power);
   a.out = out, a.lse = lse, a.parts = plan.parts;
   a.part_out = static_cast<float*>(workspace);
   a.part_ml = a.part_out + (plan.parts > 1 ? plan.rows * plan.parts * 16 * D : 0);

@@ -1,16 +1,20 @@
-"""Attention over the 8-bit cache where scores are large: one key holds a row's weight."""
+"""Attention over the 8-bit cache where scores are large, or a query's size or the scale is near the
+end of 32 bits while the scores are not: one key holds a row's weight, or several keys of equal score
+share it."""
 
 from __future__ import annotations
 
 import numpy as np
 import pytest
 
+from oracle import kv as okv
 from tests.kv_int8_cases import UNIT
 from tests.test_kv_int8_attention import _case, _run
 
-# times that a case's five tokens are taken: few rows (lists split), 1200 and 2400 tokens of four query
-# heads a key/value head (four tokens a workgroup in one tile, eight in two)
+# times that a case's five tokens are taken: few rows (lists split), 1200 and 2400 tokens of four
+# query heads a key/value head (four tokens a workgroup in one tile, eight in two)
 FORMS = [1, 240, 480]
+MOST = {"bf16": float.fromhex("0x1.fep127"), "fp16": 65504.0}
 
 
 def _five(seed, kind, d=128, page=16):
@@ -44,10 +48,10 @@ def _row(c, blocks, p, s, h, tab):
 
 
 def _check_winners(got, c, q, blocks, pos, seq, tab, scale=None):
-    """Scores are so large that the best key has all the weight wherever it leads by more than twice what
-    a score may be off (``off``, as ``kv_int8_cases.check_attention`` derives it) and 30 more (weights of
-    at most e^-30 beside it, below the 2^-25 allowed): the output is its value, its weight rounded
-    once (``w``) and the output once (``u``). Nearly every row's does."""
+    """Scores are so large that the best key has all the weight wherever it leads by more than twice
+    what a score may be off (``off``, as ``kv_int8_cases.check_attention`` derives it) and 30 more
+    (weights of at most e^-30 beside it, below the 2^-25 allowed): the output is its value, its weight
+    rounded once (``w``) and the output once (``u``). Nearly every row's does."""
     out, lse, of = got
     d, group = q.shape[2], q.shape[1] // c.k.shape[1]
     scale, u = 1 / np.sqrt(d) if scale is None else scale, UNIT[c.kind]
@@ -63,7 +67,8 @@ def _check_winners(got, c, q, blocks, pos, seq, tab, scale=None):
             best = scores.argmax()
             ahead = scores[best] - np.partition(scores, -2)[-2] > 2 * off + 30
             assert np.isfinite(out[row, g]).all() and np.isfinite(lse[row, g]), (t, g)
-            slack = off + 2.0**-20 * max(1, abs(scores[best])) + (0 if ahead else np.log(len(scores)))
+            slack = off + 2.0**-20 * max(1, abs(scores[best]))
+            slack += 0 if ahead else np.log(len(scores))
             assert abs(lse[row, g] - scores[best]) <= slack, (t, g)
             if not ahead:
                 continue
@@ -89,3 +94,62 @@ def test_far_scores(dev, kind, scale, n):
     c.kt = -np.abs(c.kt)
     q = np.abs(q) * np.float32(np.sign(scale))
     _check_winners(_repeated(dev, n, c, q, *rest, scale), c, q, *rest, scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", FORMS)
+@pytest.mark.parametrize("size", [2.0**112, 2.0**119, 2.0**121, 2.0**123, 2.0**125, 2.0**126])
+def test_large_queries(dev, size, n):
+    """bf16 queries up to the type's largest number beside keys that leave the scores finite, of
+    both signs and all below 0."""
+    print(f"queries of {size} x{n}", flush=True)
+    c, q, *rest = _five(71, "bf16")
+    most = np.float64(MOST["bf16"])
+    q = okv.round16(np.clip(q * np.float64(size), -most, most).astype(np.float32), "bf16")
+    small = np.float32(2.0**110 / size)
+    c.ks *= small
+    c.kt = okv.round16(c.kt * small, "bf16")
+    _check_winners(_repeated(dev, n, c, q, *rest), c, q, *rest)
+    c.k = -np.maximum(np.abs(c.k), 1).astype(np.int8)
+    c.kt = -np.abs(c.kt)
+    q = np.abs(q)
+    _check_winners(_repeated(dev, n, c, q, *rest), c, q, *rest)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", FORMS)
+@pytest.mark.parametrize("kind,size,scale", [("bf16", 2.0**127, None), ("bf16", -(2.0**127), None),
+                                             ("bf16", 1.0, 2.0**122), ("fp16", 1.0, 2.0**122),
+                                             ("fp16", 65504.0, -(2.0**107)),
+                                             ("bf16", 2.0**100, 2.0**-126)])
+def test_scores_of_zero_beside_large_ones(dev, kind, size, scale, n):
+    """Queries of one channel, so that every score is one product (exact but for the three behind it,
+    and for the 2^-17 that the logarithm of a block's scale and its sum are off): keys that do not hold
+    the channel score 0 and share the weight evenly where all others are below 0; then one key holds a
+    code of 1, and the weight. With a scale of the least size all scores are next to 0."""
+    print(f"{kind} {size} x {scale}, x{n}", flush=True)
+    c, q, blocks, pos, seq, tab = _five(73, kind)
+    sign = 1.0 if scale is None else np.sign(scale)
+    at, down = 37, -np.sign(size) * sign
+    q[:] = 0
+    q[:, :, at] = size
+    c.k[..., at] = down * np.where(np.arange(16) % 3 == 0, 0, np.abs(c.k[..., at].astype(np.int32)))
+    c.kt[..., at] = down * np.where(np.arange(16) % 5 == 0, 0, np.abs(c.kt[..., at]))
+    q[1] = q[1] if scale == 2.0**-126 else 0 * q[1]  # (a row of nothing: all scores 0)
+    rest = blocks, pos, seq, tab
+    used = 1 / np.sqrt(128) if scale is None else scale
+    for one in (False, True):
+        if one:
+            c.k[:, :, 3, at] = -down
+        got_out, got_lse, of = _repeated(dev, n, c, q, *rest, scale)
+        with np.errstate(under="ignore"):
+            out, lse, spread, _ = c.attention(q, *rest, used)
+        u, w = UNIT[kind], max(UNIT[kind], 2.0**-11)
+        keys = c.page * blocks.shape[2]
+        most = max(np.abs(c.v * c.vs[..., None, None]).max(), np.abs(c.vt).max())
+        least = 2.0**-32 * keys * most + 2.0**-24 * (keys / 32 + 16) * 255 * c.vs.max()
+        tol = u * np.abs(out) + (w + 2.0**-16) * spread * (1 + u) + least + 2.0**-25
+        assert np.isfinite(got_out).all() and np.isfinite(got_lse).all()
+        off = 2.0**-17 + 2.0**-20 * np.maximum(1, np.abs(lse))
+        assert (np.abs(got_lse - lse[of]) <= off[of]).all()
+        assert (np.abs(got_out - out[of]) <= tol[of]).all()
