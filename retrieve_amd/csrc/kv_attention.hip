@@ -14,7 +14,9 @@
 //                                read transposed (ds_read_tr: 4 keys of one channel a lane).
 // A lane's column is one head in both products: maxima, sums and rescaling stay in the lane. The
 // maximum is raised only where a score passes it by 8 (in powers of two: weights reach 256 at
-// most, far inside both types), so most steps do not touch the accumulators or exchange lanes.
+// most, far inside both types), so most steps do not touch the accumulators or exchange lanes. A
+// score and its maximum meet in one fused multiply-add; of scores past 2^23, where that would differ
+// from the rounded maximum by whole powers of two, each is rounded first (`far`).
 // Weights are rounded to the values' 16 bits for the matrix cores (l sums them unrounded):
 // relative 2^-9 / 2^-12 a weight, the size of the output's own rounding (against 64 bits the
 // outputs are off by 2.3e-3 / 2.9e-4 of their size, by 1.7e-3 / 2.1e-4 with weights of 32 bits).
@@ -148,8 +150,10 @@ struct AttendWave {
   using V8 = typename Op::V8;
   static constexpr int KS = D / 32, DT = D / 16, VL = D / 16;  // VL: 16-byte loads of V a lane
   static constexpr float kLift = std::is_same<E, _Float16>::value ? 5.0f : 0.0f;  // maximum - m
+  static constexpr float kFar = 0x1p23f;
   v4f acc[DT];
   float m, l;
+  bool far;  // a maximum has been past kFar, in some column
   V8 qf[KS], kf[2][KS], vf[VL];
 
   __device__ void clear() {
@@ -157,6 +161,7 @@ struct AttendWave {
     for (int i = 0; i < DT; ++i) acc[i] = v4f{0.f, 0.f, 0.f, 0.f};
     m = -3.402823466e38f;
     l = 0.0f;
+    far = false;
   }
   // This lane's column is query head `head` of token t (zeros where it is not `real`).
   __device__ void load_q(const AttendArgs& a, int64_t t, int64_t head, bool real) {
@@ -222,15 +227,20 @@ struct AttendWave {
     }
     fetch_v();
     V8 p[1];
-    weigh(a.scale, sc, whole, n, p);
+    weigh<false>(a.scale, sc, whole, n, p);
     asm volatile("" ::: "memory");  // (the staged rows are read by other lanes of this wave)
     add(lds, p);
     asm volatile("" ::: "memory");
   }
+  __device__ static float rounded(float x, float scale) {
+#pragma clang fp contract(off)
+    return x * scale;
+  }
   // The weights of the scores of N tiles (key 4 (lane / 16) + r of tile j at 4 (j % 2) + r of p[j /
   // 2]), rounded for the second product; the maximum raised and the sum extended. A column counts
-  // the first n[j] keys of tile j (all where `whole`).
-  template <int N>
+  // the first n[j] keys of tile j (all where `whole`). ALONE: far scores make the sums no numbers (the
+  // caller takes such rows alone).
+  template <bool ALONE, int N>
   __device__ void weigh(float scale, v4f (&sc)[N], bool whole, const int (&n)[N],
                         V8 (&p)[N / 2]) {
     settle(sc);
@@ -251,6 +261,12 @@ struct AttendWave {
     for (int j = 1; j < N; ++j) top[0] = fmaxf(top[0], top[j]);
     const float high = top[0] * scale;
     if (__any(high - m > 8.0f + kLift)) {
+      const bool is_far = __any(fabsf(high) > kFar && high != -INFINITY);
+      if (ALONE) {
+        if (is_far) acc[0][0] = NAN;
+      } else {
+        far |= is_far;
+      }
       float next = fmaxf(high, __shfl_xor(high, 16));
       next = fmaxf(next, __shfl_xor(next, 32));
       next = fmaxf(next - kLift, m);
@@ -263,10 +279,17 @@ struct AttendWave {
     float sum[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      float e[4];
+      float t[4], e[4];
+      if (!ALONE && far) {  // (rounded first, as the maximum is)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) t[r] = rounded(sc[j][r], scale) - m;
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) t[r] = fmaf(sc[j][r], scale, -m);
+      }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        e[r] = __builtin_amdgcn_exp2f(fmaf(sc[j][r], scale, -m));
+        e[r] = __builtin_amdgcn_exp2f(t[r]);
         p[j / 2][4 * (j % 2) + r] = static_cast<E>(e[r]);
       }
       sum[j] = (e[0] + e[1]) + (e[2] + e[3]);
@@ -369,7 +392,8 @@ __global__ void __launch_bounds__(kAttendWaves* kWave, D <= 128 ? 2 : 1)
 }
 
 // One query head of one token by a wave, key by key (a lane scores one of 64, then sums its own
-// channels): only for rows beside values that are not finite, so it spares registers, not time.
+// channels): only for rows beside values that are not finite or of far scores, so it spares
+// registers, not time.
 template <class E, int D>
 __device__ inline void attend_alone(const AttendArgs& a, int64_t t, int head, int hq, float* qs) {
   using V8 = typename Kv<E>::V8;
@@ -377,7 +401,9 @@ __device__ inline void attend_alone(const AttendArgs& a, int64_t t, int head, in
   const int lane = lane_id();
   const KvPlace p = kv_place(a.tok, t);
   const E* q = static_cast<const E*>(a.q) + t * a.q_st + hq * a.q_sh;
-  const float scale = a.minus ? -a.scale : a.scale;
+  // (a scale above 1 behind the product: a query may be large beside small keys)
+  const float below = fminf(a.scale, 1.0f), above = fmaxf(a.scale, 1.0f);
+  const float scale = a.minus ? -below : below;
   for (int d = lane; d < D; d += kWave) qs[d] = static_cast<float>(q[d]) * scale;
   asm volatile("" ::: "memory");
   const int size = 1 << a.tok.shift;
@@ -401,6 +427,7 @@ __device__ inline void attend_alone(const AttendArgs& a, int64_t t, int head, in
 #pragma unroll
           for (int e = 0; e < 8; ++e) x = fmaf(static_cast<float>(kv[e]), qs[d + e], x);
         }
+        x *= above;
       }
       float top = x;
       for (int s = 1; s < kWave; s <<= 1) top = fmaxf(top, __shfl_xor(top, s));
@@ -708,7 +735,7 @@ __global__ void __launch_bounds__(kJoinWaves* kWave, D > 128 ? 2 : MOST > kJoinM
       }
     }
     V8 p[kJoinTiles / 2];
-    w.weigh(a.scale, sc, whole, n, p);
+    w.template weigh<true>(a.scale, sc, whole, n, p);
     w.add(use + kJoinTiles * Lds::kTile, p);
   };
   Step now = next();
@@ -734,7 +761,7 @@ __global__ void __launch_bounds__(kJoinWaves* kWave, D > 128 ? 2 : MOST > kJoinM
   }
   w.join_sums();
   __syncthreads();  // (the stages are free)
-  float odd = 0.0f;  // 0 times every sum: not a number where one is not finite
+  float odd = 0.0f;  // 0 times every sum: not a number where one is not finite, or scores are far
 #pragma unroll
   for (int i = 0; i < D / 16; ++i) {
 #pragma unroll
