@@ -15,8 +15,8 @@
 // A lane's column is one head in both products: maxima, sums and rescaling stay in the lane. The
 // maximum is raised only where a score passes it by 8 (in powers of two: weights reach 256 at
 // most, far inside both types), so most steps do not touch the accumulators or exchange lanes. A
-// score and its maximum meet in one fused multiply-add; of scores past 2^23, where that would differ
-// from the rounded maximum by whole powers of two, each is rounded first (`far`).
+// score and its maximum meet in one fused multiply-add; of scores past 2^23, where that would
+// differ from the rounded maximum by whole powers of two, each is rounded first (`far`).
 // Weights are rounded to the values' 16 bits for the matrix cores (l sums them unrounded):
 // relative 2^-9 / 2^-12 a weight, the size of the output's own rounding (against 64 bits the
 // outputs are off by 2.3e-3 / 2.9e-4 of their size, by 1.7e-3 / 2.1e-4 with weights of 32 bits).
@@ -238,8 +238,8 @@ struct AttendWave {
   }
   // The weights of the scores of N tiles (key 4 (lane / 16) + r of tile j at 4 (j % 2) + r of p[j /
   // 2]), rounded for the second product; the maximum raised and the sum extended. A column counts
-  // the first n[j] keys of tile j (all where `whole`). ALONE: far scores make the sums no numbers (the
-  // caller takes such rows alone).
+  // the first n[j] keys of tile j (all where `whole`). ALONE: far scores make the sums no
+  // numbers (the caller takes such rows alone).
   template <bool ALONE, int N>
   __device__ void weigh(float scale, v4f (&sc)[N], bool whole, const int (&n)[N],
                         V8 (&p)[N / 2]) {
