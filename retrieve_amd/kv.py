@@ -719,9 +719,14 @@ class PagedCache:
             raise RuntimeError(f"{more} pages wanted, {len(self._free)} free")
         if more > 0:
             new = [self._free.pop() for _ in range(more)]
-            self.page_table[seq, len(held):need] = torch.tensor(new, dtype=torch.int32)
+            rows = self.page_table[seq, len(held):need]
+            rows.copy_(torch.tensor(new, dtype=torch.int32))
+            self._empty(rows)
             self._active += not held
             held += new
+
+    def _empty(self, pages: Tensor) -> None:
+        """Pages that a sequence takes, whatever they held."""
 
     def free(self, seq: int) -> None:
         """Returns the sequence's pages."""
@@ -782,6 +787,10 @@ class Int8PagedCache(PagedCache):
         self.v_scales = torch.zeros_like(self.k_scales)
         self.k_tail = empty(sequences, heads, page, dim, of=dtype)
         self.v_tail = empty(sequences, heads, dim, page, of=dtype)
+
+    def _empty(self, pages: Tensor) -> None:
+        for scales in (self.k_scales, self.v_scales):
+            scales.index_fill_(0, pages.long(), 0.0)  # (not full)
 
     @property
     def _tensors(self) -> tuple[Tensor, ...]:
