@@ -580,8 +580,9 @@ int rt_search_epilogue(int64_t* ids, const int32_t* raw_dots, float* out_scores,
  * codes rint(x / a * 127) with a = max(max |x|, 1e-8) and scale a / 127. The block's earlier keys are
  * taken from this call where they are the tokens right before it (same sequence, consecutive
  * positions), else from the cache: a sequence's tokens come in order, side by side. Padding
- * tokens, and tokens past cos_sin or without a page, write nothing but a zero row of q_out. Two tokens at
- * one slot are not allowed. */
+ * tokens, and tokens past cos_sin or without a page, write nothing but a zero row of q_out (all, where
+ * the table has no rows: it may be null then). Two tokens at one slot are not allowed. A call without
+ * tokens looks at no pointer. */
 int rt_kv_append(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
                  int64_t k_token_stride, int64_t k_head_stride, const void* v,
                  int64_t v_token_stride, int64_t v_head_stride, int64_t T, int64_t Hq, int64_t Hkv,

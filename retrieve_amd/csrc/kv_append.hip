@@ -252,7 +252,9 @@ extern "C" int rt_kv_append_norm(
     void* v_cache, int64_t P, int64_t page, int8_t* bounds, float* bound_scales, void* q_out,
     rt_stream_t stream) {
   if (const int st = kv_check(T, Hq, Hkv, D, dtype, B, max_pages, P, page)) return st;
-  if (const int st = kv_check_turn(D, cos_sin, table_len, rot, q_weight, k_weight, eps)) return st;
+  if (const int st = kv_check_turn(T, D, cos_sin, table_len, rot, q_weight, k_weight, eps)) {
+    return st;
+  }
   if (T == 0) return kOk;
   RT_CHECK_ARG(q && k && v && positions && seq_ids && q_out, "null pointer");
   RT_CHECK_ARG(B * max_pages == 0 || page_table, "null page table");

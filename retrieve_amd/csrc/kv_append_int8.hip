@@ -16,7 +16,9 @@ extern "C" int rt_kv_append_int8(
     int64_t P, int64_t page, int8_t* bounds, float* bound_scales, void* q_out,
     rt_stream_t stream) {
   if (const int st = kv_check(T, Hq, Hkv, D, dtype, B, max_pages, P, page)) return st;
-  if (const int st = kv_check_turn(D, cos_sin, table_len, rot, q_weight, k_weight, eps)) return st;
+  if (const int st = kv_check_turn(T, D, cos_sin, table_len, rot, q_weight, k_weight, eps)) {
+    return st;
+  }
   if (T == 0) return kOk;
   const KvInt8 cache{k_codes, v_codes, k_scales, v_scales, k_tail, v_tail};
   if (const int st = kv_check_int8(cache, B, P)) return st;

@@ -287,18 +287,19 @@ struct Pair {
   }
 };
 
-// Host: the checks of the table and the weights, and their arguments.
-inline int kv_check_turn(int64_t D, const float* cos_sin, int64_t table_len, int64_t rot,
+// Host: the checks of the table and the weights (of their pointers where there are tokens).
+inline int kv_check_turn(int64_t T, int64_t D, const float* cos_sin, int64_t table_len, int64_t rot,
                          const void* q_weight, const void* k_weight, double eps) {
   RT_CHECK_ARG(rot >= 0 && rot % 2 == 0 && rot <= D, "the rotated part must be even, at most %lld",
                static_cast<long long>(D));
   RT_CHECK_ARG(table_len >= 0 && table_len <= INT32_MAX, "the rotary table has too many rows");
+  RT_CHECK_ARG(eps >= 0.0 && eps <= 1.7e308, "eps must be finite and not negative, got %g", eps);
+  if (T == 0) return kOk;
   RT_CHECK_ARG(rot == 0 || table_len == 0 || cos_sin, "null pointer");
   for (const void* p : {static_cast<const void*>(cos_sin), q_weight, k_weight}) {
     RT_CHECK_ARG(reinterpret_cast<uintptr_t>(p) % 16 == 0,
                  "the rotary table and the norms' weights must start on 16 bytes");
   }
-  RT_CHECK_ARG(eps >= 0.0 && eps <= 1.7e308, "eps must be finite and not negative, got %g", eps);
   return kOk;
 }
 inline TurnArgs kv_turn_args(const float* cos_sin, int64_t table_len, int64_t rot,
