@@ -71,3 +71,48 @@ def test_a_sequence_does_not_see_the_last_owner(dev):
             got += [q, *c.attend_to(q, blocks, pos[a:b], one[a:b])]
         results.append([back(x) for x in (*got, *c.read(pos[:90], one[:90]))])
     assert all(np.array_equal(a, b) for a, b in zip(*results))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["bf16", "fp16"])
+def test_a_shared_page_is_copied_before_it_is_cut_into(dev, kind):
+    """Two sequences share a prompt's full pages; one is cut back into the last of them, after that
+    page was copied to one of its own: it goes on as a sequence alone does that is cut back there, and
+    the other one's results stay the same bits."""
+    import torch
+
+    from retrieve_amd import kv
+
+    page, at = 16, 41
+    dtype = getattr(torch, {"bf16": "bfloat16", "fp16": "float16"}[kind])
+    rows = to(dev, normal16(5, (60, 8, 64), kind), kind)
+    more = to(dev, normal16(6, (20, 8, 64), kind), kind)
+
+    def append(c, s, x, first):
+        pos = torch.arange(first, first + len(x), dtype=torch.int32, device=dev)
+        seq = torch.full_like(pos, s)
+        q = c.append(x[:, :4], x[:, 4:6], x[:, 6:], None, pos, seq)
+        return [q, *c.attend(q, pos, seq, 6, 1, 6)]
+
+    def held(c, s, n):
+        pos = torch.arange(n, dtype=torch.int32, device=dev)
+        return c.read(pos, torch.full_like(pos, s))
+
+    alone = kv.Int8PagedCache(8, 2, 64, page, 1, 4, dtype, dev)
+    alone.reserve(0, 64)
+    append(alone, 0, rows[:48], 0)
+    expected = [*append(alone, 0, more, at), *held(alone, 0, at + 20)]
+
+    c = kv.Int8PagedCache(8, 2, 64, page, 2, 4, dtype, dev)
+    c.reserve(0, 64)
+    c.reserve(1, 64)
+    append(c, 0, rows[:48], 0)
+    before = held(c, 0, 48)
+    own = int(c.page_table[1, 2])
+    c.page_table[1, :2] = c.page_table[0, :2]
+    shared = int(c.page_table[0, 2])
+    for x in (c.k_codes, c.v_codes, c.k_scales, c.v_scales, c.bounds, c.bound_scales):
+        x[own] = x[shared]
+    got = [*append(c, 1, more, at), *held(c, 1, at + 20)]
+    assert all(torch.equal(a, b) for a, b in zip(got, expected))
+    assert all(torch.equal(a, b) for a, b in zip(held(c, 0, 48), before))
