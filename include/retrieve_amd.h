@@ -580,9 +580,9 @@ int rt_search_epilogue(int64_t* ids, const int32_t* raw_dots, float* out_scores,
  * codes rint(x / a * 127) with a = max(max |x|, 1e-8) and scale a / 127. The block's earlier keys are
  * taken from this call where they are the tokens right before it (same sequence, consecutive
  * positions), else from the cache: a sequence's tokens come in order, side by side. Padding
- * tokens, and tokens past cos_sin or without a page, write nothing but a zero row of q_out (all, where
- * the table has no rows: it may be null then). Two tokens at one slot are not allowed. A call without
- * tokens looks at no pointer. */
+ * tokens, and tokens past cos_sin or without a page, write nothing but a zero row of q_out (all,
+ * where the table has no rows: it may be null then). Two tokens at one slot are not allowed. A call
+ * without tokens looks at no pointer. */
 int rt_kv_append(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
                  int64_t k_token_stride, int64_t k_head_stride, const void* v,
                  int64_t v_token_stride, int64_t v_head_stride, int64_t T, int64_t Hq, int64_t Hkv,
@@ -596,7 +596,8 @@ int rt_kv_append(const void* q, int64_t q_token_stride, int64_t q_head_stride, c
  * sqrt(mean(x^2) + eps) over the head's D channels (the sum in double, r, x r and the product with
  * w each rounded to float once; nothing is rounded to 16 bits before the rotation). q_weight,
  * k_weight [D], float where `wide_weights`, else of the rows' type; null: those heads are not
- * normed. eps >= 0. */
+ * normed. eps >= 0 (r is past float where mean(x^2) + eps is below 2^-256: rows of bf16's least
+ * numbers need an eps). */
 int rt_kv_append_norm(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
                       int64_t k_token_stride, int64_t k_head_stride, const void* v,
                       int64_t v_token_stride, int64_t v_head_stride, int64_t T, int64_t Hq,
@@ -611,15 +612,18 @@ int rt_kv_append_norm(const void* q, int64_t q_token_stride, int64_t q_head_stri
  * transposed), k_scales, v_scales float [P, Hkv] (a code stands for code * scale), and each
  * sequence's open block, its last one while it is not full, in 16 bits: k_tail [B, Hkv, page, D],
  * v_tail [B, Hkv, D, page]. All start on 16 bytes. A page whose scales are 0 is not full: its
- * tokens are in its sequence's open block. Bounds as in the 16-bit cache, from the 16-bit keys.
+ * tokens are in its sequence's open block. So a page's scales are set to 0 when a sequence takes it.
+ * Bounds as in the 16-bit cache, from the 16-bit keys.
  *
  * rt_kv_append_norm into it. A token at the last slot of its block completes it: its keys become
  * codes rint(127 x / a) with a = max(max |x| over the block's finite keys of the head, 1e-8) and
  * scale a / 127 (infinities +-127, NaN 0), its values the same. The other tokens' rows go to the
  * open block and their page's scales become 0. A call's tokens of a sequence lie side by side, in
- * order, at consecutive positions whose blocks have pages (or none from some block on), and are its
- * end from then on: positions behind them are no longer held. A sequence that goes on inside a
- * block that was full (it has been cut back) has the block's earlier tokens from their codes. */
+ * order, at consecutive positions whose blocks have pages (or none from some block on), the first no
+ * further than the sequence's end, and are its end from then on: positions behind them are no longer
+ * held. A sequence that goes on inside a block that was full (it has been cut back) has the block's
+ * earlier tokens from their codes. Its page's scales become 0 then: where other sequences share the
+ * page, it is copied to a page of the sequence's own first. */
 int rt_kv_append_int8(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
                       int64_t k_token_stride, int64_t k_head_stride, const void* v,
                       int64_t v_token_stride, int64_t v_head_stride, int64_t T, int64_t Hq,
@@ -632,7 +636,8 @@ int rt_kv_append_int8(const void* q, int64_t q_token_stride, int64_t q_head_stri
                       int8_t* bounds, float* bound_scales, void* q_out, rt_stream_t stream);
 
 /* Tokens of the 8-bit cache in 16 bits -> k_out, v_out [T, Hkv, D]: code * scale rounded once, the
- * open block's rows as they are. Padding tokens (and tokens without a page) give zeros. */
+ * open block's rows as they are. Padding tokens (and tokens without a page) give zeros; positions
+ * that their sequence does not hold give anything. */
 int rt_kv_read_int8(const int8_t* k_codes, const int8_t* v_codes, const float* k_scales,
                     const float* v_scales, const void* k_tail, const void* v_tail, int64_t T,
                     int64_t Hkv, int64_t D, int dtype, int64_t P, int64_t page,
@@ -672,7 +677,8 @@ int rt_kv_select_of(const void* q, int64_t q_token_stride, int64_t q_head_stride
  * any order; entries below 0, past the token's block or without a page are skipped), the keys at
  * positions up to the token's, scores scale * q . k -> out [T, Hq, D], lse float [T, Hq] (natural
  * log of the weights' sum). A row without a key: zeros and -inf. Cache slots past a token's
- * position are never used, whatever they hold. scale has to be finite (also times log2 e). */
+ * position are never used, whatever they hold. scale has to be finite (also times log2 e). Scores are
+ * float: one past its range (times log2 e) is infinite. */
 size_t rt_kv_attention_workspace(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t page,
                                  int64_t count);
 int rt_kv_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t T,

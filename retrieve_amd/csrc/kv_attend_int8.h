@@ -16,9 +16,10 @@
 // The scale of a block's keys multiplies the scores; that of its values, s_v, goes into the
 // exponent: with t = x log2 e + log2 s_v and m the running maximum of t, p = 2^(t - m) is the
 // weight that the second product wants (codes stand for s_v each), and p / s_v what the sum of
-// weights wants. So neither product is rescaled from block to block. p is rounded to fp16 (2^-11,
-// and held 2^7 times as large as the maximum says: it reaches 2^15, its step below 2^-14 is 2^-31
-// of the largest weight) whatever the queries' type; the sum takes it unrounded. The maximum is
+// weights wants. So neither product is rescaled from block to block. Beside codes p is rounded to
+// fp16 (2^-11, and held 2^7 times as large as the maximum says: it reaches 2^15, its step below
+// 2^-14 is 2^-31 of the largest weight) whatever the queries' type; beside the open block, whose
+// values are of the queries' type, to that (bf16: 2^-8). The sum takes it unrounded. The maximum is
 // raised only where a score passes it by 8 (in powers of two), so most steps exchange nothing
 // between lanes. A score and its maximum meet in one fused multiply-add; of scores past 2^23, where
 // that would differ from the rounded maximum by whole powers of two, each is rounded first (`far`).

@@ -4,8 +4,10 @@
 // [D, page], each with one scale (a code stands for code * scale). A sequence's last block, not
 // full yet, lies in 16 bits in the sequence's open block, k_tail [page, D] and v_tail [D, page];
 // its page's scales are 0 until it is full. So a code depends on its block's 16-bit numbers alone,
-// never on how many calls wrote them, and the latest keys are exact. Transposed values give
-// attention's second product its operand (16 slots of a channel) as it lies in memory.
+// never on how many calls wrote them, and the latest keys are exact. (A block that its sequence is
+// cut back into after it was full is the exception: its earlier numbers are those that the codes
+// stand for, rounded to 16 bits.) Transposed values give attention's second product its operand (16
+// slots of a channel) as it lies in memory.
 #pragma once
 
 #include "kv_common.h"

@@ -1,10 +1,12 @@
 // The rotary position, and the norm before it, of one row's chunks of 8 channels: what the paged
 // cache's appending kernels apply to queries and keys on their way.
 //
-// Norm: y = x r w with r = 1 / sqrt(mean(x^2) + eps). The sum runs in 64 bits (the squares of
-// 16-bit numbers are exact there, so r does not depend on the order in which lanes add), r is
-// rounded once to fp32 and each of the two products once more: the same bits in whichever lane
-// layout, so a block's codes do not depend on how its tokens were split over calls.
+// Norm: y = x r w with r = 1 / sqrt(mean(x^2) + eps). The sum runs in 64 bits (where the squares of
+// 16-bit numbers are exact), r is rounded once to fp32 and each of the two products once more.
+// Every kernel of the 8-bit cache adds in one order (Pair's), so a block's codes do not depend on
+// how its tokens were split over calls. The 16-bit append's rows and bounds add in two orders:
+// their sums may differ in the last of 53 bits, which the rounding to 24 almost never shows (where
+// it does, a bound may be a key's neighbour in 16 bits).
 //
 // Rotation: with (c, s) the table's cosine and sine of the token's position, a pair of channels
 // (a, b) becomes (a c - b s, b c + a s), every product and sum rounded once to fp32 (no fused

@@ -284,9 +284,9 @@ def append(q: Tensor, k: Tensor, v: Tensor, cos_sin: Tensor | None, positions: T
     0, or past the page table or ``cos_sin``; a sequence outside it; no page) write nothing and
     return a zero row.
 
-    ``q_weight``, ``k_weight`` ``[D]`` (of ``q``'s dtype, or float32): each head of the queries, of
-    the keys is normed before the rotation, ``x / sqrt(mean(x ** 2) + eps) * weight``: the sum in 64
-    bits, then fp32 up to the one rounding behind the rotation."""
+    ``q_weight``, ``k_weight`` ``[D]`` (of ``q``'s dtype, or float32; both of one): each head of the
+    queries, of the keys is normed before the rotation, ``x / sqrt(mean(x ** 2) + eps) * weight``:
+    the sum in 64 bits, then fp32 up to the one rounding behind the rotation."""
     args = (q, k, v, cos_sin, positions, seq_ids, page_table, k_cache, v_cache, bounds,
             bound_scales)
     call = _append if _eager(*args, q_weight, k_weight) else torch.ops.retrieve_kv.append
@@ -393,7 +393,8 @@ def block_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, blocks: Tensor,
     with scores ``scale * q . k`` (``1 / sqrt(D)`` by default): ``(out [T, Hq, D], lse fp32 [T,
     Hq])``, ``lse`` the natural logarithm of the weights' sum. Entries below 0, past the token's
     block or without a page are skipped; a row without a key is zeros and ``-inf``. Slots past a
-    token's position are not used, whatever they hold. ``sequences`` as in :func:`select_blocks`."""
+    token's position are not used, whatever they hold. Scores are fp32, one past its range infinite.
+    ``sequences`` as in :func:`select_blocks`."""
     args = (q, k_cache, v_cache, blocks, positions, seq_ids, page_table)
     call = _attention if _eager(*args) else torch.ops.retrieve_kv.block_attention
     return call(*args, scale, sequences)
@@ -483,10 +484,12 @@ def append_int8(q: Tensor, k: Tensor, v: Tensor, cos_sin: Tensor | None, positio
     :func:`append`'s. Until then its tokens lie in the open block and its page's scales are 0.
 
     A call's tokens of a sequence lie side by side, in order, at consecutive positions whose blocks
-    have pages (or none from some block on), and are its end from then on: what it held at later
-    positions is dropped. A sequence may be cut back so, also into a block that was
-    full (whose earlier tokens then come from their codes). Sequences may share full pages, not an
-    open block."""
+    have pages (or none from some block on), the first no further than the sequence's end, and are
+    its end from then on: what it held at later positions is dropped. A sequence may be cut back so,
+    also into a block that was full, whose earlier tokens then come from their codes and whose page
+    is no longer full. Sequences may share full pages, not an open block: before one is cut back into
+    a page that it shares, that page (codes, scales, bounds) is copied to one of its own. Scales are
+    set to 0 when a sequence takes a page (:class:`Int8PagedCache` does)."""
     args = (q, k, v, cos_sin, positions, seq_ids, page_table, k_codes, v_codes, k_scales, v_scales,
             k_tail, v_tail, bounds, bound_scales)
     call = _append_int8 if _eager(*args, q_weight, k_weight) else torch.ops.retrieve_kv_int8.append
@@ -517,8 +520,9 @@ def read_int8(k_codes: Tensor, v_codes: Tensor, k_scales: Tensor, v_scales: Tens
               ) -> tuple[Tensor, Tensor]:
     """Tokens of a cache in 8 bits (:func:`append_int8`'s tensors) in 16 bits again: ``(k, v)``,
     each ``[T, Hkv, D]``, the keys rotated as they are held. Codes times their scale, rounded once;
-    tokens of the open block as they were appended; zeros for padding and for blocks without a page.
-    Tokens may come in any order, runs of one sequence are read fastest."""
+    tokens of the open block as they were appended; zeros for padding and for blocks without a page,
+    anything for positions that the sequence does not hold. Tokens may come in any order, runs of
+    one sequence are read fastest."""
     args = (k_codes, v_codes, k_scales, v_scales, k_tail, v_tail, positions, seq_ids, page_table)
     call = _read_int8 if _eager(*args) else torch.ops.retrieve_kv_int8.read
     return call(*args)
