@@ -92,7 +92,7 @@ def test_a_shared_page_is_copied_before_it_is_cut_into(dev, kind):
         pos = torch.arange(first, first + len(x), dtype=torch.int32, device=dev)
         seq = torch.full_like(pos, s)
         q = c.append(x[:, :4], x[:, 4:6], x[:, 6:], None, pos, seq)
-        return [q, *c.attend(q, pos, seq, 6, 1, 6)]
+        return [q, *c.attend(q, pos, seq, 6, 0, 6)]
 
     def held(c, s, n):
         pos = torch.arange(n, dtype=torch.int32, device=dev)
