@@ -16,15 +16,15 @@
 // workgroup that reads the open block first, after it has read.
 //
 // What bounds it, and what was taken for it: 16384 tokens of 32 rows of 256 channels take 172 us
-// (102 at a large copy's rate), 9001 normed tokens of 48 rows of 128 70 us (43). The blocks' part
-// is three quarters of that: 16 bits to codes is 3 instructions a number and a turn through LDS for
-// the values, on rows that arrive after a chain of lookups. Rows that stay in registers between the
-// maximum and the codes (334 us when they were read twice), magnitudes and bounds two numbers an
-// instruction (230 to 212), and eight waves a workgroup where a block has more than 128 channels
-// (212 to 189: more rows under way a CU); earlier rows that come from codes are taken there, not by
-// way of the open block (189 to 172 where a call's first blocks have such rows). Workgroups of both
-// kinds alternating in the grid instead of the blocks' first were slower. A decode step is bound by
-// its launch (5 us; 203 tokens of 14 heads of 64 11 us).
+// (103 at the 4.81 TB/s of a large copy), 9001 normed tokens of 48 rows of 128 71 us (43). The
+// blocks' part is three quarters of that: 16 bits to codes is 3 instructions a number and a turn
+// through LDS for the values, on rows that arrive after a chain of lookups. Rows that stay in
+// registers between the maximum and the codes (334 us when they were read twice), magnitudes and
+// bounds two numbers an instruction (230 to 212), and eight waves a workgroup where a block has
+// more than 128 channels (212 to 189: more rows under way a CU); earlier rows that come from codes
+// are taken there, not by way of the open block (189 to 172 where a call's first blocks have such
+// rows). Workgroups of both kinds alternating in the grid instead of the blocks' first were slower.
+// A decode step is bound by its launch (5 us; 203 tokens of 14 heads of 64 11 us).
 #pragma once
 
 #include <type_traits>

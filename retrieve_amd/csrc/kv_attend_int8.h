@@ -44,9 +44,10 @@
 // Single tokens are bound by memory: 64 of them over 64 blocks of 64 keys (8 heads of 128 channels,
 // 526 MB of codes) take 93 us, 5.6 TB/s; about 15 us of that are the start (lists, pages and scales
 // are looked up one after the other before the first codes) and the end, the rest runs at 6.7 TB/s.
-// Prompts are bound by the vector instructions: 2053 tokens over 16 blocks each take 154 us, of
-// which a third makes codes into fp16 and a third is the softmax. 8 tokens share a pass there; 4,
-// whose codes are widened for one tile of columns, take 169.
+// Prompts are bound by the vector instructions (59 % of the time, a third of them makes codes into
+// fp16 and a third is the softmax) and by the waits between operands and products: 2053 tokens over
+// 16 blocks each take 152 us. 8 tokens share a pass there; 4, whose codes are widened for one tile
+// of columns, take 169.
 #pragma once
 
 #include <type_traits>

@@ -5,7 +5,7 @@
 // together: a workgroup looks at 64 tokens of one head, finds the runs of tokens within 16 slots,
 // and a wave takes a run: its keys row by row, its values 16 bytes of a channel a lane, turned
 // through LDS. Bound by memory: a token's codes are read once, its 16 bits written once; 131001
-// tokens of 8 heads of 128 channels take 173 us (4.65 TB/s, a large copy's rate is 4.86). What that
+// tokens of 8 heads of 128 channels take 174 us (4.63 TB/s; a large copy beside it 4.81). What that
 // took: a run's loads all under way before the first is waited for, and stores of which
 // neighbouring lanes write neighbouring bytes (201 us without both); nontemporal loads of the
 // values were slower, since a run's 16 bytes of a channel are a part of a line. 2003 tokens of 14
