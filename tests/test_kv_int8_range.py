@@ -118,6 +118,19 @@ def test_large_queries(dev, size, n):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("n", FORMS)
+@pytest.mark.parametrize("d,page", [(64, 64), (96, 16), (96, 128), (128, 32), (192, 64), (256, 16)])
+def test_large_queries_of_every_shape(dev, d, page, n):
+    print(f"queries of {d} channels over pages of {page}, x{n}", flush=True)
+    c, q, *rest = _five(75, "bf16", d, page)
+    q = q * np.float32(2.0**124)
+    small = np.float32(2.0**-14)
+    c.ks *= small
+    c.kt = okv.round16(c.kt * small, "bf16")
+    _check_winners(_repeated(dev, n, c, q, *rest), c, q, *rest)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", FORMS)
 @pytest.mark.parametrize("kind,size,scale", [("bf16", 2.0**127, None), ("bf16", -(2.0**127), None),
                                              ("bf16", 1.0, 2.0**122), ("fp16", 1.0, 2.0**122),
                                              ("fp16", 65504.0, -(2.0**107)),
