@@ -11,7 +11,7 @@
 // row is scaled by a power of two so that its largest magnitude is in [2^14, 2^15), where fp16
 // holds every 8-bit significand down to 2^-17; what is lost is below 2^-39 of the row's largest.
 // The row's power of two and the scale's come back as one whole exponent, applied to the block's
-// scale times the scale's significand (kShift).
+// scale times the scale's significand: infinite only beside scores that are far, or next to 0.
 //
 // The scale of a block's keys multiplies the scores; that of its values, s_v, goes into the
 // exponent: with t = x log2 e + log2 s_v and m the running maximum of t, p = 2^(t - m) is the
@@ -21,8 +21,9 @@
 // 2^-14 is 2^-31 of the largest weight) whatever the queries' type; beside the open block, whose
 // values are of the queries' type, to that (bf16: 2^-8). The sum takes it unrounded. The maximum is
 // raised only where a score passes it by 8 (in powers of two), so most steps exchange nothing
-// between lanes. A score and its maximum meet in one fused multiply-add; of scores past 2^23, where
-// that would differ from the rounded maximum by whole powers of two, each is rounded first (`far`).
+// between lanes. A score and its maximum meet in one fused multiply-add: past 2^23 that leaves the
+// rounded maximum by whole powers of two, so rows of such scores are `far`, and taken again key by
+// key (AloneSums).
 //
 // A wave holds columns, 16 query heads a tile: heads of one token, or heads of several tokens that
 // share a key/value head. It takes 64 keys a step, four subtiles of 16 slots, lane group g (lanes
@@ -236,26 +237,22 @@ struct Int8Wave {
   static constexpr float kLift = 7.0f;            // maximum - m
   static constexpr float kFar = 0x1p23f;
   static constexpr float kLeast = 1.17549435e-38f, kMost = 3.402823466e38f;  // (normal, finite)
-  // Products with codes are whole multiples of 2^-48 (query and code steps are 2^-24): with 2^48
-  // any but 0 is 1 at least, so their factor, held 2^48 times too small, is finite beside every
-  // score that is. (Below 2^-78 it loses bits then, of scores below 2^-70.)
-  static constexpr int kShift = 48;
-  static constexpr float kUnits = 0x1p48f;  // 2^kShift
   v4f acc[CT][DT], over[CT];
   float m[CT], l[CT];
-  bool far[CT];  // a maximum has been past kFar, in some column of the tile
+  bool far;  // a score was past kFar, in some column: the sums are of no use
   // Two tiles' queries stay in LDS: in registers they would spill others beside the next step's
   // keys and values.
   static constexpr bool kQueriesInLds = CT > 1;
   v8h qf[kQueriesInLds ? 1 : KS];
   const v8h* q_lds;  // [CT][KS][64]
-  int power[CT];    // a score is multiplied by its block's ks * 2^(power + kShift)
+  int power[CT];    // a score is multiplied by its block's ks * 2^power
   float start[CT];  // -128 sum(q), in units of kCodeUnit
   bool odd[CT];     // the column's query is not finite
   static constexpr int LOADS = D / 16;  // of 64 keys' codes, of their values': 1 KiB each
   static constexpr int STAGE = 64 * D;  // bytes of a step's keys in the wave's LDS; its values too
 
   __device__ void clear() {
+    far = false;
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
 #pragma unroll
@@ -263,7 +260,6 @@ struct Int8Wave {
       over[c] = v4f{0.f, 0.f, 0.f, 0.f};
       m[c] = -3.402823466e38f;
       l[c] = 0.0f;
-      far[c] = false;
     }
   }
   // The first of a lane group's eight channels in step s of the first product.
@@ -323,7 +319,7 @@ struct Int8Wave {
 #pragma unroll
     for (int i = 16; i < kWave; i <<= 1) sum += __shfl_xor(sum, i);
     start[c] = sum * (-128.0f * kCodeUnit);
-    power[c] = a.power - up + kCodeBits - kShift;
+    power[c] = a.power - up + kCodeBits;
   }
 
   // The step of quad i. Its page is one where pages hold 64 slots or more.
@@ -415,23 +411,11 @@ struct Int8Wave {
       }
     }
   }
-  // Scores as exponents t, the product (of `unit` sc) and the sum rounded once each: the largest is
-  // then its column's maximum exactly.
-  __device__ static void exponents(v4f (&sc)[4], float unit, float f, float lift) {
-#pragma clang fp contract(off)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        sc[j][r] = lift == -INFINITY ? -INFINITY : sc[j][r] * unit * f + lift;
-      }
-    }
-  }
   // The weights of tile c's scores (slot 4 j + r of this lane's subtile): the maximum raised, the
-  // sum extended. f multiplies the scores (CODES: f * 2^kShift), lift is the logarithm of what the
-  // values stand for, inv its inverse. A column has the subtile's first n keys (`some` lane's n is
-  // not 16, or its scores may not be numbers), or none of them where it does not count.
-  template <bool CODES, class P>
+  // sum extended. f multiplies the scores, lift is the logarithm of what the values stand for, inv
+  // its inverse. A column has the subtile's first n keys (`some` lane's n is not 16, or its scores
+  // may not be numbers), or none of them where it does not count.
+  template <class P>
   __device__ void weigh(int c, v4f (&sc)[4], float f, float lift, float inv, bool counts, int n,
                         bool some, P (&p)[2]) {
     settle(sc);
@@ -442,33 +426,22 @@ struct Int8Wave {
         for (int r = 0; r < 4; ++r) sc[j][r] = counts && 4 * j + r < n ? sc[j][r] : -INFINITY;
       }
     }
-    // (a score of -inf stays that, and one of 0)
-    const float held = f;
-    f = __builtin_amdgcn_fmed3f(CODES ? f * kUnits : f, kLeast, kMost);
+    // (a score of -inf stays that, one of 0 too; another whose factor was infinite is far: scores
+    // in units of the codes are 0 or 2^-48 at least)
+    f = fminf(fmaxf(f, kLeast), kMost);
     if (!counts) lift = -INFINITY;
-    float high = fmaf(most_of(sc), f, lift);
-    bool raise = __any(high - m[c] > 8.0f + kLift);
-    if (raise || far[c]) {
-      if (far[c] || __any(fabsf(high) > kFar && high != -INFINITY)) {
-        far[c] = true;
-        if (CODES) f = fminf(fmaxf(held, 0x1p-149f), kMost);
-        exponents(sc, CODES ? kUnits : 1.0f, f, lift);
-        f = 1.0f;
-        lift = 0.0f;
-        high = most_of(sc);
-        raise = __any(high - m[c] > 8.0f + kLift);
-      }
-      if (raise) {
-        float next = fmaxf(high, __shfl_xor(high, 16));
-        next = fmaxf(next, __shfl_xor(next, 32));
-        next = fmaxf(next - kLift, m[c]);
-        const float keep = __builtin_amdgcn_exp2f(m[c] - next);
-        m[c] = next;
-        l[c] *= keep;
-        over[c] *= keep;
+    const float high = fmaf(most_of(sc), f, lift);
+    if (__any(high - m[c] > 8.0f + kLift)) {
+      far |= __any(fabsf(high) > kFar && high != -INFINITY) != 0;
+      float next = fmaxf(high, __shfl_xor(high, 16));
+      next = fmaxf(next, __shfl_xor(next, 32));
+      next = fmaxf(next - kLift, m[c]);
+      const float keep = __builtin_amdgcn_exp2f(m[c] - next);
+      m[c] = next;
+      l[c] *= keep;
+      over[c] *= keep;
 #pragma unroll
-        for (int i = 0; i < DT; ++i) acc[c][i] *= keep;
-      }
+      for (int i = 0; i < DT; ++i) acc[c][i] *= keep;
     }
     const float less = lift - m[c];
     float sum[4];
@@ -562,7 +535,7 @@ struct Int8Wave {
       // (a tile none of whose columns counts the step: weights of 0, without their exponentials)
       p[c][0] = p[c][1] = v8h{};
       if (CT > 1 && !__any(counts[c])) continue;
-      weigh<true>(c, sc[c], ldexpf(s.ks, power[c]), s.lift, s.inv, counts[c], n[c], some, p[c]);
+      weigh(c, sc[c], ldexpf(s.ks, power[c]), s.lift, s.inv, counts[c], n[c], some, p[c]);
     }
     constexpr int ROW = SHIFT >= 6 ? 64 : SHIFT == 5 ? 32 : 16;  // bytes of a staged channel
     const uint32_t v_at = lds_address(values) + value_offset<D, SHIFT>(col, grp);
@@ -622,7 +595,7 @@ struct Int8Wave {
       }
     }
     V8 p[2];
-    weigh<false>(c, sc, a.scale, 0.0f, 1.0f, n > 0, n, true, p);
+    weigh(c, sc, a.scale, 0.0f, 1.0f, n > 0, n, true, p);
     const E* v = static_cast<const E*>(a.cache.v_tail) + open + (col << SHIFT) + first;
     float none = 0.0f;
 #pragma unroll
@@ -679,10 +652,125 @@ struct Int8Wave {
 };
 
 // Waves a SIMD that the registers leave room for: as many as the workgroups' LDS does (512 D bytes
-// and up to 20 KiB each of a CU's 160 KiB); heads of 64 channels over pages of 16 and 32 hold more
-// of a step's addresses, and would spill.
-constexpr int attend_int8_waves(int D, int shift) {
-  return D > 128 ? 1 : D > 64 || shift < 6 ? 2 : 3;
+// and up to 20 KiB each of a CU's 160 KiB), but for what would spill then: two tiles of 64 channels
+// over pages of 16 and 32, the split form (0 tiles) and two tiles of 96, one of 96 over pages of 16.
+constexpr int attend_int8_waves(int D, int shift, int tiles) {
+  if (D > 128) return 1;
+  return (D <= 64 && shift >= 6) || (D <= 96 && shift >= 5 && tiles == 1) ? 3 : 2;
+}
+
+// The sums of one query head of one token over a wave's share of its list (units of 64 keys part,
+// part + parts, ...), key by key, for rows of far scores: it spares registers, not time. A score is
+// summed in 64 bits and rounded once, so equal ones are equal whatever their blocks' scales; the
+// maximum is of the scores alone, and weights times a value's scale stay in fp32. Channel d of the
+// sums is in acc[d / 64] of lane d % 64.
+template <class E, int D, int SHIFT>
+struct AloneSums {
+  using V8 = typename Kv<E>::V8;
+  static constexpr int R = (D + kWave - 1) / kWave;
+  float m, l, acc[R];
+
+  __device__ void run(const AttendInt8Args& a, int64_t t, int head, int64_t hq, int part,
+                      int parts) {
+    m = -3.402823466e38f;
+    l = 0.0f;
+#pragma unroll
+    for (int r = 0; r < R; ++r) acc[r] = 0.0f;
+    const KvPlace place = kv_place(a.tok, t);
+    if (place.last < 0) return;
+    const int lane = lane_id();
+    const int64_t seq = a.tok.seq_ids[t], open = ((seq * a.Hkv + head) << SHIFT) * D;
+    const int32_t* list = a.blocks + (t * a.Hkv + head) * a.count;
+    const E* q = static_cast<const E*>(a.q) + t * a.q_st + hq * a.q_sh;
+    const E* k_tail = static_cast<const E*>(a.cache.k_tail) + open;
+    const E* v_tail = static_cast<const E*>(a.cache.v_tail) + open;
+    const double scale = a.minus ? -static_cast<double>(a.scale) : a.scale;
+    const int64_t keys = static_cast<int64_t>(a.count) << SHIFT;
+#pragma unroll 1
+    for (int64_t first = int64_t{part} * 64; first < keys; first += int64_t{parts} * 64) {
+      const int64_t key = first + lane;
+      const int32_t slot = static_cast<int32_t>(key) & ((1 << SHIFT) - 1);
+      int32_t page = -1;  // -1: no key; past the cache's: the open block
+      float x = -INFINITY, vs = 0.0f;
+      if (key < keys) {
+        const int32_t block = list[key >> SHIFT];
+        if (block >= 0 && block <= place.last && slot <= place.pos - (block << SHIFT)) {
+          page = kv_page(a.tok, place, block);
+        }
+        if (page >= 0) {
+          const int64_t row = static_cast<int64_t>(page) * a.Hkv + head;
+          const float ks = a.cache.k_scales[row];
+          if (ks > 0.0f) {
+            vs = a.cache.v_scales[row];
+          } else {
+            page = block == place.last ? a.tok.P : -1;
+          }
+          if (page >= 0) {
+            const int8_t* codes = a.cache.k_codes + ((row << SHIFT) + slot) * D;
+            double sum = 0.0, none = 0.0;
+#pragma unroll 1
+            for (int d = 0; d < D; d += 8) {
+              const V8 f = *reinterpret_cast<const V8*>(q + d);
+              V8 k{};
+              v2i c{};
+              if (ks > 0.0f) {
+                c = *reinterpret_cast<const v2i*>(codes + d);
+              } else {
+                k = *reinterpret_cast<const V8*>(k_tail + slot * D + d);
+              }
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const double of = static_cast<double>(static_cast<float>(f[e]));
+                const float code = static_cast<int8_t>(c[e >> 2] >> (8 * (e & 3)));
+                sum = __builtin_fma(of, ks > 0.0f ? code : static_cast<float>(k[e]), sum);
+                none = __builtin_fma(of, 0.0, none);
+              }
+            }
+            // (a query that is not finite: not a number, whatever the key)
+            x = static_cast<float>((sum + none) * (ks > 0.0f ? ks : 1.0f) * scale);
+          }
+        }
+      }
+      float top = x;
+#pragma unroll
+      for (int i = 1; i < kWave; i <<= 1) top = fmaxf(top, __shfl_xor(top, i));
+      const float next = fmaxf(m, top), keep = __builtin_amdgcn_exp2f(m - next);
+      const float w = page < 0 ? 0.0f : __builtin_amdgcn_exp2f(x - next);
+      float sum = w;
+#pragma unroll
+      for (int i = 1; i < kWave; i <<= 1) sum += __shfl_xor(sum, i);
+      m = next;
+      l = l * keep + sum;
+#pragma unroll
+      for (int r = 0; r < R; ++r) acc[r] *= keep;
+#pragma unroll 1
+      for (uint64_t left = __ballot(page >= 0); left != 0; left &= left - 1) {
+        const int at = __builtin_ctzll(left);
+        const int32_t pg = __builtin_amdgcn_readlane(page, at);
+        const int32_t sl = __builtin_amdgcn_readlane(slot, at);
+        const float wj = lane_value(w, at), sj = lane_value(vs, at);
+        const int8_t* codes = a.cache.v_codes +
+                              (((static_cast<int64_t>(pg) * a.Hkv + head) * D) << SHIFT) + sl;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const int d = r * kWave + lane;
+          if (d < D) {
+            const float v = pg < a.tok.P ? static_cast<float>(codes[d << SHIFT]) * sj
+                                         : static_cast<float>(v_tail[(d << SHIFT) + sl]);
+            acc[r] = fmaf(wj, v, acc[r]);
+          }
+        }
+      }
+    }
+  }
+};
+
+// The kernel's arguments, read where they are used: what a path that is seldom taken reads would
+// otherwise be held in registers from the start.
+__device__ inline const AttendInt8Args& late_args() {
+  auto* p = __builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const AttendInt8Args*)(p);
 }
 
 // Single tokens, and few rows: the workgroup's waves (and `parts` workgroups) share a row's list in
@@ -723,6 +811,37 @@ struct SplitWave : Int8Wave<E, D, SHIFT, 1> {
     full = __ballot(s.at != 0 && !is_open);
     open = __ballot(s.at != 0 && is_open);
     return true;
+  }
+  // The sums of a wave's share taken again, a column at a time, by way of `lds` (16 rows of D) and
+  // `ml`, which are the wave's own and free.
+  __device__ void alone(const AttendInt8Args& a, int64_t t, int head, int tile, int part, int parts,
+                        float* lds, float (&ml)[16][2]) {
+    const int lane = lane_id(), col = lane & 15, grp = lane >> 4;
+    const int heads = a.G - tile * 16 < 16 ? a.G - tile * 16 : 16;
+    AloneSums<E, D, SHIFT> sums;
+#pragma unroll 1
+    for (int g = 0; g < 16; ++g) {
+      if (g < heads) {
+        sums.run(a, t, head, static_cast<int64_t>(head) * a.G + tile * 16 + g, part, parts);
+      }
+#pragma unroll
+      for (int r = 0; r < sums.R; ++r) {
+        const int d = r * kWave + lane;
+        if (d < D) lds[g * D + d] = g < heads ? sums.acc[r] : 0.0f;
+      }
+      if (lane == 0) {
+        ml[g][0] = g < heads ? sums.m : -3.402823466e38f;
+        ml[g][1] = g < heads ? sums.l : 0.0f;
+      }
+    }
+    wave_sync_memory();
+    this->m[0] = ml[col][0];
+    this->l[0] = ml[col][1];
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+      this->acc[0][i] = *reinterpret_cast<const v4f*>(lds + col * D + 16 * i + 4 * grp);
+    }
+    wave_sync_memory();
   }
   // `stream`: others do not read these blocks.
   __device__ void run(const AttendInt8Args& a, int64_t t, int head, int tile, int part, int parts,
@@ -793,7 +912,7 @@ struct SplitWave : Int8Wave<E, D, SHIFT, 1> {
 };
 
 template <class E, int D, int SHIFT>
-__global__ void __launch_bounds__(kAttendWaves* kWave, attend_int8_waves(D, SHIFT))
+__global__ void __launch_bounds__(kAttendWaves* kWave, attend_int8_waves(D, SHIFT, 0))
     kv_attend_int8_split_kernel(AttendInt8Args a) {
   __shared__ __attribute__((aligned(16))) char lds[kAttendWaves][64 * D];  // keys, then sums
   __shared__ __attribute__((aligned(16))) char values[kAttendWaves][64 * D];
@@ -811,7 +930,12 @@ __global__ void __launch_bounds__(kAttendWaves* kWave, attend_int8_waves(D, SHIF
                       (t + 1 < a.T && a.tok.seq_ids[t + 1] == seq);
   const int first = part * kAttendWaves + wave, parts = a.parts * kAttendWaves;
   w.run(a, t, head, tile, first, parts, !beside, lds[wave], values[wave]);
-  w.finish();
+  if (__builtin_expect(w.far, 0)) {
+    w.alone(late_args(), t, head, tile, first, parts, reinterpret_cast<float*>(values[wave]),
+            ml[wave]);
+  } else {
+    w.finish();
+  }
   join_waves<E, D>(a, w.acc[0], w.m[0], w.l[0], t, head, tile, row, part, lds, ml);
 }
 
@@ -918,7 +1042,7 @@ __device__ inline int join_lists(const AttendInt8Args& a, int64_t t0, int tokens
 }
 
 template <class E, int D, int SHIFT, int CT>
-__global__ void __launch_bounds__(kAttendWaves* kWave, attend_int8_waves(D, SHIFT))
+__global__ void __launch_bounds__(kAttendWaves* kWave, attend_int8_waves(D, SHIFT, CT))
     kv_attend_int8_joined_kernel(AttendInt8Args a) {
   __shared__ __attribute__((aligned(16))) JoinInt8Lds<D, CT> lds;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
@@ -1052,11 +1176,34 @@ __global__ void __launch_bounds__(kAttendWaves* kWave, attend_int8_waves(D, SHIF
       }
     }
   }
+  if (lane == 0) lds.counts[wave] = w.far ? 1 : 0;
+  __syncthreads();  // (the stages are free)
+  int far = 0;
+#pragma unroll
+  for (int i = 0; i < kAttendWaves; ++i) far |= lds.counts[i];
+  if (__builtin_expect(__builtin_amdgcn_readfirstlane(far) != 0, 0)) {  // (the rows one by one)
+    const AttendInt8Args& a = late_args();
+#pragma unroll 1
+    for (int i = wave; i < tokens * a.G; i += kAttendWaves) {
+      const int64_t t = t0 + i / a.G, hq = static_cast<int64_t>(head) * a.G + i % a.G;
+      AloneSums<E, D, SHIFT> sums;
+      sums.run(a, t, head, hq, 0, 1);
+      const float inv = inverse_sum(sums.l);
+      E* out = static_cast<E*>(a.out) + (t * a.Hq + hq) * D;
+#pragma unroll
+      for (int r = 0; r < sums.R; ++r) {
+        const int d = r * kWave + lane;
+        if (d < D) out[d] = static_cast<E>(sums.acc[r] * inv);
+      }
+      if (lane == 0) a.lse[t * a.Hq + hq] = log_sum(sums.m, sums.l);
+    }
+    return;
+  }
   w.finish();
 #pragma unroll
   for (int c = 0; c < CT; ++c) {
     if (c > 0 && c * each >= tokens) continue;
-    __syncthreads();
+    if (c > 0) __syncthreads();
     join_columns<E, D>(w.acc[c], w.m[c], w.l[c], wave, lds.keys, lds.ml, each * a.G,
                        [&](int g, int ch, float m, float l, v4f sum) {
       typedef E V4 __attribute__((ext_vector_type(4)));

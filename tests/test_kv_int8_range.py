@@ -166,3 +166,42 @@ def test_scores_of_zero_beside_large_ones(dev, kind, size, scale, n):
         off = 2.0**-17 + 2.0**-20 * np.maximum(1, np.abs(lse))
         assert (np.abs(got_lse - lse[of]) <= off[of]).all()
         assert (np.abs(got_out - out[of]) <= tol[of]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", FORMS)
+@pytest.mark.parametrize("kind,page,size,scale", [("bf16", 16, 1.0, 2.0**20), ("fp16", 64, 1.0, 2.0**24),
+                                                  ("fp16", 32, -1.0, 2.0**36),
+                                                  ("bf16", 128, 2.0**123, None),
+                                                  ("bf16", 16, -(2.0**123), None)])
+def test_equal_far_scores(dev, kind, page, size, scale, n):
+    """Keys that are all alike, so that every score of a row is the same number, over full blocks whose
+    values are of unlike size: each weighs the same, and the output is the values' mean. (Off: its
+    rounding, the weights' and the 2^-17 of a scale's logarithm and its sum; the sums' roundings beside
+    the largest block's as ``kv_int8_cases.check_attention`` has them.)"""
+    print(f"{kind} page={page} {size} x {scale}, x{n}", flush=True)
+    c, q, blocks, pos, seq, tab = _case(77, kind, 8, 2, 128, page, [(9 * page + 3, 1), (7 * page, 4)], 6)
+    last = pos // page
+    for t in range(len(pos)):
+        blocks[t][blocks[t] == last[t]] = -1  # (the open block has no codes)
+    g = np.random.Generator(np.random.PCG64(78))
+    c.k[:] = c.k[:1, :1, :1]
+    c.ks[c.ks > 0] = 0.01 if abs(size) == 1 else 1e-4
+    c.vs[c.vs > 0] = np.exp2(g.uniform(-12, 3, c.vs.shape)).astype(np.float32)[c.vs > 0]
+    q = okv.round16((np.abs(q) + 1) * np.sign(c.k[0, 0, 0]) * np.float32(size), kind)
+    used = 1 / np.sqrt(128) if scale is None else scale
+    out, lse, of = _repeated(dev, n, c, q, blocks, pos, seq, tab, scale)
+    u, w = UNIT[kind], max(UNIT[kind], 2.0**-11)
+    assert np.isfinite(out).all() and np.isfinite(lse).all()
+    for row, t in enumerate(of):
+        for g in range(8):
+            kk, vv = _row(c, blocks[t, g // 4], pos[t], seq[t], g // 4, tab)
+            mean, spread, x = vv.mean(0), np.abs(vv).mean(0), q[t, g].astype(np.float64)
+            score = kk[0] @ x * used
+            assert abs(score) > 2.0**24
+            off = (128 + 16) * 2.0**-24 * (np.abs(kk[0]) @ np.abs(x)) * used
+            off += 2.0**-24 * (128 / 32 + 8) * 255 * c.ks.max() * used * np.abs(x).sum()
+            assert abs(lse[row, g] - score - np.log(len(kk))) <= off + 2.0**-20 * abs(score)
+            tol = u * np.abs(mean) + (w + 2.0**-16) * spread * (1 + u) + 2.0**-25
+            tol += 2.0**-24 * (len(kk) / 32 + 16) * 255 * c.vs.max()
+            assert (np.abs(out[row, g] - mean) <= tol).all(), (t, g, np.abs(out[row, g] - mean).max())
