@@ -47,7 +47,7 @@
 // are looked up one after the other before the first codes) and the end, the rest runs at 6.7 TB/s.
 // Prompts are bound by the vector instructions (59 % of the time, a third of them makes codes into
 // fp16 and a third is the softmax) and by the waits between operands and products: 2053 tokens over
-// 16 blocks each take 152 us. 8 tokens share a pass there; 4, whose codes are widened for one tile
+// 16 blocks each take 153 us. 8 tokens share a pass there; 4, whose codes are widened for one tile
 // of columns, take 169.
 #pragma once
 
