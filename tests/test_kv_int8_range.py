@@ -205,3 +205,60 @@ def test_equal_far_scores(dev, kind, page, size, scale, n):
             tol = u * np.abs(mean) + (w + 2.0**-16) * spread * (1 + u) + 2.0**-25
             tol += 2.0**-24 * (len(kk) / 32 + 16) * 255 * c.vs.max()
             assert (np.abs(out[row, g] - mean) <= tol).all(), (t, g, np.abs(out[row, g] - mean).max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,heads,heads_kv,d,page,count", [("bf16", 20, 1, 64, 16, 128),
+                                                              ("fp16", 4, 2, 128, 64, 60),
+                                                              ("bf16", 3, 1, 256, 32, 70)])
+def test_far_scores_of_long_lists(dev, kind, heads, heads_kv, d, page, count):
+    """Single tokens whose lists are split over workgroups, more heads than one tile has."""
+    print(f"{kind} {heads}/{heads_kv} d={d} page={page} count={count}", flush=True)
+    c, q, *rest = _case(81, kind, heads, heads_kv, d, page, [(page * 150 + 5, 1), (40, 1)], count)
+    got = (*_run(dev, c, q, *rest, 2.0**40), np.arange(2))
+    _check_winners(got, c, q, *rest, 2.0**40)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", FORMS)
+def test_rows_beside_far_ones(dev, n):
+    """Tokens of far scores beside padding, rows without a list, queries that are not finite and tokens
+    of ordinary scores: each as it is alone; captured, replayed and the same bits every time."""
+    import torch
+
+    from retrieve_amd import kv
+    from tests.kv_cases import back, to
+    from tests.kv_int8_cases import check_attention, on_gpu
+
+    c, q, blocks, pos, seq, tab = _case(83, "bf16", 8, 2, 64, 16, [(200, 2), (90, 6)], 6)
+    q[0] = okv.round16(q[0] * np.float32(2.0**60), "bf16")
+    pos[1], blocks[2], q[3, 5, 7] = -1, -1, np.nan
+    case = [np.repeat(x, n, 0) for x in (q, blocks, pos, seq)]
+    gq, gb, gp, gs, gt = to(dev, case[0], "bf16"), *(to(dev, x) for x in (*case[1:], tab))
+    cache = on_gpu(dev, c)[0]
+
+    def call():
+        return kv.block_attention_int8(gq, *cache, gb, gp, gs, gt)
+
+    out, lse = (back(x) for x in call())
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        held = call()
+    for _ in range(3):
+        for x in held:
+            x.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert np.array_equal(back(held[0]), out, equal_nan=True)
+        assert np.array_equal(back(held[1]), lse, equal_nan=True)
+    pick = np.sort(np.r_[0:len(pos) * n:n, n - 1:len(pos) * n:n])
+    of = pick // n
+    out, lse = out[pick], lse[pick]
+    none = (of == 1) | (of == 2)
+    assert (out[none] == 0).all() and np.isneginf(lse[none]).all()
+    assert np.isnan(out[of == 3, 5]).all() and np.isnan(lse[of == 3, 5]).all()
+    first = of == 0
+    _check_winners((out[first], lse[first], of[first]), c, q, blocks, pos, seq, tab)
+    rest = of > 3
+    check_attention((out[rest], lse[rest]), c, *(x[of[rest]] for x in (q, blocks, pos, seq)), tab)
