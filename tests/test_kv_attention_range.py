@@ -5,7 +5,7 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
-from tests.test_kv_attention import UNIT, _case, _run
+from tests.test_kv_attention import UNIT, _case, _check, _run
 
 
 def _check_winners(got, of, kind, q, kc, vc, blocks, pos, seq, tab, scale):
@@ -60,3 +60,33 @@ def test_far_scores(dev, kind, scale, heads, n):
         many = [np.repeat(x, n, 0) for x in (q, blocks, pos, seq)]
         out, lse = _run(dev, kind, many[0], kc, vc, *many[1:], tab, scale)
         _check_winners((out[pick], lse[pick]), pick // n, kind, q, kc, vc, blocks, pos, seq, tab, scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,heads,heads_kv,d,page,count", [("bf16", 20, 1, 64, 16, 128),
+                                                              ("fp16", 4, 2, 128, 64, 60),
+                                                              ("bf16", 3, 1, 256, 32, 70)])
+def test_far_scores_of_long_lists(dev, kind, heads, heads_kv, d, page, count):
+    """Single tokens whose lists are split over workgroups."""
+    case = _case(81, kind, heads, heads_kv, d, page, [(page * 150 + 5, 1), (40, 1)], count)
+    _check_winners(_run(dev, kind, *case, 2.0**40), np.arange(2), kind, *case, 2.0**40)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 480])
+def test_rows_beside_far_ones(dev, n):
+    """Tokens of far scores beside padding, rows without a list and tokens of ordinary scores: each as
+    it is alone."""
+    q, kc, vc, blocks, pos, seq, tab = _case(83, "bf16", 8, 2, 64, 16, [(200, 2), (90, 6)], 6)
+    q[0] *= np.float32(2.0**60)
+    pos[1], blocks[2] = -1, -1
+    many = [np.repeat(x, n, 0) for x in (q, blocks, pos, seq)]
+    out, lse = _run(dev, "bf16", many[0], kc, vc, *many[1:], tab)
+    pick = np.sort(np.r_[0:len(pos) * n:n, n - 1:len(pos) * n:n])
+    of = pick // n
+    out, lse = out[pick], lse[pick]
+    none, first, rest = (of == 1) | (of == 2), of == 0, of > 2
+    assert (out[none] == 0).all() and np.isneginf(lse[none]).all()
+    _check_winners((out[first], lse[first]), of[first], "bf16", q, kc, vc, blocks, pos, seq, tab, 0.125)
+    _check((out[rest], lse[rest]), "bf16", q[of[rest]], kc, vc, blocks[of[rest]], pos[of[rest]],
+           seq[of[rest]], tab)
